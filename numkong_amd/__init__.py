@@ -22,3 +22,16 @@ from .api import (  # noqa: F401
     library,
     library_path,
 )
+from .mx import (  # noqa: F401
+    ExpertsPlan,
+    MxMatrix,
+    MxPackedMatrix,
+    experts_plan,
+    experts_route,
+    experts_route_backward,
+    mx_dequantize,
+    mx_dots_experts,
+    mx_dots_packed,
+    mx_pack,
+    mx_quantize,
+)

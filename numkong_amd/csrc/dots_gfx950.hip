@@ -68,6 +68,15 @@ int fail_msg(char const *what) {
     return -1;
 }
 
+} // namespace
+
+namespace nk_gfx950 { // (mx_gfx950.hpp: the same channel for the kernels of the other translation units)
+int mx_fail(hipError_t status, char const *what) { return fail(status, what); }
+int mx_fail(char const *what) { return fail_msg(what); }
+} // namespace nk_gfx950
+
+namespace {
+
 /**
  *  What a host thread keeps between synchronous calls: its streams, the events that order its staging pipeline, and
  *  device and pinned staging buffers that only ever grow. Created on first use, released when the thread ends (a

@@ -1,0 +1,400 @@
+/**
+ *  @brief Routing to experts on gfx950: the choice, its gradient, the plan of the products.
+ *  @file numkong_amd/csrc/experts_gfx950.hip
+ *
+ *  Implements the experts half of <numkong_amd/mx.h> but for the products (mx_gfx950.hip).
+ */
+#include "mx_gfx950.hpp"
+
+namespace nk_gfx950 {
+namespace {
+
+// ---- reductions over a wavefront ----------------------------------------------------------------------------------
+
+template <class F>
+__device__ __forceinline__ float wave_reduce(float x, F &&join) {
+#pragma unroll
+    for (int step = 32; step; step >>= 1) x = join(x, __shfl_xor(x, step));
+    return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+    return wave_reduce(x, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+#pragma unroll
+    for (int step = 32; step; step >>= 1) {
+        uint32_t const other = (uint32_t)__shfl_xor((int)x, step);
+        x = x > other ? x : other;
+    }
+    return x;
+}
+
+/** Numbers in the order of unsigned integers: larger number, larger key; every NaN above them all, both zeros the same.
+ *  Zero is below every key: what is taken already. */
+__device__ __forceinline__ uint32_t key_of(float x) {
+    if (x != x) return 0xFFFFFFFFu;
+    uint32_t const bits = __float_as_uint(x + 0.0f);
+    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+constexpr uint32_t kMaskedKey = 0x007FFFFFu; // of -inf
+
+/** What one lane holds of a row: experts lane * J ... lane * J + J - 1, -inf past the end. */
+template <class T, int J>
+__device__ __forceinline__ void load_row(T const *row, uint32_t lane, uint32_t experts, float (&l)[J]) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        uint32_t const e = lane * J + j;
+        l[j] = e < experts ? (float)row[e] : -__builtin_inff();
+    }
+}
+
+/** Scores of a row from its logits; -inf logits have score 0, also where the whole row is -inf. */
+template <int J>
+__device__ __forceinline__ void scores_of(float const (&l)[J], int sigmoid, float (&s)[J]) {
+    if (sigmoid) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) s[j] = 1.0f / (1.0f + expf(-l[j]));
+        return;
+    }
+    float top = l[0];
+#pragma unroll
+    for (int j = 1; j < J; ++j) top = fmaxf(top, l[j]);
+    top = wave_reduce(top, [](float a, float b) { return fmaxf(a, b); });
+    float sum = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) s[j] = l[j] == -__builtin_inff() ? 0.0f : expf(l[j] - top), sum += s[j];
+    sum = wave_sum(sum);
+#pragma unroll
+    for (int j = 0; j < J; ++j) s[j] = s[j] == 0.0f ? 0.0f : s[j] / sum;
+}
+
+struct RouteArgs {
+    void const *logits;
+    uint64_t stride;
+    uint32_t tokens, experts, top_k;
+    float const *bias;
+    nk_amd_route_t how;
+    float *weights;
+    int32_t *chosen;
+};
+
+/**
+ *  A wavefront for a token: the row stays in registers, J experts a lane, adjacent ones, so that of equal keys the lowest
+ *  lane's lowest is the lowest expert. A choice is a maximum over the wavefront and a ballot.
+ */
+template <class T, int J>
+__global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
+    uint32_t const lane = threadIdx.x & 63, token = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (token >= p.tokens) return;
+    float l[J], s[J];
+    load_row<T, J>((T const *)((uint8_t const *)p.logits + token * p.stride), lane, p.experts, l);
+    scores_of<J>(l, p.how.sigmoid, s);
+    uint32_t key[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        uint32_t const e = lane * J + j;
+        bool const masked = l[j] == -__builtin_inff();
+        key[j] = e >= p.experts ? 0u : masked ? kMaskedKey : key_of(p.bias ? s[j] + p.bias[e] : l[j]);
+    }
+    if (p.how.groups > 1) {
+        uint32_t const groups = (uint32_t)p.how.groups, size = p.experts / groups;
+        uint32_t mine = 0; // the key of group `lane`
+        for (uint32_t group = 0; group < groups; ++group) {
+            uint32_t best = 0;
+            int at = 0;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                uint32_t const e = lane * J + j;
+                bool const inside = e >= group * size && e < (group + 1) * size;
+                if (inside && key[j] > best) best = key[j], at = j;
+            }
+            uint32_t const first = wave_max(best);
+            uint32_t group_key = first;
+            if (p.how.group_top == 2 && size > 1) {
+                uint64_t const holders = __ballot(best == first && first != 0);
+                bool const winner = holders && lane == (uint32_t)__builtin_ctzll(holders);
+                uint32_t next = 0;
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    uint32_t const e = lane * J + j;
+                    bool const inside = e >= group * size && e < (group + 1) * size && !(winner && j == at);
+                    if (inside && key[j] > next) next = key[j];
+                }
+                uint32_t const second = wave_max(next);
+                auto const number = [](uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); };
+                group_key = key_of(number(first) + number(second));
+            }
+            if (lane == group) mine = group_key;
+        }
+        uint64_t stays = 0;
+        for (int i = 0; i < p.how.top_groups; ++i) {
+            uint32_t const best = wave_max(mine);
+            uint32_t const which = (uint32_t)__builtin_ctzll(__ballot(mine == best));
+            stays |= 1ull << which;
+            if (lane == which) mine = 0;
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            uint32_t const e = lane * J + j;
+            if (e < p.experts && !(stays >> (e / size) & 1)) key[j] = kMaskedKey;
+        }
+    }
+    float weight = 0;
+    int32_t expert = -1;
+    for (uint32_t i = 0; i < p.top_k; ++i) {
+        uint32_t best = key[0], score = __float_as_uint(s[0]);
+        int at = 0;
+#pragma unroll
+        for (int j = 1; j < J; ++j)
+            if (key[j] > best) best = key[j], at = j, score = __float_as_uint(s[j]);
+        uint32_t const top = wave_max(best);
+        if (top <= kMaskedKey) break; // the rest of the slots stay empty
+        uint32_t const which = (uint32_t)__builtin_ctzll(__ballot(best == top));
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+            if (lane == which && j == at) key[j] = 0;
+        float const its_score = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)score, (int)which));
+        int32_t const its_expert = (int32_t)which * J + __builtin_amdgcn_readlane(at, (int)which);
+        if (lane == i) weight = its_score, expert = its_expert;
+    }
+    if (p.how.renormalize) weight /= wave_sum(weight) + 1e-20f;
+    weight *= p.how.scale;
+    if (lane < p.top_k) {
+        p.weights[(uint64_t)token * p.top_k + lane] = expert < 0 ? 0.0f : weight;
+        p.chosen[(uint64_t)token * p.top_k + lane] = expert;
+    }
+}
+
+/**
+ *  With s the scores, S the chosen, D = sum_S s + 1e-20:  ds_j = scale (g_j - sum_S g s / D) / D where weights are
+ *  renormalised, scale g_j where not, 0 outside S; then dl_j = ds_j s_j (1 - s_j) for sigmoid scores, and
+ *  dl_i = s_i (ds_i - sum_S ds s) for softmax.
+ */
+template <class T, int J>
+__global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs p, float const *grad, T *out, uint64_t out_stride) {
+    uint32_t const lane = threadIdx.x & 63, token = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (token >= p.tokens) return;
+    float l[J], s[J];
+    load_row<T, J>((T const *)((uint8_t const *)p.logits + token * p.stride), lane, p.experts, l);
+    scores_of<J>(l, p.how.sigmoid, s);
+    float const its_grad = lane < p.top_k ? grad[(uint64_t)token * p.top_k + lane] : 0.0f;
+    int32_t const its_expert = lane < p.top_k ? p.chosen[(uint64_t)token * p.top_k + lane] : -1;
+    float g[J];
+    bool in[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) g[j] = 0, in[j] = false;
+    for (uint32_t i = 0; i < p.top_k; ++i) {
+        int32_t const e = __builtin_amdgcn_readlane(its_expert, (int)i);
+        float const of_e = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(__float_as_int(its_grad), (int)i));
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+            if (e == (int32_t)(lane * J + j) && e < (int32_t)p.experts) g[j] = of_e, in[j] = true;
+    }
+    float total = 0, along = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+        if (in[j]) total += s[j], along += g[j] * s[j];
+    total = wave_sum(total) + 1e-20f, along = wave_sum(along);
+    float ds[J], inner = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        ds[j] = !in[j] ? 0.0f : p.how.scale * (p.how.renormalize ? (g[j] - along / total) / total : g[j]);
+        inner += in[j] ? ds[j] * s[j] : 0.0f;
+    }
+    inner = wave_sum(inner);
+    T *row = (T *)((uint8_t *)out + token * out_stride);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        uint32_t const e = lane * J + j;
+        // (1 - s of a sigmoid is the score of the opposite logit, without its cancellation)
+        float const slope = p.how.sigmoid ? (in[j] ? ds[j] * s[j] / (1.0f + expf(l[j])) : 0.0f) : s[j] * (ds[j] - inner);
+        if (e < p.experts) row[e] = (T)(l[j] == -__builtin_inff() ? 0.0f : slope);
+    }
+}
+
+// ---- the plan -----------------------------------------------------------------------------------------------------
+
+constexpr int kPlanWaves = 16;
+/** Lanes of the wavefront that hold the same bucket, by one ballot for each bit. */
+__device__ __forceinline__ uint64_t same_bucket(uint32_t bucket, int bits, bool active) {
+    uint64_t mask = __ballot(active);
+    for (int bit = 0; bit < bits; ++bit) {
+        bool const set = bucket >> bit & 1;
+        uint64_t const with = __ballot(active && set);
+        mask &= set ? with : ~with;
+    }
+    return mask;
+}
+
+/**
+ *  Counting sort of the slots by expert in one workgroup: each wavefront takes a stretch of the slots, counts it, learns
+ *  where its slots of each expert go, and goes over it again in order, so that no atomic decides an order. Bucket
+ *  `experts` is for slots of none.
+ */
+__global__ __launch_bounds__(64 * kPlanWaves) void plan_kernel(int32_t const *chosen, uint32_t slots, uint32_t experts,
+                                                               PlanHeader header, uint32_t offsets, uint32_t order,
+                                                               uint32_t place, uint32_t tiles, int bits, uint32_t *plan) {
+    extern __shared__ uint32_t plan_lds[]; // [wave][bucket] counts, then where the wave's next slot of the bucket goes
+    __shared__ uint32_t wave_total[2][kPlanWaves];
+    uint32_t const buckets = experts + 1, thread = threadIdx.x, lane = thread & 63;
+    uint32_t const wave = __builtin_amdgcn_readfirstlane(thread >> 6);
+    for (uint32_t i = thread; i < buckets * kPlanWaves; i += 64 * kPlanWaves) plan_lds[i] = 0;
+    __syncthreads();
+    uint32_t const stretch = ((slots + kPlanWaves - 1) / kPlanWaves + 63) & ~63u;
+    uint32_t const begin = wave * stretch < slots ? wave * stretch : slots, end = begin + stretch < slots ? begin + stretch : slots;
+    uint32_t *counts = plan_lds + wave * buckets;
+    for (uint32_t at = begin + lane; at < end; at += 64) {
+        uint32_t const e = (uint32_t)chosen[at];
+        atomicAdd(counts + (e < experts ? e : experts), 1u);
+    }
+    __syncthreads();
+    // a thread for a bucket (two where there are more than threads): its size, then rows and tiles before it
+    uint32_t rows_before = 0, tiles_before = 0;
+    for (uint32_t base = 0; base < buckets; base += 64 * kPlanWaves) {
+        uint32_t const bucket = base + thread;
+        uint32_t size = 0;
+        if (bucket < buckets)
+            for (int w = 0; w < kPlanWaves; ++w) size += plan_lds[w * buckets + bucket];
+        uint32_t const its_tiles = (size + header.tile_rows - 1) / header.tile_rows;
+        uint32_t rows = size, tiles_upto = its_tiles; // inclusive sums over the wavefront, then over wavefronts
+#pragma unroll
+        for (int step = 1; step < 64; step <<= 1) {
+            uint32_t const r = (uint32_t)__shfl_up((int)rows, step), t = (uint32_t)__shfl_up((int)tiles_upto, step);
+            if (lane >= (uint32_t)step) rows += r, tiles_upto += t;
+        }
+        if (lane == 63) wave_total[0][wave] = rows, wave_total[1][wave] = tiles_upto;
+        __syncthreads();
+        uint32_t first = rows_before + rows - size, first_tile = tiles_before + tiles_upto - its_tiles;
+        for (uint32_t w = 0; w < (uint32_t)kPlanWaves; ++w) {
+            if (w < wave) first += wave_total[0][w], first_tile += wave_total[1][w];
+            rows_before += wave_total[0][w], tiles_before += wave_total[1][w];
+        }
+        if (bucket < buckets) {
+            plan[offsets + bucket] = first;
+            uint32_t next = first;
+            for (int w = 0; w < kPlanWaves; ++w) {
+                uint32_t const here = plan_lds[w * buckets + bucket];
+                plan_lds[w * buckets + bucket] = next;
+                next += here;
+            }
+            for (uint32_t t = 0; t < its_tiles; ++t) {
+                uint32_t const from = first + t * header.tile_rows, to = from + header.tile_rows;
+                PlanTile const tile = {(int32_t)bucket, (int32_t)from, (int32_t)(to < first + size ? to : first + size), 0};
+                *(PlanTile *)(plan + tiles + (first_tile + t) * 4) = tile;
+            }
+            if (bucket == experts) header.valid_rows = first, plan[offsets + buckets] = first + size;
+        }
+        __syncthreads();
+    }
+    if ((experts & (64 * kPlanWaves - 1)) == thread) { // the thread that had the last bucket
+        header.tile_count = tiles_before;
+        *(PlanHeader *)plan = header;
+    }
+    for (uint32_t base = begin; base < end; base += 64) {
+        uint32_t const at = base + lane;
+        bool const active = at < end;
+        uint32_t const e = active ? (uint32_t)chosen[at] : 0, bucket = e < experts ? e : experts;
+        uint64_t const same = same_bucket(bucket, bits, active);
+        uint32_t const rank = (uint32_t)__popcll(same & ((1ull << lane) - 1));
+        if (active) {
+            uint32_t const row = counts[bucket] + rank;
+            plan[order + row] = at;
+            plan[place + at] = bucket < experts ? row : 0xFFFFFFFFu;
+        }
+        __builtin_amdgcn_wave_barrier(); // (every lane has read its count before the first of each bucket moves it on)
+        if (active && !rank) counts[bucket] += (uint32_t)__popcll(same);
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+int check_route(nk_dtype_t dtype, void const *logits, nk_size_t stride, nk_size_t tokens, nk_size_t experts, nk_size_t top_k,
+                nk_amd_route_t const *how) {
+    int const bytes = dtype == nk_f32_k ? 4 : dtype == nk_bf16_k || dtype == nk_f16_k ? 2 : 0;
+    if (!bytes) return mx_fail("experts_route: logits have to be f32, bf16 or f16");
+    if (!how) return mx_fail("experts_route: NULL operand");
+    if (!experts || experts > kMaxExperts || !top_k || top_k > kMaxTopK || top_k > experts) return mx_fail("experts_route: 1 to 1024 experts, top_k at most 64 and no more than there are");
+    if (tokens >= (1ull << 31)) return mx_fail("experts_route: too many tokens");
+    if (how->groups < 1 || how->groups > (int)kMaxGroups || experts % how->groups || how->top_groups < 1 || how->top_groups > how->groups ||
+        how->group_top < 1 || how->group_top > 2)
+        return mx_fail("experts_route: groups have to divide the experts, at most 64, top_groups 1 to groups, group_top 1 or 2");
+    if (tokens && (!logits || (((uintptr_t)logits | stride) & (bytes - 1)))) return mx_fail("experts_route: logits are NULL or not aligned to their elements");
+    return 0;
+}
+
+/** Calls `f` with a value of the logits' type and one that says how many experts a lane holds. */
+template <class F>
+int with_row(nk_dtype_t dtype, size_t experts, F &&f) {
+    auto const of_type = [&](auto value) {
+        if (experts <= 64) return f(value, Number<1>());
+        if (experts <= 128) return f(value, Number<2>());
+        if (experts <= 256) return f(value, Number<4>());
+        if (experts <= 512) return f(value, Number<8>());
+        return f(value, Number<16>());
+    };
+    if (dtype == nk_f32_k) return of_type(float());
+    if (dtype == nk_bf16_k) return of_type(__bf16());
+    return of_type(_Float16());
+}
+
+} // namespace
+} // namespace nk_gfx950
+
+using namespace nk_gfx950;
+
+extern "C" {
+
+int nk_amd_experts_route_async(nk_dtype_t dtype, void const *logits, nk_size_t logits_stride, nk_size_t tokens, nk_size_t experts,
+                               nk_size_t top_k, float const *bias, nk_amd_route_t const *how, float *weights, nk_i32_t *chosen,
+                               void *stream) {
+    if (int const status = check_route(dtype, logits, logits_stride, tokens, experts, top_k, how)) return status;
+    if ((size_t)how->top_groups * (experts / how->groups) < top_k) return mx_fail("experts_route: the groups that stay hold fewer than top_k experts");
+    if (!tokens) return 0;
+    if (!weights || !chosen) return mx_fail("experts_route: NULL operand");
+    RouteArgs const p = {logits, logits_stride, (uint32_t)tokens, (uint32_t)experts, (uint32_t)top_k, bias, *how, weights, chosen};
+    return with_row(dtype, experts, [&](auto value, auto per_lane) {
+        typedef decltype(value) T;
+        hipLaunchKernelGGL((route_kernel<T, decltype(per_lane)::value>), dim3((uint32_t)((tokens + 3) / 4)), dim3(256), 0, (hipStream_t)stream, p);
+        hipError_t const e = hipGetLastError();
+        return e == hipSuccess ? 0 : mx_fail(e, "route_kernel");
+    });
+}
+
+int nk_amd_experts_route_backward_async(nk_dtype_t dtype, void const *logits, nk_size_t logits_stride, nk_size_t tokens,
+                                        nk_size_t experts, nk_size_t top_k, nk_amd_route_t const *how, nk_i32_t const *chosen,
+                                        float const *grad_weights, void *grad_logits, nk_size_t grad_stride, void *stream) {
+    if (int const status = check_route(dtype, logits, logits_stride, tokens, experts, top_k, how)) return status;
+    if (!tokens) return 0;
+    if (!chosen || !grad_weights || !grad_logits) return mx_fail("experts_route_backward: NULL operand");
+    int const bytes = dtype == nk_f32_k ? 4 : 2;
+    if (((uintptr_t)grad_logits | grad_stride) & (bytes - 1)) return mx_fail("experts_route_backward: grad_logits is not aligned to its elements");
+    RouteArgs const p = {logits, logits_stride, (uint32_t)tokens, (uint32_t)experts, (uint32_t)top_k, nullptr, *how, nullptr, (int32_t *)chosen};
+    return with_row(dtype, experts, [&](auto value, auto per_lane) {
+        typedef decltype(value) T;
+        hipLaunchKernelGGL((route_backward_kernel<T, decltype(per_lane)::value>), dim3((uint32_t)((tokens + 3) / 4)), dim3(256), 0,
+                           (hipStream_t)stream, p, grad_weights, (T *)grad_logits, (uint64_t)grad_stride);
+        hipError_t const e = hipGetLastError();
+        return e == hipSuccess ? 0 : mx_fail(e, "route_backward_kernel");
+    });
+}
+
+nk_size_t nk_amd_experts_plan_size(nk_size_t slots, nk_size_t experts) {
+    PlanGeometry g;
+    return plan_geometry(slots, experts, g) ? g.total_words * 4 : 0;
+}
+
+int nk_amd_experts_plan_async(nk_i32_t const *chosen, nk_size_t slots, nk_size_t experts, void *plan, void *stream) {
+    PlanGeometry g;
+    if (!plan_geometry(slots, experts, g)) return mx_fail("experts_plan: 1 to 1024 experts, fewer than 2^30 slots");
+    if (!plan || ((uintptr_t)plan & 15)) return mx_fail("experts_plan: the plan has to be 16-byte aligned");
+    if (slots && (!chosen || ((uintptr_t)chosen & 3))) return mx_fail("experts_plan: chosen is NULL or misaligned");
+    PlanHeader const header = {kPlanMagic, (uint32_t)slots, (uint32_t)experts, g.tile_rows, 0, 0, {0, 0}};
+    int bits = 0;
+    while (experts >> bits) ++bits;
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(64 * kPlanWaves), (uint32_t)((experts + 1) * kPlanWaves * 4), (hipStream_t)stream,
+                       chosen, (uint32_t)slots, (uint32_t)experts, header, (uint32_t)g.offsets, (uint32_t)g.order, (uint32_t)g.place,
+                       (uint32_t)g.tiles, bits, (uint32_t *)plan);
+    hipError_t const e = hipGetLastError();
+    return e == hipSuccess ? 0 : mx_fail(e, "plan_kernel");
+}
+
+} // extern "C"
