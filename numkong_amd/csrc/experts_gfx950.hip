@@ -256,7 +256,8 @@ __global__ __launch_bounds__(64 * kPlanWaves) void plan_kernel(int32_t const *ch
         if (bucket < buckets)
             for (int w = 0; w < kPlanWaves; ++w) size += plan_lds[w * buckets + bucket];
         uint32_t const its_tiles = (size + header.tile_rows - 1) / header.tile_rows;
-        uint32_t rows = size, tiles_upto = its_tiles; // inclusive sums over the wavefront, then over wavefronts
+        uint32_t const its_rows = (size + 15) / 16 * 16;
+        uint32_t rows = its_rows, tiles_upto = its_tiles; // inclusive sums over the wavefront, then over wavefronts
 #pragma unroll
         for (int step = 1; step < 64; step <<= 1) {
             uint32_t const r = (uint32_t)__shfl_up((int)rows, step), t = (uint32_t)__shfl_up((int)tiles_upto, step);
@@ -264,7 +265,7 @@ __global__ __launch_bounds__(64 * kPlanWaves) void plan_kernel(int32_t const *ch
         }
         if (lane == 63) wave_total[0][wave] = rows, wave_total[1][wave] = tiles_upto;
         __syncthreads();
-        uint32_t first = rows_before + rows - size, first_tile = tiles_before + tiles_upto - its_tiles;
+        uint32_t first = rows_before + rows - its_rows, first_tile = tiles_before + tiles_upto - its_tiles;
         for (uint32_t w = 0; w < (uint32_t)kPlanWaves; ++w) {
             if (w < wave) first += wave_total[0][w], first_tile += wave_total[1][w];
             rows_before += wave_total[0][w], tiles_before += wave_total[1][w];
@@ -282,14 +283,12 @@ __global__ __launch_bounds__(64 * kPlanWaves) void plan_kernel(int32_t const *ch
                 PlanTile const tile = {(int32_t)bucket, (int32_t)from, (int32_t)(to < first + size ? to : first + size), 0};
                 *(PlanTile *)(plan + tiles + (first_tile + t) * 4) = tile;
             }
-            if (bucket == experts) header.valid_rows = first, plan[offsets + buckets] = first + size;
+            for (uint32_t at = first + size; at < first + its_rows; ++at) plan[order + at] = 0xFFFFFFFFu;
+            if (bucket == experts) header.tile_count = first_tile, header.zero_tiles = its_tiles, header.first_zero = first, header.end_zero = first + size, plan[offsets + buckets] = first + size;
         }
         __syncthreads();
     }
-    if ((experts & (64 * kPlanWaves - 1)) == thread) { // the thread that had the last bucket
-        header.tile_count = tiles_before;
-        *(PlanHeader *)plan = header;
-    }
+    if ((experts & (64 * kPlanWaves - 1)) == thread) *(PlanHeader *)plan = header; // (the thread that had the last bucket)
     for (uint32_t base = begin; base < end; base += 64) {
         uint32_t const at = base + lane;
         bool const active = at < end;
@@ -387,7 +386,7 @@ int nk_amd_experts_plan_async(nk_i32_t const *chosen, nk_size_t slots, nk_size_t
     if (!plan_geometry(slots, experts, g)) return mx_fail("experts_plan: 1 to 1024 experts, fewer than 2^30 slots");
     if (!plan || ((uintptr_t)plan & 15)) return mx_fail("experts_plan: the plan has to be 16-byte aligned");
     if (slots && (!chosen || ((uintptr_t)chosen & 3))) return mx_fail("experts_plan: chosen is NULL or misaligned");
-    PlanHeader const header = {kPlanMagic, (uint32_t)slots, (uint32_t)experts, g.tile_rows, 0, 0, {0, 0}};
+    PlanHeader const header = {kPlanMagic, (uint32_t)slots, (uint32_t)experts, g.tile_rows, 0, 0, 0, 0};
     int bits = 0;
     while (experts >> bits) ++bits;
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(64 * kPlanWaves), (uint32_t)((experts + 1) * kPlanWaves * 4), (hipStream_t)stream,

@@ -13,10 +13,9 @@ namespace {
 
 /**
  *  One thread for eight adjacent values, four for a block, so that a wavefront reads 1 KiB (2 KiB of f32) in one piece.
- *  STAGED: rows padded with zeros to whole steps and scales in the order of the products' operands (mx_gfx950.hpp);
- *  otherwise rows as the caller has them. `pieces`: eights of a row, whole blocks (STAGED: whole steps).
+ *  `pieces`: eights of a row, whole blocks.
  */
-template <class T, bool STAGED>
+template <class T>
 __global__ __launch_bounds__(256) void quantize_kernel(T const *x, uint64_t x_stride, uint32_t rows, uint32_t k, uint32_t pieces,
                                                        bool wide, uint8_t *codes, uint64_t codes_stride, bool whole_words,
                                                        uint8_t *scales, uint64_t scales_stride) {
@@ -30,11 +29,6 @@ __global__ __launch_bounds__(256) void quantize_kernel(T const *x, uint64_t x_st
     uint32_t const word = quantize_eight(v, scale);
     uint32_t const block = piece >> 2;
     uint8_t *to = codes + row * codes_stride + piece * 4;
-    if (STAGED) {
-        *(uint32_t *)to = word;
-        if (!(piece & 3)) scales[row * scales_stride + (block & ~15u) + (block & 3) * 4 + (block >> 2 & 3)] = (uint8_t)scale;
-        return;
-    }
     uint32_t const bytes = col >= k ? 0 : (k - col + 1) / 2;
     if (whole_words && bytes >= 4) *(uint32_t *)to = word;
     else
@@ -42,34 +36,73 @@ __global__ __launch_bounds__(256) void quantize_kernel(T const *x, uint64_t x_st
     if (!(piece & 3)) scales[row * scales_stride + block] = (uint8_t)scale;
 }
 
-/** Rows of codes and scales as callers have them, to the staged form. One thread for a block. */
-__global__ __launch_bounds__(256) void stage_codes_kernel(uint8_t const *codes, uint64_t codes_stride, uint8_t const *scales,
-                                                          uint64_t scales_stride, uint32_t rows, uint32_t k, uint32_t blocks,
-                                                          bool wide, uint8_t *to, uint64_t to_stride, uint8_t *to_scales,
-                                                          uint64_t to_scales_stride) {
-    uint32_t const index = blockIdx.x * 256 + threadIdx.x;
-    uint32_t const row = index / blocks, block = index - row * blocks;
-    if (row >= rows) return;
-    uint8_t const *from = codes + row * codes_stride + block * 16;
-    bool const inside = block * 32 < k;
+/** 16 bytes of a row's codes from `byte` on, which start a block; zeros from column k on. */
+__device__ __forceinline__ v4u load_codes(uint8_t const *row, uint32_t block, uint32_t k, bool wide) {
     v4u word = {0, 0, 0, 0};
-    if (wide && block * 32 + 32 <= k) word = *(v4u const *)from;
-    else if (inside)
-        for (uint32_t i = 0; i < 16; ++i) {
-            uint32_t const col = block * 32 + 2 * i;
-            uint32_t const byte = col + 1 < k ? from[i] : col < k ? from[i] & 15u : 0u;
-            word[i / 4] |= byte << 8 * (i % 4);
+    if (wide && block * 32 + 32 <= k) return *(v4u const *)(row + block * 16);
+    for (uint32_t i = 0; i < 16; ++i) {
+        uint32_t const col = block * 32 + 2 * i;
+        uint32_t const byte = col + 1 < k ? row[col / 2] : col < k ? row[col / 2] & 15u : 0u;
+        word[i / 4] |= byte << 8 * (i % 4);
+    }
+    return word;
+}
+
+struct StageArgs {
+    void const *a;
+    uint64_t a_stride;
+    uint8_t const *scales; // A as codes: its scales
+    uint64_t scales_stride;
+    uint8_t *to, *to_scales;
+    uint32_t const *plan; // rows in the plan's order, or NULL
+    uint32_t rows, k, supers, order, a_share;
+    bool wide;
+};
+/**
+ *  A into fragments: a workgroup for 16 rows of a super, a wavefront for a step of it, a lane for a block, whose 32 values
+ *  it has all to itself, so that the fragment is written in one piece. In: the type of A's values, or `uint8_t`: codes.
+ */
+template <class In>
+__global__ __launch_bounds__(256) void stage_kernel(StageArgs p) {
+    __shared__ uint8_t bytes[256];
+    uint32_t const tile = blockIdx.x / p.supers, super = blockIdx.x - tile * p.supers;
+    uint32_t const lane = threadIdx.x & 63, u = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    uint32_t const row = tile * 16 + r, block = (super * 4 + u) * 4 + g;
+    bool there = row < p.rows;
+    uint64_t source = row;
+    if (p.plan) {
+        if (tile * 16 >= ((PlanHeader const *)p.plan)->first_zero) return;
+        uint32_t const slot = p.plan[p.order + row];
+        there = (int32_t)slot >= 0, source = slot / p.a_share;
+    }
+    v4u words = {0, 0, 0, 0};
+    uint32_t scale = 0;
+    if (there && block * 32 < p.k) {
+        uint8_t const *from = (uint8_t const *)p.a + source * p.a_stride;
+        if constexpr (sizeof(In) == 1) words = load_codes(from, block, p.k, p.wide), scale = p.scales[source * p.scales_stride + block];
+        else {
+            float v[32];
+#pragma unroll
+            for (int part = 0; part < 4; ++part) {
+                float eight[8];
+                load_eight((In const *)from, block * 32 + part * 8, p.k, p.wide, eight);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[part * 8 + i] = eight[i];
+            }
+            words = quantize_block(v, scale);
         }
-    *(v4u *)(to + row * to_stride + block * 16) = word;
-    uint8_t const scale = inside ? scales[row * scales_stride + block] : (uint8_t)0;
-    to_scales[row * to_scales_stride + (block & ~15u) + (block & 3) * 4 + (block >> 2 & 3)] = scale;
+    }
+    *(v4u *)(p.to + (((uint64_t)tile * p.supers + super) * 4 + u) * 1024 + lane * 16) = words;
+    bytes[scale_word(r, g) * 4 + u] = (uint8_t)scale;
+    __syncthreads();
+    if (threadIdx.x < 64) *(uint32_t *)(p.to_scales + ((uint64_t)tile * p.supers + super) * 256 + lane * 4) = *(uint32_t const *)(bytes + lane * 4);
 }
 
 /** value = q * 2^(s - 127), built from the bits: 2 |q| is a whole number up to 12, and 12 * 2^(s - 128) fits 32 bits. */
 template <class T>
 __global__ __launch_bounds__(256) void dequantize_kernel(uint8_t const *codes, uint64_t codes_stride, bool whole_words,
                                                          uint8_t const *scales, uint64_t scales_stride, uint32_t rows,
-                                                         uint32_t k, uint32_t pieces, T *x, uint64_t x_stride, bool wide) {
+                                                         uint32_t k, uint32_t pieces, T *x, uint64_t x_stride) {
     uint32_t const index = blockIdx.x * 256 + threadIdx.x;
     uint32_t const row = index / pieces, col = (index - row * pieces) * 8;
     if (row >= rows) return;
@@ -88,7 +121,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(uint8_t const *codes, u
         float const magnitude = scale == 255 ? __uint_as_float(0x7FC00000u) : ldexpf((float)twice, (int)scale - 128);
         v[i] = code & 8u ? -magnitude : magnitude;
     }
-    store_some<T, 8>((T *)((uint8_t *)x + row * x_stride) + col, v, k - col, wide);
+    store_some<T, 8>((T *)((uint8_t *)x + row * x_stride) + col, v, k - col);
 }
 
 // ---- packing ------------------------------------------------------------------------------------------------------
@@ -96,35 +129,25 @@ __global__ __launch_bounds__(256) void dequantize_kernel(uint8_t const *codes, u
 /** One thread for 16 bytes of a tile's codes or for a word of its scales; the header by the first workgroup. */
 __global__ __launch_bounds__(256) void mx_pack_kernel(uint8_t const *codes, uint64_t codes_stride, uint64_t codes_matrix,
                                                       uint8_t const *scales, uint64_t scales_stride, uint64_t scales_matrix,
-                                                      MxHeader header, uint32_t steps, uint32_t supers, uint32_t tiles,
-                                                      uint64_t first, uint64_t code_lanes, uint64_t scale_lanes, bool wide,
-                                                      uint8_t *image) {
+                                                      MxHeader header, uint32_t supers, uint32_t tiles, uint64_t first,
+                                                      uint64_t code_lanes, uint64_t scale_lanes, bool wide, uint8_t *image) {
     uint64_t const index = first + (uint64_t)blockIdx.x * 256 + threadIdx.x;
     if (index == 0) *(MxHeader *)image = header;
-    uint32_t const lane = index & 63, g = lane >> 4;
-    bool const of_codes = index < code_lanes * header.count;
-    uint64_t const at = (of_codes ? index : index - code_lanes * header.count) >> 6;
-    if (!of_codes && at >= scale_lanes / 64 * header.count) return;
-    uint32_t const across = of_codes ? steps : supers;
-    uint32_t const which = (uint32_t)(at % across); // step or super
+    uint32_t const lane = index & 63;
+    bool const of_codes = index < code_lanes;
+    uint64_t const at = (of_codes ? index : index - code_lanes) >> 6;
+    if (!of_codes && at >= scale_lanes / 64) return;
+    uint32_t const across = of_codes ? supers * 4 : supers, which = (uint32_t)(at % across); // step or super
     uint64_t const tile_of_all = at / across;
     uint32_t const tile = (uint32_t)(tile_of_all % tiles);
     uint64_t const matrix = tile_of_all / tiles;
-    uint32_t const q = lane & 15, column = (tile >> 2) * 64 + (q >> 2) * 16 + (tile & 3) * 4 + (q & 3);
+    uint32_t const q = of_codes ? lane & 15 : lane >> 2, g = of_codes ? lane >> 4 : (lane & 1) * 2 + (lane >> 1 & 1); // (scale_word)
+    uint32_t const column = (tile >> 2) * 64 + (q >> 2) * 16 + (tile & 3) * 4 + (q & 3);
     uint32_t const k = header.k;
     if (of_codes) {
         uint32_t const block = which * 4 + g;
-        uint8_t const *from = codes + matrix * codes_matrix + column * codes_stride + block * 16;
         v4u word = {0, 0, 0, 0};
-        if (column < header.n) {
-            if (wide && block * 32 + 32 <= k) word = *(v4u const *)from;
-            else
-                for (uint32_t i = 0; i < 16; ++i) {
-                    uint32_t const col = block * 32 + 2 * i;
-                    uint32_t const byte = col + 1 < k ? from[i] : col < k ? from[i] & 15u : 0u;
-                    word[i / 4] |= byte << 8 * (i % 4);
-                }
-        }
+        if (column < header.n && block * 32 < k) word = load_codes(codes + matrix * codes_matrix + column * codes_stride, block, k, wide);
         *(v4u *)(image + kMxHeaderBytes + index * 16) = word;
         return;
     }
@@ -134,7 +157,7 @@ __global__ __launch_bounds__(256) void mx_pack_kernel(uint8_t const *codes, uint
         if (column < header.n && block * 32 < k)
             word |= (uint32_t)scales[matrix * scales_matrix + column * scales_stride + block] << 8 * u;
     }
-    *(uint32_t *)(image + kMxHeaderBytes + code_lanes * header.count * 16 + (index - code_lanes * header.count) * 4) = word;
+    *(uint32_t *)(image + kMxHeaderBytes + code_lanes * 16 + (index - code_lanes) * 4) = word;
 }
 
 // ---- products -----------------------------------------------------------------------------------------------------
@@ -145,199 +168,272 @@ struct MxArgs {
     uint8_t const *image;
     uint8_t *c;
     uint32_t const *plan; // NULL: one matrix, rows in order
-    uint64_t a_pitch, scales_pitch, c_stride;
+    uint64_t a_pitch, c_stride;
     uint32_t m, n, k, steps, supers, tiles, count;
     uint32_t tiles_m, tiles_n; // the grid: tiles of rows, tiles of columns
     uint32_t order, tile_list; // words into the plan
     uint32_t a_share;          // slots that share a row of A
     uint32_t sorted;           // 1: results in the plan's order of rows (and nothing for rows of no expert), 0: at their slots
-    uint32_t a_wide, c_wide;
+    uint32_t a_wide;
 };
 
 /** The rows of one tile. */
 struct RowTile {
     uint32_t matrix, first, last; // rows [first, last): of C, or of the plan
-    bool zero;                    // rows of no expert
 };
-__device__ __forceinline__ bool row_tile_of(MxArgs const &p, uint32_t tile, uint32_t rows, RowTile &t) {
+__device__ __forceinline__ RowTile row_tile_of(MxArgs const &p, uint32_t tile, uint32_t rows) {
     if (!p.plan) {
-        t.matrix = 0, t.first = tile * rows, t.last = t.first + rows < p.m ? t.first + rows : p.m, t.zero = false;
-        return true;
+        uint32_t const first = tile * rows;
+        return {0, first, first + rows < p.m ? first + rows : p.m};
     }
-    if (tile >= ((PlanHeader const *)p.plan)->tile_count) return false;
     PlanTile const entry = *(PlanTile const *)(p.plan + p.tile_list + tile * 4);
-    t.matrix = (uint32_t)entry.expert, t.first = (uint32_t)entry.first, t.last = (uint32_t)entry.last;
-    t.zero = t.matrix >= p.count;
-    return !(t.zero && p.sorted);
+    return {(uint32_t)entry.expert, (uint32_t)entry.first, (uint32_t)entry.last};
 }
 __device__ __forceinline__ bool image_matches(MxArgs const &p) {
     MxHeader const h = *(MxHeader const *)p.image;
     return h.magic == kMxMagic && h.version == 1 && h.count == p.count && h.n == p.n && h.k == p.k;
 }
-/** Workgroup to tile: each of the eight dies gets one stretch of the walk, `bands` of eight tiles of rows at a time. */
-__device__ __forceinline__ bool grid_tile(MxArgs const &p, uint32_t &tile_m, uint32_t &tile_n) {
-    uint32_t const total = p.tiles_m * p.tiles_n, per = (total + 7) / 8;
-    uint32_t const index = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= per || index >= total) return false;
-    if (p.plan) { // the tiles of one expert stand side by side: their rows stay while the columns go by
-        tile_m = index / p.tiles_n, tile_n = index - tile_m * p.tiles_n;
-        return true;
-    }
-    uint32_t const band = index / (8 * p.tiles_n), first = band * 8, inside = index - band * 8 * p.tiles_n;
-    uint32_t const high = p.tiles_m - first < 8 ? p.tiles_m - first : 8;
-    tile_n = inside / high, tile_m = first + inside - tile_n * high;
-    return true;
-}
 
 /**
- *  The product for many rows: 16 WM FM rows x 64 WN columns by WM x WN wavefronts, each FM x 4 fragments of 16 x 16.
- *  Both operands go straight into LDS (four stages of one step, fetched three ahead), in the order in which fragments are
- *  read, so that no read meets another's bank; scales the same way, one super ahead. A stage's fetches are counted, not
- *  drained: every wavefront waits for its own, then all meet.
+ *  The product for many rows: four wavefronts side by side, each 32 FM rows x 64 columns in blocks of 32 x 32 by
+ *  v_mfma_scale_f32_32x32x64_f8f6f4 (in blocks of 16 x 16 the accumulators are four times as many values of the compiler's,
+ *  and at 256 registers of them it moved these about, 632 moves for 256 products). A block's operand of half a step is
+ *  lane l = row l % 32, block l / 32: sixteen rows' worth from each of two fragments, 256 bytes at a time.
+ *
+ *  A goes straight into LDS (a ring of four steps, fetched three ahead) in the order in which it is read, so that no read
+ *  meets another's bank; each wavefront reads all of it, kAhead operands ahead of the products. B comes from the image straight
+ *  into registers, each column of it into one wavefront's, the halves of a step refilled kSets steps ahead as they fall free.
+ *  Fetches are counted, not drained: shortly before a step reads the first of the next step's A, the fetches of two steps ago
+ *  have arrived, and everybody says so. Scales come a super ahead.
+ *
+ *  Workgroups stay: one walks its tiles, and the fetches of the next tile's first steps go out under the last steps of the one
+ *  before, so that a tile starts at once. Each of the eight dies gets one stretch of the walk, eight tiles of rows at a time.
  */
-template <int FM, int WM, int WN, class Out, bool GROUPED>
-__global__ __launch_bounds__(64 * WM * WN) void mx_gemm_kernel(MxArgs p) {
-    constexpr int kWaves = WM * WN, kA = WM * FM, kFragments = kA + WN * 4, kLoads = kFragments / kWaves;
-    static_assert(kFragments % kWaves == 0, "every wavefront fetches the same number of fragments");
-    constexpr int kRows = kA * 16, kColumns = WN * 64;
-    __shared__ __attribute__((aligned(1024))) uint8_t ring0[kFragments * 1024];
-    __shared__ __attribute__((aligned(1024))) uint8_t ring1[kFragments * 1024];
-    __shared__ __attribute__((aligned(1024))) uint8_t ring2[kFragments * 1024];
-    __shared__ __attribute__((aligned(1024))) uint8_t ring3[kFragments * 1024];
-    __shared__ __attribute__((aligned(1024))) uint8_t scale0[kFragments * 256];
-    __shared__ __attribute__((aligned(1024))) uint8_t scale1[kFragments * 256];
+template <int FM, class Out, bool GROUPED>
+__global__ __launch_bounds__(256, FM >= 8 ? 1 : 2) void mx_gemm_kernel(MxArgs p) {
+    constexpr int FN = 2, kA = 2 * FM, kFetches = kA / 4, kScales = FM + FN, kAhead = 4, kSets = FM >= 8 ? 4 : 2, kMeet = 2 * FM - kAhead;
+    static_assert(kA % 4 == 0 && kA % kAhead == 0, "whole fetches; operands of A keep their registers from step to step");
+    static_assert(kMeet > kFetches && kMeet >= FM, "before a step's meeting: its fetches of A, its scales, B's first half");
+    constexpr int kRows = FM * 32, kColumns = 256;
+    constexpr int kPieces = 64 * (int)sizeof(Out) / 16, kEach = 16 / (int)sizeof(Out); // 16-byte pieces of a wavefront's row of C
+    __shared__ __attribute__((aligned(1024))) uint8_t ring0[kA * 1024];
+    __shared__ __attribute__((aligned(1024))) uint8_t ring1[kA * 1024];
+    __shared__ __attribute__((aligned(1024))) uint8_t ring2[kA * 1024];
+    __shared__ __attribute__((aligned(1024))) uint8_t ring3[kA * 1024];
+    __shared__ __attribute__((aligned(1024))) uint8_t results[4][32 * kPieces * 16];
 
-    uint32_t tile_m, tile_n;
-    if (!grid_tile(p, tile_m, tile_n)) return;
-    RowTile rows;
-    if (!row_tile_of(p, tile_m, kRows, rows)) return;
-    uint32_t const lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    uint32_t const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+    uint32_t const lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+    uint32_t const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (GROUPED && !p.sorted) { // rows of no expert are zeros
+        PlanHeader const &h = *(PlanHeader const *)p.plan;
+        for (uint32_t at = h.first_zero + blockIdx.x; at < h.end_zero; at += gridDim.x) {
+            Out *row = (Out *)(p.c + p.plan[p.order + at] * p.c_stride);
+            for (uint32_t column = threadIdx.x; column < p.n; column += 256) row[column] = (Out)0.0f;
+        }
+    }
+    uint32_t const tiles_m = GROUPED ? ((PlanHeader const *)p.plan)->tile_count : p.tiles_m;
+    uint32_t const total = tiles_m * p.tiles_n, stretch = (total + 7) / 8, turns = gridDim.x / 8;
     bool const good = image_matches(p);
 
-    v4f acc[FM][4];
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = v4f {0, 0, 0, 0};
-
-    if (good && !(GROUPED && rows.zero) && p.steps) {
-        // what this wavefront fetches: fragments wave * kLoads ... of the stage, A's first
-        uint8_t const *from[kLoads], *scale_from[kLoads];
-        uint32_t advance[kLoads], scale_advance[kLoads];
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            uint32_t const f = wave * kLoads + i;
-            if (f < (uint32_t)kA) {
-                uint32_t at = rows.first + f * 16 + r;
-                at = at < rows.last ? at : rows.last - 1; // (results of rows past the end are not stored)
-                uint32_t const row = GROUPED ? p.plan[p.order + at] / p.a_share : at;
-                from[i] = p.a + row * p.a_pitch + g * 16, advance[i] = 64;
-                scale_from[i] = p.a_scales + row * p.scales_pitch + g * 4, scale_advance[i] = 16;
-            }
-            else {
-                uint32_t tile = tile_n * (WN * 4) + f - kA;
-                tile = tile < p.tiles ? tile : p.tiles - 1;
-                uint64_t const of_all = (uint64_t)rows.matrix * p.tiles + tile;
-                from[i] = p.image + kMxHeaderBytes + of_all * p.steps * 1024 + lane * 16, advance[i] = 1024;
-                scale_from[i] = p.image + kMxHeaderBytes + (uint64_t)p.count * p.tiles * p.steps * 1024 + of_all * p.supers * 256 + lane * 4;
-                scale_advance[i] = 256;
-            }
+    struct Tile {
+        RowTile rows;
+        uint32_t tile_n;
+        uint8_t const *a, *a_scales, *b, *b_scales;
+    };
+    uint64_t const row_bytes = (uint64_t)p.supers * 4096, scale_row_bytes = (uint64_t)p.supers * 256; // of 16 rows or columns
+    auto tile_at = [&](uint32_t turn, Tile &t) __attribute__((always_inline)) -> bool {
+        uint32_t const inside = turn * turns + (blockIdx.x >> 3), index = (blockIdx.x & 7) * stretch + inside;
+        if (inside >= stretch || index >= total) return false;
+        uint32_t tile_m;
+        if (GROUPED) tile_m = index / p.tiles_n, t.tile_n = index - tile_m * p.tiles_n; // (an expert's tiles side by side)
+        else {
+            uint32_t const band = index / (8 * p.tiles_n), first = band * 8, at = index - band * 8 * p.tiles_n;
+            uint32_t const high = tiles_m - first < 8 ? tiles_m - first : 8;
+            t.tile_n = at / high, tile_m = first + at - t.tile_n * high;
         }
-        uint32_t const last_step = p.steps - 1, last_super = p.supers - 1;
-        auto fetch = [&](uint32_t step, uint8_t *ring) __attribute__((always_inline)) {
-            step = step < last_step ? step : last_step; // (past the end: the last once more, so that the counts stay)
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i)
-                fetch_16(from[i] + (uint64_t)step * advance[i], ring + (wave * kLoads + i) * 1024);
-        };
-        auto fetch_scales = [&](uint32_t super, uint8_t *ring) __attribute__((always_inline)) {
-            super = super < last_super ? super : last_super;
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i)
-                fetch_4(scale_from[i] + (uint64_t)super * scale_advance[i], ring + (wave * kLoads + i) * 256);
-        };
-        uint32_t a_scale[FM], w_scale[4];
-        auto read_scales = [&](uint8_t const *ring) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < FM; ++i) a_scale[i] = *(uint32_t const *)(ring + (wm * FM + i) * 256 + lane * 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w_scale[j] = *(uint32_t const *)(ring + (kA + wn * 4 + j) * 256 + lane * 4);
-        };
-        auto step_of = [&](auto byte, uint8_t const *ring) __attribute__((always_inline)) {
-            constexpr int U = decltype(byte)::value;
-            v4u w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = *(v4u const *)(ring + (kA + wn * 4 + j) * 1024 + lane * 16);
-#pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                v4u const a = *(v4u const *)(ring + (wm * FM + i) * 1024 + lane * 16);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = mx_multiply<U>(w[j], a, acc[i][j], w_scale[j], a_scale[i]);
+        t.rows = row_tile_of(p, tile_m, kRows);
+        // (staged A has room for the rows of a whole tile behind its last; results of such rows are not stored)
+        t.a = p.a + t.rows.first / 16 * row_bytes, t.a_scales = p.a_scales + t.rows.first / 16 * scale_row_bytes;
+        // this wavefront's group of columns, four tiles side by side in the image; a group past its end is its last
+        uint32_t const group = t.tile_n * 4 + wave, first_tile = (group * 4 < p.tiles ? group : p.tiles / 4 - 1) * 4;
+        uint64_t const of_all = (uint64_t)t.rows.matrix * p.tiles + first_tile;
+        t.b = p.image + kMxHeaderBytes + of_all * row_bytes;
+        t.b_scales = p.image + kMxHeaderBytes + (uint64_t)p.count * p.tiles * row_bytes + of_all * scale_row_bytes;
+        return true;
+    };
+    Tile now, then;
+    if (!good || !p.supers) { // no depth: zeros; an image of something else: NaNs
+        Out const value = (Out)(good ? 0.0f : __uint_as_float(0x7FC00000u));
+        for (uint32_t turn = 0; tile_at(turn, now); ++turn)
+            for (uint32_t at = now.rows.first; at < now.rows.last; ++at) {
+                uint32_t const row = GROUPED && !p.sorted ? p.plan[p.order + at] : at, column = now.tile_n * kColumns + threadIdx.x;
+                if (column < p.n) ((Out *)(p.c + row * p.c_stride))[column] = value;
             }
-        };
-        // Every fetch into what is read next has arrived (`younger` were issued behind it and may be in flight), this
-        // wavefront's reads are done, and everybody says so.
-        auto meet = [&](auto younger_) __attribute__((always_inline)) {
-            constexpr int younger = decltype(younger_)::value;
-            static_assert(younger < 64, "what a wait can count to");
-            __builtin_amdgcn_sched_barrier(0);
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_s_waitcnt(0x0070 | (younger & 15) | (younger >> 4) << 14);
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        Number<0> const zero;
-        Number<1> const one;
-        Number<2> const two;
-        Number<3> const three;
-        Number<2 * kLoads> const few;  // two stages behind
-        Number<3 * kLoads> const more; // two stages and a super's scales
-        fetch_scales(0, scale0);
-        fetch(0, ring0), fetch(1, ring1), fetch(2, ring2);
-        uint32_t const whole = p.steps / 4, rest = p.steps % 4;
-        // Stage s: wait for its fetches (three stages old), then fetch stage s + 3 into what stage s - 1 has left.
-        auto super_of = [&](uint32_t q, uint8_t *scales_now, uint8_t *scales_next) __attribute__((always_inline)) {
-            meet(few);
-            fetch_scales(q + 1, scales_next), fetch(4 * q + 3, ring3);
-            read_scales(scales_now);
-            step_of(zero, ring0);
-            meet(more);
-            fetch(4 * q + 4, ring0);
-            step_of(one, ring1);
-            meet(more);
-            fetch(4 * q + 5, ring1);
-            step_of(two, ring2);
-            meet(few);
-            fetch(4 * q + 6, ring2);
-            step_of(three, ring3);
-        };
-        uint32_t q = 0;
-        for (; q + 2 <= whole; q += 2) super_of(q, scale0, scale1), super_of(q + 1, scale1, scale0);
-        if (q < whole) super_of(q, scale0, scale1), ++q;
-        meet(Number<0>()); // (nothing is fetched from here on)
-        if (rest) {
-            read_scales(q & 1 ? scale1 : scale0);
-            step_of(zero, ring0);
-            if (rest > 1) step_of(one, ring1);
-            if (rest > 2) step_of(two, ring2);
-        }
+        return;
     }
+    if (!tile_at(0, now)) return;
 
-    float const poison = __uint_as_float(0x7FC00000u);
+    uint32_t const steps = p.supers * 4, lane16 = lane * 16;
+    // where a lane's 16 bytes of the first half of a step are: in LDS, in the image; and its two words of scales
+    uint32_t const a_lane = (r >> 4) * 1024 + (g * 16 + (r & 15)) * 16;
+    uint32_t const b_lane = (r >> 4) * (uint32_t)row_bytes + (g * 16 + (r & 15)) * 16;
+    uint32_t const scale_lane = (r >> 4) * (uint32_t)scale_row_bytes + ((r & 15) * 4 + g * 2) * 4;
+
+    v16f acc[FM][FN];
+    v4u a[kAhead], b[kSets][2][FN]; // [step % kSets][half][block]
+    v2u a_scale[FM], b_scale[FN], a_scale_next[FM], b_scale_next[FN]; // [half]
+    auto fetch_a = [&](Tile const &t, uint32_t step, uint8_t *ring, int i) __attribute__((always_inline)) {
+        uint32_t const f = wave * kFetches + i;
+        fetch_16(buffer_of(t.a), ring + f * 1024, lane16, f * (uint32_t)row_bytes + step * 1024);
+    };
+    auto read_a = [&](uint8_t const *ring, int half, int i) __attribute__((always_inline)) -> v4u {
+        return *(v4u const *)(ring + i * 2048 + half * 512 + a_lane);
+    };
+    auto load_b = [&](Tile const &t, uint32_t step, int half, int j) __attribute__((always_inline)) -> v4u {
+        return load_16(buffer_of(t.b), b_lane, 2 * j * (uint32_t)row_bytes + step * 1024 + half * 512);
+    };
+    auto load_scale = [&](Tile const &t, uint32_t super, int i) __attribute__((always_inline)) { // FM of A's, then FN of B's
+        if (i < FM) a_scale_next[i < FM ? i : 0] = load_8(buffer_of(t.a_scales), scale_lane, 2 * i * (uint32_t)scale_row_bytes + super * 256);
+        else b_scale_next[i < FM ? 0 : i - FM] = load_8(buffer_of(t.b_scales), scale_lane, 2 * (i - FM) * (uint32_t)scale_row_bytes + super * 256);
+    };
+    // All but the last `younger` of this wavefront's fetches have arrived (< 0: they have anyway), what it has read from LDS as
+    // well, and everybody says so.
+    auto meet = [&](auto younger_) __attribute__((always_inline)) {
+        constexpr int given = decltype(younger_)::value, younger = given < 0 ? 63 : given; // (63: no wait)
+        static_assert(younger < 64, "what a wait can count to");
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070 | (younger & 15) | (younger >> 4) << 14);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // Step s, byte U of its super's scales. FRESH: of a tile's first super.
+    auto step_of = [&](auto byte, auto fresh, uint32_t s, uint8_t const *here, uint8_t const *next, uint8_t *free) __attribute__((always_inline)) {
+        constexpr int U = decltype(byte)::value, P = U % kSets;
+        constexpr bool FRESH = decltype(fresh)::value != 0;
+        bool const wrap_a = s + 3 >= steps, wrap_b = s + kSets >= steps, wrap_scales = s + 4 >= steps;
+        uint32_t const step_a = wrap_a ? s + 3 - steps : s + 3, step_b = wrap_b ? s + kSets - steps : s + kSets;
+        uint32_t const super = wrap_scales ? 0 : (s >> 2) + 1;
+        if (U == 0) {
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        uint32_t const at = rows.first + (wm * FM + i) * 16 + r;
-        if (at >= rows.last) continue;
-        uint32_t const row = GROUPED && !p.sorted ? p.plan[p.order + at] : at;
-        uint32_t const column = tile_n * kColumns + wn * 64 + g * 16;
-        if (column >= p.n) continue;
-        float v[16];
+            for (int i = 0; i < FM; ++i) a_scale[i] = a_scale_next[i];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = good ? acc[i][j / 4][j % 4] : poison;
-        store_some<Out, 16>((Out *)(p.c + row * p.c_stride) + column, v, p.n - column, p.c_wide);
+            for (int j = 0; j < FN; ++j) b_scale[j] = b_scale_next[j];
+        }
+#pragma unroll
+        for (int at = 0; at < 2 * FM; ++at) {
+            int const half = at / FM, i = at % FM, ahead = at + kAhead;
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                acc[i][j] = mx_multiply<U>(b[P][half][j], a[at % kAhead], FRESH && U == 0 && half == 0 ? v16f {} : acc[i][j], b_scale[j][half], a_scale[i][half]);
+            // What went out behind the fetches of two steps ago: B's and scales of that step, all of the last, this one's so far.
+            // (Fetches from before a tile's first step were waited for before the last tile's results were stored.)
+            if (at == kMeet) meet(Number<FRESH && U < 2 ? -1 : 5 * FN + 2 * kFetches + (U < 3 ? kScales : 0)>());
+            a[at % kAhead] = ahead < 2 * FM ? read_a(here, ahead / FM % 2, ahead % FM) : read_a(next, ahead % (2 * FM) / FM, ahead % FM);
+            if (at < kFetches) fetch_a(wrap_a ? then : now, step_a, free, at < kFetches ? at : 0);
+            if (U == 0 && at >= kFetches && at < kMeet)
+#pragma unroll
+                for (int k = (at - kFetches) * kScales / (kMeet - kFetches); k < (at - kFetches + 1) * kScales / (kMeet - kFetches); ++k)
+                    load_scale(wrap_scales ? then : now, super, k);
+            if (i == FM - 1)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) b[P][half][j] = load_b(wrap_b ? then : now, step_b, half, j);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+#pragma unroll
+    for (int i = 0; i < kScales; ++i) load_scale(now, 0, i);
+#pragma unroll
+    for (int t = 0; t < 3; ++t)
+#pragma unroll
+        for (int i = 0; i < kFetches; ++i) fetch_a(now, t, t == 0 ? ring0 : t == 1 ? ring1 : ring2, i);
+#pragma unroll
+    for (int t = 0; t < kSets; ++t)
+#pragma unroll
+        for (int j = 0; j < 2 * FN; ++j) b[t][j / FN][j % FN] = load_b(now, t, j / FN, j % FN);
+    meet(Number<0>());
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) a[i] = read_a(ring0, i / FM, i % FM);
+    for (uint32_t turn = 1;; ++turn) {
+        bool const more = tile_at(turn, then);
+        if (!more) then = now; // (its first steps are fetched once more and not used)
+        uint32_t slots[(kRows + 63) / 64]; // where the rows of this tile go
+        if (GROUPED && !p.sorted)
+#pragma unroll
+            for (int x = 0; x < (kRows + 63) / 64; ++x) {
+                uint32_t const at = now.rows.first + x * 64 + lane;
+                slots[x] = p.plan[p.order + (at < now.rows.last ? at : now.rows.last - 1)];
+            }
+        step_of(Number<0>(), Number<1>(), 0, ring0, ring1, ring3);
+        step_of(Number<1>(), Number<1>(), 1, ring1, ring2, ring0);
+        step_of(Number<2>(), Number<1>(), 2, ring2, ring3, ring1);
+        step_of(Number<3>(), Number<1>(), 3, ring3, ring0, ring2);
+        for (uint32_t s = 4; s < steps; s += 4) {
+            step_of(Number<0>(), Number<0>(), s, ring0, ring1, ring3);
+            step_of(Number<1>(), Number<0>(), s + 1, ring1, ring2, ring0);
+            step_of(Number<2>(), Number<0>(), s + 2, ring2, ring3, ring1);
+            step_of(Number<3>(), Number<0>(), s + 3, ring3, ring0, ring2);
+        }
+
+        // Rows of the image's columns in a block: 8 (t / 4) + 4 g + t % 4 of value t, which the image's order of columns makes
+        // two runs of 16 adjacent columns (2 x + g of the four in a group, x = 0, 1), four values from each of the group's four
+        // tiles. 32 rows at a time they go through the wavefront's own part of LDS (16-byte pieces, piece c of row r at
+        // c ^ (r & 7)), so that a row is stored in one piece: 128 or 256 adjacent bytes, whatever address it starts at.
+        uint8_t *const mine = results[wave];
+        uint32_t const wave_column = now.tile_n * kColumns + wave * 64;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int part = 0; part < 2 * 16 / kEach; ++part) {
+                int const x = part * kEach / 16;
+                struct alignas(16) Piece {
+                    Out v[kEach];
+                } values;
+#pragma unroll
+                for (int t = 0; t < kEach; ++t) {
+                    int const j = part * kEach % 16 + t;
+                    values.v[t] = (Out)acc[i][j / 8][(j / 4) % 2 * 8 + x * 4 + j % 4];
+                }
+                uint32_t const piece = ((2 * x + g) * 16 + part * kEach % 16) / kEach;
+                *(Piece *)(mine + (r * kPieces + (piece ^ (r & 7))) * 16) = values;
+            }
+            __builtin_amdgcn_wave_barrier();
+            if (i == 0) { // (what the next tile's first steps need: from here on stores are behind it)
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_s_waitcnt(0x0F70);
+                asm volatile("" ::: "memory");
+            }
+            auto const store_row = [&](int round, bool whole) __attribute__((always_inline)) {
+                uint32_t const local = round * (64 / kPieces) + lane / kPieces, piece = lane % kPieces;
+                v4u const values = *(v4u const *)(mine + (local * kPieces + (piece ^ (local & 7))) * 16);
+                uint32_t const at = now.rows.first + i * 32 + local, column = wave_column + piece * kEach;
+                uint32_t row = at;
+                if (GROUPED && !p.sorted) row = (uint32_t)__shfl((int)slots[i / 2], i % 2 * 32 + local);
+                if (at >= now.rows.last || (!whole && column >= p.n)) return;
+                Out *to = (Out *)(p.c + row * p.c_stride) + column;
+                if (whole || column + kEach <= p.n) store_16(to, values);
+                else
+                    for (uint32_t t = 0; t < p.n - column; ++t) { // (every element with its own word: no array of them)
+                        uint32_t const word = t * sizeof(Out) / 4 == 0 ? values[0] : t * sizeof(Out) / 4 == 1 ? values[1] : t * sizeof(Out) / 4 == 2 ? values[2] : values[3];
+                        if constexpr (sizeof(Out) == 4) ((uint32_t *)to)[t] = word;
+                        else ((uint16_t *)to)[t] = (uint16_t)(word >> 16 * (t & 1));
+                    }
+            };
+            if (wave_column + 64 <= p.n) {
+#pragma unroll
+                for (int round = 0; round < kPieces / 2; ++round) store_row(round, true);
+            }
+            else
+#pragma unroll 1
+                for (int round = 0; round < kPieces / 2; ++round) store_row(round, false);
+        }
+        if (!more) break;
+        now = then;
     }
+    __builtin_amdgcn_s_waitcnt(0x0F70); // (nothing is on its way into LDS when the workgroup ends)
 }
 
 /**
@@ -351,8 +447,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx_few_kernel(MxArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t few_lds[];
     constexpr bool FUSED = sizeof(In) != 1;
     uint32_t const tile_m = blockIdx.x / p.tiles_n, tile_n = blockIdx.x - tile_m * p.tiles_n;
-    RowTile rows;
-    if (!row_tile_of(p, tile_m, FM * 16, rows)) return;
+    if (GROUPED) {
+        PlanHeader const &h = *(PlanHeader const *)p.plan;
+        if (tile_m >= h.tile_count + (p.sorted ? 0 : h.zero_tiles)) return;
+    }
+    RowTile const rows = row_tile_of(p, tile_m, FM * 16);
     uint32_t const lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     uint32_t const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     bool const good = image_matches(p);
@@ -365,7 +464,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx_few_kernel(MxArgs p) {
 
     uint32_t const lds_pitch = p.steps * 64 + 16; // (16 bytes on: rows start in different banks)
     uint8_t *lds_scales = few_lds + here * lds_pitch;
-    bool const computes = good && !(GROUPED && rows.zero) && p.steps;
+    bool const computes = good && !(GROUPED && rows.matrix >= p.count) && p.steps;
     if (FUSED && computes) {
         uint32_t const pieces = p.steps * 16;
         for (uint32_t index = threadIdx.x; index < here * pieces; index += 64 * kFewWaves) {
@@ -382,9 +481,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx_few_kernel(MxArgs p) {
     if (FUSED) __syncthreads();
     if (computes) {
         uint32_t const begin = (uint32_t)((uint64_t)wave * p.steps / kFewWaves), end = (uint32_t)((uint64_t)(wave + 1) * p.steps / kFewWaves);
-        uint64_t const of_all = (uint64_t)rows.matrix * p.tiles + tile_n * NT;
-        uint8_t const *w_from = p.image + kMxHeaderBytes + of_all * p.steps * 1024 + lane * 16;
-        uint8_t const *w_scale_from = p.image + kMxHeaderBytes + (uint64_t)p.count * p.tiles * p.steps * 1024 + of_all * p.supers * 256 + lane * 4;
+        uint64_t const of_all = (uint64_t)rows.matrix * p.tiles + tile_n * NT, row_bytes = (uint64_t)p.supers * 4096, scale_row_bytes = (uint64_t)p.supers * 256;
+        uint32_t const scale_lane = scale_word(r, g) * 4;
+        uint8_t const *w_from = p.image + kMxHeaderBytes + of_all * row_bytes + lane * 16;
+        uint8_t const *w_scale_from = p.image + kMxHeaderBytes + (uint64_t)p.count * p.tiles * row_bytes + of_all * scale_row_bytes + scale_lane;
         uint8_t const *a_from[FM], *a_scale_from[FM];
         bool there[FM];
 #pragma unroll
@@ -392,10 +492,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx_few_kernel(MxArgs p) {
             there[i] = i * 16 + r < here;
             uint32_t const row = there[i] ? i * 16 + r : 0;
             if constexpr (FUSED) a_from[i] = few_lds + row * lds_pitch + g * 16, a_scale_from[i] = lds_scales + row * (p.steps * 4) + g;
-            else {
-                uint32_t const at = rows.first + row, source = GROUPED ? p.plan[p.order + at] / p.a_share : at;
-                a_from[i] = p.a + source * p.a_pitch + g * 16, a_scale_from[i] = p.a_scales + source * p.scales_pitch + g * 4;
-            }
+            else a_from[i] = p.a + (rows.first / 16 + i) * row_bytes + lane * 16, a_scale_from[i] = p.a_scales + (rows.first / 16 + i) * scale_row_bytes + scale_lane;
         }
         constexpr int kBatch = 4;
         for (uint32_t base = begin; base < end; base += kBatch) {
@@ -406,14 +503,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx_few_kernel(MxArgs p) {
                 uint32_t const s = base + u < end ? base + u : end - 1;
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    w[u][j] = *(v4u const *)(w_from + ((uint64_t)j * p.steps + s) * 1024);
-                    w_scale[u][j] = *(uint32_t const *)(w_scale_from + ((uint64_t)j * p.supers + (s >> 2)) * 256) >> 8 * (s & 3);
+                    w[u][j] = *(v4u const *)(w_from + j * row_bytes + (uint64_t)s * 1024);
+                    w_scale[u][j] = *(uint32_t const *)(w_scale_from + j * scale_row_bytes + (s >> 2) * 256) >> 8 * (s & 3);
                 }
 #pragma unroll
                 for (int i = 0; i < FM; ++i) {
-                    a[u][i] = *(v4u const *)(a_from[i] + (uint64_t)s * 64);
+                    a[u][i] = *(v4u const *)(a_from[i] + (uint64_t)s * (FUSED ? 64 : 1024));
                     if constexpr (FUSED) a_scale[u][i] = a_scale_from[i][s * 4];
-                    else a_scale[u][i] = *(uint32_t const *)(a_scale_from[i] + (s >> 2) * 16) >> 8 * (s & 3);
+                    else a_scale[u][i] = *(uint32_t const *)(a_scale_from[i] + (s >> 2) * 256) >> 8 * (s & 3);
                 }
             }
 #pragma unroll
@@ -450,7 +547,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx_few_kernel(MxArgs p) {
         float v[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) v[t] = good ? sum[t] : poison;
-        store_some<Out, 4>((Out *)(p.c + row * p.c_stride) + column, v, p.n - column, p.c_wide);
+        store_some<Out, 4>((Out *)(p.c + row * p.c_stride) + column, v, p.n - column);
     }
 }
 
@@ -458,7 +555,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx_few_kernel(MxArgs p) {
 template <class In, class Out>
 __global__ __launch_bounds__(256) void combine_kernel(In const *rows, uint64_t row_values, uint32_t const *plan, uint32_t place,
                                                       float const *weights, uint32_t top_k, uint32_t tokens, uint32_t n,
-                                                      uint32_t pieces, Out *c, uint64_t c_stride, bool wide) {
+                                                      uint32_t pieces, Out *c, uint64_t c_stride) {
     uint32_t const index = blockIdx.x * 256 + threadIdx.x;
     uint32_t const token = index / pieces, column = (index - token * pieces) * 4;
     if (token >= tokens) return;
@@ -474,7 +571,7 @@ __global__ __launch_bounds__(256) void combine_kernel(In const *rows, uint64_t r
 #pragma unroll
         for (int t = 0; t < 4; ++t) sum[t] = __builtin_fmaf(weight, (float)four.x[t], sum[t]);
     }
-    store_some<Out, 4>((Out *)((uint8_t *)c + token * c_stride) + column, sum, n - column, wide);
+    store_some<Out, 4>((Out *)((uint8_t *)c + token * c_stride) + column, sum, n - column);
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------
@@ -491,11 +588,9 @@ int with_type(int dtype, F &&f) {
     return f(_Float16());
 }
 
-template <bool STAGED>
 int launch_quantize(int dtype, void const *x, uint64_t rows, uint32_t k, uint64_t x_stride, uint8_t *codes, uint64_t codes_stride,
                     uint8_t *scales, uint64_t scales_stride, hipStream_t stream) {
-    uint64_t const pieces = STAGED ? (uint64_t)(k + 127) / 128 * 16 : (uint64_t)(k + 31) / 32 * 4;
-    if (!rows || !pieces) return 0;
+    uint64_t const pieces = (uint64_t)(k + 31) / 32 * 4;
     bool const wide = aligned(x, x_stride, 16), whole_words = aligned(codes, codes_stride, 4);
     uint64_t const slab = kMostThreads / pieces; // rows of one launch
     for (uint64_t first = 0; first < rows; first += slab) {
@@ -503,7 +598,7 @@ int launch_quantize(int dtype, void const *x, uint64_t rows, uint32_t k, uint64_
         uint8_t const *from = (uint8_t const *)x + first * x_stride;
         int const status = with_type(dtype, [&](auto value) {
             typedef decltype(value) T;
-            hipLaunchKernelGGL((quantize_kernel<T, STAGED>), dim3((uint32_t)((here * pieces + 255) / 256)), dim3(256), 0, stream,
+            hipLaunchKernelGGL((quantize_kernel<T>), dim3((uint32_t)((here * pieces + 255) / 256)), dim3(256), 0, stream,
                                (T const *)from, x_stride, (uint32_t)here, k, (uint32_t)pieces, wide, codes + first * codes_stride,
                                codes_stride, whole_words, scales + first * scales_stride, scales_stride);
             hipError_t const e = hipGetLastError();
@@ -514,38 +609,34 @@ int launch_quantize(int dtype, void const *x, uint64_t rows, uint32_t k, uint64_
     return 0;
 }
 
-/** How A is laid out in the workspace. */
+/** How A is laid out in the workspace: room for `rows` and, behind them, for what the last tile reads past its last row. */
 struct Staging {
-    uint64_t pitch, scales_pitch, scales_at, bytes;
+    uint64_t scales_at, bytes;
 };
+constexpr uint64_t kMostTileRows = 256;
 Staging staging_of(uint64_t rows, MxGeometry const &g) {
+    uint64_t const fragments = (rows + 15) / 16 + kMostTileRows / 16;
     Staging s;
-    // rows an odd number of 256 bytes apart: a stage reads 64 bytes of each row of a tile, and with a power of two between
-    // rows these would all come from the same few channels of the L2
-    s.pitch = (uint64_t)g.steps * 64;
-    s.pitch = (s.pitch + 255) / 256 * 256;
-    if (!(s.pitch & 256)) s.pitch += 256;
-    s.scales_pitch = (uint64_t)g.supers * 16;
-    s.scales_at = rows * s.pitch;
-    s.bytes = (s.scales_at + rows * s.scales_pitch + 255) / 256 * 256;
+    s.scales_at = fragments * g.supers * 4096;
+    s.bytes = (s.scales_at + fragments * g.supers * 256 + 255) / 256 * 256;
     return s;
 }
-int stage(int a_dtype, void const *a, uint64_t a_stride, void const *a_scales, uint64_t a_scales_stride, uint64_t rows, uint32_t k,
-          MxGeometry const &g, Staging const &s, uint8_t *to, hipStream_t stream) {
-    if (!a_scales) return launch_quantize<true>(a_dtype, a, rows, k, a_stride, to, s.pitch, to + s.scales_at, s.scales_pitch, stream);
-    uint32_t const blocks = g.steps * 4;
-    if (!rows || !blocks) return 0;
-    uint64_t const slab = kMostThreads / blocks;
-    for (uint64_t first = 0; first < rows; first += slab) {
-        uint64_t const here = rows - first < slab ? rows - first : slab;
-        hipLaunchKernelGGL(stage_codes_kernel, dim3((uint32_t)((here * blocks + 255) / 256)), dim3(256), 0, stream,
-                           (uint8_t const *)a + first * a_stride, a_stride, (uint8_t const *)a_scales + first * a_scales_stride,
-                           a_scales_stride, (uint32_t)here, k, blocks, aligned(a, a_stride, 16), to + first * s.pitch, s.pitch,
-                           to + s.scales_at + first * s.scales_pitch, s.scales_pitch);
-        hipError_t const e = hipGetLastError();
-        if (e != hipSuccess) return mx_fail(e, "stage_codes_kernel");
-    }
-    return 0;
+/** A into the workspace: rows in order, or the rows of a plan. */
+int stage(int a_dtype, void const *a, uint64_t a_stride, void const *a_scales, uint64_t a_scales_stride, uint32_t rows, uint32_t k,
+          MxGeometry const &g, Staging const &s, uint8_t *to, void const *plan, size_t order, uint32_t a_share, hipStream_t stream) {
+    uint64_t const grid = (uint64_t)((rows + 15) / 16) * g.supers;
+    if (!grid) return 0;
+    if (grid > 0x7FFFFFFFull) return mx_fail("mx product: A is too large");
+    StageArgs const p = {a, a_stride, (uint8_t const *)a_scales, a_scales_stride, to, to + s.scales_at, (uint32_t const *)plan, rows, k,
+                         g.supers, (uint32_t)order, a_share, aligned(a, a_stride, 16)};
+    if (a_scales) hipLaunchKernelGGL(stage_kernel<uint8_t>, dim3((uint32_t)grid), dim3(256), 0, stream, p);
+    else
+        with_type(a_dtype, [&](auto value) {
+            hipLaunchKernelGGL(stage_kernel<decltype(value)>, dim3((uint32_t)grid), dim3(256), 0, stream, p);
+            return 0;
+        });
+    hipError_t const e = hipGetLastError();
+    return e == hipSuccess ? 0 : mx_fail(e, "stage_kernel");
 }
 
 /** Can products of few rows quantise A themselves? What a workgroup holds of it has to fit, and to stay small. */
@@ -564,13 +655,15 @@ int launch_few(MxArgs &p, uint32_t max_rows, MxGeometry const &g, hipStream_t st
     hipError_t const e = hipGetLastError();
     return e == hipSuccess ? 0 : mx_fail(e, "mx_few_kernel");
 }
-template <int FM, int WM, int WN, class Out, bool GROUPED>
+template <int FM, class Out, bool GROUPED>
 int launch_gemm(MxArgs &p, hipStream_t stream) {
-    p.tiles_n = (p.tiles + WN * 4 - 1) / (WN * 4);
-    if (!GROUPED) p.tiles_m = (p.m + 16 * WM * FM - 1) / (16 * WM * FM);
-    uint64_t const grid = ((uint64_t)p.tiles_m * p.tiles_n + 7) / 8 * 8;
-    if (grid > 0x7FFFFFFFull) return mx_fail("mx product: too many tiles");
-    hipLaunchKernelGGL((mx_gemm_kernel<FM, WM, WN, Out, GROUPED>), dim3((uint32_t)grid), dim3(64 * WM * WN), 0, stream, p);
+    p.tiles_n = (p.tiles + 15) / 16;
+    if (!GROUPED) p.tiles_m = (p.m + 32 * FM - 1) / (32 * FM);
+    uint64_t const tiles = (uint64_t)p.tiles_m * p.tiles_n, resident = (uint64_t)compute_unit_count() * (FM >= 8 ? 1 : 2);
+    if (tiles > 0x7FFFFFFFull) return mx_fail("mx product: too many tiles");
+    if (!resident) return mx_fail("mx product: no GPU");
+    uint64_t const grid = ((tiles < resident ? tiles : resident) + 7) / 8 * 8;
+    hipLaunchKernelGGL((mx_gemm_kernel<FM, Out, GROUPED>), dim3((uint32_t)grid), dim3(256), 0, stream, p);
     hipError_t const e = hipGetLastError();
     return e == hipSuccess ? 0 : mx_fail(e, "mx_gemm_kernel");
 }
@@ -588,8 +681,8 @@ int launch_product(MxArgs &p, uint32_t rows, int a_dtype, bool fused, uint32_t f
         if (rows <= 32) return launch_few<2, 2, uint8_t, Out, GROUPED>(p, rows, g, stream);
         return launch_few<4, 2, uint8_t, Out, GROUPED>(p, rows, g, stream);
     }
-    if (GROUPED ? rows <= 128 : (uint64_t)((p.m + 255) / 256) * ((p.n + 255) / 256) < 256) return launch_gemm<4, 2, 2, Out, GROUPED>(p, stream);
-    return launch_gemm<8, 2, 4, Out, GROUPED>(p, stream);
+    if (GROUPED ? rows <= 128 : (uint64_t)((p.m + 255) / 256) * ((p.n + 255) / 256) < 256) return launch_gemm<4, Out, GROUPED>(p, stream);
+    return launch_gemm<8, Out, GROUPED>(p, stream);
 }
 
 int check_a(int a_dtype, void const *a, void const *a_scales, uint64_t a_stride) {
@@ -613,18 +706,17 @@ struct ExpertsLayout {
     int sums_dtype;
     bool fused;
 };
-ExpertsLayout experts_layout(uint64_t slots, uint64_t a_share, uint64_t experts, uint64_t n, MxGeometry const &g, bool a_is_codes,
-                             int c_dtype, bool weighted) {
+ExpertsLayout experts_layout(PlanGeometry const &shape, uint64_t n, MxGeometry const &g, bool a_is_codes, int c_dtype, bool weighted) {
     ExpertsLayout l = {};
-    l.fused = !a_is_codes && plan_tile_rows(slots, experts) == 16 && fuses(16, g);
-    if (!l.fused) l.staged = staging_of((slots + a_share - 1) / a_share, g);
+    l.fused = !a_is_codes && shape.tile_rows == 16 && fuses(16, g);
+    if (!l.fused) l.staged = staging_of(shape.max_rows, g);
     l.sums_at = l.staged.bytes;
     // rows that are still to be summed by weight: as wide as the result where that is bf16 (each is rounded once more, by at
     // most 2^-9 of itself, half of what the result's own rounding may do to it; at 32 bits they are most of the traffic),
     // 32 bits otherwise (f16 might overflow where the sum does not)
     l.sums_dtype = c_dtype == nk_bf16_k ? nk_bf16_k : nk_f32_k;
     l.sums_values = (n + 15) / 16 * 16;
-    l.bytes = l.sums_at + (weighted ? (slots * l.sums_values * element_bytes(l.sums_dtype) + 255) / 256 * 256 : 0);
+    l.bytes = l.sums_at + (weighted ? (shape.max_rows * l.sums_values * element_bytes(l.sums_dtype) + 255) / 256 * 256 : 0);
     return l;
 }
 
@@ -643,7 +735,7 @@ int nk_amd_mx_quantize_async(nk_dtype_t dtype, void const *x, nk_size_t rows, nk
     if (!rows || !depth) return 0;
     if (!x || !codes || !scales) return mx_fail("mx_quantize: NULL operand");
     if (!aligned(x, x_stride, bytes)) return mx_fail("mx_quantize: x is not aligned to its elements");
-    return launch_quantize<false>(dtype, x, rows, (uint32_t)depth, x_stride, (uint8_t *)codes, codes_stride, (uint8_t *)scales,
+    return launch_quantize(dtype, x, rows, (uint32_t)depth, x_stride, (uint8_t *)codes, codes_stride, (uint8_t *)scales,
                                   scales_stride, (hipStream_t)stream);
 }
 
@@ -663,7 +755,7 @@ int nk_amd_mx_dequantize_async(nk_dtype_t dtype, void const *codes, nk_size_t co
             hipLaunchKernelGGL((dequantize_kernel<T>), dim3((uint32_t)((here * pieces + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
                                (uint8_t const *)codes + first * codes_stride, codes_stride, aligned(codes, codes_stride, 4),
                                (uint8_t const *)scales + first * scales_stride, scales_stride, (uint32_t)here, (uint32_t)depth,
-                               (uint32_t)pieces, (T *)((uint8_t *)x + first * x_stride), x_stride, aligned(x, x_stride, 16));
+                               (uint32_t)pieces, (T *)((uint8_t *)x + first * x_stride), x_stride);
             hipError_t const e = hipGetLastError();
             return e == hipSuccess ? 0 : mx_fail(e, "dequantize_kernel");
         });
@@ -685,15 +777,15 @@ int nk_amd_mx_pack_async(void const *codes, nk_size_t codes_stride, nk_size_t co
     if (!packed || ((uintptr_t)packed & 15)) return mx_fail("mx_pack: the image has to be 16-byte aligned");
     if (count && width && depth && (!codes || !scales)) return mx_fail("mx_pack: NULL operand");
     MxHeader const header = {kMxMagic, 1, (uint32_t)count, (uint32_t)width, (uint32_t)depth, {0, 0, 0}};
-    uint64_t const code_lanes = g.code_bytes / 16, scale_lanes = g.scale_bytes / 4;
-    uint64_t const total = count * (code_lanes + scale_lanes);
+    uint64_t const code_lanes = count * (g.code_bytes / 16), scale_lanes = count * (g.scale_bytes / 4);
+    uint64_t const total = code_lanes + scale_lanes;
     bool const wide = aligned(codes, codes_stride | codes_matrix, 16);
-    uint64_t const steps = g.steps ? g.steps : 1, supers = g.supers ? g.supers : 1, tiles = g.tiles ? g.tiles : 1;
+    uint64_t const supers = g.supers ? g.supers : 1, tiles = g.tiles ? g.tiles : 1;
     for (uint64_t first = 0; first == 0 || first < total; first += kMostThreads) {
         uint64_t const here = total - first < kMostThreads ? total - first : kMostThreads;
         hipLaunchKernelGGL(mx_pack_kernel, dim3((uint32_t)(here ? (here + 255) / 256 : 1)), dim3(256), 0, (hipStream_t)stream,
                            (uint8_t const *)codes, codes_stride, codes_matrix, (uint8_t const *)scales, scales_stride,
-                           scales_matrix, header, (uint32_t)steps, (uint32_t)supers, (uint32_t)tiles, first, code_lanes, scale_lanes,
+                           scales_matrix, header, (uint32_t)supers, (uint32_t)tiles, first, code_lanes, scale_lanes,
                            wide, (uint8_t *)packed);
         hipError_t const e = hipGetLastError();
         if (e != hipSuccess) return mx_fail(e, "mx_pack_kernel");
@@ -722,15 +814,15 @@ int nk_amd_mx_dots_packed_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_s
     MxArgs p = {};
     p.image = (uint8_t const *)packed, p.c = (uint8_t *)c, p.c_stride = c_stride;
     p.m = (uint32_t)height, p.n = (uint32_t)width, p.k = (uint32_t)depth, p.count = 1, p.a_share = 1;
-    p.steps = g.steps, p.supers = g.supers, p.tiles = g.tiles, p.c_wide = aligned(c, c_stride, 16);
+    p.steps = g.steps, p.supers = g.supers, p.tiles = g.tiles;
     if (fused) p.a = (uint8_t const *)a, p.a_pitch = a_stride, p.a_wide = aligned(a, a_stride, 16);
     else {
         Staging const s = staging_of(height, g);
         if (s.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < s.bytes))
             return mx_fail("mx_dots_packed: the workspace is too small or not 256-byte aligned");
-        if (int const status = stage(a_dtype, a, a_stride, a_scales, a_scales_stride, height, p.k, g, s, (uint8_t *)workspace, stream))
+        if (int const status = stage(a_dtype, a, a_stride, a_scales, a_scales_stride, p.m, p.k, g, s, (uint8_t *)workspace, nullptr, 0, 1, stream))
             return status;
-        p.a = (uint8_t const *)workspace, p.a_scales = p.a + s.scales_at, p.a_pitch = s.pitch, p.scales_pitch = s.scales_pitch;
+        p.a = (uint8_t const *)workspace, p.a_scales = p.a + s.scales_at;
     }
     return with_type(c_dtype, [&](auto value) {
         uint32_t const rows = height > 256 ? 256 : (uint32_t)height;
@@ -741,8 +833,9 @@ int nk_amd_mx_dots_packed_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_s
 nk_size_t nk_amd_mx_experts_workspace_size(nk_size_t slots, nk_size_t a_share, nk_size_t experts, nk_size_t width,
                                            nk_size_t depth, int a_is_codes, nk_dtype_t c_dtype, int weighted) {
     MxGeometry g;
-    if (!slots || !a_share || slots >= (1ull << 30) || !mx_geometry(experts, width, depth, g)) return 0;
-    return experts_layout(slots, a_share, experts, width, g, a_is_codes != 0, c_dtype, weighted != 0).bytes;
+    PlanGeometry shape;
+    if (!slots || !a_share || !mx_geometry(experts, width, depth, g) || !plan_geometry(slots, experts, shape)) return 0;
+    return experts_layout(shape, width, g, a_is_codes != 0, c_dtype, weighted != 0).bytes;
 }
 
 int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_stride, void const *a_scales,
@@ -759,7 +852,7 @@ int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_
     if (int const status = depth ? check_a(a_dtype, a, a_scales, a_stride) : 0) return status;
     if (int const status = check_c(c_dtype, c, c_stride)) return status;
     if (!packed || ((uintptr_t)packed & 15) || !plan || ((uintptr_t)plan & 15)) return mx_fail("mx_dots_experts: image and plan have to be 16-byte aligned");
-    ExpertsLayout const l = experts_layout(slots, a_share, experts, width, g, a_scales != nullptr, c_dtype, weights != nullptr);
+    ExpertsLayout const l = experts_layout(shape, width, g, a_scales != nullptr, c_dtype, weights != nullptr);
     if (l.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < l.bytes))
         return mx_fail("mx_dots_experts: the workspace is too small or not 256-byte aligned");
     MxArgs p = {};
@@ -769,14 +862,14 @@ int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_
     p.tiles_m = shape.max_tiles, p.order = (uint32_t)shape.order, p.tile_list = (uint32_t)shape.tiles;
     if (l.fused) p.a = (uint8_t const *)a, p.a_pitch = a_stride, p.a_wide = aligned(a, a_stride, 16);
     else {
-        if (int const status = stage(a_dtype, a, a_stride, a_scales, a_scales_stride, slots / a_share, p.k, g, l.staged, (uint8_t *)workspace, stream))
+        if (int const status = stage(a_dtype, a, a_stride, a_scales, a_scales_stride, shape.max_rows, p.k, g, l.staged, (uint8_t *)workspace, plan, shape.order, p.a_share, stream))
             return status;
-        p.a = (uint8_t const *)workspace, p.a_scales = p.a + l.staged.scales_at, p.a_pitch = l.staged.pitch, p.scales_pitch = l.staged.scales_pitch;
+        p.a = (uint8_t const *)workspace, p.a_scales = p.a + l.staged.scales_at;
     }
     uint8_t *sums = (uint8_t *)workspace + l.sums_at;
     int const product_dtype = weights ? l.sums_dtype : (int)c_dtype;
-    if (weights) p.sorted = 1, p.c = sums, p.c_stride = l.sums_values * element_bytes(l.sums_dtype), p.c_wide = 1;
-    else p.c = (uint8_t *)c, p.c_stride = c_stride, p.c_wide = aligned(c, c_stride, 16);
+    if (weights) p.sorted = 1, p.c = sums, p.c_stride = l.sums_values * element_bytes(l.sums_dtype);
+    else p.c = (uint8_t *)c, p.c_stride = c_stride;
     int const status = with_type(product_dtype, [&](auto value) {
         return launch_product<decltype(value), true>(p, shape.tile_rows, a_dtype, l.fused, 16, g, stream);
     });
@@ -791,7 +884,7 @@ int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_
             typedef decltype(out) Out;
             hipLaunchKernelGGL((combine_kernel<In, Out>), dim3((uint32_t)((here * pieces + 255) / 256)), dim3(256), 0, stream,
                                (In const *)sums, l.sums_values, p.plan, place, weights + first * top_k, (uint32_t)top_k, (uint32_t)here,
-                               p.n, (uint32_t)pieces, (Out *)((uint8_t *)c + first * c_stride), (uint64_t)c_stride, aligned(c, c_stride, 16));
+                               p.n, (uint32_t)pieces, (Out *)((uint8_t *)c + first * c_stride), (uint64_t)c_stride);
             hipError_t const e = hipGetLastError();
             return e == hipSuccess ? 0 : mx_fail(e, "combine_kernel");
         };

@@ -13,19 +13,21 @@
  *  whole depth. A scale of 255 gives NaN also where every code of the block is zero.
  *
  *  Depth is walked in steps of 128 values, 64 bytes of codes a row; four steps (a super) share a 32-bit word of scales per
- *  lane, byte u for step u, which the instruction picks by an immediate.
+ *  lane, byte u for step u, which the instruction picks by an immediate. What is stored is padded to whole supers with zeros.
+ *
+ *  Fragments: 16 rows of a step are 1024 bytes, lane l's 16 bytes at 16 l (row l % 16, block l / 16 of the step's four), so a
+ *  wavefront moves one with a single instruction and in one piece. Their scales of a super are 256 bytes, the word of row r
+ *  and block g at word 4 r + 2 (g % 2) + g / 2: instructions of 32 rows take two blocks at a time, and their lanes find the
+ *  words of both halves of a step side by side. Both operands of a product are held like this:
  *
  *  Packed image (B, n columns of depth k, `count` matrices), little-endian:
  *
- *      [ 128-byte header ][ codes of every matrix ][ scales of every matrix ]
- *      codes:  [tile][step][lane] 16 bytes      1024 bytes that one wavefront loads at once and feeds to the instruction
- *      scales: [tile][super][lane] 4 bytes
+ *      [ 128-byte header ][ codes of every matrix: [tile][step] ][ scales of every matrix: [tile][super] ]
  *
  *  A tile is 16 columns, four tiles a group of 64. Row q of tile j of a group is column 16 (q / 4) + 4 j + q % 4: a lane's
  *  results of the four tiles are then 16 adjacent columns of one row of C, and are stored as such.
  *
- *  Staged A (in the workspace): rows of codes `a_pitch` bytes apart, padded with zeros to whole steps; rows of scales
- *  [super][l / 16] 4 bytes, again byte u for step u.
+ *  Staged A (in the workspace): [16 rows][step] and [16 rows][super] likewise, rows in order (with experts: in the plan's).
  */
 #ifndef NUMKONG_AMD_MX_GFX950_HPP
 #define NUMKONG_AMD_MX_GFX950_HPP
@@ -43,6 +45,7 @@ namespace nk_gfx950 {
 /** The text that nk_hip_last_error() gives on this thread; both return a status for the caller to hand on. */
 int mx_fail(hipError_t status, char const *what);
 int mx_fail(char const *what);
+int compute_unit_count(); // of the current device (dots_gfx950.hip)
 
 constexpr uint32_t kMxMagic = 0x34584D4Eu; // "NMX4"
 constexpr uint32_t kMxHeaderBytes = 128;
@@ -50,47 +53,58 @@ struct MxHeader {
     uint32_t magic, version, count, n, k, reserved[3];
 };
 
+/** Depths of products: below 2^25, so that eight tiles of the image, and 256 rows of A, lie within 32-bit offsets. */
+constexpr uint64_t kMxMaxDepth = 1ull << 25;
+
 struct MxGeometry {
-    uint32_t steps, supers, tiles; // of one matrix
+    uint32_t steps, supers, tiles; // of one matrix (steps: those that hold values)
     uint64_t code_bytes, scale_bytes, total_bytes; // of one matrix, of one matrix, of the image
 };
 inline bool mx_geometry(size_t count, size_t n, size_t k, MxGeometry &g) {
-    if (n >= (1ull << 31) || k >= (1ull << 31) || count >= (1ull << 20)) return false;
+    if (n >= (1ull << 31) || k >= kMxMaxDepth || count >= (1ull << 20)) return false;
     g.steps = (uint32_t)((k + 127) / 128), g.supers = (g.steps + 3) / 4, g.tiles = (uint32_t)((n + 63) / 64) * 4;
-    g.code_bytes = (uint64_t)g.tiles * g.steps * 1024, g.scale_bytes = (uint64_t)g.tiles * g.supers * 256;
+    g.code_bytes = (uint64_t)g.tiles * g.supers * 4096, g.scale_bytes = (uint64_t)g.tiles * g.supers * 256;
     if (count && g.code_bytes + g.scale_bytes > (1ull << 46) / count) return false;
     g.total_bytes = kMxHeaderBytes + count * (g.code_bytes + g.scale_bytes);
     return true;
 }
 
+/** Where, of a fragment's 64 words of scales, that of row r and block g is. */
+__host__ __device__ inline uint32_t scale_word(uint32_t r, uint32_t g) { return r * 4 + (g & 1) * 2 + (g >> 1); }
+
 /**
- *  The plan of the experts' products, 32-bit words: header, first row of each expert, rows (slots sorted by expert), the
- *  row of each slot (-1: no expert), tiles of rows. Bucket `experts` holds the slots of no expert, in the last rows.
+ *  The plan of the experts' products, 32-bit words: header, first row of each expert, the slot of each row, the row of each
+ *  slot (-1: no expert), tiles of rows. Rows are the slots sorted by expert; an expert's rows start at a multiple of 16, so
+ *  that its fragments are its own, and rows in between have slot -1. Bucket `experts` holds the slots of no expert, last.
  */
 struct PlanHeader {
-    uint32_t magic, slots, experts, tile_rows, tile_count, valid_rows, reserved[2];
+    uint32_t magic, slots, experts, tile_rows;
+    uint32_t tile_count, zero_tiles; // tiles of the experts' rows; tiles of the rows of none, behind them
+    uint32_t first_zero, end_zero;   // rows of the experts end, and rows of none begin, at the first; these end at the second
 };
 constexpr uint32_t kPlanMagic = 0x504C414Eu;
 struct PlanTile {
     int32_t expert, first, last, reserved; // rows [first, last) of one expert; expert == experts: rows of none
 };
 struct PlanGeometry {
-    uint32_t tile_rows, max_tiles;
+    uint32_t tile_rows, max_tiles, max_rows;
     size_t offsets, order, place, tiles, total_words; // in words
 };
 /** Rows of a tile: what an expert has on average decides which kernel will run, and with it how its rows are cut. */
 inline uint32_t plan_tile_rows(size_t slots, size_t experts) {
     size_t const mean = experts ? slots / experts : 0;
-    return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 96 ? 64 : mean <= 256 ? 128 : 256;
+    return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 256 ? 128 : 256;
 }
 constexpr size_t kMaxExperts = 1024, kMaxTopK = 64, kMaxGroups = 64;
 inline bool plan_geometry(size_t slots, size_t experts, PlanGeometry &g) {
     if (!experts || experts > kMaxExperts || slots >= (1ull << 30)) return false;
+    size_t const buckets = slots < experts + 1 ? slots : experts + 1; // that can have any
     g.tile_rows = plan_tile_rows(slots, experts);
-    g.max_tiles = (uint32_t)(slots / g.tile_rows + (slots < experts + 1 ? slots : experts + 1));
+    g.max_tiles = (uint32_t)(slots / g.tile_rows + buckets);
+    g.max_rows = (uint32_t)((slots + buckets * 15 + 15) / 16 * 16);
     g.offsets = sizeof(PlanHeader) / 4;
     g.order = g.offsets + ((experts + 2 + 3) & ~(size_t)3);
-    g.place = g.order + slots;
+    g.place = g.order + g.max_rows;
     g.tiles = (g.place + slots + 3) & ~(size_t)3;
     g.total_words = g.tiles + (size_t)g.max_tiles * 4;
     return true;
@@ -101,6 +115,7 @@ inline bool plan_geometry(size_t slots, size_t experts, PlanGeometry &g) {
 #endif
 
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef int v8i __attribute__((ext_vector_type(8)));
@@ -171,6 +186,32 @@ __device__ __forceinline__ uint32_t quantize_eight(float const (&v)[8], uint32_t
     return field == 255 ? 0u : codes;
 }
 
+/** The same with a block's 32 values in one lane: four words of codes. */
+__device__ __forceinline__ v4u quantize_block(float const (&v)[32], uint32_t &scale) {
+    uint32_t largest = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        uint32_t const magnitude = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+        largest = largest > magnitude ? largest : magnitude;
+    }
+    uint32_t const field = largest >> 23;
+    scale = field == 255 ? 255 : field > 2 ? field - 2 : 0;
+    float const power = __uint_as_float(scale ? scale << 23 : 0x00400000u);
+    v4u words = {0, 0, 0, 0};
+#ifdef NK_MX_DEVICE_BUILTINS
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t codes = 0;
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[8 * i], v[8 * i + 1], power, 0);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[8 * i + 2], v[8 * i + 3], power, 1);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[8 * i + 4], v[8 * i + 5], power, 2);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[8 * i + 6], v[8 * i + 7], power, 3);
+        words[i] = codes;
+    }
+#endif
+    return field == 255 ? v4u {0, 0, 0, 0} : words;
+}
+
 /** acc += W-fragment x A-fragment: rows of the result are the image's columns. `U`: which byte of the scale words. */
 template <int U>
 __device__ __forceinline__ v4f mx_multiply(v4u w, v4u a, v4f acc, uint32_t w_scale, uint32_t a_scale) {
@@ -183,18 +224,50 @@ __device__ __forceinline__ v4f mx_multiply(v4u w, v4u a, v4f acc, uint32_t w_sca
 #endif
 }
 
-typedef __attribute__((address_space(3))) void mx_lds_t;
-typedef __attribute__((address_space(1))) void const mx_global_t;
-/** 16 or 4 bytes per lane from each lane's own address into LDS at `dst` + 16 or 4 x lane (`dst` the same in all lanes). */
-__device__ __forceinline__ void fetch_16(void const *src, void *dst) {
+/** The same with v_mfma_scale_f32_32x32x64_f8f6f4: lane l brings row l % 32, block l / 32 of two. */
+template <int U>
+__device__ __forceinline__ v16f mx_multiply(v4u w, v4u a, v16f acc, uint32_t w_scale, uint32_t a_scale) {
 #ifdef NK_MX_DEVICE_BUILTINS
-    __builtin_amdgcn_global_load_lds((mx_global_t *)src, (mx_lds_t *)dst, 16, 0, 0);
+    v8i const x = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+    v8i const y = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc, 4, 4, U, (int)w_scale, U, (int)a_scale);
+#else
+    return acc;
 #endif
 }
-__device__ __forceinline__ void fetch_4(void const *src, void *dst) {
+
+typedef __attribute__((address_space(3))) void mx_lds_t;
+/** 16 bytes per lane at `lane_offset` + `offset` (the same in all lanes) of a buffer into LDS at `dst` + 16 x lane. */
+__device__ __forceinline__ void fetch_16(__amdgpu_buffer_rsrc_t buffer, void *dst, uint32_t lane_offset, uint32_t offset) {
 #ifdef NK_MX_DEVICE_BUILTINS
-    __builtin_amdgcn_global_load_lds((mx_global_t *)src, (mx_lds_t *)dst, 4, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (mx_lds_t *)dst, 16, (int)lane_offset, (int)offset, 0, 0);
 #endif
+}
+
+/** 16 or 8 bytes per lane at `lane_offset` + `offset` (the same in all lanes) of a buffer. */
+__device__ __forceinline__ v4u load_16(__amdgpu_buffer_rsrc_t buffer, uint32_t lane_offset, uint32_t offset) {
+#ifdef NK_MX_DEVICE_BUILTINS
+    return __builtin_amdgcn_raw_buffer_load_b128(buffer, (int)lane_offset, (int)offset, 0);
+#else
+    return v4u {0, 0, 0, 0};
+#endif
+}
+__device__ __forceinline__ v2u load_8(__amdgpu_buffer_rsrc_t buffer, uint32_t lane_offset, uint32_t offset) {
+#ifdef NK_MX_DEVICE_BUILTINS
+    return __builtin_amdgcn_raw_buffer_load_b64(buffer, (int)lane_offset, (int)offset, 0);
+#else
+    return v2u {0, 0};
+#endif
+}
+/** What is at `base`, the same in all lanes, as a buffer (callers stay inside what they address by it). */
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(void const *base) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, 0xFFFFFFFFu, 0x00020000);
+}
+
+/** 16 bytes to any address that is even. */
+__device__ __forceinline__ void store_16(void *to, v4u values) {
+    typedef v4u __attribute__((aligned(2))) anywhere;
+    *(anywhere *)to = values;
 }
 
 /** A number that a lambda's argument carries at compile time. */
@@ -203,16 +276,16 @@ struct Number {
     static constexpr int value = N;
 };
 
-/** `count` (up to N) adjacent results at `to`; all N as one vector where `wide` says that the address allows it. */
+/** `count` (up to N) adjacent results at `to`: all N as vectors, which global memory takes at any element's address. */
 template <class Out, int N>
-__device__ __forceinline__ void store_some(Out *to, float const (&v)[N], uint32_t count, bool wide) {
-    if (wide && count >= N) {
-        struct alignas(sizeof(Out) * N < 16 ? sizeof(Out) * N : 16) Pack {
+__device__ __forceinline__ void store_some(Out *to, float const (&v)[N], uint32_t count) {
+    if (count >= N) {
+        struct __attribute__((packed, aligned(sizeof(Out)))) Pack {
             Out x[N];
         } pack;
 #pragma unroll
         for (int i = 0; i < N; ++i) pack.x[i] = (Out)v[i];
-        *(Pack *)to = pack;
+        __builtin_memcpy(to, &pack, sizeof(pack));
         return;
     }
 #pragma unroll

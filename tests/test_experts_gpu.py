@@ -193,22 +193,26 @@ def test_plan(tokens, top_k, experts, kind):
     words = plan.buffer.view(torch.int32).cpu().numpy()
     flat = chosen.reshape(-1)
     bucket = np.where((flat >= 0) & (flat < experts), flat, experts)
-    order = np.argsort(bucket, kind="stable")
     counts = np.bincount(bucket, minlength=experts + 1)
-    first = 8 + (experts + 2 + 3) // 4 * 4
-    np.testing.assert_array_equal(words[8:8 + experts + 2], np.concatenate([[0], np.cumsum(counts)]))
-    np.testing.assert_array_equal(words[first:first + len(flat)], order)
-    place = np.empty(len(flat), np.int64)
-    place[order] = np.arange(len(flat))
-    np.testing.assert_array_equal(words[first + len(flat):first + 2 * len(flat)], np.where(bucket < experts, place, -1))
-    tile_rows, tile_count = words[3], words[4]
-    tiles = words[(first + 2 * len(flat) + 3) // 4 * 4:].reshape(-1, 4)[:tile_count]
-    want, start = [], 0
+    sizes = (counts + 15) // 16 * 16  # an expert's rows start at a multiple of 16; rows between have slot -1
+    starts = np.concatenate([[0], np.cumsum(sizes)])[:-1]
+    tile_rows, tile_count, zero_tiles, first_zero, end_zero = words[3:8]
+    assert (first_zero, end_zero) == (starts[experts], starts[experts] + counts[experts])
+    np.testing.assert_array_equal(words[8:8 + experts + 2], np.concatenate([starts, [end_zero]]))
+    buckets = min(len(flat), experts + 1)
+    first, room = 8 + (experts + 2 + 3) // 4 * 4, (len(flat) + buckets * 15 + 15) // 16 * 16
+    order, place = np.full(sizes.sum(), -1), np.full(len(flat), -1)
     for e in range(experts + 1):
-        for row in range(0, counts[e], tile_rows):
-            want.append((e, start + row, min(start + row + tile_rows, start + counts[e])))
-        start += counts[e]
+        slots = np.flatnonzero(bucket == e)
+        order[starts[e]:starts[e] + counts[e]] = slots
+        place[slots] = starts[e] + np.arange(counts[e]) if e < experts else -1
+    np.testing.assert_array_equal(words[first:first + len(order)], order)
+    np.testing.assert_array_equal(words[first + room:first + room + len(flat)], place)
+    tiles = words[(first + room + len(flat) + 3) // 4 * 4:].reshape(-1, 4)[:tile_count + zero_tiles]
+    want = [(e, starts[e] + row, min(starts[e] + row + tile_rows, starts[e] + counts[e]))
+            for e in range(experts + 1) for row in range(0, counts[e], tile_rows)]
     np.testing.assert_array_equal(tiles[:, :3], np.array(want).reshape(-1, 3))
+    assert tile_count == sum(tile[0] < experts for tile in want)
 
 
 @pytest.mark.parametrize("tokens,top_k,experts,kind", CASES)
