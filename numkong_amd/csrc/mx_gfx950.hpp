@@ -122,32 +122,39 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-/** Eight adjacent values of a row from column `col` on, as 32-bit floats; zeros from column `k` on. `wide`: rows start on
- *  16-byte addresses. (Widening is exact, so whatever follows sees the values themselves.) */
+/** Eight adjacent values as they lie in memory, 16-byte aligned, and as 32-bit floats. (Widening is exact, so whatever
+ *  follows sees the values themselves; a kernel loads several before it widens the first.) */
 template <class T>
-__device__ __forceinline__ void load_eight(T const *row, uint32_t col, uint32_t k, bool wide, float (&v)[8]) {
-    if (wide && col + 8 <= k) {
-        if constexpr (sizeof(T) == 4) {
-            v4f const low = *(v4f const *)(row + col), high = *(v4f const *)(row + col + 4);
+struct Eight {
+    v4u words[sizeof(T) / 2];
+};
+template <class T>
+__device__ __forceinline__ Eight<T> load_eight(T const *from) {
+    Eight<T> e;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = low[i], v[4 + i] = high[i];
-        }
-        else {
-            v4u const words = *(v4u const *)(row + col);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) e.words[i] = ((v4u const *)from)[i];
+    return e;
+}
+template <class T>
+__device__ __forceinline__ void widen_eight(Eight<T> const &e, float (&v)[8]) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (__is_same(T, __bf16))
-                    v[2 * i] = __uint_as_float(words[i] << 16), v[2 * i + 1] = __uint_as_float(words[i] & 0xFFFF0000u);
-                else {
-                    f16x2 const pair = __builtin_bit_cast(f16x2, (uint32_t)words[i]);
-                    v[2 * i] = (float)pair[0], v[2 * i + 1] = (float)pair[1];
-                }
-            }
-        }
-        return;
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(e.words[i / 4][i % 4]);
+        else if constexpr (__is_same(T, __bf16)) v[i] = __uint_as_float(i % 2 ? e.words[0][i / 2] & 0xFFFF0000u : e.words[0][i / 2] << 16);
+        else v[i] = (float)__builtin_bit_cast(f16x2, (uint32_t)e.words[0][i / 2])[i % 2];
     }
+}
+/** Eight values of a row from column `col` on, wherever they lie; zeros from column `k` on. */
+template <class T>
+__device__ __forceinline__ void load_some(T const *row, uint32_t col, uint32_t k, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = col + i < k ? (float)row[col + i] : 0.0f;
+}
+/** `wide`: rows start on 16-byte addresses. */
+template <class T>
+__device__ __forceinline__ void load_eight(T const *row, uint32_t col, uint32_t k, bool wide, float (&v)[8]) {
+    if (wide && col + 8 <= k) widen_eight(load_eight(row + col), v);
+    else load_some(row, col, k, v);
 }
 
 /** The largest of four adjacent lanes, in all four. */
@@ -184,32 +191,6 @@ __device__ __forceinline__ uint32_t quantize_eight(float const (&v)[8], uint32_t
     codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[6], v[7], power, 3);
 #endif
     return field == 255 ? 0u : codes;
-}
-
-/** The same with a block's 32 values in one lane: four words of codes. */
-__device__ __forceinline__ v4u quantize_block(float const (&v)[32], uint32_t &scale) {
-    uint32_t largest = 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        uint32_t const magnitude = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-        largest = largest > magnitude ? largest : magnitude;
-    }
-    uint32_t const field = largest >> 23;
-    scale = field == 255 ? 255 : field > 2 ? field - 2 : 0;
-    float const power = __uint_as_float(scale ? scale << 23 : 0x00400000u);
-    v4u words = {0, 0, 0, 0};
-#ifdef NK_MX_DEVICE_BUILTINS
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t codes = 0;
-        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[8 * i], v[8 * i + 1], power, 0);
-        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[8 * i + 2], v[8 * i + 3], power, 1);
-        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[8 * i + 4], v[8 * i + 5], power, 2);
-        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[8 * i + 6], v[8 * i + 7], power, 3);
-        words[i] = codes;
-    }
-#endif
-    return field == 255 ? v4u {0, 0, 0, 0} : words;
 }
 
 /** acc += W-fragment x A-fragment: rows of the result are the image's columns. `U`: which byte of the scale words. */
