@@ -14,7 +14,6 @@ from __future__ import annotations
 
 import ctypes
 import math
-from contextlib import nullcontext
 from dataclasses import dataclass
 
 from . import api
@@ -29,13 +28,18 @@ class _Route(ctypes.Structure):
 
 
 _LIB = None
+_device = _stream = None  # the current device's index, a device's current stream as a number: torch's own (see _library)
 
 
 def _library():
     """The shared library with the entry points of mx.h bound, and the torch module."""
-    global _LIB
+    global _LIB, _device, _stream
     if _LIB is None:
         import torch
+
+        _device = torch.cuda.current_device
+        # (a Stream object of torch's takes 2 us to make; a product of few rows takes 8)
+        _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
         lib = api.library()
         sz, vp, i32 = ctypes.c_uint64, ctypes.c_void_p, ctypes.c_int
@@ -76,84 +80,90 @@ def _tensor(t, what: str):
 
 def _floats(t, what: str, dims: int = 2):
     """The tensor of a float operand, rows of adjacent values."""
-    lib, torch, codes = _library()
-    t = _tensor(t, what)
+    lib, torch, codes = _LIB or _library()
+    if not isinstance(t, torch.Tensor):
+        t = _tensor(t, what)
     if t.dtype not in codes:
         raise TypeError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
     if t.dim() != dims:
         raise ValueError(f"{what} must be {dims}-dimensional, got {t.dim()} dimensions")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{what} rows must be contiguous (stride of the last dimension must be 1)")
-    if t.shape[0] > 1 and t.stride(0) < 0:
-        raise ValueError(f"{what} rows must not run backwards")
     return t
 
 
 def _row_bytes(t) -> int:
     """Bytes from one row of a matrix to the next."""
-    return (t.stride(0) if t.shape[0] > 1 else t.shape[1]) * t.element_size()
-
-
-def _on(device):
-    """What makes `device` the current one while a call queues its work (nothing where it is)."""
-    import torch
-
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-def _stream(torch, device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    rows, columns = t.shape
+    return (t.stride(0) if rows > 1 else columns) * t.itemsize
 
 
 def _home(*operands):
-    """The GPU that a call runs on (where its device operands are), and whether its results go back to host memory."""
+    """The index of the GPU that the operands are on, None where all are in host memory."""
+    home, host = None, False
+    for t in operands:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            host = True
+        elif home is None:
+            home = t.get_device()
+        elif t.get_device() != home:
+            raise ValueError(f"operands are on different devices: cuda:{home} and {t.device}")
+    if home is not None and host:
+        raise ValueError("operands are partly in GPU memory and partly in host memory")
+    return home
+
+
+def _to_gpu(t):
+    """An operand of host memory (a tensor, or an MxMatrix) on the current GPU."""
     import torch
 
-    devices = {t.device for t in operands if t is not None and t.is_cuda}
-    if len(devices) > 1:
-        raise ValueError(f"operands are on different devices: {sorted(map(str, devices))}")
-    if devices:
-        for t in operands:
-            if t is not None and not t.is_cuda:
-                raise ValueError("operands are partly in GPU memory and partly in host memory")
-        return devices.pop(), False
     if not torch.cuda.is_available():
         raise NumKongAmdError("no GPU: this library has no CPU fallback")
-    return torch.device("cuda", torch.cuda.current_device()), True
+    if isinstance(t, MxMatrix):
+        return MxMatrix(_tensor(t.codes, "codes").cuda(), _tensor(t.scales, "scales").cuda(), t.depth)
+    return None if t is None else t.cuda()
 
 
-def _given_back(result, host: bool, as_numpy: bool, out=None):
-    """A result as the caller has its operands: in host memory, as a numpy array, or in `out`."""
+def _to_host(result, as_numpy: bool, out=None):
+    """A result as a caller with operands in host memory has them: a CPU tensor, a numpy array, or in `out`."""
     if out is not None:
-        target = _tensor(out, "out")
-        if target.data_ptr() != result.data_ptr():
-            target.copy_(result)
+        _tensor(out, "out").copy_(result)
         return out
-    if host:
-        result = result.cpu()
-    return result.numpy() if as_numpy else result
+    return result.cpu().numpy() if as_numpy else result.cpu()
 
 
-def _result(torch, out, shape, dtype, device, host: bool):
-    """The matrix that a call writes: `out` where it can be written in place, else a new one."""
+def _result(torch, out, shape, dtype, like):
+    """The matrix that a call writes: `out` where one is given, else a new one."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty(shape, dtype=dtype, device=like.device)
     t = _tensor(out, "out")
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"out has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != dtype:
         raise TypeError(f"out must have dtype {dtype}")
-    if host:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if t.device != device:
-        raise ValueError(f"out is on {t.device}, the operands on {device}")
-    if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.device != like.device:
+        raise ValueError(f"out is on {t.device}, the operands on {like.device}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError("out rows must be contiguous")
     return t
 
 
+def _check_host_out(out, shape, dtype):
+    """What `_result` asks of an `out` in host memory."""
+    if out is not None:
+        t = _tensor(out, "out")
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError(f"out has shape {tuple(t.shape)}, expected {tuple(shape)}")
+        if t.dtype != dtype:
+            raise TypeError(f"out must have dtype {dtype}")
+        if t.is_cuda:
+            raise ValueError("out is in GPU memory, the operands in host memory")
+
+
 def _out_dtype(out, out_dtype):
-    lib, torch, codes = _library()
+    lib, torch, codes = _LIB or _library()
     if out_dtype is None:
         out_dtype = _tensor(out, "out").dtype if out is not None else torch.float32
     if out_dtype not in codes:
@@ -192,8 +202,12 @@ class MxMatrix:
     def shape(self):
         return (*self.codes.shape[:-1], self.depth)
 
-    def _to(self, device):
-        return self if self.codes.device == device else MxMatrix(self.codes.to(device), self.scales.to(device), self.depth)
+    @classmethod
+    def _made(cls, codes, scales, depth):
+        """One whose parts are known to be right."""
+        matrix = cls.__new__(cls)
+        matrix.codes, matrix.scales, matrix.depth = codes, scales, depth
+        return matrix
 
     def __repr__(self):
         return f"MxMatrix(shape={tuple(self.shape)}, device={self.codes.device})"
@@ -222,35 +236,30 @@ class MxPackedMatrix:
         return int(_library()[0].nk_amd_mx_packed_size(count, width, depth))
 
 
-def _quantized(lib, torch, dtype_codes, x, device):
-    """Codes and scales of the rows of a device matrix."""
-    rows, depth = x.shape
-    codes = torch.empty((rows, (depth + 1) // 2), dtype=torch.uint8, device=device)
-    scales = torch.empty((rows, (depth + BLOCK - 1) // BLOCK), dtype=torch.uint8, device=device)
-    _check(lib.nk_amd_mx_quantize_async(dtype_codes[x.dtype], x.data_ptr(), rows, depth, _row_bytes(x), codes.data_ptr(),
-                                        codes.shape[1], scales.data_ptr(), scales.shape[1], _stream(torch, device)), "mx_quantize")
-    return codes, scales
-
-
 def mx_quantize(x) -> MxMatrix:
     """The rows of ``x`` (float32, bfloat16 or float16) as 4-bit codes with a scale for each 32 values: the power of two
     that brings the block's largest magnitude into [4, 8); codes to nearest, ties to even, stopping at 6. A block that holds a
     NaN or an infinity becomes NaN."""
-    lib, torch, dtype_codes = _library()
-    as_numpy, x = _is_numpy(x), _floats(x, "x")
-    device, host = _home(x)
-    with _on(device):
-        codes, scales = _quantized(lib, torch, dtype_codes, x.to(device) if host else x, device)
-    if host:
-        codes, scales = codes.cpu(), scales.cpu()
-    matrix = MxMatrix(codes, scales, x.shape[1])
-    if as_numpy:
-        matrix.codes, matrix.scales = matrix.codes.numpy(), matrix.scales.numpy()
-    return matrix
+    lib, torch, dtype_codes = _LIB or _library()
+    t = _floats(x, "x")
+    rows, depth = t.shape
+    if not t.is_cuda:
+        m = mx_quantize(_to_gpu(t))
+        codes, scales = m.codes.cpu(), m.scales.cpu()
+        return MxMatrix._made(codes.numpy(), scales.numpy(), depth) if _is_numpy(x) else MxMatrix._made(codes, scales, depth)
+    if t.get_device() != _device():
+        with torch.cuda.device(t.device):
+            return mx_quantize(t)
+    code_bytes, blocks = (depth + 1) // 2, (depth + BLOCK - 1) // BLOCK
+    codes = torch.empty((rows, code_bytes), dtype=torch.uint8, device=t.device)
+    scales = torch.empty((rows, blocks), dtype=torch.uint8, device=t.device)
+    _check(lib.nk_amd_mx_quantize_async(dtype_codes[t.dtype], t.data_ptr(), rows, depth, _row_bytes(t), codes.data_ptr(), code_bytes,
+                                        scales.data_ptr(), blocks, _stream(t.get_device())), "mx_quantize")
+    return MxMatrix._made(codes, scales, depth)
 
 
 def _matrix_of(a, what: str) -> MxMatrix:
-    """An MxMatrix whose parts are tensors (one made of numpy arrays is looked at anew)."""
+    """An MxMatrix whose parts are tensors (mx_quantize of a numpy array has given one of arrays)."""
     if not isinstance(a, MxMatrix):
         raise TypeError(f"{what} must be an MxMatrix")
     return a if hasattr(a.codes, "data_ptr") else MxMatrix(a.codes, a.scales, a.depth)
@@ -258,95 +267,94 @@ def _matrix_of(a, what: str) -> MxMatrix:
 
 def mx_dequantize(matrix: MxMatrix, dtype=None, out=None):
     """The values that a matrix of codes and scales stands for, in float32 (default), bfloat16 (both exact) or float16."""
-    lib, torch, dtype_codes = _library()
-    as_numpy = isinstance(matrix, MxMatrix) and _is_numpy(matrix.codes)
-    matrix = _matrix_of(matrix, "matrix")
+    lib, torch, dtype_codes = _LIB or _library()
+    m = _matrix_of(matrix, "matrix")
     dtype = _out_dtype(out, dtype)
-    if matrix.codes.dim() != 2:
+    if m.codes.dim() != 2:
         raise ValueError("mx_dequantize takes one matrix, not a stack")
-    device, host = _home(matrix.codes)
-    rows, depth = matrix.shape
-    with _on(device):
-        m = matrix._to(device)
-        result = _result(torch, out, (rows, depth), dtype, device, host)
-        _check(lib.nk_amd_mx_dequantize_async(dtype_codes[dtype], m.codes.data_ptr(), _row_bytes(m.codes), m.scales.data_ptr(),
-                                              _row_bytes(m.scales), rows, depth, result.data_ptr(), _row_bytes(result),
-                                              _stream(torch, device)), "mx_dequantize")
-        return _given_back(result, host, as_numpy, out)
+    rows, depth = m.shape
+    if not m.codes.is_cuda:
+        _check_host_out(out, (rows, depth), dtype)
+        return _to_host(mx_dequantize(_to_gpu(m), dtype), _is_numpy(matrix.codes), out)
+    if m.codes.get_device() != _device():
+        with torch.cuda.device(m.codes.device):
+            return mx_dequantize(m, dtype, out)
+    result = _result(torch, out, (rows, depth), dtype, m.codes)
+    _check(lib.nk_amd_mx_dequantize_async(dtype_codes[dtype], m.codes.data_ptr(), _row_bytes(m.codes), m.scales.data_ptr(),
+                                          _row_bytes(m.scales), rows, depth, result.data_ptr(), _row_bytes(result),
+                                          _stream(m.codes.get_device())), "mx_dequantize")
+    return result if out is None else out
 
 
 def mx_pack(b) -> MxPackedMatrix:
     """Lay ``b`` out for products: an MxMatrix or floats (quantised first), width x depth, or count x width x depth for a
     stack of matrices (``mx_dots_experts``). The image is in GPU memory."""
-    lib, torch, dtype_codes = _library()
+    lib, torch, dtype_codes = _LIB or _library()
     if not isinstance(b, MxMatrix):
         b = _tensor(b, "b")
         b = _floats(b, "b", 3 if b.dim() == 3 else 2)
-        device, host = _home(b)
-        b = b.to(device) if host else b
-        with _on(device):
-            flat = b if b.dim() == 2 else b.reshape(-1, b.shape[2])
-            codes, scales = _quantized(lib, torch, dtype_codes, flat, device)
-        b = MxMatrix(codes.reshape(*b.shape[:-1], -1) if codes.numel() else codes.new_empty((*b.shape[:-1], codes.shape[-1])),
-                     scales.reshape(*b.shape[:-1], -1) if scales.numel() else scales.new_empty((*b.shape[:-1], scales.shape[-1])), b.shape[-1])
+        flat = mx_quantize((b if b.is_cuda else _to_gpu(b)).reshape(-1, b.shape[-1]) if b.dim() == 3 else b if b.is_cuda else _to_gpu(b))
+        b = MxMatrix(flat.codes.reshape(*b.shape[:-1], flat.codes.shape[-1]), flat.scales.reshape(*b.shape[:-1], flat.scales.shape[-1]), b.shape[-1])
     b = _matrix_of(b, "b")
-    device, _ = _home(b.codes)
-    count, width = (1, b.codes.shape[0]) if b.codes.dim() == 2 else b.codes.shape[:2]
+    if not b.codes.is_cuda:
+        b = _to_gpu(b)
+    if b.codes.get_device() != _device():
+        with torch.cuda.device(b.codes.device):
+            return mx_pack(b)
+    stacked = b.codes.dim() == 3
+    count, width = b.codes.shape[:2] if stacked else (1, b.codes.shape[0])
     size = lib.nk_amd_mx_packed_size(count, width, b.depth)
     if size == 0:
         raise NumKongAmdError("nk_amd_mx_packed_size returned 0 (unsupported dimensions)")
-    with _on(device):
-        b = b._to(device)
-        if min(*b.codes.stride(), *b.scales.stride(), 0) < 0:
-            raise ValueError("rows must not run backwards")
-        stacked = b.codes.dim() == 3
-        buffer = torch.empty(size, dtype=torch.uint8, device=device)
-        _check(lib.nk_amd_mx_pack_async(b.codes.data_ptr(), b.codes.stride(-2), b.codes.stride(0) if stacked else 0,
-                                        b.scales.data_ptr(), b.scales.stride(-2), b.scales.stride(0) if stacked else 0, count, width,
-                                        b.depth, buffer.data_ptr(), _stream(torch, device)), "mx_pack")
+    buffer = torch.empty(size, dtype=torch.uint8, device=b.codes.device)
+    _check(lib.nk_amd_mx_pack_async(b.codes.data_ptr(), b.codes.stride(-2), b.codes.stride(0) if stacked else 0, b.scales.data_ptr(),
+                                    b.scales.stride(-2), b.scales.stride(0) if stacked else 0, count, width, b.depth,
+                                    buffer.data_ptr(), _stream(buffer.get_device())), "mx_pack")
     return MxPackedMatrix(count, width, b.depth, buffer)
 
 
-def _left_operand(a, dtype_codes, what="a"):
-    """What a product's call says of A: (tensor, scales or None, depth, dtype code, whether it came as numpy)."""
+def _left_operand(a, dtype_codes):
+    """What a product's call says of A: (tensor, scales or None, depth, dtype code, bytes between rows of scales)."""
     if isinstance(a, MxMatrix):
-        as_numpy = _is_numpy(a.codes)
-        a = _matrix_of(a, what)
+        a = _matrix_of(a, "a")
         if a.codes.dim() != 2:
-            raise ValueError(f"{what} must be one matrix, not a stack")
-        return a.codes, a.scales, a.depth, 0, as_numpy
-    as_numpy, a = _is_numpy(a), _floats(a, what)
-    return a, None, a.shape[1], dtype_codes[a.dtype], as_numpy
+            raise ValueError("a must be one matrix, not a stack")
+        return a.codes, a.scales, a.depth, 0, _row_bytes(a.scales)
+    a = _floats(a, "a")
+    return a, None, a.shape[1], dtype_codes[a.dtype], 0
 
 
 def mx_dots_packed(a, packed: MxPackedMatrix, out=None, out_dtype=None):
     """``C[height x width] = a @ B.T`` with 4-bit operands and 32-bit sums. ``a``: floats, quantised on the way exactly as
     ``mx_quantize`` does, or an MxMatrix; the result is float32 (default), bfloat16 or float16 (``out_dtype``, or ``out``'s)."""
-    lib, torch, dtype_codes = _library()
+    lib, torch, dtype_codes = _LIB or _library()
     if not isinstance(packed, MxPackedMatrix):
         raise TypeError("packed must be an MxPackedMatrix from mx_pack()")
     if packed.count != 1:
         raise ValueError("packed is a stack of matrices: mx_dots_experts() takes it")
-    a, scales, depth, a_dtype, as_numpy = _left_operand(a, dtype_codes)
+    t, scales, depth, a_dtype, scales_stride = _left_operand(a, dtype_codes)
     if depth != packed.depth:
         raise ValueError(f"depth mismatch: a has {depth} columns, packed matrix has depth {packed.depth}")
     out_dtype = _out_dtype(out, out_dtype)
-    device, host = _home(a)
-    if packed.buffer.device != device:
-        raise ValueError(f"a is on {device}, packed on {packed.buffer.device}")
-    height = a.shape[0]
-    with _on(device):
-        if host:
-            a, scales = a.to(device), scales.to(device) if scales is not None else None
-        result = _result(torch, out, (height, packed.width), out_dtype, device, host)
-        needed = lib.nk_amd_mx_dots_workspace_size(height, packed.width, depth, scales is not None)
-        workspace = torch.empty(needed, dtype=torch.uint8, device=device) if needed else None
-        _check(lib.nk_amd_mx_dots_packed_async(
-            a_dtype, a.data_ptr(), _row_bytes(a), scales.data_ptr() if scales is not None else None,
-            _row_bytes(scales) if scales is not None else 0, packed.buffer.data_ptr(), dtype_codes[out_dtype], result.data_ptr(),
-            _row_bytes(result), height, packed.width, depth, workspace.data_ptr() if needed else None, needed,
-            _stream(torch, device)), "mx_dots_packed")
-        return _given_back(result, host, as_numpy, out)
+    height, width = t.shape[0], packed.width
+    if not t.is_cuda:
+        _check_host_out(out, (height, width), out_dtype)
+        as_numpy = _is_numpy(a.codes if isinstance(a, MxMatrix) else a)
+        return _to_host(mx_dots_packed(_to_gpu(a if isinstance(a, MxMatrix) else t), packed, None, out_dtype), as_numpy, out)
+    index = t.get_device()
+    if packed.buffer.get_device() != index:
+        raise ValueError(f"a is on {t.device}, packed on {packed.buffer.device}")
+    if index != _device():
+        with torch.cuda.device(index):
+            return mx_dots_packed(a, packed, out, out_dtype)
+    result = _result(torch, out, (height, width), out_dtype, t)
+    needed = lib.nk_amd_mx_dots_workspace_size(height, width, depth, scales is not None)
+    workspace = torch.empty(needed, dtype=torch.uint8, device=t.device) if needed else None
+    _check(lib.nk_amd_mx_dots_packed_async(
+        a_dtype, t.data_ptr(), _row_bytes(t), scales.data_ptr() if scales is not None else None, scales_stride,
+        packed.buffer.data_ptr(), dtype_codes[out_dtype], result.data_ptr(), _row_bytes(result), height, width, depth,
+        workspace.data_ptr() if needed else None, needed, _stream(index)), "mx_dots_packed")
+    return result if out is None else out
 
 
 # ---- experts -------------------------------------------------------------------------------------------------------
@@ -372,51 +380,55 @@ def experts_route(logits, top_k: int, score: str = "softmax", bias=None, groups:
     the chosen where ``renormalize`` is set, times ``scale``. With ``groups`` > 1 the experts stand in groups of equal size, of
     which the ``top_groups`` stay whose ``group_top`` (1 or 2) best selection scores have the largest sum (without a bias:
     the sum of logits). A logit of -inf is never chosen; a row with too few others gets expert -1 with weight 0."""
-    lib, torch, dtype_codes = _library()
-    as_numpy, logits = _is_numpy(logits), _floats(logits, "logits")
-    tokens, experts = logits.shape
+    lib, torch, dtype_codes = _LIB or _library()
+    t = _floats(logits, "logits")
+    tokens, experts = t.shape
     how = _route_kind(score, renormalize, scale, groups, top_groups, group_top)
     if bias is not None:
         bias = _tensor(bias, "bias")
         if bias.dtype != torch.float32 or tuple(bias.shape) != (experts,):
             raise ValueError(f"bias must be {experts} float32 values")
-    device, host = _home(logits, bias)
-    with _on(device):
-        if host:
-            logits, bias = logits.to(device), bias.to(device) if bias is not None else None
-        if bias is not None:
-            bias = bias.contiguous()
-        weights = torch.empty((tokens, top_k), dtype=torch.float32, device=device)
-        chosen = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
-        _check(lib.nk_amd_experts_route_async(dtype_codes[logits.dtype], logits.data_ptr(), _row_bytes(logits), tokens, experts, top_k,
-                                              bias.data_ptr() if bias is not None else None, how, weights.data_ptr(),
-                                              chosen.data_ptr(), _stream(torch, device)), "experts_route")
-        return _given_back(weights, host, as_numpy), _given_back(chosen, host, as_numpy)
+        bias = bias.contiguous()
+    index = _home(t, bias)
+    if index is None:
+        found = experts_route(_to_gpu(t), top_k, score, _to_gpu(bias), groups, top_groups, group_top, renormalize, scale)
+        return tuple(_to_host(one, _is_numpy(logits)) for one in found)
+    if index != _device():
+        with torch.cuda.device(index):
+            return experts_route(t, top_k, score, bias, groups, top_groups, group_top, renormalize, scale)
+    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=t.device)
+    chosen = torch.empty((tokens, top_k), dtype=torch.int32, device=t.device)
+    _check(lib.nk_amd_experts_route_async(dtype_codes[t.dtype], t.data_ptr(), _row_bytes(t), tokens, experts, top_k,
+                                          bias.data_ptr() if bias is not None else None, how, weights.data_ptr(), chosen.data_ptr(),
+                                          _stream(index)), "experts_route")
+    return weights, chosen
 
 
 def experts_route_backward(grad_weights, logits, experts, score: str = "softmax", renormalize: bool = True, scale: float = 1.0):
     """The gradient of ``logits`` (their type and shape) from ``grad_weights``, that of the weights that ``experts_route``
     gave for them together with ``experts``. The selection itself has none, and neither has a bias."""
-    lib, torch, dtype_codes = _library()
-    as_numpy, logits = _is_numpy(logits), _floats(logits, "logits")
+    lib, torch, dtype_codes = _LIB or _library()
+    t = _floats(logits, "logits")
     grad_weights, experts = _tensor(grad_weights, "grad_weights"), _tensor(experts, "experts")
-    tokens, count = logits.shape
+    tokens, count = t.shape
     how = _route_kind(score, renormalize, scale)
     if grad_weights.dim() != 2 or grad_weights.shape != experts.shape or grad_weights.shape[0] != tokens:
         raise ValueError(f"grad_weights {tuple(grad_weights.shape)} and experts {tuple(experts.shape)} must be tokens x top_k, tokens {tokens}")
     if grad_weights.dtype != torch.float32 or experts.dtype != torch.int32:
         raise TypeError("grad_weights must be float32 and experts int32")
-    device, host = _home(logits, grad_weights, experts)
-    with _on(device):
-        if host:
-            logits, grad_weights, experts = logits.to(device), grad_weights.to(device), experts.to(device)
-        grad_weights, experts = grad_weights.contiguous(), experts.contiguous()
-        result = torch.empty((tokens, count), dtype=logits.dtype, device=device)
-        _check(lib.nk_amd_experts_route_backward_async(
-            dtype_codes[logits.dtype], logits.data_ptr(), _row_bytes(logits), tokens, count, experts.shape[1], how,
-            experts.data_ptr(), grad_weights.data_ptr(), result.data_ptr(), _row_bytes(result), _stream(torch, device)),
-            "experts_route_backward")
-        return _given_back(result, host, as_numpy)
+    index = _home(t, grad_weights, experts)
+    if index is None:
+        found = experts_route_backward(_to_gpu(grad_weights), _to_gpu(t), _to_gpu(experts), score, renormalize, scale)
+        return _to_host(found, _is_numpy(logits))
+    if index != _device():
+        with torch.cuda.device(index):
+            return experts_route_backward(grad_weights, t, experts, score, renormalize, scale)
+    grad_weights, experts = grad_weights.contiguous(), experts.contiguous()
+    result = torch.empty((tokens, count), dtype=t.dtype, device=t.device)
+    _check(lib.nk_amd_experts_route_backward_async(
+        dtype_codes[t.dtype], t.data_ptr(), _row_bytes(t), tokens, count, experts.shape[1], how, experts.data_ptr(),
+        grad_weights.data_ptr(), result.data_ptr(), _row_bytes(result), _stream(index)), "experts_route_backward")
+    return result
 
 
 @dataclass
@@ -432,20 +444,23 @@ class ExpertsPlan:
 def experts_plan(chosen, experts: int) -> ExpertsPlan:
     """Sort the slots of ``chosen`` (tokens x top_k, int32, as ``experts_route`` gives them) by expert, keeping their order.
     Entries outside [0, ``experts``) go to no expert: -1 for padding, or experts that another process holds."""
-    lib, torch, _ = _library()
+    lib, torch, _ = _LIB or _library()
     chosen = _tensor(chosen, "chosen")
     if chosen.dim() != 2 or chosen.dtype != torch.int32:
         raise ValueError("chosen must be a tokens x top_k matrix of int32")
     tokens, top_k = chosen.shape
-    size = lib.nk_amd_experts_plan_size(chosen.numel(), experts) if experts > 0 else 0
+    size = lib.nk_amd_experts_plan_size(tokens * top_k, experts) if experts > 0 else 0
     if size == 0:
         raise ValueError("a plan is for 1 to 1024 experts and fewer than 2^30 slots")
-    device, host = _home(chosen)
-    with _on(device):
-        chosen = chosen.to(device).contiguous()
-        buffer = torch.empty(size, dtype=torch.uint8, device=device)
-        _check(lib.nk_amd_experts_plan_async(chosen.data_ptr(), chosen.numel(), experts, buffer.data_ptr(), _stream(torch, device)),
-               "experts_plan")
+    if not chosen.is_cuda:
+        chosen = _to_gpu(chosen)
+    index = chosen.get_device()
+    if index != _device():
+        with torch.cuda.device(index):
+            return experts_plan(chosen, experts)
+    chosen = chosen.contiguous()
+    buffer = torch.empty(size, dtype=torch.uint8, device=chosen.device)
+    _check(lib.nk_amd_experts_plan_async(chosen.data_ptr(), tokens * top_k, experts, buffer.data_ptr(), _stream(index)), "experts_plan")
     return ExpertsPlan(tokens, top_k, experts, buffer)
 
 
@@ -454,49 +469,53 @@ def mx_dots_experts(a, packed: MxPackedMatrix, plan: ExpertsPlan, weights=None, 
     has a row for each token, or one for each slot (tokens * top_k rows); floats or an MxMatrix as in ``mx_dots_packed``.
     With ``weights`` (tokens x top_k, float32) the rows of a token are summed by weight instead: tokens x width, slots without
     an expert left out."""
-    lib, torch, dtype_codes = _library()
+    lib, torch, dtype_codes = _LIB or _library()
     if not isinstance(packed, MxPackedMatrix):
         raise TypeError("packed must be an MxPackedMatrix from mx_pack()")
     if not isinstance(plan, ExpertsPlan):
         raise TypeError("plan must be an ExpertsPlan from experts_plan()")
     if packed.count != plan.experts:
         raise ValueError(f"packed holds {packed.count} matrices, the plan is for {plan.experts} experts")
-    a, scales, depth, a_dtype, as_numpy = _left_operand(a, dtype_codes)
+    t, scales, depth, a_dtype, scales_stride = _left_operand(a, dtype_codes)
     if depth != packed.depth:
         raise ValueError(f"depth mismatch: a has {depth} columns, packed matrices have depth {packed.depth}")
-    slots, rows = plan.tokens * plan.top_k, a.shape[0]
-    if rows not in (plan.tokens, slots):
-        raise ValueError(f"a has {rows} rows, expected {plan.tokens} (one for each token) or {slots} (one for each slot)")
-    share = plan.top_k if rows == plan.tokens else 1
+    tokens, top_k, width, rows = plan.tokens, plan.top_k, packed.width, t.shape[0]
+    slots = tokens * top_k
+    if rows not in (tokens, slots):
+        raise ValueError(f"a has {rows} rows, expected {tokens} (one for each token) or {slots} (one for each slot)")
     if weights is not None:
         weights = _tensor(weights, "weights")
-        if weights.dtype != torch.float32 or tuple(weights.shape) != (plan.tokens, plan.top_k):
-            raise ValueError(f"weights must be {plan.tokens} x {plan.top_k} float32 values")
+        if weights.dtype != torch.float32 or tuple(weights.shape) != (tokens, top_k):
+            raise ValueError(f"weights must be {tokens} x {top_k} float32 values")
     out_dtype = _out_dtype(out, out_dtype)
-    device, host = _home(a, weights)
+    shape = (tokens, width) if weights is not None else (tokens, top_k, width)
+    index = _home(t, weights)
+    if index is None:
+        _check_host_out(out, shape, out_dtype)
+        as_numpy = _is_numpy(a.codes if isinstance(a, MxMatrix) else a)
+        found = mx_dots_experts(_to_gpu(a if isinstance(a, MxMatrix) else t), packed, plan, _to_gpu(weights), None, out_dtype)
+        return _to_host(found, as_numpy, out)
     for buffer, what in ((packed.buffer, "packed"), (plan.buffer, "plan")):
-        if buffer.device != device:
-            raise ValueError(f"a is on {device}, {what} on {buffer.device}")
-    shape = (plan.tokens, packed.width) if weights is not None else (plan.tokens, plan.top_k, packed.width)
-    with _on(device):
-        if host:
-            a, scales = a.to(device), scales.to(device) if scales is not None else None
-            weights = weights.to(device) if weights is not None else None
-        if weights is not None:
-            weights = weights.contiguous()
-        result = _result(torch, out, shape, out_dtype, device, host)
-        if weights is None and not result.is_contiguous():
-            raise ValueError("out must be contiguous")
-        if not slots:
-            return _given_back(result.zero_(), host, as_numpy, out)
-        flat = result if weights is not None else result.view(slots, packed.width)
-        code = dtype_codes[out_dtype]
-        needed = lib.nk_amd_mx_experts_workspace_size(slots, share, plan.experts, packed.width, depth, scales is not None, code,
-                                                      weights is not None)
-        workspace = torch.empty(needed, dtype=torch.uint8, device=device) if needed else None
-        _check(lib.nk_amd_mx_dots_experts_async(
-            a_dtype, a.data_ptr(), _row_bytes(a), scales.data_ptr() if scales is not None else None,
-            _row_bytes(scales) if scales is not None else 0, share, packed.buffer.data_ptr(), plan.buffer.data_ptr(), slots,
-            plan.experts, plan.top_k, weights.data_ptr() if weights is not None else None, code, flat.data_ptr(), _row_bytes(flat),
-            packed.width, depth, workspace.data_ptr() if needed else None, needed, _stream(torch, device)), "mx_dots_experts")
-        return _given_back(result, host, as_numpy, out)
+        if buffer.get_device() != index:
+            raise ValueError(f"a is on {t.device}, {what} on {buffer.device}")
+    if index != _device():
+        with torch.cuda.device(index):
+            return mx_dots_experts(a, packed, plan, weights, out, out_dtype)
+    result = _result(torch, out, shape, out_dtype, t)
+    if weights is not None:
+        weights, stride = weights.contiguous(), _row_bytes(result)
+    elif result.is_contiguous():
+        stride = width * result.itemsize
+    else:
+        raise ValueError("out must be contiguous")
+    if not slots:
+        result.zero_()
+        return result if out is None else out
+    share, code, is_codes = top_k if rows == tokens else 1, dtype_codes[out_dtype], scales is not None
+    needed = lib.nk_amd_mx_experts_workspace_size(slots, share, plan.experts, width, depth, is_codes, code, weights is not None)
+    workspace = torch.empty(needed, dtype=torch.uint8, device=t.device) if needed else None
+    _check(lib.nk_amd_mx_dots_experts_async(
+        a_dtype, t.data_ptr(), _row_bytes(t), scales.data_ptr() if is_codes else None, scales_stride, share, packed.buffer.data_ptr(),
+        plan.buffer.data_ptr(), slots, plan.experts, top_k, weights.data_ptr() if weights is not None else None, code,
+        result.data_ptr(), stride, width, depth, workspace.data_ptr() if needed else None, needed, _stream(index)), "mx_dots_experts")
+    return result if out is None else out
