@@ -214,7 +214,7 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs p, float 
 
 // ---- the plan -----------------------------------------------------------------------------------------------------
 
-constexpr int kPlanWaves = 16;
+constexpr int kPlanWaves = 4, kPlanThreads = 64 * kPlanWaves;
 /** Lanes of the wavefront that hold the same bucket, by one ballot for each bit. */
 __device__ __forceinline__ uint64_t same_bucket(uint32_t bucket, int bits, bool active) {
     uint64_t mask = __ballot(active);
@@ -226,37 +226,72 @@ __device__ __forceinline__ uint64_t same_bucket(uint32_t bucket, int bits, bool 
     return mask;
 }
 
+/** The slots of one lane: `BATCH` of its wavefront's stretch of 64 BATCH, which starts at `begin`; `experts` for none. */
+template <int BATCH>
+__device__ __forceinline__ void load_stretch(int32_t const *chosen, uint32_t begin, uint32_t slots, uint32_t experts, uint32_t (&mine)[BATCH]) {
+    uint32_t const lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) mine[i] = begin + i * 64 + lane < slots ? (uint32_t)chosen[begin + i * 64 + lane] : 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) mine[i] = mine[i] < experts ? mine[i] : experts;
+}
+
+/** How many slots of each bucket each workgroup of plan_kernel will have: table[workgroup][bucket]. */
+template <int BATCH>
+__global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(int32_t const *chosen, uint32_t slots, uint32_t experts, uint32_t *table) {
+    extern __shared__ uint32_t plan_lds[];
+    uint32_t const buckets = experts + 1, lane = threadIdx.x & 63, begin = (blockIdx.x * kPlanWaves + (threadIdx.x >> 6)) * 64 * BATCH;
+    uint32_t mine[BATCH];
+    load_stretch(chosen, begin, slots, experts, mine);
+    for (uint32_t i = threadIdx.x; i < buckets; i += kPlanThreads) plan_lds[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+        if (begin + i * 64 + lane < slots) atomicAdd(plan_lds + mine[i], 1u);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < buckets; i += kPlanThreads) table[blockIdx.x * buckets + i] = plan_lds[i];
+}
+
 /**
- *  Counting sort of the slots by expert in one workgroup: each wavefront takes a stretch of the slots, counts it, learns
- *  where its slots of each expert go, and goes over it again in order, so that no atomic decides an order. Bucket
- *  `experts` is for slots of none.
+ *  Counting sort of the slots by expert. A wavefront has a stretch of them in registers; it counts them, learns where its slots
+ *  of each bucket go (behind those of the wavefronts before it, whose counts are in LDS, and of the workgroups before, in
+ *  `table`; NULL where there is one workgroup), and goes over them again in order, so that no atomic decides an order. The first
+ *  workgroup also writes the header, the tiles and the slots of rows that stand between experts.
  */
-__global__ __launch_bounds__(64 * kPlanWaves) void plan_kernel(int32_t const *chosen, uint32_t slots, uint32_t experts,
-                                                               PlanHeader header, uint32_t offsets, uint32_t order,
-                                                               uint32_t place, uint32_t tiles, int bits, uint32_t *plan) {
+template <int BATCH>
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(int32_t const *chosen, uint32_t slots, uint32_t experts, PlanHeader header,
+                                                            uint32_t offsets, uint32_t order, uint32_t place, uint32_t tiles, int bits,
+                                                            uint32_t const *table, uint32_t *plan) {
     extern __shared__ uint32_t plan_lds[]; // [wave][bucket] counts, then where the wave's next slot of the bucket goes
     __shared__ uint32_t wave_total[2][kPlanWaves];
     uint32_t const buckets = experts + 1, thread = threadIdx.x, lane = thread & 63;
-    uint32_t const wave = __builtin_amdgcn_readfirstlane(thread >> 6);
-    for (uint32_t i = thread; i < buckets * kPlanWaves; i += 64 * kPlanWaves) plan_lds[i] = 0;
+    uint32_t const wave = __builtin_amdgcn_readfirstlane(thread >> 6), begin = (blockIdx.x * kPlanWaves + wave) * 64 * BATCH;
+    uint32_t mine[BATCH];
+    load_stretch(chosen, begin, slots, experts, mine);
+    for (uint32_t i = thread; i < buckets * kPlanWaves; i += kPlanThreads) plan_lds[i] = 0;
     __syncthreads();
-    uint32_t const stretch = ((slots + kPlanWaves - 1) / kPlanWaves + 63) & ~63u;
-    uint32_t const begin = wave * stretch < slots ? wave * stretch : slots, end = begin + stretch < slots ? begin + stretch : slots;
     uint32_t *counts = plan_lds + wave * buckets;
-    for (uint32_t at = begin + lane; at < end; at += 64) {
-        uint32_t const e = (uint32_t)chosen[at];
-        atomicAdd(counts + (e < experts ? e : experts), 1u);
-    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+        if (begin + i * 64 + lane < slots) atomicAdd(counts + mine[i], 1u);
     __syncthreads();
-    // a thread for a bucket (two where there are more than threads): its size, then rows and tiles before it
     uint32_t rows_before = 0, tiles_before = 0;
-    for (uint32_t base = 0; base < buckets; base += 64 * kPlanWaves) {
+    for (uint32_t base = 0; base < buckets; base += kPlanThreads) { // a thread for a bucket
         uint32_t const bucket = base + thread;
-        uint32_t size = 0;
-        if (bucket < buckets)
-            for (int w = 0; w < kPlanWaves; ++w) size += plan_lds[w * buckets + bucket];
-        uint32_t const its_tiles = (size + header.tile_rows - 1) / header.tile_rows;
-        uint32_t const its_rows = (size + 15) / 16 * 16;
+        uint32_t here[kPlanWaves] = {}, size = 0, earlier = 0;
+        if (bucket < buckets) {
+#pragma unroll
+            for (int w = 0; w < kPlanWaves; ++w) here[w] = plan_lds[w * buckets + bucket], size += here[w];
+            if (table) {
+                size = 0;
+#pragma unroll 8
+                for (uint32_t block = 0; block < gridDim.x; ++block) {
+                    uint32_t const its = table[block * buckets + bucket];
+                    size += its, earlier += block < blockIdx.x ? its : 0;
+                }
+            }
+        }
+        uint32_t const its_tiles = (size + header.tile_rows - 1) / header.tile_rows, its_rows = (size + 15) / 16 * 16;
         uint32_t rows = its_rows, tiles_upto = its_tiles; // inclusive sums over the wavefront, then over wavefronts
 #pragma unroll
         for (int step = 1; step < 64; step <<= 1) {
@@ -266,33 +301,38 @@ __global__ __launch_bounds__(64 * kPlanWaves) void plan_kernel(int32_t const *ch
         if (lane == 63) wave_total[0][wave] = rows, wave_total[1][wave] = tiles_upto;
         __syncthreads();
         uint32_t first = rows_before + rows - its_rows, first_tile = tiles_before + tiles_upto - its_tiles;
+#pragma unroll
         for (uint32_t w = 0; w < (uint32_t)kPlanWaves; ++w) {
             if (w < wave) first += wave_total[0][w], first_tile += wave_total[1][w];
             rows_before += wave_total[0][w], tiles_before += wave_total[1][w];
         }
         if (bucket < buckets) {
-            plan[offsets + bucket] = first;
-            uint32_t next = first;
-            for (int w = 0; w < kPlanWaves; ++w) {
-                uint32_t const here = plan_lds[w * buckets + bucket];
-                plan_lds[w * buckets + bucket] = next;
-                next += here;
+            uint32_t next = first + earlier;
+#pragma unroll
+            for (int w = 0; w < kPlanWaves; ++w) plan_lds[w * buckets + bucket] = next, next += here[w];
+            if (blockIdx.x == 0) {
+                plan[offsets + bucket] = first;
+                for (uint32_t t = 0; t < its_tiles; ++t) {
+                    uint32_t const from = first + t * header.tile_rows, to = from + header.tile_rows;
+                    PlanTile const tile = {(int32_t)bucket, (int32_t)from, (int32_t)(to < first + size ? to : first + size), 0};
+                    *(PlanTile *)(plan + tiles + (first_tile + t) * 4) = tile;
+                }
+                for (uint32_t at = first + size; at < first + its_rows; ++at) plan[order + at] = 0xFFFFFFFFu;
+                if (bucket == experts) {
+                    header.tile_count = first_tile, header.zero_tiles = its_tiles;
+                    header.first_zero = first, header.end_zero = first + size;
+                    plan[offsets + buckets] = first + size;
+                    *(PlanHeader *)plan = header;
+                }
             }
-            for (uint32_t t = 0; t < its_tiles; ++t) {
-                uint32_t const from = first + t * header.tile_rows, to = from + header.tile_rows;
-                PlanTile const tile = {(int32_t)bucket, (int32_t)from, (int32_t)(to < first + size ? to : first + size), 0};
-                *(PlanTile *)(plan + tiles + (first_tile + t) * 4) = tile;
-            }
-            for (uint32_t at = first + size; at < first + its_rows; ++at) plan[order + at] = 0xFFFFFFFFu;
-            if (bucket == experts) header.tile_count = first_tile, header.zero_tiles = its_tiles, header.first_zero = first, header.end_zero = first + size, plan[offsets + buckets] = first + size;
         }
         __syncthreads();
     }
-    if ((experts & (64 * kPlanWaves - 1)) == thread) *(PlanHeader *)plan = header; // (the thread that had the last bucket)
-    for (uint32_t base = begin; base < end; base += 64) {
-        uint32_t const at = base + lane;
-        bool const active = at < end;
-        uint32_t const e = active ? (uint32_t)chosen[at] : 0, bucket = e < experts ? e : experts;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+        uint32_t const at = begin + i * 64 + lane, bucket = mine[i];
+        if (begin + i * 64 >= slots) break;
+        bool const active = at < slots;
         uint64_t const same = same_bucket(bucket, bits, active);
         uint32_t const rank = (uint32_t)__popcll(same & ((1ull << lane) - 1));
         if (active) {
@@ -389,9 +429,20 @@ int nk_amd_experts_plan_async(nk_i32_t const *chosen, nk_size_t slots, nk_size_t
     PlanHeader const header = {kPlanMagic, (uint32_t)slots, (uint32_t)experts, g.tile_rows, 0, 0, 0, 0};
     int bits = 0;
     while (experts >> bits) ++bits;
-    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(64 * kPlanWaves), (uint32_t)((experts + 1) * kPlanWaves * 4), (hipStream_t)stream,
-                       chosen, (uint32_t)slots, (uint32_t)experts, header, (uint32_t)g.offsets, (uint32_t)g.order, (uint32_t)g.place,
-                       (uint32_t)g.tiles, bits, (uint32_t *)plan);
+    auto const launch = [&](auto batch) {
+        constexpr int BATCH = decltype(batch)::value;
+        uint32_t const blocks = (uint32_t)((slots + BATCH * kPlanThreads - 1) / (BATCH * kPlanThreads)), lds = (uint32_t)((experts + 1) * 4);
+        uint32_t *const table = blocks > 1 ? (uint32_t *)plan + g.table : nullptr;
+        if (table) hipLaunchKernelGGL(plan_count_kernel<BATCH>, dim3(blocks), dim3(kPlanThreads), lds, (hipStream_t)stream, chosen, (uint32_t)slots, (uint32_t)experts, table);
+        hipLaunchKernelGGL(plan_kernel<BATCH>, dim3(blocks ? blocks : 1), dim3(kPlanThreads), lds * kPlanWaves, (hipStream_t)stream,
+                           chosen, (uint32_t)slots, (uint32_t)experts, header, (uint32_t)g.offsets, (uint32_t)g.order, (uint32_t)g.place,
+                           (uint32_t)g.tiles, bits, table, (uint32_t *)plan);
+    };
+    // one workgroup while its lanes hold all slots, four each at the most; then a launch that counts comes first (eight each:
+    // 4,004 slots took 12 us, 32,768 15.5 us; four: 9.3 and 12.5)
+    static_assert(kPlanBlockSlots == 4 * kPlanThreads, "what plan_geometry leaves room for");
+    if (slots <= kPlanThreads) launch(Number<1>());
+    else launch(Number<4>());
     hipError_t const e = hipGetLastError();
     return e == hipSuccess ? 0 : mx_fail(e, "plan_kernel");
 }

@@ -457,13 +457,13 @@ __global__ __launch_bounds__(256, FM >= 8 ? 1 : 2) void mx_gemm_kernel(MxArgs p)
 }
 
 /**
- *  The product for few rows: the stream of B is the work, so a workgroup takes 16 NT columns and its eight wavefronts a
- *  stretch of the depth each, B straight into registers, and their sums meet in LDS. In: the type of A's values, which
- *  the workgroup quantises into LDS itself (one launch, and A is read by all lanes), or `uint8_t`: A is staged already.
+ *  The product for few rows: the stream of B is the work, so a workgroup takes 16 NT columns and its wavefronts the supers of
+ *  the depth in turn, B straight into registers, and their sums meet in LDS. In: the type of A's values, which the workgroup
+ *  quantises into LDS itself (one launch, and A is read by all lanes), or `uint8_t`: A is staged already. B's first loads are
+ *  on their way while A is quantised.
  */
-constexpr int kFewWaves = 8;
-template <int FM, int NT, class In, class Out, bool GROUPED>
-__global__ __launch_bounds__(64 * kFewWaves) void mx_few_kernel(MxArgs p) {
+template <int WAVES, int FM, int NT, class In, class Out, bool GROUPED>
+__global__ __launch_bounds__(64 * WAVES, FM >= 4 ? 2 : 4) void mx_few_kernel(MxArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t few_lds[];
     constexpr bool FUSED = sizeof(In) != 1;
     uint32_t const tile_m = blockIdx.x / p.tiles_n, tile_n = blockIdx.x - tile_m * p.tiles_n;
@@ -474,20 +474,38 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx_few_kernel(MxArgs p) {
     RowTile const rows = row_tile_of(p, tile_m, FM * 16);
     uint32_t const lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     uint32_t const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    bool const good = image_matches(p);
+    bool const good = image_matches(p), computes = good && !(GROUPED && rows.matrix >= p.count) && p.steps;
     uint32_t const here = rows.last - rows.first;
+    uint32_t const row_bytes = p.supers * 4096, scale_row_bytes = p.supers * 256, lane16 = lane * 16, scale_lane = scale_word(r, g) * 4;
     v4f acc[FM][NT];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = v4f {0, 0, 0, 0};
 
+    uint64_t const of_all = (uint64_t)rows.matrix * p.tiles + tile_n * NT;
+    uint8_t const *const codes = p.image + kMxHeaderBytes;
+    __amdgpu_buffer_rsrc_t const w_from = buffer_of(codes + of_all * row_bytes);
+    __amdgpu_buffer_rsrc_t const w_scale_from = buffer_of(codes + (uint64_t)p.count * p.tiles * row_bytes + of_all * scale_row_bytes);
+    v4u w[4][NT];
+    uint32_t w_scale[NT];
+    auto load_w = [&](uint32_t super) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            uint32_t const s = super * 4 + u < p.steps ? super * 4 + u : p.steps - 1; // (what pads the last super is not fetched)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) w[u][j] = load_16(w_from, lane16, j * row_bytes + s * 1024);
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) w_scale[j] = load_4(w_scale_from, scale_lane, j * scale_row_bytes + super * 256);
+    };
+    if (computes && wave < p.supers) load_w(wave);
+
     uint32_t const lds_pitch = p.steps * 64 + 16; // (16 bytes on: rows start in different banks)
     uint8_t *lds_scales = few_lds + here * lds_pitch;
-    bool const computes = good && !(GROUPED && rows.matrix >= p.count) && p.steps;
     if (FUSED && computes) {
         uint32_t const pieces = p.steps * 16;
-        for (uint32_t index = threadIdx.x; index < here * pieces; index += 64 * kFewWaves) {
+        for (uint32_t index = threadIdx.x; index < here * pieces; index += 64 * WAVES) {
             uint32_t const row = index / pieces, piece = index - row * pieces;
             uint32_t const at = rows.first + row, source = GROUPED ? p.plan[p.order + at] / p.a_share : at;
             float v[8];
@@ -500,50 +518,41 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx_few_kernel(MxArgs p) {
     }
     if (FUSED) __syncthreads();
     if (computes) {
-        uint32_t const begin = (uint32_t)((uint64_t)wave * p.steps / kFewWaves), end = (uint32_t)((uint64_t)(wave + 1) * p.steps / kFewWaves);
-        uint64_t const of_all = (uint64_t)rows.matrix * p.tiles + tile_n * NT, row_bytes = (uint64_t)p.supers * 4096, scale_row_bytes = (uint64_t)p.supers * 256;
-        uint32_t const scale_lane = scale_word(r, g) * 4;
-        uint8_t const *w_from = p.image + kMxHeaderBytes + of_all * row_bytes + lane * 16;
-        uint8_t const *w_scale_from = p.image + kMxHeaderBytes + (uint64_t)p.count * p.tiles * row_bytes + of_all * scale_row_bytes + scale_lane;
-        uint8_t const *a_from[FM], *a_scale_from[FM];
-        bool there[FM];
+        uint32_t const fragment = rows.first / 16;
+        __amdgpu_buffer_rsrc_t const a_from = buffer_of(p.a + (uint64_t)fragment * row_bytes), a_scale_from = buffer_of(p.a_scales + (uint64_t)fragment * scale_row_bytes);
+        for (uint32_t super = wave; super < p.supers; super += WAVES) {
+            if (super != wave) load_w(super);
+            v4u a[4][FM];
+            uint32_t a_scale[FM];
+            if constexpr (!FUSED) {
 #pragma unroll
-        for (int i = 0; i < FM; ++i) {
-            there[i] = i * 16 + r < here;
-            uint32_t const row = there[i] ? i * 16 + r : 0;
-            if constexpr (FUSED) a_from[i] = few_lds + row * lds_pitch + g * 16, a_scale_from[i] = lds_scales + row * (p.steps * 4) + g;
-            else a_from[i] = p.a + (rows.first / 16 + i) * row_bytes + lane * 16, a_scale_from[i] = p.a_scales + (rows.first / 16 + i) * scale_row_bytes + scale_lane;
-        }
-        constexpr int kBatch = 4;
-        for (uint32_t base = begin; base < end; base += kBatch) {
-            v4u w[kBatch][NT], a[kBatch][FM];
-            uint32_t w_scale[kBatch][NT], a_scale[kBatch][FM];
+                for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                uint32_t const s = base + u < end ? base + u : end - 1;
+                    for (int i = 0; i < FM; ++i) a[u][i] = load_16(a_from, lane16, i * row_bytes + (super * 4 + u) * 1024);
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    w[u][j] = *(v4u const *)(w_from + j * row_bytes + (uint64_t)s * 1024);
-                    w_scale[u][j] = *(uint32_t const *)(w_scale_from + j * scale_row_bytes + (s >> 2) * 256) >> 8 * (s & 3);
-                }
-#pragma unroll
-                for (int i = 0; i < FM; ++i) {
-                    a[u][i] = *(v4u const *)(a_from[i] + (uint64_t)s * (FUSED ? 64 : 1024));
-                    if constexpr (FUSED) a_scale[u][i] = a_scale_from[i][s * 4];
-                    else a_scale[u][i] = *(uint32_t const *)(a_scale_from[i] + (s >> 2) * 256) >> 8 * (s & 3);
-                }
+                for (int i = 0; i < FM; ++i) a_scale[i] = load_4(a_scale_from, scale_lane, i * scale_row_bytes + super * 256);
             }
+            auto step_of = [&](auto byte) __attribute__((always_inline)) {
+                constexpr int U = decltype(byte)::value;
+                uint32_t const s = super * 4 + U;
+                if (s >= p.steps) return;
+                if constexpr (FUSED) {
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                if (base + u >= end) break;
-#pragma unroll
-                for (int i = 0; i < FM; ++i) {
-                    v4u const rows_of_a = there[i] ? a[u][i] : v4u {0, 0, 0, 0};
-                    uint32_t const scale_of_a = there[i] ? a_scale[u][i] : 0;
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j] = mx_multiply<0>(w[u][j], rows_of_a, acc[i][j], w_scale[u][j], scale_of_a);
+                    for (int i = 0; i < FM; ++i) {
+                        bool const there = i * 16 + r < here;
+                        uint32_t const row = there ? i * 16 + r : 0;
+                        v4u const codes_of_a = *(v4u const *)(few_lds + row * lds_pitch + s * 64 + g * 16);
+                        uint32_t const scale_of_a = lds_scales[row * (p.steps * 4) + s * 4 + g];
+                        a[U][i] = there ? codes_of_a : v4u {0, 0, 0, 0};
+                        a_scale[i] = there ? scale_of_a << 8 * U : 0u;
+                    }
                 }
-            }
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[i][j] = mx_multiply<U>(w[U][j], a[U][i], acc[i][j], w_scale[j], a_scale[i]);
+            };
+            step_of(Number<0>()), step_of(Number<1>()), step_of(Number<2>()), step_of(Number<3>());
         }
     }
     if (FUSED) __syncthreads(); // (the sums go where A was)
@@ -554,13 +563,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx_few_kernel(MxArgs p) {
         for (int j = 0; j < NT; ++j) sums[(wave * FM * NT + i * NT + j) * 64 + lane] = acc[i][j];
     __syncthreads();
     float const poison = __uint_as_float(0x7FC00000u);
-    for (uint32_t index = threadIdx.x; index < FM * NT * 64; index += 64 * kFewWaves) {
+    for (uint32_t index = threadIdx.x; index < FM * NT * 64; index += 64 * WAVES) {
         uint32_t const of_lane = index & 63, fragment = index >> 6, i = fragment / NT, j = fragment % NT;
         uint32_t const local = i * 16 + (of_lane & 15);
         if (local >= here) continue;
         v4f sum = sums[index];
 #pragma unroll
-        for (int w = 1; w < kFewWaves; ++w) sum += sums[w * FM * NT * 64 + index];
+        for (int w = 1; w < WAVES; ++w) sum += sums[w * FM * NT * 64 + index];
         uint32_t const at = rows.first + local, row = GROUPED && !p.sorted ? p.plan[p.order + at] : at;
         uint32_t const tile = tile_n * NT + j, column = (tile >> 2) * 64 + (of_lane >> 4) * 16 + (tile & 3) * 4;
         if (column >= p.n) continue;
@@ -664,16 +673,20 @@ constexpr uint32_t kFusedBytes = 64 * 1024;
 uint32_t fused_bytes(uint32_t rows, MxGeometry const &g) { return rows * (g.steps * 64 + 16) + rows * g.steps * 4; }
 bool fuses(uint64_t rows, MxGeometry const &g) { return rows <= 16 && (uint64_t)rows * (g.steps * 68 + 16) <= kFusedBytes; }
 
-template <int FM, int NT, class In, class Out, bool GROUPED>
-int launch_few(MxArgs &p, uint32_t max_rows, MxGeometry const &g, hipStream_t stream) {
+template <int WAVES, int FM, int NT, class In, class Out, bool GROUPED>
+int launch_few_of(MxArgs &p, uint32_t max_rows, MxGeometry const &g, hipStream_t stream) {
     p.tiles_n = (p.tiles + NT - 1) / NT;
     uint64_t const grid = (uint64_t)p.tiles_m * p.tiles_n;
     if (grid > 0x7FFFFFFFull) return mx_fail("mx product: too many tiles");
-    uint32_t lds = kFewWaves * FM * NT * 1024;
+    uint32_t lds = WAVES * FM * NT * 1024;
     if (sizeof(In) != 1 && fused_bytes(max_rows, g) > lds) lds = fused_bytes(max_rows, g);
-    hipLaunchKernelGGL((mx_few_kernel<FM, NT, In, Out, GROUPED>), dim3((uint32_t)grid), dim3(64 * kFewWaves), lds, stream, p);
+    hipLaunchKernelGGL((mx_few_kernel<WAVES, FM, NT, In, Out, GROUPED>), dim3((uint32_t)grid), dim3(64 * WAVES), lds, stream, p);
     hipError_t const e = hipGetLastError();
     return e == hipSuccess ? 0 : mx_fail(e, "mx_few_kernel");
+}
+template <int FM, int NT, class In, class Out, bool GROUPED>
+int launch_few(MxArgs &p, uint32_t max_rows, MxGeometry const &g, hipStream_t stream) {
+    return g.steps < 32 ? launch_few_of<4, FM, NT, In, Out, GROUPED>(p, max_rows, g, stream) : launch_few_of<8, FM, NT, In, Out, GROUPED>(p, max_rows, g, stream);
 }
 template <int FM, class Out, bool GROUPED>
 int launch_gemm(MxArgs &p, hipStream_t stream) {

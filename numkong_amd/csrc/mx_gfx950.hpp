@@ -88,13 +88,14 @@ struct PlanTile {
 };
 struct PlanGeometry {
     uint32_t tile_rows, max_tiles, max_rows;
-    size_t offsets, order, place, tiles, total_words; // in words
+    size_t offsets, order, place, tiles, table, total_words; // in words
 };
 /** Rows of a tile: what an expert has on average decides which kernel will run, and with it how its rows are cut. */
 inline uint32_t plan_tile_rows(size_t slots, size_t experts) {
     size_t const mean = experts ? slots / experts : 0;
     return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 256 ? 128 : 256;
 }
+constexpr size_t kPlanBlockSlots = 1024; // slots of a workgroup that makes the plan; its counts stand behind the tiles
 constexpr size_t kMaxExperts = 1024, kMaxTopK = 64, kMaxGroups = 64;
 inline bool plan_geometry(size_t slots, size_t experts, PlanGeometry &g) {
     if (!experts || experts > kMaxExperts || slots >= (1ull << 30)) return false;
@@ -106,7 +107,8 @@ inline bool plan_geometry(size_t slots, size_t experts, PlanGeometry &g) {
     g.order = g.offsets + ((experts + 2 + 3) & ~(size_t)3);
     g.place = g.order + g.max_rows;
     g.tiles = (g.place + slots + 3) & ~(size_t)3;
-    g.total_words = g.tiles + (size_t)g.max_tiles * 4;
+    g.table = g.tiles + (size_t)g.max_tiles * 4;
+    g.total_words = g.table + (slots + kPlanBlockSlots - 1) / kPlanBlockSlots * (experts + 1);
     return true;
 }
 
@@ -225,12 +227,19 @@ __device__ __forceinline__ void fetch_16(__amdgpu_buffer_rsrc_t buffer, void *ds
 #endif
 }
 
-/** 16 or 8 bytes per lane at `lane_offset` + `offset` (the same in all lanes) of a buffer. */
+/** 16, 4 or 8 bytes per lane at `lane_offset` + `offset` (the same in all lanes) of a buffer. */
 __device__ __forceinline__ v4u load_16(__amdgpu_buffer_rsrc_t buffer, uint32_t lane_offset, uint32_t offset) {
 #ifdef NK_MX_DEVICE_BUILTINS
     return __builtin_amdgcn_raw_buffer_load_b128(buffer, (int)lane_offset, (int)offset, 0);
 #else
     return v4u {0, 0, 0, 0};
+#endif
+}
+__device__ __forceinline__ uint32_t load_4(__amdgpu_buffer_rsrc_t buffer, uint32_t lane_offset, uint32_t offset) {
+#ifdef NK_MX_DEVICE_BUILTINS
+    return __builtin_amdgcn_raw_buffer_load_b32(buffer, (int)lane_offset, (int)offset, 0);
+#else
+    return 0;
 #endif
 }
 __device__ __forceinline__ v2u load_8(__amdgpu_buffer_rsrc_t buffer, uint32_t lane_offset, uint32_t offset) {

@@ -208,7 +208,7 @@ def test_plan(tokens, top_k, experts, kind):
         place[slots] = starts[e] + np.arange(counts[e]) if e < experts else -1
     np.testing.assert_array_equal(words[first:first + len(order)], order)
     np.testing.assert_array_equal(words[first + room:first + room + len(flat)], place)
-    tiles = words[(first + room + len(flat) + 3) // 4 * 4:].reshape(-1, 4)[:tile_count + zero_tiles]
+    tiles = words[(first + room + len(flat) + 3) // 4 * 4:][:4 * (tile_count + zero_tiles)].reshape(-1, 4)
     want = [(e, starts[e] + row, min(starts[e] + row + tile_rows, starts[e] + counts[e]))
             for e in range(experts + 1) for row in range(0, counts[e], tile_rows)]
     np.testing.assert_array_equal(tiles[:, :3], np.array(want).reshape(-1, 3))
