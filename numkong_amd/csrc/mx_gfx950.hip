@@ -466,8 +466,14 @@ template <int WAVES, int FM, int NT, class In, class Out, bool GROUPED>
 __global__ __launch_bounds__(64 * WAVES, FM >= 4 ? 2 : 4) void mx_few_kernel(MxArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t few_lds[];
     constexpr bool FUSED = sizeof(In) != 1;
-    uint32_t const tile_m = blockIdx.x / p.tiles_n, tile_n = blockIdx.x - tile_m * p.tiles_n;
-    if (GROUPED) {
+    uint32_t tile_m, tile_n;
+    if (!GROUPED) { // the tiles of rows of the same columns on one die, one after the other: it reads them once
+        uint32_t const index = blockIdx.x >> 3, column = index / p.tiles_m;
+        tile_m = index - column * p.tiles_m, tile_n = column * 8 + (blockIdx.x & 7);
+        if (tile_n >= p.tiles_n) return;
+    }
+    else {
+        tile_m = blockIdx.x / p.tiles_n, tile_n = blockIdx.x - tile_m * p.tiles_n;
         PlanHeader const &h = *(PlanHeader const *)p.plan;
         if (tile_m >= h.tile_count + (p.sorted ? 0 : h.zero_tiles)) return;
     }
@@ -668,15 +674,22 @@ int stage(int a_dtype, void const *a, uint64_t a_stride, void const *a_scales, u
     return e == hipSuccess ? 0 : mx_fail(e, "stage_kernel");
 }
 
-/** Can products of few rows quantise A themselves? What a workgroup holds of it has to fit, and to stay small. */
-constexpr uint32_t kFusedBytes = 64 * 1024;
+/**
+ *  Do products of few rows quantise A themselves? Every workgroup then does it for all columns that it has, and no launch goes
+ *  before: 1 x 8192 against 8192 columns takes 9.1 us so, 8 x 8192 16.1 us, and 10.9 us where a launch stages A first; 4 x 4096 against 4096 columns 4.7 us so.
+ *  `values`: of A, as many as a workgroup is expected to have; `rows`: the most that it may have, which have to fit.
+ */
+constexpr uint32_t kFusedBytes = 64 * 1024, kFusedValues = 16 * 1024;
 uint32_t fused_bytes(uint32_t rows, MxGeometry const &g) { return rows * (g.steps * 64 + 16) + rows * g.steps * 4; }
-bool fuses(uint64_t rows, MxGeometry const &g) { return rows <= 16 && (uint64_t)rows * (g.steps * 68 + 16) <= kFusedBytes; }
+bool fuses(uint64_t rows, uint64_t values, MxGeometry const &g) {
+    return rows <= 16 && values <= kFusedValues && (uint64_t)rows * (g.steps * 68 + 16) <= kFusedBytes;
+}
 
 template <int WAVES, int FM, int NT, class In, class Out, bool GROUPED>
 int launch_few_of(MxArgs &p, uint32_t max_rows, MxGeometry const &g, hipStream_t stream) {
     p.tiles_n = (p.tiles + NT - 1) / NT;
-    uint64_t const grid = (uint64_t)p.tiles_m * p.tiles_n;
+    if (!GROUPED) p.tiles_m = (p.m + 16 * FM - 1) / (16 * FM);
+    uint64_t const grid = (uint64_t)p.tiles_m * (GROUPED ? p.tiles_n : (p.tiles_n + 7) / 8 * 8);
     if (grid > 0x7FFFFFFFull) return mx_fail("mx product: too many tiles");
     uint32_t lds = WAVES * FM * NT * 1024;
     if (sizeof(In) != 1 && fused_bytes(max_rows, g) > lds) lds = fused_bytes(max_rows, g);
@@ -701,21 +714,28 @@ int launch_gemm(MxArgs &p, hipStream_t stream) {
     return e == hipSuccess ? 0 : mx_fail(e, "mx_gemm_kernel");
 }
 
-/** Which kernel: by the rows of a tile (the plan's where there is one). */
+/**
+ *  Which kernel. With experts, the rows of a tile decide (plan_tile_rows). Otherwise products of fewer than 64 tiles of 128 x 256
+ *  are of few rows, in tiles of up to 64: those tiles would each take as long as it takes to walk the depth, with most of the
+ *  compute units idle (us, few rows against many: 128 x 8192 x 8192 19.1 and 27.1, 512 x 2048 x 2048 10.6 and 12.5, 1024 x 1024 x
+ *  8192 23.1 and 30.8; at 64 tiles 256 x 8192 x 8192 29.9 and 28.5, 1024 x 2048 x 2048 15.4 and 13.9). A workgroup of few rows
+ *  takes one tile of columns while there are fewer than 512 (64 x 2048 x 2048 7.0 us with one, 7.5 with two; 64 x 8192 x 8192
+ *  17.0 and 15.0). Tiles of 256 rows from 256 of them on: less of B is read for the same work, the compute units are full.
+ */
 template <class Out, bool GROUPED>
-int launch_product(MxArgs &p, uint32_t rows, int a_dtype, bool fused, uint32_t fused_rows, MxGeometry const &g, hipStream_t stream) {
+int launch_product(MxArgs &p, uint32_t tile_rows, int a_dtype, bool fused, uint32_t fused_rows, MxGeometry const &g, hipStream_t stream) {
+    auto const tiles_of = [&](uint64_t rows, uint64_t columns) { return (p.m + rows - 1) / rows * ((p.n + columns - 1) / columns); };
+    uint32_t const rows = GROUPED ? tile_rows : p.m <= 32 || tiles_of(128, 256) < 64 ? (p.m < 64 ? p.m : 64) : tiles_of(256, 256) < 256 ? 128 : 256;
     if (rows <= 16) {
-        if (!GROUPED) p.tiles_m = 1;
-        if (!fused) return launch_few<1, 2, uint8_t, Out, GROUPED>(p, rows, g, stream);
-        return with_type(a_dtype, [&](auto value) { return launch_few<1, 2, decltype(value), Out, GROUPED>(p, fused_rows, g, stream); });
+        if (!fused) return launch_few<1, 1, uint8_t, Out, GROUPED>(p, rows, g, stream);
+        return with_type(a_dtype, [&](auto value) { return launch_few<1, 1, decltype(value), Out, GROUPED>(p, fused_rows, g, stream); });
     }
     if (rows <= 64) {
-        if (!GROUPED) p.tiles_m = 1;
-        if (rows <= 32) return launch_few<2, 2, uint8_t, Out, GROUPED>(p, rows, g, stream);
-        return launch_few<4, 2, uint8_t, Out, GROUPED>(p, rows, g, stream);
+        bool const narrow = p.tiles * (GROUPED ? (uint64_t)p.tiles_m : tiles_of(64, p.n)) < 512;
+        if (rows <= 32) return narrow ? launch_few<2, 1, uint8_t, Out, GROUPED>(p, rows, g, stream) : launch_few<2, 2, uint8_t, Out, GROUPED>(p, rows, g, stream);
+        return narrow ? launch_few<4, 1, uint8_t, Out, GROUPED>(p, rows, g, stream) : launch_few<4, 2, uint8_t, Out, GROUPED>(p, rows, g, stream);
     }
-    if (GROUPED ? rows <= 128 : (uint64_t)((p.m + 255) / 256) * ((p.n + 255) / 256) < 256) return launch_gemm<4, Out, GROUPED>(p, stream);
-    return launch_gemm<8, Out, GROUPED>(p, stream);
+    return rows <= 128 ? launch_gemm<4, Out, GROUPED>(p, stream) : launch_gemm<8, Out, GROUPED>(p, stream);
 }
 
 int check_a(int a_dtype, void const *a, void const *a_scales, uint64_t a_stride) {
@@ -739,9 +759,10 @@ struct ExpertsLayout {
     int sums_dtype;
     bool fused;
 };
-ExpertsLayout experts_layout(PlanGeometry const &shape, uint64_t n, MxGeometry const &g, bool a_is_codes, int c_dtype, bool weighted) {
+ExpertsLayout experts_layout(PlanGeometry const &shape, uint64_t slots, uint64_t experts, uint64_t n, uint64_t k, MxGeometry const &g,
+                             bool a_is_codes, int c_dtype, bool weighted) {
     ExpertsLayout l = {};
-    l.fused = !a_is_codes && shape.tile_rows == 16 && fuses(16, g);
+    l.fused = !a_is_codes && shape.tile_rows == 16 && fuses(16, (slots / experts + 1) * k, g);
     if (!l.fused) l.staged = staging_of(shape.max_rows, g);
     l.sums_at = l.staged.bytes;
     // rows that are still to be summed by weight: as wide as the result where that is bf16 (each is rounded once more, by at
@@ -829,7 +850,7 @@ int nk_amd_mx_pack_async(void const *codes, nk_size_t codes_stride, nk_size_t co
 nk_size_t nk_amd_mx_dots_workspace_size(nk_size_t height, nk_size_t width, nk_size_t depth, int a_is_codes) {
     MxGeometry g;
     if (!height || !width || height >= (1ull << 31) || !mx_geometry(1, width, depth, g)) return 0;
-    return !a_is_codes && fuses(height, g) ? 0 : staging_of(height, g).bytes;
+    return !a_is_codes && fuses(height, height * depth, g) ? 0 : staging_of(height, g).bytes;
 }
 
 int nk_amd_mx_dots_packed_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_stride, void const *a_scales,
@@ -843,7 +864,7 @@ int nk_amd_mx_dots_packed_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_s
     if (int const status = depth ? check_a(a_dtype, a, a_scales, a_stride) : 0) return status;
     if (int const status = check_c(c_dtype, c, c_stride)) return status;
     if (!packed || ((uintptr_t)packed & 15)) return mx_fail("mx_dots_packed: the image has to be 16-byte aligned");
-    bool const fused = !a_scales && fuses(height, g);
+    bool const fused = !a_scales && fuses(height, height * depth, g);
     MxArgs p = {};
     p.image = (uint8_t const *)packed, p.c = (uint8_t *)c, p.c_stride = c_stride;
     p.m = (uint32_t)height, p.n = (uint32_t)width, p.k = (uint32_t)depth, p.count = 1, p.a_share = 1;
@@ -858,8 +879,7 @@ int nk_amd_mx_dots_packed_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_s
         p.a = (uint8_t const *)workspace, p.a_scales = p.a + s.scales_at;
     }
     return with_type(c_dtype, [&](auto value) {
-        uint32_t const rows = height > 256 ? 256 : (uint32_t)height;
-        return launch_product<decltype(value), false>(p, rows, a_dtype, fused, rows, g, stream);
+        return launch_product<decltype(value), false>(p, 0, a_dtype, fused, p.m, g, stream);
     });
 }
 
@@ -868,7 +888,7 @@ nk_size_t nk_amd_mx_experts_workspace_size(nk_size_t slots, nk_size_t a_share, n
     MxGeometry g;
     PlanGeometry shape;
     if (!slots || !a_share || !mx_geometry(experts, width, depth, g) || !plan_geometry(slots, experts, shape)) return 0;
-    return experts_layout(shape, width, g, a_is_codes != 0, c_dtype, weighted != 0).bytes;
+    return experts_layout(shape, slots, experts, width, depth, g, a_is_codes != 0, c_dtype, weighted != 0).bytes;
 }
 
 int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_stride, void const *a_scales,
@@ -885,7 +905,7 @@ int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_
     if (int const status = depth ? check_a(a_dtype, a, a_scales, a_stride) : 0) return status;
     if (int const status = check_c(c_dtype, c, c_stride)) return status;
     if (!packed || ((uintptr_t)packed & 15) || !plan || ((uintptr_t)plan & 15)) return mx_fail("mx_dots_experts: image and plan have to be 16-byte aligned");
-    ExpertsLayout const l = experts_layout(shape, width, g, a_scales != nullptr, c_dtype, weights != nullptr);
+    ExpertsLayout const l = experts_layout(shape, slots, experts, width, depth, g, a_scales != nullptr, c_dtype, weights != nullptr);
     if (l.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < l.bytes))
         return mx_fail("mx_dots_experts: the workspace is too small or not 256-byte aligned");
     MxArgs p = {};
