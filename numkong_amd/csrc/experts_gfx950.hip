@@ -11,22 +11,68 @@ namespace {
 
 // ---- reductions over a wavefront ----------------------------------------------------------------------------------
 
-template <class F>
-__device__ __forceinline__ float wave_reduce(float x, F &&join) {
-#pragma unroll
-    for (int step = 32; step; step >>= 1) x = join(x, __shfl_xor(x, step));
+/** The value of the lane that stands across: in pairs, fours, eights (within each the same already), sixteens and so on, for
+ *  reductions whose every lane gets the result. Moves within 16 lanes come with the instruction that uses them, others are
+ *  swaps of rows: a maximum over the wavefront costs six instructions (and six round trips to LDS by shuffles). */
+template <int STEP>
+__device__ __forceinline__ v2u swapped(uint32_t x) { // what the lower and the upper of two rows (halves) of lanes hold
+#ifdef NK_MX_DEVICE_BUILTINS
+    auto const both = STEP == 16 ? __builtin_amdgcn_permlane16_swap(x, x, false, false) : __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return v2u {both[0], both[1]};
+#else
+    return v2u {x, x};
+#endif
+}
+template <int STEP>
+__device__ __forceinline__ uint32_t across(uint32_t x) {
+#ifdef NK_MX_DEVICE_BUILTINS
+    if constexpr (STEP == 1) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xF, 0xF, true);       // lanes 1 0 3 2
+    else if constexpr (STEP == 2) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xF, 0xF, true);  // lanes 2 3 0 1
+    else if constexpr (STEP == 4) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xF, 0xF, true); // eights mirrored
+    else if constexpr (STEP == 8) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x140, 0xF, 0xF, true); // sixteens mirrored
+    else {
+        v2u const both = swapped<STEP>(x);
+        return threadIdx.x & STEP ? both[0] : both[1];
+    }
+#else
     return x;
+#endif
+}
+/** `join` of what two lanes that stand across hold, in both. */
+template <int STEP, class F>
+__device__ __forceinline__ uint32_t joined(uint32_t x, F &&join) {
+    if constexpr (STEP < 16) return join(x, across<STEP>(x));
+    else {
+        v2u const both = swapped<STEP>(x);
+        return join((uint32_t)both[0], (uint32_t)both[1]);
+    }
+}
+/** `join` over groups of `lanes` (a power of two) adjacent lanes. */
+template <class F>
+__device__ __forceinline__ void reduce_steps(uint32_t lanes, F &&join) {
+    if (lanes > 1) join(Number<1>());
+    if (lanes > 2) join(Number<2>());
+    if (lanes > 4) join(Number<4>());
+    if (lanes > 8) join(Number<8>());
+    if (lanes > 16) join(Number<16>());
+    if (lanes > 32) join(Number<32>());
 }
 __device__ __forceinline__ float wave_sum(float x) {
-    return wave_reduce(x, [](float a, float b) { return a + b; });
+    auto const sum = [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); };
+    uint32_t bits = __float_as_uint(x);
+    reduce_steps(64, [&](auto step) __attribute__((always_inline)) { bits = joined<decltype(step)::value>(bits, sum); });
+    return __uint_as_float(bits);
 }
+__device__ __forceinline__ float wave_max(float x) {
+    auto const most = [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); };
+    uint32_t bits = __float_as_uint(x);
+    reduce_steps(64, [&](auto step) __attribute__((always_inline)) { bits = joined<decltype(step)::value>(bits, most); });
+    return __uint_as_float(bits);
+}
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-#pragma unroll
-    for (int step = 32; step; step >>= 1) {
-        uint32_t const other = (uint32_t)__shfl_xor((int)x, step);
-        x = x > other ? x : other;
-    }
-    return x;
+    reduce_steps(64, [&](auto step) __attribute__((always_inline)) { x = joined<decltype(step)::value>(x, larger); });
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
 }
 
 /** Numbers in the order of unsigned integers: larger number, larger key; every NaN above them all, both zeros the same.
@@ -38,9 +84,20 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 constexpr uint32_t kMaskedKey = 0x007FFFFFu; // of -inf
 
+__device__ __forceinline__ float number_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); }
+
 /** What one lane holds of a row: experts lane * J ... lane * J + J - 1, -inf past the end. */
 template <class T, int J>
 __device__ __forceinline__ void load_row(T const *row, uint32_t lane, uint32_t experts, float (&l)[J]) {
+    if (lane * J + J <= experts) {
+        struct __attribute__((packed, aligned(sizeof(T)))) Several {
+            T x[J];
+        } several;
+        __builtin_memcpy(&several, row + lane * J, sizeof(several));
+#pragma unroll
+        for (int j = 0; j < J; ++j) l[j] = (float)several.x[j];
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         uint32_t const e = lane * J + j;
@@ -59,7 +116,7 @@ __device__ __forceinline__ void scores_of(float const (&l)[J], int sigmoid, floa
     float top = l[0];
 #pragma unroll
     for (int j = 1; j < J; ++j) top = fmaxf(top, l[j]);
-    top = wave_reduce(top, [](float a, float b) { return fmaxf(a, b); });
+    top = wave_max(top);
     float sum = 0;
 #pragma unroll
     for (int j = 0; j < J; ++j) s[j] = l[j] == -__builtin_inff() ? 0.0f : expf(l[j] - top), sum += s[j];
@@ -80,88 +137,113 @@ struct RouteArgs {
 
 /**
  *  A wavefront for a token: the row stays in registers, J experts a lane, adjacent ones, so that of equal keys the lowest
- *  lane's lowest is the lowest expert. A choice is a maximum over the wavefront and a ballot.
+ *  lane's lowest is the lowest expert. Each lane sorts its own; a choice is a maximum over the lanes' first, a ballot, and the
+ *  winner moves up. Nothing here waits for memory twice: what bounds it is the number of instructions (16,384 tokens of 256
+ *  experts, sigmoid, 4 of 8 groups, 8 chosen: 20 us, 46 us with shuffles and a search in every lane for every choice).
  */
 template <class T, int J>
 __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
-    uint32_t const lane = threadIdx.x & 63, token = blockIdx.x * 4 + (threadIdx.x >> 6);
+    __shared__ float score_of[4][64 * J];
+    uint32_t const lane = threadIdx.x & 63, wave = threadIdx.x >> 6, token = blockIdx.x * 4 + wave;
     if (token >= p.tokens) return;
     float l[J], s[J];
     load_row<T, J>((T const *)((uint8_t const *)p.logits + token * p.stride), lane, p.experts, l);
     scores_of<J>(l, p.how.sigmoid, s);
-    uint32_t key[J];
+    uint32_t key[J], expert[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         uint32_t const e = lane * J + j;
         bool const masked = l[j] == -__builtin_inff();
+        expert[j] = e, score_of[wave][e] = s[j];
         key[j] = e >= p.experts ? 0u : masked ? kMaskedKey : key_of(p.bias ? s[j] + p.bias[e] : l[j]);
     }
     if (p.how.groups > 1) {
-        uint32_t const groups = (uint32_t)p.how.groups, size = p.experts / groups;
-        uint32_t mine = 0; // the key of group `lane`
-        for (uint32_t group = 0; group < groups; ++group) {
-            uint32_t best = 0;
-            int at = 0;
+        uint32_t const groups = (uint32_t)p.how.groups, size = p.experts / groups, lanes = size / J;
+        bool const two = p.how.group_top == 2 && size > 1;
+        if (size % J == 0 && (lanes & (lanes - 1)) == 0) { // a group is some whole lanes, side by side
+            uint32_t first = key[0], second = 0;
+#pragma unroll
+            for (int j = 1; j < J; ++j) {
+                uint32_t const lesser = key[j] < first ? key[j] : first;
+                first = larger(first, key[j]), second = larger(second, lesser);
+            }
+            reduce_steps(lanes, [&](auto step) __attribute__((always_inline)) {
+                uint32_t const other = across<decltype(step)::value>(first), next = across<decltype(step)::value>(second);
+                uint32_t const lesser = other < first ? other : first;
+                first = larger(first, other), second = larger(larger(second, next), lesser);
+            });
+            uint32_t mine = lane >= groups * lanes ? 0 : two ? key_of(number_of(first) + number_of(second)) : first;
+            bool stays = false;
+            for (int i = 0; i < p.how.top_groups; ++i) {
+                uint32_t const best = wave_max(mine), which = (uint32_t)__builtin_ctzll(__ballot(mine == best));
+                if (lane / lanes == which / lanes) stays = true, mine = 0;
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+                if (!stays && lane * J + j < p.experts) key[j] = kMaskedKey;
+        }
+        else { // groups that start anywhere, one after the other
+            uint32_t mine = 0; // the key of group `lane`
+            for (uint32_t group = 0; group < groups; ++group) {
+                uint32_t best = 0;
+                int at = 0;
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+                    if (lane * J + j >= group * size && lane * J + j < (group + 1) * size && key[j] > best) best = key[j], at = j;
+                uint32_t const first = wave_max(best);
+                uint32_t group_key = first;
+                if (two) {
+                    uint64_t const holders = __ballot(best == first && first != 0);
+                    bool const winner = holders && lane == (uint32_t)__builtin_ctzll(holders);
+                    uint32_t next = 0;
+#pragma unroll
+                    for (int j = 0; j < J; ++j)
+                        if (lane * J + j >= group * size && lane * J + j < (group + 1) * size && !(winner && j == at)) next = larger(next, key[j]);
+                    group_key = key_of(number_of(first) + number_of(wave_max(next)));
+                }
+                if (lane == group) mine = group_key;
+            }
+            uint64_t stays = 0;
+            for (int i = 0; i < p.how.top_groups; ++i) {
+                uint32_t const best = wave_max(mine), which = (uint32_t)__builtin_ctzll(__ballot(mine == best));
+                stays |= 1ull << which;
+                if (lane == which) mine = 0;
+            }
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 uint32_t const e = lane * J + j;
-                bool const inside = e >= group * size && e < (group + 1) * size;
-                if (inside && key[j] > best) best = key[j], at = j;
+                if (e < p.experts && !(stays >> (e / size) & 1)) key[j] = kMaskedKey;
             }
-            uint32_t const first = wave_max(best);
-            uint32_t group_key = first;
-            if (p.how.group_top == 2 && size > 1) {
-                uint64_t const holders = __ballot(best == first && first != 0);
-                bool const winner = holders && lane == (uint32_t)__builtin_ctzll(holders);
-                uint32_t next = 0;
-#pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    uint32_t const e = lane * J + j;
-                    bool const inside = e >= group * size && e < (group + 1) * size && !(winner && j == at);
-                    if (inside && key[j] > next) next = key[j];
-                }
-                uint32_t const second = wave_max(next);
-                auto const number = [](uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); };
-                group_key = key_of(number(first) + number(second));
-            }
-            if (lane == group) mine = group_key;
-        }
-        uint64_t stays = 0;
-        for (int i = 0; i < p.how.top_groups; ++i) {
-            uint32_t const best = wave_max(mine);
-            uint32_t const which = (uint32_t)__builtin_ctzll(__ballot(mine == best));
-            stays |= 1ull << which;
-            if (lane == which) mine = 0;
-        }
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            uint32_t const e = lane * J + j;
-            if (e < p.experts && !(stays >> (e / size) & 1)) key[j] = kMaskedKey;
         }
     }
-    float weight = 0;
-    int32_t expert = -1;
+#pragma unroll
+    for (int end = J - 1; end > 0; --end) // largest first; equal ones stay as they stand, the lower expert before the higher
+#pragma unroll
+        for (int j = 0; j < end; ++j) {
+            bool const swaps = key[j + 1] > key[j];
+            uint32_t const k = key[j], e = expert[j];
+            key[j] = swaps ? key[j + 1] : k, expert[j] = swaps ? expert[j + 1] : e;
+            key[j + 1] = swaps ? k : key[j + 1], expert[j + 1] = swaps ? e : expert[j + 1];
+        }
+    int32_t chosen = -1;
     for (uint32_t i = 0; i < p.top_k; ++i) {
-        uint32_t best = key[0], score = __float_as_uint(s[0]);
-        int at = 0;
-#pragma unroll
-        for (int j = 1; j < J; ++j)
-            if (key[j] > best) best = key[j], at = j, score = __float_as_uint(s[j]);
-        uint32_t const top = wave_max(best);
+        uint32_t const top = wave_max(key[0]);
         if (top <= kMaskedKey) break; // the rest of the slots stay empty
-        uint32_t const which = (uint32_t)__builtin_ctzll(__ballot(best == top));
+        uint32_t const which = (uint32_t)__builtin_ctzll(__ballot(key[0] == top));
+        int32_t const its = __builtin_amdgcn_readlane((int)expert[0], (int)which);
+        if (lane == i) chosen = its;
+        bool const winner = lane == which;
 #pragma unroll
-        for (int j = 0; j < J; ++j)
-            if (lane == which && j == at) key[j] = 0;
-        float const its_score = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)score, (int)which));
-        int32_t const its_expert = (int32_t)which * J + __builtin_amdgcn_readlane(at, (int)which);
-        if (lane == i) weight = its_score, expert = its_expert;
+        for (int j = 0; j + 1 < J; ++j) key[j] = winner ? key[j + 1] : key[j], expert[j] = winner ? expert[j + 1] : expert[j];
+        if (winner) key[J - 1] = 0;
     }
+    __builtin_amdgcn_wave_barrier(); // (the wavefront's own scores, written above)
+    float weight = chosen < 0 ? 0.0f : score_of[wave][chosen];
     if (p.how.renormalize) weight /= wave_sum(weight) + 1e-20f;
     weight *= p.how.scale;
     if (lane < p.top_k) {
-        p.weights[(uint64_t)token * p.top_k + lane] = expert < 0 ? 0.0f : weight;
-        p.chosen[(uint64_t)token * p.top_k + lane] = expert;
+        p.weights[(uint64_t)token * p.top_k + lane] = chosen < 0 ? 0.0f : weight;
+        p.chosen[(uint64_t)token * p.top_k + lane] = chosen;
     }
 }
 

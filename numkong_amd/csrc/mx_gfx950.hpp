@@ -124,64 +124,57 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-/** Eight adjacent values as they lie in memory, 16-byte aligned, and as 32-bit floats. (Widening is exact, so whatever
- *  follows sees the values themselves; a kernel loads several before it widens the first.) */
+/** What a lane loads at once: 16 adjacent bytes of a row, four values of f32 and eight of bf16 and f16. */
 template <class T>
-struct Eight {
-    v4u words[sizeof(T) / 2];
-};
+constexpr int kEach = 16 / (int)sizeof(T);
+/** They as 32-bit floats. (Widening is exact, so whatever follows sees the values themselves; a kernel loads several times
+ *  before it widens the first.) */
 template <class T>
-__device__ __forceinline__ Eight<T> load_eight(T const *from) {
-    Eight<T> e;
+__device__ __forceinline__ void widen(v4u words, float (&v)[kEach<T>]) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) e.words[i] = ((v4u const *)from)[i];
-    return e;
-}
-template <class T>
-__device__ __forceinline__ void widen_eight(Eight<T> const &e, float (&v)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(e.words[i / 4][i % 4]);
-        else if constexpr (__is_same(T, __bf16)) v[i] = __uint_as_float(i % 2 ? e.words[0][i / 2] & 0xFFFF0000u : e.words[0][i / 2] << 16);
-        else v[i] = (float)__builtin_bit_cast(f16x2, (uint32_t)e.words[0][i / 2])[i % 2];
+    for (int i = 0; i < kEach<T>; ++i) {
+        if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(words[i]);
+        else if constexpr (__is_same(T, __bf16)) v[i] = __uint_as_float(i % 2 ? words[i / 2] & 0xFFFF0000u : words[i / 2] << 16);
+        else v[i] = (float)__builtin_bit_cast(f16x2, (uint32_t)words[i / 2])[i % 2];
     }
 }
-/** Eight values of a row from column `col` on, wherever they lie; zeros from column `k` on. */
+/** Values of a row from column `col` on, wherever they lie; zeros from column `k` on. */
 template <class T>
-__device__ __forceinline__ void load_some(T const *row, uint32_t col, uint32_t k, float (&v)[8]) {
+__device__ __forceinline__ void load_some(T const *row, uint32_t col, uint32_t k, float (&v)[kEach<T>]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < k ? (float)row[col + i] : 0.0f;
-}
-/** `wide`: rows start on 16-byte addresses. */
-template <class T>
-__device__ __forceinline__ void load_eight(T const *row, uint32_t col, uint32_t k, bool wide, float (&v)[8]) {
-    if (wide && col + 8 <= k) widen_eight(load_eight(row + col), v);
-    else load_some(row, col, k, v);
+    for (int i = 0; i < kEach<T>; ++i) v[i] = col + i < k ? (float)row[col + i] : 0.0f;
 }
 
-/** The largest of four adjacent lanes, in all four. */
-__device__ __forceinline__ uint32_t quad_max(uint32_t x) {
+/** The largest of the adjacent lanes that share a block, in all of them: four lanes, or eight of f32. */
+template <int LANES>
+__device__ __forceinline__ uint32_t block_max(uint32_t x) {
     uint32_t const y = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xF, 0xF, true); // lanes 1 0 3 2
     x = x > y ? x : y;
     uint32_t const z = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xF, 0xF, true); // lanes 2 3 0 1
-    return x > z ? x : z;
+    x = x > z ? x : z;
+    if (LANES == 8) {
+        uint32_t const w = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xF, 0xF, true); // eights mirrored
+        x = x > w ? x : w;
+    }
+    return x;
 }
 
 /**
- *  Eight values of a block of 32 that four adjacent lanes hold, to eight codes and the block's scale byte. The exponent
- *  field of the largest magnitude, less 2, is the scale: e2m1's largest exponent is 2. (Magnitudes are compared as integers;
- *  a NaN or an infinity has the largest exponent field and so decides for its block; subnormal blocks end at 2^-127.) The
- *  conversion divides by the scale, rounds to nearest even and saturates: measured equal to that definition on every bf16
- *  value and on f32 and f16 values of every size, at scales from 2^-127 to 2^127.
+ *  A lane's values of a block of 32 that adjacent lanes hold, to codes (four bits each, the first lowest) and the block's scale
+ *  byte. The exponent field of the largest magnitude, less 2, is the scale: e2m1's largest exponent is 2. (Magnitudes are
+ *  compared as integers; a NaN or an infinity has the largest exponent field and so decides for its block; subnormal blocks end
+ *  at 2^-127.) The conversion divides by the scale, rounds to nearest even and saturates: measured equal to that definition on
+ *  every bf16 value and on f32 and f16 values of every size, at scales from 2^-127 to 2^127.
  */
-__device__ __forceinline__ uint32_t quantize_eight(float const (&v)[8], uint32_t &scale) {
+template <int N>
+__device__ __forceinline__ uint32_t quantize_some(float const (&v)[N], uint32_t &scale) {
     uint32_t largest = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < N; ++i) {
         uint32_t const magnitude = __float_as_uint(v[i]) & 0x7FFFFFFFu;
         largest = largest > magnitude ? largest : magnitude;
     }
-    largest = quad_max(largest);
+    largest = block_max<32 / N>(largest);
     uint32_t const field = largest >> 23;
     scale = field == 255 ? 255 : field > 2 ? field - 2 : 0;
     float const power = __uint_as_float(scale ? scale << 23 : 0x00400000u);
@@ -189,8 +182,10 @@ __device__ __forceinline__ uint32_t quantize_eight(float const (&v)[8], uint32_t
 #ifdef NK_MX_DEVICE_BUILTINS
     codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[0], v[1], power, 0);
     codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[2], v[3], power, 1);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[4], v[5], power, 2);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[6], v[7], power, 3);
+    if constexpr (N == 8) {
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[4], v[5], power, 2);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[6], v[7], power, 3);
+    }
 #endif
     return field == 255 ? 0u : codes;
 }
