@@ -92,71 +92,81 @@ struct StageArgs {
     uint32_t rows, k, supers, order, a_share;
     bool wide;
 };
+/** The row of A that row `row` of the fragments is; false where there is none. */
+__device__ __forceinline__ bool source_of(StageArgs const &p, uint32_t row, uint64_t &source) {
+    source = row;
+    if (!p.plan) return row < p.rows;
+    uint32_t const slot = p.plan[p.order + row];
+    source = slot / p.a_share;
+    return (int32_t)slot >= 0;
+}
+
 /**
  *  A into fragments: a workgroup for 16 rows of a super, a wavefront for a step of it. Four lanes share a block, 16 lanes read
  *  the 128 values of a row side by side, four rows at a time, and the codes change places in LDS, so that the fragment is
  *  written in one piece as well. (A lane with a block to itself reads 64-byte pieces 16 bytes at a time: 8192 x 8192 bf16 took
- *  46 us so, and takes 37 us.) In: the type of A's values, or `uint8_t`: codes.
+ *  46 us so, and takes 37 us.)
  */
 template <class In>
 __global__ __launch_bounds__(256) void stage_kernel(StageArgs p) {
     __shared__ __attribute__((aligned(16))) uint32_t words[4][256];
     __shared__ __attribute__((aligned(4))) uint8_t bytes[256];
+    constexpr int kLoads = sizeof(In) / 2; // 16-byte loads of a lane's eight values
     uint32_t const tile = blockIdx.x / p.supers, super = blockIdx.x - tile * p.supers;
     uint32_t const lane = threadIdx.x & 63, u = threadIdx.x >> 6, piece = lane & 15, g = piece >> 2;
-    uint32_t const block = (super * 4 + u) * 4 + g;
+    uint32_t const block = (super * 4 + u) * 4 + g, col = block * 32 + (piece & 3) * 8;
     if (p.plan && tile * 16 >= ((PlanHeader const *)p.plan)->first_zero) return;
-    uint8_t const *from[4];
+    bool const whole = p.wide && col + 8 <= p.k;
+    In const *from[4];
     bool there[4];
+    v4u raw[4][kLoads];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        uint32_t const row = tile * 16 + t * 4 + (lane >> 4);
-        uint64_t source = row;
-        there[t] = row < p.rows && block * 32 < p.k;
-        if (p.plan) {
-            uint32_t const slot = p.plan[p.order + row];
-            there[t] = there[t] && (int32_t)slot >= 0, source = slot / p.a_share;
-        }
-        from[t] = (uint8_t const *)p.a + source * p.a_stride;
-        if (sizeof(In) == 1 && !(piece & 3)) {
-            v4u codes = {0, 0, 0, 0};
-            uint32_t scale = 0;
-            if (there[t]) codes = load_codes(from[t], block, p.k, p.wide), scale = p.scales[source * p.scales_stride + block];
-            uint32_t const r = t * 4 + (lane >> 4);
-            *(v4u *)(words[u] + (g * 16 + r) * 4) = codes;
-            bytes[scale_word(r, g) * 4 + u] = (uint8_t)scale;
-        }
+        uint64_t source;
+        there[t] = source_of(p, tile * 16 + t * 4 + (lane >> 4), source) && col < p.k;
+        from[t] = (In const *)((uint8_t const *)p.a + source * p.a_stride);
     }
-    if constexpr (sizeof(In) != 1) {
-        constexpr int kLoads = sizeof(In) / 2;
-        uint32_t const col = block * 32 + (piece & 3) * 8;
-        bool const whole = p.wide && col + 8 <= p.k;
-        v4u raw[4][kLoads];
-        if (whole)
+    if (whole)
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int i = 0; i < kLoads; ++i) raw[t][i] = ((v4u const *)((In const *)(there[t] ? from[t] : (uint8_t const *)p.a) + col))[i];
+            for (int i = 0; i < kLoads; ++i) raw[t][i] = ((v4u const *)((there[t] ? from[t] : (In const *)p.a) + col))[i];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (there[t])
+    for (int t = 0; t < 4; ++t) {
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (there[t])
 #pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    float part[kEach<In>];
-                    if (whole) widen<In>(raw[t][i], part);
-                    else load_some((In const *)from[t], col + i * kEach<In>, p.k, part);
+            for (int i = 0; i < kLoads; ++i) {
+                float part[kEach<In>];
+                if (whole) widen<In>(raw[t][i], part);
+                else load_some(from[t], col + i * kEach<In>, p.k, part);
 #pragma unroll
-                    for (int j = 0; j < kEach<In>; ++j) v[i * kEach<In> + j] = part[j];
-                }
-            uint32_t scale;
-            uint32_t const r = t * 4 + (lane >> 4), codes = quantize_some(v, scale);
-            words[u][(g * 16 + r) * 4 + (piece & 3)] = codes;
-            if (!(piece & 3)) bytes[scale_word(r, g) * 4 + u] = (uint8_t)scale;
-        }
+                for (int j = 0; j < kEach<In>; ++j) v[i * kEach<In> + j] = part[j];
+            }
+        uint32_t scale;
+        uint32_t const r = t * 4 + (lane >> 4), codes = quantize_some(v, scale);
+        words[u][(g * 16 + r) * 4 + (piece & 3)] = codes;
+        if (!(piece & 3)) bytes[scale_word(r, g) * 4 + u] = (uint8_t)scale;
     }
     __syncthreads();
     *(v4u *)(p.to + (((uint64_t)tile * p.supers + super) * 4 + u) * 1024 + lane * 16) = *(v4u const *)(words[u] + lane * 4);
+    if (threadIdx.x < 64) *(uint32_t *)(p.to_scales + ((uint64_t)tile * p.supers + super) * 256 + lane * 4) = *(uint32_t const *)(bytes + lane * 4);
+}
+
+/** The same from codes: a lane's 16 bytes of a row are its 16 bytes of the fragment. */
+__global__ __launch_bounds__(256) void stage_codes_kernel(StageArgs p) {
+    __shared__ __attribute__((aligned(4))) uint8_t bytes[256];
+    uint32_t const tile = blockIdx.x / p.supers, super = blockIdx.x - tile * p.supers;
+    uint32_t const lane = threadIdx.x & 63, u = threadIdx.x >> 6, r = lane & 15, g = lane >> 4, block = (super * 4 + u) * 4 + g;
+    if (p.plan && tile * 16 >= ((PlanHeader const *)p.plan)->first_zero) return;
+    uint64_t source;
+    v4u codes = {0, 0, 0, 0};
+    uint32_t scale = 0;
+    if (source_of(p, tile * 16 + r, source) && block * 32 < p.k)
+        codes = load_codes((uint8_t const *)p.a + source * p.a_stride, block, p.k, p.wide), scale = p.scales[source * p.scales_stride + block];
+    *(v4u *)(p.to + (((uint64_t)tile * p.supers + super) * 4 + u) * 1024 + lane * 16) = codes;
+    bytes[scale_word(r, g) * 4 + u] = (uint8_t)scale;
+    __syncthreads();
     if (threadIdx.x < 64) *(uint32_t *)(p.to_scales + ((uint64_t)tile * p.supers + super) * 256 + lane * 4) = *(uint32_t const *)(bytes + lane * 4);
 }
 
@@ -475,6 +485,8 @@ __global__ __launch_bounds__(256, FM >= 8 ? 1 : 2) void mx_gemm_kernel(MxArgs p)
         // two runs of 16 adjacent columns (2 x + g of the four in a group, x = 0, 1), four values from each of the group's four
         // tiles. 32 rows at a time they go through the wavefront's own part of LDS (16-byte pieces, piece c of row r at
         // c ^ (r & 7)), so that a row is stored in one piece: 128 or 256 adjacent bytes, whatever address it starts at.
+        // (Stores past the caches: 273 against 277 us for 8192^3, 116 against 85 where rows do not start on 128-byte lines; a choice
+        // between the two in the kernel costs what it brings.)
         uint8_t *const mine = results[wave];
         uint32_t const wave_column = now.tile_n * kColumns + wave * 64;
 #pragma unroll
@@ -752,7 +764,7 @@ int stage(int a_dtype, void const *a, uint64_t a_stride, void const *a_scales, u
     if (grid > 0x7FFFFFFFull) return mx_fail("mx product: A is too large");
     StageArgs const p = {a, a_stride, (uint8_t const *)a_scales, a_scales_stride, to, to + s.scales_at, (uint32_t const *)plan, rows, k,
                          g.supers, (uint32_t)order, a_share, aligned(a, a_stride, 16)};
-    if (a_scales) hipLaunchKernelGGL(stage_kernel<uint8_t>, dim3((uint32_t)grid), dim3(256), 0, stream, p);
+    if (a_scales) hipLaunchKernelGGL(stage_codes_kernel, dim3((uint32_t)grid), dim3(256), 0, stream, p);
     else
         with_type(a_dtype, [&](auto value) {
             hipLaunchKernelGGL(stage_kernel<decltype(value)>, dim3((uint32_t)grid), dim3(256), 0, stream, p);
@@ -824,7 +836,9 @@ int launch_product(MxArgs &p, uint32_t tile_rows, int a_dtype, bool fused, uint3
         if (rows <= 32) return narrow ? launch_few<2, 1, uint8_t, Out, GROUPED>(p, rows, g, stream) : launch_few<2, 2, uint8_t, Out, GROUPED>(p, rows, g, stream);
         return narrow ? launch_few<4, 1, uint8_t, Out, GROUPED>(p, rows, g, stream) : launch_few<4, 2, uint8_t, Out, GROUPED>(p, rows, g, stream);
     }
-    return rows <= 128 ? launch_gemm<4, Out, GROUPED>(p, stream) : launch_gemm<8, Out, GROUPED>(p, stream);
+    if constexpr (!GROUPED)
+        if (rows > 128) return launch_gemm<8, Out, GROUPED>(p, stream);
+    return launch_gemm<4, Out, GROUPED>(p, stream);
 }
 
 int check_a(int a_dtype, void const *a, void const *a_scales, uint64_t a_stride) {
@@ -844,16 +858,26 @@ int check_c(int c_dtype, void const *c, uint64_t c_stride) {
 /** Where the parts of the experts' workspace are. */
 struct ExpertsLayout {
     Staging staged;
+    uint64_t codes_at, codes_stride, codes_scales_at, codes_scales_stride; // A's rows as codes, where they are quantised first
     uint64_t sums_at, sums_values, bytes; // rows of the plan before they are summed: values a row
     int sums_dtype;
-    bool fused;
+    bool fused, quantised;
 };
-ExpertsLayout experts_layout(PlanGeometry const &shape, uint64_t slots, uint64_t experts, uint64_t n, uint64_t k, MxGeometry const &g,
-                             bool a_is_codes, int c_dtype, bool weighted) {
+ExpertsLayout experts_layout(PlanGeometry const &shape, uint64_t slots, uint64_t a_share, uint64_t experts, uint64_t n, uint64_t k,
+                             MxGeometry const &g, bool a_is_codes, int c_dtype, bool weighted) {
     ExpertsLayout l = {};
     l.fused = !a_is_codes && shape.tile_rows == 16 && fuses(16, (slots / experts + 1) * k, g);
     if (!l.fused) l.staged = staging_of(shape.max_rows, g);
-    l.sums_at = l.staged.bytes;
+    uint64_t at = l.staged.bytes;
+    // Rows that go to several experts are quantised once and gathered as codes, where that is worth a launch more (32,768 slots
+    // of 4,096 rows of 2048: 26 us as floats, 19 us so).
+    l.quantised = !l.fused && !a_is_codes && a_share > 1 && slots * k >= 1ull << 24;
+    if (l.quantised) {
+        l.codes_stride = (k / 2 + 15) / 16 * 16 + 16, l.codes_scales_stride = (k + 31) / 32;
+        l.codes_at = at, l.codes_scales_at = at + (slots / a_share + 1) * l.codes_stride;
+        at = (l.codes_scales_at + (slots / a_share + 1) * l.codes_scales_stride + 255) / 256 * 256;
+    }
+    l.sums_at = at;
     // rows that are still to be summed by weight: as wide as the result where that is bf16 (each is rounded once more, by at
     // most 2^-9 of itself, half of what the result's own rounding may do to it; at 32 bits they are most of the traffic),
     // 32 bits otherwise (f16 might overflow where the sum does not)
@@ -973,7 +997,7 @@ nk_size_t nk_amd_mx_experts_workspace_size(nk_size_t slots, nk_size_t a_share, n
     MxGeometry g;
     PlanGeometry shape;
     if (!slots || !a_share || !mx_geometry(experts, width, depth, g) || !plan_geometry(slots, experts, shape)) return 0;
-    return experts_layout(shape, slots, experts, width, depth, g, a_is_codes != 0, c_dtype, weighted != 0).bytes;
+    return experts_layout(shape, slots, a_share, experts, width, depth, g, a_is_codes != 0, c_dtype, weighted != 0).bytes;
 }
 
 int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_stride, void const *a_scales,
@@ -990,7 +1014,7 @@ int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_
     if (int const status = depth ? check_a(a_dtype, a, a_scales, a_stride) : 0) return status;
     if (int const status = check_c(c_dtype, c, c_stride)) return status;
     if (!packed || ((uintptr_t)packed & 15) || !plan || ((uintptr_t)plan & 15)) return mx_fail("mx_dots_experts: image and plan have to be 16-byte aligned");
-    ExpertsLayout const l = experts_layout(shape, slots, experts, width, depth, g, a_scales != nullptr, c_dtype, weights != nullptr);
+    ExpertsLayout const l = experts_layout(shape, slots, a_share, experts, width, depth, g, a_scales != nullptr, c_dtype, weights != nullptr);
     if (l.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < l.bytes))
         return mx_fail("mx_dots_experts: the workspace is too small or not 256-byte aligned");
     MxArgs p = {};
@@ -1000,6 +1024,12 @@ int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_
     p.tiles_m = shape.max_tiles, p.order = (uint32_t)shape.order, p.tile_list = (uint32_t)shape.tiles;
     if (l.fused) p.a = (uint8_t const *)a, p.a_pitch = a_stride, p.a_wide = aligned(a, a_stride, 16);
     else {
+        if (l.quantised) {
+            uint8_t *const codes = (uint8_t *)workspace + l.codes_at, *const scales = (uint8_t *)workspace + l.codes_scales_at;
+            if (int const status = launch_quantize(a_dtype, a, slots / a_share, depth, a_stride, codes, l.codes_stride, scales, l.codes_scales_stride, stream))
+                return status;
+            a = codes, a_stride = l.codes_stride, a_scales = scales, a_scales_stride = l.codes_scales_stride;
+        }
         if (int const status = stage(a_dtype, a, a_stride, a_scales, a_scales_stride, shape.max_rows, p.k, g, l.staged, (uint8_t *)workspace, plan, shape.order, p.a_share, stream))
             return status;
         p.a = (uint8_t const *)workspace, p.a_scales = p.a + l.staged.scales_at;

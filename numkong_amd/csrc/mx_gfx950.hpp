@@ -90,10 +90,11 @@ struct PlanGeometry {
     uint32_t tile_rows, max_tiles, max_rows;
     size_t offsets, order, place, tiles, table, total_words; // in words
 };
-/** Rows of a tile: what an expert has on average decides which kernel will run, and with it how its rows are cut. */
+/** Rows of a tile: what an expert has on average decides which kernel will run, and with it how its rows are cut. (Tiles of 256
+ *  rows: 117 us for 64 experts of 512 rows on average, against 104 us; more of the last tile of each expert is empty.) */
 inline uint32_t plan_tile_rows(size_t slots, size_t experts) {
     size_t const mean = experts ? slots / experts : 0;
-    return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 256 ? 128 : 256;
+    return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
 }
 constexpr size_t kPlanBlockSlots = 1024; // slots of a workgroup that makes the plan; its counts stand behind the tiles
 constexpr size_t kMaxExperts = 1024, kMaxTopK = 64, kMaxGroups = 64;

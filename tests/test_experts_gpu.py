@@ -251,6 +251,20 @@ def test_experts_products(tokens, top_k, experts, kind, n, k, dtype, out):
     mx.close(got, summed, magnitudes, k, extra)
 
 
+@pytest.mark.parametrize("tokens,top_k,experts,n,k", [(4200, 8, 16, 130, 513), (3000, 6, 40, 77, 1000)])
+def test_rows_that_go_to_many(tokens, top_k, experts, n, k):
+    """So many slots that the rows are quantised first and gathered as codes: the same values as one product for each expert."""
+    chosen = torch.from_numpy(routing(tokens, top_k, experts, "some", 3))
+    a, stack = normal(tokens, k, torch.bfloat16, 1, 0.2).to(DEV), normal(experts * n, k, torch.float32, 2, 0.2).reshape(experts, n, k).to(DEV)
+    got = nk.mx_dots_experts(a, nk.mx_pack(stack), nk.experts_plan(chosen.to(DEV), experts))
+    left, right = mx.rounded(a.cpu()), mx.rounded(stack.reshape(-1, k).cpu()).reshape(experts, n, k)
+    for e in range(experts):
+        token, slot = torch.nonzero(chosen == e, as_tuple=True)
+        truth, magnitude = left[token] @ right[e].T, np.abs(left[token]) @ np.abs(right[e]).T
+        mx.close(got[token, slot], truth, magnitude, k)
+    assert not got[((chosen < 0) | (chosen >= experts)).to(DEV)].any()
+
+
 def test_no_tokens():
     packed = nk.mx_pack(torch.ones((4, 64, 64), device=DEV))
     plan = nk.experts_plan(torch.zeros((0, 2), dtype=torch.int32, device=DEV), 4)

@@ -113,7 +113,7 @@ def product_of(a, b):
 
 SHAPES = [(1, 1, 1), (1, 17, 31), (2, 64, 32), (1, 256, 4096), (3, 65, 129), (15, 200, 512), (16, 130, 640), (17, 33, 127), (31, 100, 384),
           (32, 64, 1000), (33, 257, 96), (64, 192, 513), (65, 64, 128), (65, 300, 1), (129, 255, 500), (200, 131, 1024), (257, 129, 2100),
-          (300, 1000, 160), (1030, 520, 700)]
+          (300, 1000, 160), (1030, 520, 700), (1030, 2100, 700), (8200, 300, 260), (2050, 8200, 130), (2049, 8001, 641)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -129,10 +129,10 @@ def test_product(m, n, k):
         mx.close(nk.mx_dots_packed(nk.mx_quantize(a.to(DEV)), packed, out_dtype=out), truth, magnitude, k)
 
 
-@pytest.mark.parametrize("m", [1, 9, 40, 100, 300])
-def test_product_of_views(m):
+@pytest.mark.parametrize("m,n", [(1, 77), (9, 77), (40, 77), (100, 77), (300, 77), (1100, 2077), (2100, 8003)])
+def test_product_of_views(m, n):
     """Rows that start anywhere, a result inside a larger matrix, nothing beside it written."""
-    k, n = 333, 77
+    k = 333
     a, b = normal(m, k, torch.bfloat16, 1), normal(n, k, torch.bfloat16, 2)
     truth, magnitude = product_of(a, b)
     packed = nk.mx_pack(strided(b, 5, 1))
@@ -145,9 +145,9 @@ def test_product_of_views(m):
         assert bool((store == 77.0).all())
 
 
-@pytest.mark.parametrize("m", [1, 20, 70, 260])
-def test_special_values_stay_in_their_rows(m):
-    k, n = 200, 90
+@pytest.mark.parametrize("m,n", [(1, 90), (20, 90), (70, 90), (260, 90), (1100, 2100), (2100, 8200)])
+def test_special_values_stay_in_their_rows(m, n):
+    k = 200
     a, b = normal(m, k, torch.float32, 3), normal(n, k, torch.float32, 4)
     a[m // 2, 77], b[5, 199], b[60, 0] = float("inf"), float("nan"), -float("inf")
     a[0, 32:64] = 0  # a NaN of the other side meets zeros only
@@ -212,10 +212,10 @@ def test_host_operands():
     np.testing.assert_array_equal(nk.mx_dequantize(matrix), mx.rounded(a).astype(np.float32))
 
 
-@pytest.mark.parametrize("m", [4, 50, 300])
-def test_streams_and_replays(m):
+@pytest.mark.parametrize("m,n", [(4, 200), (50, 200), (300, 200), (1100, 2100), (2100, 8200)])
+def test_streams_and_replays(m, n):
     """Work follows the current stream; a captured call is replayed on new values, with eager work between."""
-    a, b = normal(m, 640, torch.bfloat16, 8).to(DEV), normal(200, 640, torch.bfloat16, 9).to(DEV)
+    a, b = normal(m, 640, torch.bfloat16, 8).to(DEV), normal(n, 640, torch.bfloat16, 9).to(DEV)
     packed = nk.mx_pack(b)
     eager = nk.mx_dots_packed(a, packed).clone()
     torch.cuda.synchronize()
