@@ -103,7 +103,7 @@ NK_DYNAMIC int nk_amd_experts_plan_async(nk_i32_t const *chosen, nk_size_t slots
  */
 NK_DYNAMIC nk_size_t nk_amd_mx_experts_workspace_size(nk_size_t slots, nk_size_t a_share, nk_size_t experts,
                                                       nk_size_t width, nk_size_t depth, int a_is_codes,
-                                                      nk_dtype_t c_dtype, int weighted);
+                                                      int weighted);
 NK_DYNAMIC int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_stride, void const *a_scales,
                                             nk_size_t a_scales_stride, nk_size_t a_share, void const *packed,
                                             void const *plan, nk_size_t slots, nk_size_t experts, nk_size_t top_k,

@@ -676,25 +676,32 @@ __global__ __launch_bounds__(64 * WAVES, FM >= 4 ? 2 : 4) void mx_few_kernel(MxA
     }
 }
 
-/** out[token] = sum over its slots of weight * row of the plan, slots without an expert left out; a thread for four columns. */
-template <class In, class Out>
-__global__ __launch_bounds__(256) void combine_kernel(In const *rows, uint64_t row_values, uint32_t const *plan, uint32_t place,
+/** out[token] = sum over its slots of weight * row of the plan, slots without an expert left out; a thread for four columns, four
+ *  rows under way at a time. */
+template <class Out>
+__global__ __launch_bounds__(256) void combine_kernel(float const *rows, uint64_t row_values, uint32_t const *plan, uint32_t place,
                                                       float const *weights, uint32_t top_k, uint32_t tokens, uint32_t n,
                                                       uint32_t pieces, Out *c, uint64_t c_stride) {
     uint32_t const index = blockIdx.x * 256 + threadIdx.x;
     uint32_t const token = index / pieces, column = (index - token * pieces) * 4;
     if (token >= tokens) return;
     float sum[4] = {0, 0, 0, 0};
-    for (uint32_t i = 0; i < top_k; ++i) {
-        uint32_t const slot = token * top_k + i;
-        int32_t const row = (int32_t)plan[place + slot];
-        if (row < 0) continue;
-        float const weight = weights[slot];
-        struct alignas(4 * sizeof(In)) Four {
-            In x[4];
-        } const four = *(Four const *)(rows + (uint64_t)row * row_values + column); // (rows are padded to whole fours)
+    for (uint32_t first = 0; first < top_k; first += 4) {
+        int32_t row[4];
+        float weight[4];
+        v4f values[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) sum[t] = __builtin_fmaf(weight, (float)four.x[t], sum[t]);
+        for (int i = 0; i < 4; ++i) {
+            uint32_t const slot = token * top_k + (first + i < top_k ? first + i : 0);
+            row[i] = first + i < top_k ? (int32_t)plan[place + slot] : -1, weight[i] = weights[slot];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) // (rows are padded to whole fours; row 0 is there, whatever it holds)
+            values[i] = *(v4f const *)(rows + (uint64_t)(row[i] < 0 ? 0 : row[i]) * row_values + column);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) sum[t] = row[i] < 0 ? sum[t] : __builtin_fmaf(weight[i], values[i][t], sum[t]);
     }
     store_some<Out, 4>((Out *)((uint8_t *)c + token * c_stride) + column, sum, n - column);
 }
@@ -860,11 +867,10 @@ struct ExpertsLayout {
     Staging staged;
     uint64_t codes_at, codes_stride, codes_scales_at, codes_scales_stride; // A's rows as codes, where they are quantised first
     uint64_t sums_at, sums_values, bytes; // rows of the plan before they are summed: values a row
-    int sums_dtype;
     bool fused, quantised;
 };
 ExpertsLayout experts_layout(PlanGeometry const &shape, uint64_t slots, uint64_t a_share, uint64_t experts, uint64_t n, uint64_t k,
-                             MxGeometry const &g, bool a_is_codes, int c_dtype, bool weighted) {
+                             MxGeometry const &g, bool a_is_codes, bool weighted) {
     ExpertsLayout l = {};
     l.fused = !a_is_codes && shape.tile_rows == 16 && fuses(16, (slots / experts + 1) * k, g);
     if (!l.fused) l.staged = staging_of(shape.max_rows, g);
@@ -878,12 +884,10 @@ ExpertsLayout experts_layout(PlanGeometry const &shape, uint64_t slots, uint64_t
         at = (l.codes_scales_at + (slots / a_share + 1) * l.codes_scales_stride + 255) / 256 * 256;
     }
     l.sums_at = at;
-    // rows that are still to be summed by weight: as wide as the result where that is bf16 (each is rounded once more, by at
-    // most 2^-9 of itself, half of what the result's own rounding may do to it; at 32 bits they are most of the traffic),
-    // 32 bits otherwise (f16 might overflow where the sum does not)
-    l.sums_dtype = c_dtype == nk_bf16_k ? nk_bf16_k : nk_f32_k;
+    // (rows that are still to be summed by weight stand in 32 bits, whatever the result has: rounded to 16 they would err as much
+    // again as the result's own rounding, and without bound against a sum that cancels)
     l.sums_values = (n + 15) / 16 * 16;
-    l.bytes = l.sums_at + (weighted ? (shape.max_rows * l.sums_values * element_bytes(l.sums_dtype) + 255) / 256 * 256 : 0);
+    l.bytes = l.sums_at + (weighted ? (shape.max_rows * l.sums_values * 4 + 255) / 256 * 256 : 0);
     return l;
 }
 
@@ -993,11 +997,11 @@ int nk_amd_mx_dots_packed_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_s
 }
 
 nk_size_t nk_amd_mx_experts_workspace_size(nk_size_t slots, nk_size_t a_share, nk_size_t experts, nk_size_t width,
-                                           nk_size_t depth, int a_is_codes, nk_dtype_t c_dtype, int weighted) {
+                                           nk_size_t depth, int a_is_codes, int weighted) {
     MxGeometry g;
     PlanGeometry shape;
     if (!slots || !a_share || !mx_geometry(experts, width, depth, g) || !plan_geometry(slots, experts, shape)) return 0;
-    return experts_layout(shape, slots, a_share, experts, width, depth, g, a_is_codes != 0, c_dtype, weighted != 0).bytes;
+    return experts_layout(shape, slots, a_share, experts, width, depth, g, a_is_codes != 0, weighted != 0).bytes;
 }
 
 int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_stride, void const *a_scales,
@@ -1014,7 +1018,7 @@ int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_
     if (int const status = depth ? check_a(a_dtype, a, a_scales, a_stride) : 0) return status;
     if (int const status = check_c(c_dtype, c, c_stride)) return status;
     if (!packed || ((uintptr_t)packed & 15) || !plan || ((uintptr_t)plan & 15)) return mx_fail("mx_dots_experts: image and plan have to be 16-byte aligned");
-    ExpertsLayout const l = experts_layout(shape, slots, a_share, experts, width, depth, g, a_scales != nullptr, c_dtype, weights != nullptr);
+    ExpertsLayout const l = experts_layout(shape, slots, a_share, experts, width, depth, g, a_scales != nullptr, weights != nullptr);
     if (l.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < l.bytes))
         return mx_fail("mx_dots_experts: the workspace is too small or not 256-byte aligned");
     MxArgs p = {};
@@ -1035,8 +1039,8 @@ int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_
         p.a = (uint8_t const *)workspace, p.a_scales = p.a + l.staged.scales_at;
     }
     uint8_t *sums = (uint8_t *)workspace + l.sums_at;
-    int const product_dtype = weights ? l.sums_dtype : (int)c_dtype;
-    if (weights) p.sorted = 1, p.c = sums, p.c_stride = l.sums_values * element_bytes(l.sums_dtype);
+    int const product_dtype = weights ? (int)nk_f32_k : (int)c_dtype;
+    if (weights) p.sorted = 1, p.c = sums, p.c_stride = l.sums_values * 4;
     else p.c = (uint8_t *)c, p.c_stride = c_stride;
     int const status = with_type(product_dtype, [&](auto value) {
         return launch_product<decltype(value), true>(p, shape.tile_rows, a_dtype, l.fused, 16, g, stream);
@@ -1047,16 +1051,14 @@ int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_
     for (uint64_t first = 0; first < tokens; first += slab) {
         uint64_t const here = tokens - first < slab ? tokens - first : slab;
         uint32_t const place = (uint32_t)(shape.place + first * top_k);
-        auto const combine = [&](auto in, auto out) {
-            typedef decltype(in) In;
-            typedef decltype(out) Out;
-            hipLaunchKernelGGL((combine_kernel<In, Out>), dim3((uint32_t)((here * pieces + 255) / 256)), dim3(256), 0, stream,
-                               (In const *)sums, l.sums_values, p.plan, place, weights + first * top_k, (uint32_t)top_k, (uint32_t)here,
+        int const done = with_type(c_dtype, [&](auto value) {
+            typedef decltype(value) Out;
+            hipLaunchKernelGGL((combine_kernel<Out>), dim3((uint32_t)((here * pieces + 255) / 256)), dim3(256), 0, stream,
+                               (float const *)sums, l.sums_values, p.plan, place, weights + first * top_k, (uint32_t)top_k, (uint32_t)here,
                                p.n, (uint32_t)pieces, (Out *)((uint8_t *)c + first * c_stride), (uint64_t)c_stride);
             hipError_t const e = hipGetLastError();
             return e == hipSuccess ? 0 : mx_fail(e, "combine_kernel");
-        };
-        int const done = c_dtype == nk_bf16_k ? combine(__bf16(), __bf16()) : c_dtype == nk_f32_k ? combine(float(), float()) : combine(float(), _Float16());
+        });
         if (done) return done;
     }
     return 0;

@@ -55,7 +55,7 @@ def _library():
             ("experts_route_backward_async", i32, [i32, vp, sz, sz, sz, sz, how, vp, vp, vp, sz, vp]),
             ("experts_plan_size", sz, [sz, sz]),
             ("experts_plan_async", i32, [vp, sz, sz, vp, vp]),
-            ("mx_experts_workspace_size", sz, [sz, sz, sz, sz, sz, i32, i32, i32]),
+            ("mx_experts_workspace_size", sz, [sz, sz, sz, sz, sz, i32, i32]),
             ("mx_dots_experts_async", i32, [i32, vp, sz, vp, sz, sz, vp, vp, sz, sz, sz, vp, i32, vp, sz, sz, sz, vp, sz, vp]),
         ):
             function = getattr(lib, "nk_amd_" + name)
@@ -512,7 +512,7 @@ def mx_dots_experts(a, packed: MxPackedMatrix, plan: ExpertsPlan, weights=None, 
         result.zero_()
         return result if out is None else out
     share, code, is_codes = top_k if rows == tokens else 1, dtype_codes[out_dtype], scales is not None
-    needed = lib.nk_amd_mx_experts_workspace_size(slots, share, plan.experts, width, depth, is_codes, code, weights is not None)
+    needed = lib.nk_amd_mx_experts_workspace_size(slots, share, plan.experts, width, depth, is_codes, weights is not None)
     workspace = torch.empty(needed, dtype=torch.uint8, device=t.device) if needed else None
     _check(lib.nk_amd_mx_dots_experts_async(
         a_dtype, t.data_ptr(), _row_bytes(t), scales.data_ptr() if is_codes else None, scales_stride, share, packed.buffer.data_ptr(),
