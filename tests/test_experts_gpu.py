@@ -245,7 +245,7 @@ def test_experts_products(tokens, top_k, experts, kind, n, k, dtype, out):
     summed = (truth * weight[..., None]).sum(1)
     magnitudes = (magnitude * np.abs(weight)[..., None]).sum(1)
     sizes = (np.abs(truth * weight[..., None])).sum(1)
-    extra = (mx.ROUNDING[torch.bfloat16] if out == torch.bfloat16 else 0.0) * (sizes + magnitudes * k * 2.0**-24) + top_k * 2.0**-23 * sizes
+    extra = top_k * 2.0**-23 * sizes
     got = nk.mx_dots_experts(a.to(DEV), packed, plan, weights.to(DEV), out_dtype=out)
     assert got.shape == (tokens, n)
     mx.close(got, summed, magnitudes, k, extra)
@@ -299,3 +299,38 @@ def test_layer_replays():
         torch.cuda.synchronize()
         assert torch.equal(captured, eager[replay % 2]), replay
         assert torch.equal(layer(x[0], logits[0]), eager[0])
+
+
+def test_example_layer():
+    """The layer of the example, from the router's scores to the sum by weight, against 64-bit forms step by step."""
+    from numkong_amd.examples import experts_layer
+
+    experts, hidden, depth, top_k, tokens = 12, 160, 224, 3, 50
+    layer, (router, up, down) = experts_layer.make(experts, hidden, depth, top_k)
+    x = normal(tokens, depth, torch.bfloat16, 9, 0.0).to(DEV)
+    logits = layer.scores(x)
+    exact = x.double() @ router.double().T
+    assert ((logits.double() - exact).abs() <= depth * 2.0**-23 * (x.double().abs() @ router.double().abs().T)).all()
+    y = layer(x)
+    weights, chosen = nk.experts_route(logits, top_k)
+    first = nk.mx_dots_experts(x, layer.up, nk.experts_plan(chosen, experts), out_dtype=torch.bfloat16)
+    rows, matrices = mx.rounded(x), [mx.rounded(one) for one in up]
+    choice = chosen.cpu().numpy()
+    truth = np.stack([[matrices[e] @ rows[t] for e in choice[t]] for t in range(tokens)])
+    magnitude = np.stack([[np.abs(matrices[e]) @ np.abs(rows[t]) for e in choice[t]] for t in range(tokens)])
+    mx.close(first, truth, magnitude, depth)
+    rows = mx.rounded(torch.relu(first).reshape(-1, hidden)).reshape(tokens, top_k, hidden)
+    matrices = [mx.rounded(one) for one in down]
+    parts = np.stack([[matrices[e] @ rows[t, i] for i, e in enumerate(choice[t])] for t in range(tokens)])
+    sizes = np.stack([[np.abs(matrices[e]) @ np.abs(rows[t, i]) for i, e in enumerate(choice[t])] for t in range(tokens)])
+    weight = weights.double().cpu().numpy()[..., None]
+    mx.close(y, (parts * weight).sum(1), (sizes * weight).sum(1), hidden, top_k * 2.0**-23 * (np.abs(parts) * weight).sum(1))
+
+
+def test_example_trains_a_router():
+    from numkong_amd.examples import experts_layer
+
+    wanted = torch.arange(200, device=DEV) % 10
+    x = torch.nn.functional.one_hot(wanted, 16).float()
+    first, last = experts_layer.train_router(x, wanted, 10, 3, 30, 5.0)
+    assert last < first / 2  # separable tokens: the gradient leads there
