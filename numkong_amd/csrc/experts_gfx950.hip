@@ -57,30 +57,45 @@ __device__ __forceinline__ void reduce_steps(uint32_t lanes, F &&join) {
     if (lanes > 16) join(Number<16>());
     if (lanes > 32) join(Number<32>());
 }
-__device__ __forceinline__ float wave_sum(float x) {
+template <int L>
+__device__ __forceinline__ float lanes_sum(float x) {
     auto const sum = [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); };
     uint32_t bits = __float_as_uint(x);
-    reduce_steps(64, [&](auto step) __attribute__((always_inline)) { bits = joined<decltype(step)::value>(bits, sum); });
+    reduce_steps(L, [&](auto step) __attribute__((always_inline)) { bits = joined<decltype(step)::value>(bits, sum); });
     return __uint_as_float(bits);
 }
-__device__ __forceinline__ float wave_max(float x) {
+template <int L>
+__device__ __forceinline__ float lanes_max(float x) {
     auto const most = [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); };
     uint32_t bits = __float_as_uint(x);
-    reduce_steps(64, [&](auto step) __attribute__((always_inline)) { bits = joined<decltype(step)::value>(bits, most); });
+    reduce_steps(L, [&](auto step) __attribute__((always_inline)) { bits = joined<decltype(step)::value>(bits, most); });
     return __uint_as_float(bits);
 }
 __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-    reduce_steps(64, [&](auto step) __attribute__((always_inline)) { x = joined<decltype(step)::value>(x, larger); });
-    return (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+template <int L>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
+    reduce_steps(L, [&](auto step) __attribute__((always_inline)) { x = joined<decltype(step)::value>(x, larger); });
+    return x;
+}
+/** The lowest of L lanes for which `is` holds; L and more where it does for none. */
+template <int L>
+__device__ __forceinline__ uint32_t first_lane(bool is) {
+    uint64_t const all = __ballot(is);
+    if constexpr (L == 64) return all ? (uint32_t)__builtin_ctzll(all) : 64u;
+    else return (uint32_t)__builtin_ctz(((uint32_t)(all >> (threadIdx.x & 63 & ~(L - 1))) & ((1u << L) - 1)) | 1u << L);
+}
+/** What lanes of a wavefront have written to LDS is there for its other lanes. */
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 /** Numbers in the order of unsigned integers: larger number, larger key; every NaN above them all, both zeros the same.
  *  Zero is below every key: what is taken already. */
 __device__ __forceinline__ uint32_t key_of(float x) {
-    if (x != x) return 0xFFFFFFFFu;
-    uint32_t const bits = __float_as_uint(x + 0.0f);
-    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+    uint32_t const bits = __float_as_uint(x + 0.0f), key = bits ^ ((uint32_t)((int32_t)bits >> 31) | 0x80000000u);
+    return x != x ? 0xFFFFFFFFu : key;
 }
 constexpr uint32_t kMaskedKey = 0x007FFFFFu; // of -inf
 
@@ -105,24 +120,73 @@ __device__ __forceinline__ void load_row(T const *row, uint32_t lane, uint32_t e
     }
 }
 
-/** Scores of a row from its logits; -inf logits have score 0, also where the whole row is -inf. */
-template <int J>
-__device__ __forceinline__ void scores_of(float const (&l)[J], int sigmoid, float (&s)[J]) {
-    if (sigmoid) {
+template <class T, int J>
+__device__ __forceinline__ void store_row(T *row, uint32_t lane, uint32_t experts, float const (&l)[J]) {
+    if (lane * J + J <= experts) {
+        struct __attribute__((packed, aligned(sizeof(T)))) Several {
+            T x[J];
+        } several;
 #pragma unroll
-        for (int j = 0; j < J; ++j) s[j] = 1.0f / (1.0f + expf(-l[j]));
+        for (int j = 0; j < J; ++j) several.x[j] = (T)l[j];
+        __builtin_memcpy(row + lane * J, &several, sizeof(several));
         return;
     }
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+        if (lane * J + j < experts) row[lane * J + j] = (T)l[j];
+}
+
+/** What scores are made of besides the logit: the row's largest logit and the sum of exponentials (softmax). */
+struct ScoreOf {
+    int sigmoid;
+    float top, sum;
+    template <int J>
+    __device__ __forceinline__ void operator()(float const (&l)[J], float (&s)[J]) const {
+        if (sigmoid) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) s[j] = 1.0f / (1.0f + expf(-l[j]));
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) { // -inf has score 0, also where the whole row is -inf
+            float const e = expf(l[j] - top);
+            s[j] = l[j] == -__builtin_inff() || e == 0.0f ? 0.0f : e / sum;
+        }
+    }
+};
+template <int L, int J>
+__device__ __forceinline__ ScoreOf score_of_row(float const (&l)[J], int sigmoid) {
+    if (sigmoid) return {sigmoid, 0.0f, 0.0f};
     float top = l[0];
 #pragma unroll
     for (int j = 1; j < J; ++j) top = fmaxf(top, l[j]);
-    top = wave_max(top);
+    top = lanes_max<L>(top);
     float sum = 0;
 #pragma unroll
-    for (int j = 0; j < J; ++j) s[j] = l[j] == -__builtin_inff() ? 0.0f : expf(l[j] - top), sum += s[j];
-    sum = wave_sum(sum);
+    for (int j = 0; j < J; ++j) {
+        float const e = expf(l[j] - top);
+        sum += l[j] == -__builtin_inff() ? 0.0f : e;
+    }
+    return {sigmoid, top, lanes_sum<L>(sum)};
+}
+
+/** Takes the largest key of L lanes out, the first of equal ones: its place in the lane that held it, -1 in others and where
+ *  none is above `floor`. */
+template <int L, int J>
+__device__ __forceinline__ int take_largest(uint32_t (&key)[J], uint32_t lane, uint32_t floor, bool &any) {
+    uint32_t mine = key[0];
 #pragma unroll
-    for (int j = 0; j < J; ++j) s[j] = s[j] == 0.0f ? 0.0f : s[j] / sum;
+    for (int j = 1; j < J; ++j) mine = larger(mine, key[j]);
+    uint32_t const top = lanes_max<L>(mine);
+    any = top > floor;
+    bool here = first_lane<L>(mine == top) == lane && any;
+    int at = -1;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        bool const hit = here && key[j] == top;
+        at = hit ? j : at, key[j] = hit ? 0u : key[j], here = here && !hit;
+    }
+    return at;
 }
 
 struct RouteArgs {
@@ -136,31 +200,42 @@ struct RouteArgs {
 };
 
 /**
- *  A wavefront for a token: the row stays in registers, J experts a lane, adjacent ones, so that of equal keys the lowest
- *  lane's lowest is the lowest expert. Each lane sorts its own; a choice is a maximum over the lanes' first, a ballot, and the
- *  winner moves up. Nothing here waits for memory twice: what bounds it is the number of instructions (16,384 tokens of 256
- *  experts, sigmoid, 4 of 8 groups, 8 chosen: 20 us, 46 us with shuffles and a search in every lane for every choice).
+ *  L lanes for a token: its row stays in registers, J experts a lane, adjacent ones, so that of equal keys the lowest lane's
+ *  lowest is the lowest expert. A choice is a maximum over each lane's keys and over the lanes; the lane that holds it takes it
+ *  out and notes it. What bounds this is the number of instructions, so 16 lanes serve a token while they can hold its row, and
+ *  four tokens share what a choice takes (16,384 tokens of 256 experts, sigmoid and bias, 4 of 8 groups, 8 chosen: 14.9 us with 16
+ *  lanes, 20.5 with 64, at 3 us for the traffic; 8192 tokens of 128 experts, 8 chosen: 5.7 and 7.3 us, the gradient 5.8 and 7.7).
+ *  Groups of whole lanes are found in registers, others through LDS (the same 16,384 tokens all through LDS: 23.6 us).
  */
-template <class T, int J>
+template <class T, int L, int J>
 __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
-    __shared__ float score_of[4][64 * J];
-    uint32_t const lane = threadIdx.x & 63, wave = threadIdx.x >> 6, token = blockIdx.x * 4 + wave;
-    if (token >= p.tokens) return;
-    float l[J], s[J];
-    load_row<T, J>((T const *)((uint8_t const *)p.logits + token * p.stride), lane, p.experts, l);
-    scores_of<J>(l, p.how.sigmoid, s);
-    uint32_t key[J], expert[J];
+    constexpr uint32_t kTokens = 256 / L;
+    constexpr int kOfLane = 64 / L; // groups, and choices, that a lane looks after
+    __shared__ uint32_t keys[kTokens][L * J];
+    __shared__ int32_t notes[kTokens][64];
+    uint32_t const lane = threadIdx.x % L, local = threadIdx.x / L, token = blockIdx.x * kTokens + local;
+    if (token >= p.tokens) return; // (with all lanes that it exchanges anything with)
+    T const *const row = (T const *)((uint8_t const *)p.logits + token * p.stride);
+    float l[J];
+    load_row<T, J>(row, lane, p.experts, l);
+    ScoreOf const score = score_of_row<L, J>(l, p.how.sigmoid);
+    uint32_t key[J];
+    if (p.bias) {
+        float bias[J], s[J];
+        load_row<float, J>(p.bias, lane, p.experts, bias);
+        score(l, s);
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-        uint32_t const e = lane * J + j;
-        bool const masked = l[j] == -__builtin_inff();
-        expert[j] = e, score_of[wave][e] = s[j];
-        key[j] = e >= p.experts ? 0u : masked ? kMaskedKey : key_of(p.bias ? s[j] + p.bias[e] : l[j]);
+        for (int j = 0; j < J; ++j) key[j] = key_of(l[j] == -__builtin_inff() ? l[j] : s[j] + bias[j]);
     }
+    else
+#pragma unroll
+        for (int j = 0; j < J; ++j) key[j] = key_of(l[j]);
+    bool any;
     if (p.how.groups > 1) {
         uint32_t const groups = (uint32_t)p.how.groups, size = p.experts / groups, lanes = size / J;
         bool const two = p.how.group_top == 2 && size > 1;
-        if (size % J == 0 && (lanes & (lanes - 1)) == 0) { // a group is some whole lanes, side by side
+        auto const group_key = [&](uint32_t first, uint32_t second) { return two ? key_of(number_of(first) + number_of(second)) : first; };
+        if (size % J == 0 && (lanes & (lanes - 1)) == 0) { // a group is some whole lanes, side by side, and stays in registers
             uint32_t first = key[0], second = 0;
 #pragma unroll
             for (int j = 1; j < J; ++j) {
@@ -172,78 +247,75 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
                 uint32_t const lesser = other < first ? other : first;
                 first = larger(first, other), second = larger(larger(second, next), lesser);
             });
-            uint32_t mine = lane >= groups * lanes ? 0 : two ? key_of(number_of(first) + number_of(second)) : first;
+            uint32_t mine = lane >= groups * lanes ? 0 : group_key(first, second);
             bool stays = false;
-            for (int i = 0; i < p.how.top_groups; ++i) {
-                uint32_t const best = wave_max(mine), which = (uint32_t)__builtin_ctzll(__ballot(mine == best));
-                if (lane / lanes == which / lanes) stays = true, mine = 0;
-            }
+            for (int i = 0; i < p.how.top_groups; ++i)
+                if ((lane ^ first_lane<L>(mine == lanes_max<L>(mine))) < lanes) stays = true, mine = 0;
 #pragma unroll
-            for (int j = 0; j < J; ++j)
-                if (!stays && lane * J + j < p.experts) key[j] = kMaskedKey;
+            for (int j = 0; j < J; ++j) key[j] = stays ? key[j] : kMaskedKey;
         }
-        else { // groups that start anywhere, one after the other
-            uint32_t mine = 0; // the key of group `lane`
-            for (uint32_t group = 0; group < groups; ++group) {
-                uint32_t best = 0;
-                int at = 0;
+        else { // the keys go through LDS, and each lane finds the best of its own groups
+            uint32_t const per_lane = (groups + L - 1) / L;
 #pragma unroll
-                for (int j = 0; j < J; ++j)
-                    if (lane * J + j >= group * size && lane * J + j < (group + 1) * size && key[j] > best) best = key[j], at = j;
-                uint32_t const first = wave_max(best);
-                uint32_t group_key = first;
-                if (two) {
-                    uint64_t const holders = __ballot(best == first && first != 0);
-                    bool const winner = holders && lane == (uint32_t)__builtin_ctzll(holders);
-                    uint32_t next = 0;
+            for (int j = 0; j < J; ++j) keys[local][lane * J + j] = key[j];
+            wave_fence();
+            uint32_t of_group[kOfLane], stay = 0;
 #pragma unroll
-                    for (int j = 0; j < J; ++j)
-                        if (lane * J + j >= group * size && lane * J + j < (group + 1) * size && !(winner && j == at)) next = larger(next, key[j]);
-                    group_key = key_of(number_of(first) + number_of(wave_max(next)));
+            for (int q = 0; q < kOfLane; ++q) {
+                uint32_t const group = lane * per_lane + q;
+                of_group[q] = 0;
+                if (q >= per_lane || group >= groups) continue;
+                uint32_t first = 0, second = 0, at = lane % size; // (not all lanes at the same bank)
+                for (uint32_t i = 0; i < size; ++i) {
+                    uint32_t const k = keys[local][group * size + at], lesser = k < first ? k : first;
+                    first = larger(first, k), second = larger(second, lesser);
+                    at = at + 1 == size ? 0 : at + 1;
                 }
-                if (lane == group) mine = group_key;
+                of_group[q] = group_key(first, second);
             }
-            uint64_t stays = 0;
             for (int i = 0; i < p.how.top_groups; ++i) {
-                uint32_t const best = wave_max(mine), which = (uint32_t)__builtin_ctzll(__ballot(mine == best));
-                stays |= 1ull << which;
-                if (lane == which) mine = 0;
+                int const at = take_largest<L, kOfLane>(of_group, lane, 0u, any);
+                stay |= at < 0 ? 0u : 1u << at;
             }
+#pragma unroll
+            for (int q = 0; q < kOfLane; ++q)
+                if (q < per_lane && lane * per_lane + q < 64) notes[local][lane * per_lane + q] = (int32_t)(stay >> q & 1);
+            wave_fence();
+            uint32_t group = lane * J / size, left = size - (lane * J - group * size);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                uint32_t const e = lane * J + j;
-                if (e < p.experts && !(stays >> (e / size) & 1)) key[j] = kMaskedKey;
+                if (group >= groups || !notes[local][group]) key[j] = kMaskedKey;
+                if (--left == 0) left = size, ++group;
             }
+            wave_fence();
         }
     }
-#pragma unroll
-    for (int end = J - 1; end > 0; --end) // largest first; equal ones stay as they stand, the lower expert before the higher
-#pragma unroll
-        for (int j = 0; j < end; ++j) {
-            bool const swaps = key[j + 1] > key[j];
-            uint32_t const k = key[j], e = expert[j];
-            key[j] = swaps ? key[j + 1] : k, expert[j] = swaps ? expert[j + 1] : e;
-            key[j + 1] = swaps ? k : key[j + 1], expert[j + 1] = swaps ? e : expert[j + 1];
-        }
-    int32_t chosen = -1;
     for (uint32_t i = 0; i < p.top_k; ++i) {
-        uint32_t const top = wave_max(key[0]);
-        if (top <= kMaskedKey) break; // the rest of the slots stay empty
-        uint32_t const which = (uint32_t)__builtin_ctzll(__ballot(key[0] == top));
-        int32_t const its = __builtin_amdgcn_readlane((int)expert[0], (int)which);
-        if (lane == i) chosen = its;
-        bool const winner = lane == which;
-#pragma unroll
-        for (int j = 0; j + 1 < J; ++j) key[j] = winner ? key[j + 1] : key[j], expert[j] = winner ? expert[j + 1] : expert[j];
-        if (winner) key[J - 1] = 0;
+        int const at = take_largest<L, J>(key, lane, kMaskedKey, any);
+        if (any ? at >= 0 : lane == 0) notes[local][i] = any ? (int32_t)(lane * J) + at : -1;
     }
-    __builtin_amdgcn_wave_barrier(); // (the wavefront's own scores, written above)
-    float weight = chosen < 0 ? 0.0f : score_of[wave][chosen];
-    if (p.how.renormalize) weight /= wave_sum(weight) + 1e-20f;
-    weight *= p.how.scale;
-    if (lane < p.top_k) {
-        p.weights[(uint64_t)token * p.top_k + lane] = chosen < 0 ? 0.0f : weight;
-        p.chosen[(uint64_t)token * p.top_k + lane] = chosen;
+    wave_fence();
+    float weight[kOfLane], sum = 0;
+    int32_t chosen[kOfLane];
+#pragma unroll
+    for (int q = 0; q < kOfLane; ++q) {
+        uint32_t const i = q * L + lane;
+        chosen[q] = -1, weight[q] = 0;
+        if (q * L >= p.top_k) continue;
+        if (i < p.top_k) chosen[q] = notes[local][i];
+        float const its[1] = {chosen[q] < 0 ? -__builtin_inff() : (float)row[chosen[q]]}; // (-inf: of both kinds the score is 0)
+        float of_it[1];
+        score(its, of_it);
+        weight[q] = of_it[0], sum += weight[q];
+    }
+    if (p.how.renormalize) sum = lanes_sum<L>(sum) + 1e-20f;
+#pragma unroll
+    for (int q = 0; q < kOfLane; ++q) {
+        uint32_t const i = q * L + lane;
+        if (i >= p.top_k) continue;
+        if (p.how.renormalize) weight[q] /= sum;
+        p.weights[(uint64_t)token * p.top_k + i] = chosen[q] < 0 ? 0.0f : weight[q] * p.how.scale;
+        p.chosen[(uint64_t)token * p.top_k + i] = chosen[q];
     }
 }
 
@@ -252,46 +324,49 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
  *  renormalised, scale g_j where not, 0 outside S; then dl_j = ds_j s_j (1 - s_j) for sigmoid scores, and
  *  dl_i = s_i (ds_i - sum_S ds s) for softmax.
  */
-template <class T, int J>
+template <class T, int L, int J>
 __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs p, float const *grad, T *out, uint64_t out_stride) {
-    uint32_t const lane = threadIdx.x & 63, token = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (token >= p.tokens) return;
-    float l[J], s[J];
+    constexpr uint32_t kTokens = 256 / L;
+    __shared__ uint32_t choice_of[kTokens][L * J]; // of each expert, 1 for the first; 0: it was not chosen
+    __shared__ float grads[kTokens][64];
+    uint32_t const lane = threadIdx.x % L, local = threadIdx.x / L, token = blockIdx.x * kTokens + local;
+    if (token >= p.tokens) return; // (with all lanes that it exchanges anything with)
+    float l[J], s[J], g[J];
     load_row<T, J>((T const *)((uint8_t const *)p.logits + token * p.stride), lane, p.experts, l);
-    scores_of<J>(l, p.how.sigmoid, s);
-    float const its_grad = lane < p.top_k ? grad[(uint64_t)token * p.top_k + lane] : 0.0f;
-    int32_t const its_expert = lane < p.top_k ? p.chosen[(uint64_t)token * p.top_k + lane] : -1;
-    float g[J];
-    bool in[J];
 #pragma unroll
-    for (int j = 0; j < J; ++j) g[j] = 0, in[j] = false;
-    for (uint32_t i = 0; i < p.top_k; ++i) {
-        int32_t const e = __builtin_amdgcn_readlane(its_expert, (int)i);
-        float const of_e = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(__float_as_int(its_grad), (int)i));
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-            if (e == (int32_t)(lane * J + j) && e < (int32_t)p.experts) g[j] = of_e, in[j] = true;
+    for (int j = 0; j < J; ++j) choice_of[local][lane * J + j] = 0;
+    wave_fence();
+    for (uint32_t i = lane; i < p.top_k; i += L) {
+        uint32_t const e = (uint32_t)p.chosen[(uint64_t)token * p.top_k + i];
+        grads[local][i] = grad[(uint64_t)token * p.top_k + i];
+        if (e < p.experts) choice_of[local][e] = i + 1;
     }
+    ScoreOf const score = score_of_row<L, J>(l, p.how.sigmoid);
+    wave_fence();
+    bool in[J];
     float total = 0, along = 0;
+    score(l, s);
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+    for (int j = 0; j < J; ++j) {
+        uint32_t const choice = choice_of[local][lane * J + j];
+        in[j] = choice != 0, g[j] = in[j] ? grads[local][choice - 1] : 0.0f;
         if (in[j]) total += s[j], along += g[j] * s[j];
-    total = wave_sum(total) + 1e-20f, along = wave_sum(along);
+    }
+    total = lanes_sum<L>(total) + 1e-20f, along = lanes_sum<L>(along);
     float ds[J], inner = 0;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         ds[j] = !in[j] ? 0.0f : p.how.scale * (p.how.renormalize ? (g[j] - along / total) / total : g[j]);
         inner += in[j] ? ds[j] * s[j] : 0.0f;
     }
-    inner = wave_sum(inner);
-    T *row = (T *)((uint8_t *)out + token * out_stride);
+    inner = lanes_sum<L>(inner);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-        uint32_t const e = lane * J + j;
         // (1 - s of a sigmoid is the score of the opposite logit, without its cancellation)
         float const slope = p.how.sigmoid ? (in[j] ? ds[j] * s[j] / (1.0f + expf(l[j])) : 0.0f) : s[j] * (ds[j] - inner);
-        if (e < p.experts) row[e] = (T)(l[j] == -__builtin_inff() ? 0.0f : slope);
+        g[j] = l[j] == -__builtin_inff() ? 0.0f : slope;
     }
+    store_row<T, J>((T *)((uint8_t *)out + token * out_stride), lane, p.experts, g);
 }
 
 // ---- the plan -----------------------------------------------------------------------------------------------------
@@ -442,15 +517,15 @@ int check_route(nk_dtype_t dtype, void const *logits, nk_size_t stride, nk_size_
     return 0;
 }
 
-/** Calls `f` with a value of the logits' type and one that says how many experts a lane holds. */
+/** Calls `f` with a value of the logits' type, and with how many lanes a token has and how many experts a lane holds. */
 template <class F>
 int with_row(nk_dtype_t dtype, size_t experts, F &&f) {
     auto const of_type = [&](auto value) {
-        if (experts <= 64) return f(value, Number<1>());
-        if (experts <= 128) return f(value, Number<2>());
-        if (experts <= 256) return f(value, Number<4>());
-        if (experts <= 512) return f(value, Number<8>());
-        return f(value, Number<16>());
+        if (experts <= 64) return f(value, Number<16>(), Number<4>());
+        if (experts <= 128) return f(value, Number<16>(), Number<8>());
+        if (experts <= 256) return f(value, Number<16>(), Number<16>());
+        if (experts <= 512) return f(value, Number<64>(), Number<8>());
+        return f(value, Number<64>(), Number<16>());
     };
     if (dtype == nk_f32_k) return of_type(float());
     if (dtype == nk_bf16_k) return of_type(__bf16());
@@ -472,9 +547,10 @@ int nk_amd_experts_route_async(nk_dtype_t dtype, void const *logits, nk_size_t l
     if (!tokens) return 0;
     if (!weights || !chosen) return mx_fail("experts_route: NULL operand");
     RouteArgs const p = {logits, logits_stride, (uint32_t)tokens, (uint32_t)experts, (uint32_t)top_k, bias, *how, weights, chosen};
-    return with_row(dtype, experts, [&](auto value, auto per_lane) {
+    return with_row(dtype, experts, [&](auto value, auto lanes, auto per_lane) {
         typedef decltype(value) T;
-        hipLaunchKernelGGL((route_kernel<T, decltype(per_lane)::value>), dim3((uint32_t)((tokens + 3) / 4)), dim3(256), 0, (hipStream_t)stream, p);
+        constexpr int L = decltype(lanes)::value, J = decltype(per_lane)::value;
+        hipLaunchKernelGGL((route_kernel<T, L, J>), dim3((uint32_t)((tokens + 256 / L - 1) / (256 / L))), dim3(256), 0, (hipStream_t)stream, p);
         hipError_t const e = hipGetLastError();
         return e == hipSuccess ? 0 : mx_fail(e, "route_kernel");
     });
@@ -489,9 +565,10 @@ int nk_amd_experts_route_backward_async(nk_dtype_t dtype, void const *logits, nk
     int const bytes = dtype == nk_f32_k ? 4 : 2;
     if (((uintptr_t)grad_logits | grad_stride) & (bytes - 1)) return mx_fail("experts_route_backward: grad_logits is not aligned to its elements");
     RouteArgs const p = {logits, logits_stride, (uint32_t)tokens, (uint32_t)experts, (uint32_t)top_k, nullptr, *how, nullptr, (int32_t *)chosen};
-    return with_row(dtype, experts, [&](auto value, auto per_lane) {
+    return with_row(dtype, experts, [&](auto value, auto lanes, auto per_lane) {
         typedef decltype(value) T;
-        hipLaunchKernelGGL((route_backward_kernel<T, decltype(per_lane)::value>), dim3((uint32_t)((tokens + 3) / 4)), dim3(256), 0,
+        constexpr int L = decltype(lanes)::value, J = decltype(per_lane)::value;
+        hipLaunchKernelGGL((route_backward_kernel<T, L, J>), dim3((uint32_t)((tokens + 256 / L - 1) / (256 / L))), dim3(256), 0,
                            (hipStream_t)stream, p, grad_weights, (T *)grad_logits, (uint64_t)grad_stride);
         hipError_t const e = hipGetLastError();
         return e == hipSuccess ? 0 : mx_fail(e, "route_backward_kernel");
