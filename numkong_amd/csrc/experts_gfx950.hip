@@ -84,13 +84,6 @@ __device__ __forceinline__ uint32_t first_lane(bool is) {
     if constexpr (L == 64) return all ? (uint32_t)__builtin_ctzll(all) : 64u;
     else return (uint32_t)__builtin_ctz(((uint32_t)(all >> (threadIdx.x & 63 & ~(L - 1))) & ((1u << L) - 1)) | 1u << L);
 }
-/** What lanes of a wavefront have written to LDS is there for its other lanes. */
-__device__ __forceinline__ void wave_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 /** Numbers in the order of unsigned integers: larger number, larger key; every NaN above them all, both zeros the same.
  *  Zero is below every key: what is taken already. */
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -497,9 +490,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(int32_t const *chose
             plan[order + row] = at;
             plan[place + at] = bucket < experts ? row : 0xFFFFFFFFu;
         }
-        __builtin_amdgcn_wave_barrier(); // (every lane has read its count before the first of each bucket moves it on)
+        wave_fence(); // (every lane has read its count before the first of each bucket moves it on)
         if (active && !rank) counts[bucket] += (uint32_t)__popcll(same);
-        __builtin_amdgcn_wave_barrier();
+        wave_fence();
     }
 }
 

@@ -491,7 +491,7 @@ __global__ __launch_bounds__(256, FM >= 8 ? 1 : 2) void mx_gemm_kernel(MxArgs p)
         uint32_t const wave_column = now.tile_n * kColumns + wave * 64;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
-            __builtin_amdgcn_wave_barrier();
+            wave_fence();
 #pragma unroll
             for (int part = 0; part < 2 * 16 / kEach; ++part) {
                 int const x = part * kEach / 16;
@@ -506,7 +506,7 @@ __global__ __launch_bounds__(256, FM >= 8 ? 1 : 2) void mx_gemm_kernel(MxArgs p)
                 uint32_t const piece = ((2 * x + g) * 16 + part * kEach % 16) / kEach;
                 *(Piece *)(mine + (r * kPieces + (piece ^ (r & 7))) * 16) = values;
             }
-            __builtin_amdgcn_wave_barrier();
+            wave_fence();
             if (i == 0) { // (what the next tile's first steps need: from here on stores are behind it)
                 asm volatile("" ::: "memory");
                 __builtin_amdgcn_s_waitcnt(0x0F70);

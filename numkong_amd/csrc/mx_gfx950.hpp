@@ -256,6 +256,13 @@ __device__ __forceinline__ void store_16(void *to, v4u values) {
     *(anywhere *)to = values;
 }
 
+/** What lanes of a wavefront have written to LDS is there for its other lanes. */
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 /** A number that a lambda's argument carries at compile time. */
 template <int N>
 struct Number {
