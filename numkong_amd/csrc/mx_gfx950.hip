@@ -827,12 +827,15 @@ int launch_gemm(MxArgs &p, hipStream_t stream) {
  *  compute units idle (us, few rows against many: 128 x 8192 x 8192 19.1 and 27.1, 512 x 2048 x 2048 10.6 and 12.5, 1024 x 1024 x
  *  8192 23.1 and 30.8; at 64 tiles 256 x 8192 x 8192 29.9 and 28.5, 1024 x 2048 x 2048 15.4 and 13.9). A workgroup of few rows
  *  takes one tile of columns while there are fewer than 512 (64 x 2048 x 2048 7.0 us with one, 7.5 with two; 64 x 8192 x 8192
- *  17.0 and 15.0). Tiles of 256 rows from 256 of them on: less of B is read for the same work, the compute units are full.
+ *  17.0 and 15.0). Tiles of 256 rows from 256 of them on: less of B is read for the same work, the compute units are full. But a
+ *  workgroup's results hold up its next tile (stores are waited for in order), and where 16-bit results come every 16 steps or more
+ *  often, two workgroups of 128 rows that hide that from each other are faster (8192 x 8192, us, 128 rows and 256: bf16 depth 512
+ *  45.3 and 56.0, 1024 62.2 and 69.8, 2048 88.4 and 94.2, 4096 174 and 156; f32 depth 1024 105 and 96).
  */
 template <class Out, bool GROUPED>
 int launch_product(MxArgs &p, uint32_t tile_rows, int a_dtype, bool fused, uint32_t fused_rows, MxGeometry const &g, hipStream_t stream) {
     auto const tiles_of = [&](uint64_t rows, uint64_t columns) { return (p.m + rows - 1) / rows * ((p.n + columns - 1) / columns); };
-    uint32_t const rows = GROUPED ? tile_rows : p.m <= 32 || tiles_of(128, 256) < 64 ? (p.m < 64 ? p.m : 64) : tiles_of(256, 256) < 256 ? 128 : 256;
+    uint32_t const rows = GROUPED ? tile_rows : p.m <= 32 || tiles_of(128, 256) < 64 ? (p.m < 64 ? p.m : 64) : tiles_of(256, 256) < 256 || (sizeof(Out) == 2 && g.steps <= 16) ? 128 : 256;
     if (rows <= 16) {
         constexpr int NT = GROUPED ? 2 : 1; // (experts of 4 tokens, 28 matrices of 2048 x 2048: 13.0 us with two, 14.0 with one)
         if (!fused) return launch_few<1, NT, uint8_t, Out, GROUPED>(p, rows, g, stream);

@@ -134,10 +134,15 @@ def _to_host(result, as_numpy: bool, out=None):
     return result.cpu().numpy() if as_numpy else result.cpu()
 
 
+def _new(torch, rows, columns, dtype, device):
+    """A matrix of whatever (by its strides: torch.empty takes half as long again, and a call of few tokens makes several)."""
+    return torch.empty_strided((rows, columns), (columns or 1, 1), dtype=dtype, device=device)
+
+
 def _result(torch, out, shape, dtype, like):
     """The matrix that a call writes: `out` where one is given, else a new one."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return _new(torch, *shape, dtype, like.device) if len(shape) == 2 else torch.empty(shape, dtype=dtype, device=like.device)
     t = _tensor(out, "out")
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"out has shape {tuple(t.shape)}, expected {tuple(shape)}")
@@ -251,8 +256,8 @@ def mx_quantize(x) -> MxMatrix:
         with torch.cuda.device(t.device):
             return mx_quantize(t)
     code_bytes, blocks = (depth + 1) // 2, (depth + BLOCK - 1) // BLOCK
-    codes = torch.empty((rows, code_bytes), dtype=torch.uint8, device=t.device)
-    scales = torch.empty((rows, blocks), dtype=torch.uint8, device=t.device)
+    device, u8 = t.device, torch.uint8
+    codes, scales = _new(torch, rows, code_bytes, u8, device), _new(torch, rows, blocks, u8, device)
     _check(lib.nk_amd_mx_quantize_async(dtype_codes[t.dtype], t.data_ptr(), rows, depth, _row_bytes(t), codes.data_ptr(), code_bytes,
                                         scales.data_ptr(), blocks, _stream(t.get_device())), "mx_quantize")
     return MxMatrix._made(codes, scales, depth)
@@ -349,7 +354,7 @@ def mx_dots_packed(a, packed: MxPackedMatrix, out=None, out_dtype=None):
             return mx_dots_packed(a, packed, out, out_dtype)
     result = _result(torch, out, (height, width), out_dtype, t)
     needed = lib.nk_amd_mx_dots_workspace_size(height, width, depth, scales is not None)
-    workspace = torch.empty(needed, dtype=torch.uint8, device=t.device) if needed else None
+    workspace = torch.empty_strided((needed,), (1,), dtype=torch.uint8, device=t.device) if needed else None
     _check(lib.nk_amd_mx_dots_packed_async(
         a_dtype, t.data_ptr(), _row_bytes(t), scales.data_ptr() if scales is not None else None, scales_stride,
         packed.buffer.data_ptr(), dtype_codes[out_dtype], result.data_ptr(), _row_bytes(result), height, width, depth,
@@ -396,8 +401,8 @@ def experts_route(logits, top_k: int, score: str = "softmax", bias=None, groups:
     if index != _device():
         with torch.cuda.device(index):
             return experts_route(t, top_k, score, bias, groups, top_groups, group_top, renormalize, scale)
-    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=t.device)
-    chosen = torch.empty((tokens, top_k), dtype=torch.int32, device=t.device)
+    device = t.device
+    weights, chosen = _new(torch, tokens, top_k, torch.float32, device), _new(torch, tokens, top_k, torch.int32, device)
     _check(lib.nk_amd_experts_route_async(dtype_codes[t.dtype], t.data_ptr(), _row_bytes(t), tokens, experts, top_k,
                                           bias.data_ptr() if bias is not None else None, how, weights.data_ptr(), chosen.data_ptr(),
                                           _stream(index)), "experts_route")
@@ -424,7 +429,7 @@ def experts_route_backward(grad_weights, logits, experts, score: str = "softmax"
         with torch.cuda.device(index):
             return experts_route_backward(grad_weights, t, experts, score, renormalize, scale)
     grad_weights, experts = grad_weights.contiguous(), experts.contiguous()
-    result = torch.empty((tokens, count), dtype=t.dtype, device=t.device)
+    result = _new(torch, tokens, count, t.dtype, t.device)
     _check(lib.nk_amd_experts_route_backward_async(
         dtype_codes[t.dtype], t.data_ptr(), _row_bytes(t), tokens, count, experts.shape[1], how, experts.data_ptr(),
         grad_weights.data_ptr(), result.data_ptr(), _row_bytes(result), _stream(index)), "experts_route_backward")
@@ -459,7 +464,7 @@ def experts_plan(chosen, experts: int) -> ExpertsPlan:
         with torch.cuda.device(index):
             return experts_plan(chosen, experts)
     chosen = chosen.contiguous()
-    buffer = torch.empty(size, dtype=torch.uint8, device=chosen.device)
+    buffer = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=chosen.device)
     _check(lib.nk_amd_experts_plan_async(chosen.data_ptr(), tokens * top_k, experts, buffer.data_ptr(), _stream(index)), "experts_plan")
     return ExpertsPlan(tokens, top_k, experts, buffer)
 
@@ -513,7 +518,7 @@ def mx_dots_experts(a, packed: MxPackedMatrix, plan: ExpertsPlan, weights=None, 
         return result if out is None else out
     share, code, is_codes = top_k if rows == tokens else 1, dtype_codes[out_dtype], scales is not None
     needed = lib.nk_amd_mx_experts_workspace_size(slots, share, plan.experts, width, depth, is_codes, weights is not None)
-    workspace = torch.empty(needed, dtype=torch.uint8, device=t.device) if needed else None
+    workspace = torch.empty_strided((needed,), (1,), dtype=torch.uint8, device=t.device) if needed else None
     _check(lib.nk_amd_mx_dots_experts_async(
         a_dtype, t.data_ptr(), _row_bytes(t), scales.data_ptr() if is_codes else None, scales_stride, share, packed.buffer.data_ptr(),
         plan.buffer.data_ptr(), slots, plan.experts, top_k, weights.data_ptr() if weights is not None else None, code,
