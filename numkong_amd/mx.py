@@ -28,12 +28,13 @@ class _Route(ctypes.Structure):
 
 
 _LIB = None
+_CALLS = None  # csrc/mx_calls.cpp: the calls in their ordinary form; each gives None for what is to go the general way below
 _device = _stream = None  # the current device's index, a device's current stream as a number: torch's own (see _library)
 
 
 def _library():
     """The shared library with the entry points of mx.h bound, and the torch module."""
-    global _LIB, _device, _stream
+    global _LIB, _CALLS, _device, _stream
     if _LIB is None:
         import torch
 
@@ -62,6 +63,15 @@ def _library():
             function.restype, function.argtypes = result, arguments
         codes = {torch.float32: NK_F32, torch.bfloat16: NK_BF16, torch.float16: NK_F16}
         _LIB = lib, torch, codes
+        try:
+            from .lib import _mx_calls
+        except ImportError:  # built for another torch, or not at all
+            _mx_calls = None
+        else:
+            _mx_calls.bind(*(ctypes.cast(getattr(lib, "nk_amd_" + name), ctypes.c_void_p).value for name in (
+                "mx_quantize_async", "mx_dequantize_async", "mx_dots_workspace_size", "mx_dots_packed_async", "experts_route_async",
+                "experts_route_backward_async", "experts_plan_size", "experts_plan_async", "mx_experts_workspace_size", "mx_dots_experts_async")))
+        _CALLS = _mx_calls
     return _LIB
 
 
@@ -245,6 +255,8 @@ def mx_quantize(x) -> MxMatrix:
     """The rows of ``x`` (float32, bfloat16 or float16) as 4-bit codes with a scale for each 32 values: the power of two
     that brings the block's largest magnitude into [4, 8); codes to nearest, ties to even, stopping at 6. A block that holds a
     NaN or an infinity becomes NaN."""
+    if _CALLS is not None and (made := _CALLS.quantize(x)) is not None:
+        return MxMatrix._made(*made, x.shape[1])
     lib, torch, dtype_codes = _LIB or _library()
     t = _floats(x, "x")
     rows, depth = t.shape
@@ -273,6 +285,9 @@ def _matrix_of(a, what: str) -> MxMatrix:
 def mx_dequantize(matrix: MxMatrix, dtype=None, out=None):
     """The values that a matrix of codes and scales stands for, in float32 (default), bfloat16 (both exact) or float16."""
     lib, torch, dtype_codes = _LIB or _library()
+    if _CALLS is not None and out is None and type(matrix) is MxMatrix:
+        if (made := _CALLS.dequantize(matrix.codes, matrix.scales, matrix.depth, dtype or torch.float32)) is not None:
+            return made
     m = _matrix_of(matrix, "matrix")
     dtype = _out_dtype(out, dtype)
     if m.codes.dim() != 2:
@@ -333,6 +348,10 @@ def mx_dots_packed(a, packed: MxPackedMatrix, out=None, out_dtype=None):
     """``C[height x width] = a @ B.T`` with 4-bit operands and 32-bit sums. ``a``: floats, quantised on the way exactly as
     ``mx_quantize`` does, or an MxMatrix; the result is float32 (default), bfloat16 or float16 (``out_dtype``, or ``out``'s)."""
     lib, torch, dtype_codes = _LIB or _library()
+    if _CALLS is not None and out is None and type(packed) is MxPackedMatrix and packed.count == 1:
+        values, scales, depth = (a.codes, a.scales, a.depth) if type(a) is MxMatrix else (a, None, None)
+        if (made := _CALLS.dots(values, scales, depth, packed.buffer, packed.width, packed.depth, out_dtype or torch.float32)) is not None:
+            return made
     if not isinstance(packed, MxPackedMatrix):
         raise TypeError("packed must be an MxPackedMatrix from mx_pack()")
     if packed.count != 1:
@@ -385,6 +404,9 @@ def experts_route(logits, top_k: int, score: str = "softmax", bias=None, groups:
     the chosen where ``renormalize`` is set, times ``scale``. With ``groups`` > 1 the experts stand in groups of equal size, of
     which the ``top_groups`` stay whose ``group_top`` (1 or 2) best selection scores have the largest sum (without a bias:
     the sum of logits). A logit of -inf is never chosen; a row with too few others gets expert -1 with weight 0."""
+    if _CALLS is not None:
+        if (made := _CALLS.route(logits, top_k, bias, _SCORES.get(score), bool(renormalize), scale, groups, top_groups, group_top)) is not None:
+            return made
     lib, torch, dtype_codes = _LIB or _library()
     t = _floats(logits, "logits")
     tokens, experts = t.shape
@@ -412,6 +434,9 @@ def experts_route(logits, top_k: int, score: str = "softmax", bias=None, groups:
 def experts_route_backward(grad_weights, logits, experts, score: str = "softmax", renormalize: bool = True, scale: float = 1.0):
     """The gradient of ``logits`` (their type and shape) from ``grad_weights``, that of the weights that ``experts_route``
     gave for them together with ``experts``. The selection itself has none, and neither has a bias."""
+    if _CALLS is not None:
+        if (made := _CALLS.route_backward(grad_weights, logits, experts, _SCORES.get(score), bool(renormalize), scale)) is not None:
+            return made
     lib, torch, dtype_codes = _LIB or _library()
     t = _floats(logits, "logits")
     grad_weights, experts = _tensor(grad_weights, "grad_weights"), _tensor(experts, "experts")
@@ -449,6 +474,8 @@ class ExpertsPlan:
 def experts_plan(chosen, experts: int) -> ExpertsPlan:
     """Sort the slots of ``chosen`` (tokens x top_k, int32, as ``experts_route`` gives them) by expert, keeping their order.
     Entries outside [0, ``experts``) go to no expert: -1 for padding, or experts that another process holds."""
+    if _CALLS is not None and (made := _CALLS.plan(chosen, experts)) is not None:
+        return ExpertsPlan(*chosen.shape, experts, made)
     lib, torch, _ = _LIB or _library()
     chosen = _tensor(chosen, "chosen")
     if chosen.dim() != 2 or chosen.dtype != torch.int32:
@@ -475,6 +502,11 @@ def mx_dots_experts(a, packed: MxPackedMatrix, plan: ExpertsPlan, weights=None, 
     With ``weights`` (tokens x top_k, float32) the rows of a token are summed by weight instead: tokens x width, slots without
     an expert left out."""
     lib, torch, dtype_codes = _LIB or _library()
+    if _CALLS is not None and out is None and type(packed) is MxPackedMatrix and type(plan) is ExpertsPlan:
+        values, scales, depth = (a.codes, a.scales, a.depth) if type(a) is MxMatrix else (a, None, None)
+        if (made := _CALLS.experts(values, scales, depth, packed.buffer, packed.count, packed.width, packed.depth, plan.buffer, plan.tokens,
+                                   plan.top_k, plan.experts, weights, out_dtype or torch.float32)) is not None:
+            return made
     if not isinstance(packed, MxPackedMatrix):
         raise TypeError("packed must be an MxPackedMatrix from mx_pack()")
     if not isinstance(plan, ExpertsPlan):

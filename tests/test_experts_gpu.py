@@ -334,3 +334,36 @@ def test_example_trains_a_router():
     x = torch.nn.functional.one_hot(wanted, 16).float()
     first, last = experts_layer.train_router(x, wanted, 10, 3, 30, 5.0)
     assert last < first / 2  # separable tokens: the gradient leads there
+
+
+def test_the_short_way_and_the_general_one_agree(monkeypatch):
+    """Every call in its ordinary form, on the default stream and on another, against the same call the general way."""
+    from numkong_amd import mx as binding
+
+    x, b = normal(40, 200, torch.bfloat16, 1).to(DEV), normal(70, 200, torch.float32, 2).to(DEV)
+    stack, logits = normal(6 * 33, 200, torch.float32, 3).reshape(6, 33, 200).to(DEV), normal(40, 6, torch.float32, 4, 0.0).to(DEV)
+    bias, grad = torch.rand(6, device=DEV), torch.rand((40, 2), device=DEV)
+    packed, packed_stack = nk.mx_pack(b), nk.mx_pack(stack)
+
+    def calls():
+        q = nk.mx_quantize(x)
+        weights, chosen = nk.experts_route(logits, 2, "sigmoid", bias, groups=3, top_groups=2, scale=1.5)
+        plan = nk.experts_plan(chosen, 6)
+        found = [q.codes, q.scales, nk.mx_dequantize(q), nk.mx_dequantize(q, torch.float16), nk.mx_dots_packed(x, packed),
+                 nk.mx_dots_packed(q, packed, out_dtype=torch.bfloat16), nk.mx_dots_packed(x[:, 3:103], nk.mx_pack(b[:, :100])), weights, chosen,
+                 nk.experts_route_backward(grad, logits, chosen, "sigmoid", scale=1.5), plan.buffer.view(torch.int32)[:8],
+                 nk.mx_dots_experts(x, packed_stack, plan), nk.mx_dots_experts(q, packed_stack, plan, out_dtype=torch.float16),
+                 nk.mx_dots_experts(x, packed_stack, plan, weights, out_dtype=torch.bfloat16),
+                 nk.mx_dots_experts(x.repeat_interleave(2, 0), packed_stack, plan, weights)]
+        assert (plan.tokens, plan.top_k, plan.experts) == (40, 2, 6) and q.shape == (40, 200)
+        return found
+
+    assert binding._CALLS is not None
+    short = calls()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        elsewhere = calls()
+    torch.cuda.synchronize()
+    monkeypatch.setattr(binding, "_CALLS", None)
+    for one, other, general in zip(short, elsewhere, calls()):
+        assert one.dtype == general.dtype and one.shape == general.shape and one.stride() == general.stride()
+        assert torch.equal(one, general) and torch.equal(other, general)

@@ -236,6 +236,29 @@ def test_no_gpu_is_an_error(call):
         call()
 
 
+def test_the_short_way_leaves_the_rest_to_the_general_one():
+    """Operands in host memory, other types and shapes, and things that are no tensors: None, and no error."""
+    lib()
+    calls = binding._CALLS
+    assert calls is not None, "numkong_amd/lib/_mx_calls.so is not built"
+    x, u8 = torch.zeros((4, 64)), torch.zeros((4, 32), dtype=torch.uint8)
+    i32, image_ = torch.zeros((4, 2), dtype=torch.int32), torch.zeros(8, dtype=torch.uint8)
+    for a in (x, x.T, x[0], x.double(), x.numpy(), None, "x", 1):
+        assert calls.quantize(a) is None
+        assert calls.dequantize(u8, a, 64, torch.float32) is None and calls.dequantize(a, u8, 64, torch.float32) is None
+        assert calls.dots(a, None, None, image_, 8, 64, torch.float32) is None and calls.dots(x, None, None, a, 8, 64, a) is None
+        assert calls.route(a, 2, None, 0, True, 1.0, 1, 1, 1) is None and calls.route(x, 2, a, 0, True, 1.0, 1, 1, 1) is None
+        assert calls.route_backward(a, x, i32, 0, True, 1.0) is None and calls.route_backward(x[:, :2], a, i32, 0, True, 1.0) is None
+        assert calls.plan(a, 8) is None and calls.plan(i32, a) is None
+        assert calls.experts(a, None, None, image_, 8, 8, 64, image_, 4, 2, 8, None, torch.float32) is None
+    for name in ("quantize", "dequantize", "dots", "route", "route_backward", "plan", "experts"):
+        assert getattr(calls, name)() is None  # (and too few of them)
+    with pytest.raises(TypeError):
+        calls.bind(1, 2)
+    with pytest.raises(ValueError):
+        calls.bind(*[0] * 10)
+
+
 # ---- the plain forms that the GPU's results are compared with ---------------------------------------------------------
 
 def test_plain_quantising():
