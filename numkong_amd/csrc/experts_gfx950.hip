@@ -195,10 +195,10 @@ struct RouteArgs {
 /**
  *  L lanes for a token: its row stays in registers, J experts a lane, adjacent ones, so that of equal keys the lowest lane's
  *  lowest is the lowest expert. A choice is a maximum over each lane's keys and over the lanes; the lane that holds it takes it
- *  out and notes it. What bounds this is the number of instructions, so 16 lanes serve a token while they can hold its row, and
- *  four tokens share what a choice takes (16,384 tokens of 256 experts, sigmoid and bias, 4 of 8 groups, 8 chosen: 14.9 us with 16
- *  lanes, 20.5 with 64, at 3 us for the traffic; 8192 tokens of 128 experts, 8 chosen: 5.7 and 7.3 us, the gradient 5.8 and 7.7).
- *  Groups of whole lanes are found in registers, others through LDS (the same 16,384 tokens all through LDS: 23.6 us).
+ *  out and notes it. What bounds this is the number of instructions, which 16 lanes to a token share among four of them, and for few
+ *  tokens the time that they take one after the other (with_row). 16,384 tokens of 256 experts, sigmoid and bias, 4 of 8 groups,
+ *  8 chosen: 14 us, at 3 us for the traffic; 8192 tokens of 128 experts, 8 chosen: 5.7 us. Groups of whole lanes are found in
+ *  registers, others through LDS (the same 16,384 tokens through LDS, a lane for four groups: 23.6 us).
  */
 template <class T, int L, int J>
 __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
@@ -228,6 +228,13 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
         uint32_t const groups = (uint32_t)p.how.groups, size = p.experts / groups, lanes = size / J;
         bool const two = p.how.group_top == 2 && size > 1;
         auto const group_key = [&](uint32_t first, uint32_t second) { return two ? key_of(number_of(first) + number_of(second)) : first; };
+        auto const best_two = [&](uint32_t lanes, uint32_t &first, uint32_t &second) __attribute__((always_inline)) { // of adjacent lanes, in all
+            reduce_steps(lanes, [&](auto step) __attribute__((always_inline)) {
+                uint32_t const other = across<decltype(step)::value>(first), next = across<decltype(step)::value>(second);
+                uint32_t const lesser = other < first ? other : first;
+                first = larger(first, other), second = larger(larger(second, next), lesser);
+            });
+        };
         if (size % J == 0 && (lanes & (lanes - 1)) == 0) { // a group is some whole lanes, side by side, and stays in registers
             uint32_t first = key[0], second = 0;
 #pragma unroll
@@ -235,11 +242,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
                 uint32_t const lesser = key[j] < first ? key[j] : first;
                 first = larger(first, key[j]), second = larger(second, lesser);
             }
-            reduce_steps(lanes, [&](auto step) __attribute__((always_inline)) {
-                uint32_t const other = across<decltype(step)::value>(first), next = across<decltype(step)::value>(second);
-                uint32_t const lesser = other < first ? other : first;
-                first = larger(first, other), second = larger(larger(second, next), lesser);
-            });
+            best_two(lanes, first, second);
             uint32_t mine = lane >= groups * lanes ? 0 : group_key(first, second);
             bool stays = false;
             for (int i = 0; i < p.how.top_groups; ++i)
@@ -247,24 +250,29 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
 #pragma unroll
             for (int j = 0; j < J; ++j) key[j] = stays ? key[j] : kMaskedKey;
         }
-        else { // the keys go through LDS, and each lane finds the best of its own groups
+        else { // the keys go through LDS, and some lanes (or one, which may have several groups) find the best of each group
             uint32_t const per_lane = (groups + L - 1) / L;
+            uint32_t share = 1;
+            while (share * 2 * groups <= L) share *= 2;
+            uint32_t const part = lane & (share - 1);
 #pragma unroll
             for (int j = 0; j < J; ++j) keys[local][lane * J + j] = key[j];
             wave_fence();
             uint32_t of_group[kOfLane], stay = 0;
 #pragma unroll
             for (int q = 0; q < kOfLane; ++q) {
-                uint32_t const group = lane * per_lane + q;
+                uint32_t const group = lane / share * per_lane + q;
+                bool const has = q < per_lane && group < groups;
+                uint32_t first = 0, second = 0;
                 of_group[q] = 0;
-                if (q >= per_lane || group >= groups) continue;
-                uint32_t first = 0, second = 0, at = lane % size; // (not all lanes at the same bank)
-                for (uint32_t i = 0; i < size; ++i) {
-                    uint32_t const k = keys[local][group * size + at], lesser = k < first ? k : first;
+                if (q >= per_lane) continue;
+#pragma unroll 4
+                for (uint32_t i = part; has && i < size; i += share) {
+                    uint32_t const k = keys[local][group * size + i], lesser = k < first ? k : first;
                     first = larger(first, k), second = larger(second, lesser);
-                    at = at + 1 == size ? 0 : at + 1;
                 }
-                of_group[q] = group_key(first, second);
+                best_two(share, first, second);
+                if (has && part == 0) of_group[q] = group_key(first, second);
             }
             for (int i = 0; i < p.how.top_groups; ++i) {
                 int const at = take_largest<L, kOfLane>(of_group, lane, 0u, any);
@@ -272,7 +280,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
             }
 #pragma unroll
             for (int q = 0; q < kOfLane; ++q)
-                if (q < per_lane && lane * per_lane + q < 64) notes[local][lane * per_lane + q] = (int32_t)(stay >> q & 1);
+                if (q < per_lane && part == 0 && lane / share * per_lane + q < 64) notes[local][lane / share * per_lane + q] = (int32_t)(stay >> q & 1);
             wave_fence();
             uint32_t group = lane * J / size, left = size - (lane * J - group * size);
 #pragma unroll
@@ -527,13 +535,21 @@ int check_route(nk_dtype_t dtype, void const *logits, nk_size_t stride, nk_size_
     return 0;
 }
 
-/** Calls `f` with a value of the logits' type, and with how many lanes a token has and how many experts a lane holds. */
-template <class F>
-int with_row(nk_dtype_t dtype, size_t experts, F &&f) {
+/**
+ *  Calls `f` with a value of the logits' type, and with how many lanes a token has and how many experts a lane holds. A wavefront
+ *  for a token (`wide`) is done sooner, 16 lanes take fewer instructions in all: with 64 lanes and with 16, 128 experts took 3.6 and
+ *  4.5 us for up to 1,024 tokens, 4.2 and 4.7 for 2,048, 5.3 and 4.9 for 4,096, 12.7 and 8.3 for 16,384; 256 experts in groups 4.4 and 6.1,
+ *  4.9 and 6.2, 6.5 and 6.3, 17.1 and 13.3. The gradient, 128 experts: 2.5 and 3.9, 3.0 and 4.0, 3.9 and 4.2, 8.7 and 7.5; 256 experts:
+ *  3.1 and 6.8, 3.5 and 6.9, 4.6 and 7.5, 12.6 and 14.6, so there a wavefront it is for any number. (Up to 64 experts: no difference.)
+ */
+template <bool ALL_WIDE_PAST_128, class F>
+int with_row(nk_dtype_t dtype, bool wide, size_t experts, F &&f) {
     auto const of_type = [&](auto value) {
         if (experts <= 64) return f(value, Number<16>(), Number<4>());
-        if (experts <= 128) return f(value, Number<16>(), Number<8>());
-        if (experts <= 256) return f(value, Number<16>(), Number<16>());
+        if (experts <= 128) return wide ? f(value, Number<64>(), Number<2>()) : f(value, Number<16>(), Number<8>());
+        if constexpr (!ALL_WIDE_PAST_128)
+            if (experts <= 256 && !wide) return f(value, Number<16>(), Number<16>());
+        if (experts <= 256) return f(value, Number<64>(), Number<4>());
         if (experts <= 512) return f(value, Number<64>(), Number<8>());
         return f(value, Number<64>(), Number<16>());
     };
@@ -557,7 +573,7 @@ int nk_amd_experts_route_async(nk_dtype_t dtype, void const *logits, nk_size_t l
     if (!tokens) return 0;
     if (!weights || !chosen) return mx_fail("experts_route: NULL operand");
     RouteArgs const p = {logits, logits_stride, (uint32_t)tokens, (uint32_t)experts, (uint32_t)top_k, bias, *how, weights, chosen};
-    return with_row(dtype, experts, [&](auto value, auto lanes, auto per_lane) {
+    return with_row<false>(dtype, tokens <= (experts > 128 ? 4096 : 2048), experts, [&](auto value, auto lanes, auto per_lane) {
         typedef decltype(value) T;
         constexpr int L = decltype(lanes)::value, J = decltype(per_lane)::value;
         hipLaunchKernelGGL((route_kernel<T, L, J>), dim3((uint32_t)((tokens + 256 / L - 1) / (256 / L))), dim3(256), 0, (hipStream_t)stream, p);
@@ -575,7 +591,7 @@ int nk_amd_experts_route_backward_async(nk_dtype_t dtype, void const *logits, nk
     int const bytes = dtype == nk_f32_k ? 4 : 2;
     if (((uintptr_t)grad_logits | grad_stride) & (bytes - 1)) return mx_fail("experts_route_backward: grad_logits is not aligned to its elements");
     RouteArgs const p = {logits, logits_stride, (uint32_t)tokens, (uint32_t)experts, (uint32_t)top_k, nullptr, *how, nullptr, (int32_t *)chosen};
-    return with_row(dtype, experts, [&](auto value, auto lanes, auto per_lane) {
+    return with_row<true>(dtype, tokens <= 4096, experts, [&](auto value, auto lanes, auto per_lane) {
         typedef decltype(value) T;
         constexpr int L = decltype(lanes)::value, J = decltype(per_lane)::value;
         hipLaunchKernelGGL((route_backward_kernel<T, L, J>), dim3((uint32_t)((tokens + 256 / L - 1) / (256 / L))), dim3(256), 0,
