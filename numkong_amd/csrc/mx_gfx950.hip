@@ -311,7 +311,8 @@ __device__ __forceinline__ bool image_matches(MxArgs const &p) {
  *  have arrived, and everybody says so. Scales come a super ahead.
  *
  *  Workgroups stay: one walks its tiles, and the fetches of the next tile's first steps go out under the last steps of the one
- *  before, so that a tile starts at once. Each of the eight dies gets one stretch of the walk, eight tiles of rows at a time.
+ *  before, so that a tile starts at once. Each of the eight dies gets one stretch of the walk, in bands of some tiles of rows (bf16,
+ *  us, bands of 8, 4, 2 and 1: tiles of 256 rows, 8192^3 280, 274, 273, 281; tiles of 128, 8192 x 8192 x 1024 51, 54, 55, 65).
  */
 template <int FM, class Out, bool GROUPED>
 __global__ __launch_bounds__(256, FM >= 8 ? 1 : 2) void mx_gemm_kernel(MxArgs p) {
@@ -319,6 +320,7 @@ __global__ __launch_bounds__(256, FM >= 8 ? 1 : 2) void mx_gemm_kernel(MxArgs p)
     static_assert(kA % 4 == 0 && kA % kAhead == 0, "whole fetches; operands of A keep their registers from step to step");
     static_assert(kMeet > kFetches && kMeet >= FM, "before a step's meeting: its fetches of A, its scales, B's first half");
     constexpr int kRows = FM * 32, kColumns = 256;
+    constexpr uint32_t kBand = FM >= 8 ? 4 : 8; // tiles of rows that are walked side by side
     constexpr int kPieces = 64 * (int)sizeof(Out) / 16, kEach = 16 / (int)sizeof(Out); // 16-byte pieces of a wavefront's row of C
     __shared__ __attribute__((aligned(1024))) uint8_t ring0[kA * 1024];
     __shared__ __attribute__((aligned(1024))) uint8_t ring1[kA * 1024];
@@ -351,8 +353,8 @@ __global__ __launch_bounds__(256, FM >= 8 ? 1 : 2) void mx_gemm_kernel(MxArgs p)
         uint32_t tile_m;
         if (GROUPED) tile_m = index / p.tiles_n, t.tile_n = index - tile_m * p.tiles_n; // (an expert's tiles side by side)
         else {
-            uint32_t const band = index / (8 * p.tiles_n), first = band * 8, at = index - band * 8 * p.tiles_n;
-            uint32_t const high = tiles_m - first < 8 ? tiles_m - first : 8;
+            uint32_t const band = index / (kBand * p.tiles_n), first = band * kBand, at = index - band * kBand * p.tiles_n;
+            uint32_t const high = tiles_m - first < kBand ? tiles_m - first : kBand;
             t.tile_n = at / high, tile_m = first + at - t.tile_n * high;
         }
         t.rows = row_tile_of(p, tile_m, kRows);
