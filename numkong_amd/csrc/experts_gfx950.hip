@@ -373,7 +373,6 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs p, float 
 // ---- the plan -----------------------------------------------------------------------------------------------------
 
 constexpr int kPlanWaves = 4, kPlanThreads = 64 * kPlanWaves;
-constexpr size_t kPlanCounted = 4096;
 static_assert(kPlanBlockSlots == 4 * kPlanThreads, "what plan_geometry leaves room for");
 /** Lanes of the wavefront that hold the same bucket, by one ballot for each bit. */
 __device__ __forceinline__ uint64_t same_bucket(uint32_t bucket, int bits, bool active) {
@@ -414,37 +413,24 @@ __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(int32_t const 
 
 /**
  *  Counting sort of the slots by expert. A wavefront has a stretch of them in registers; it counts them, learns where its slots
- *  of each bucket go (behind those of the wavefronts before it, whose counts are in LDS, and of the workgroups before, which it
- *  counts itself where `table` is NULL and has from there where the slots are many), and goes over them again in order, so that
- *  no atomic decides an order. The first workgroup also writes the header, the tiles and the slots of rows that stand between
- *  experts.
+ *  of each bucket go (behind those of the wavefronts before it, whose counts are in LDS, and of the workgroups before, in
+ *  `table`; NULL where there is one workgroup), and goes over them again in order, so that no atomic decides an order. The first
+ *  workgroup also writes the header, the tiles and the slots of rows that stand between experts. Its time is that of a few loads
+ *  and LDS round trips one after the other: 32 slots 3.4 us, 1,024 5.3, 4,004 with the launch that counts 8.5, 32,768 9.4.
  */
 template <int BATCH>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(int32_t const *chosen, uint32_t slots, uint32_t experts, PlanHeader header,
                                                             uint32_t offsets, uint32_t order, uint32_t place, uint32_t tiles, int bits,
                                                             uint32_t const *table, uint32_t *plan) {
-    // [wave][bucket] counts, then where the wave's next slot of the bucket goes; slots of the workgroups before, of those after
-    extern __shared__ uint32_t plan_lds[];
+    extern __shared__ uint32_t plan_lds[]; // [wave][bucket] counts, then where the wave's next slot of the bucket goes
     __shared__ uint32_t wave_total[2][kPlanWaves];
     uint32_t const buckets = experts + 1, thread = threadIdx.x, lane = thread & 63;
     uint32_t const wave = __builtin_amdgcn_readfirstlane(thread >> 6), begin = (blockIdx.x * kPlanWaves + wave) * 64 * BATCH;
     uint32_t mine[BATCH];
     load_stretch(chosen, begin, slots, experts, mine);
-    for (uint32_t i = thread; i < buckets * (kPlanWaves + 2); i += kPlanThreads) plan_lds[i] = 0;
+    for (uint32_t i = thread; i < buckets * kPlanWaves; i += kPlanThreads) plan_lds[i] = 0;
     __syncthreads();
-    uint32_t *counts = plan_lds + wave * buckets, *const of_others = plan_lds + kPlanWaves * buckets;
-    if (!table) {
-        // (stretches of 1024 slots, which are one workgroup's each)
-        for (uint32_t base = wave * 1024; base < slots; base += kPlanWaves * 1024) {
-            if (base / 1024 == blockIdx.x) continue;
-            uint32_t *const there = of_others + (base / 1024 < blockIdx.x ? 0 : buckets);
-            uint32_t its[16];
-            load_stretch(chosen, base, slots, experts, its);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (base + i * 64 + lane < slots) atomicAdd(there + its[i], 1u);
-        }
-    }
+    uint32_t *counts = plan_lds + wave * buckets;
 #pragma unroll
     for (int i = 0; i < BATCH; ++i)
         if (begin + i * 64 + lane < slots) atomicAdd(counts + mine[i], 1u);
@@ -464,7 +450,6 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(int32_t const *chose
                     size += its, earlier += block < blockIdx.x ? its : 0;
                 }
             }
-            else earlier = of_others[bucket], size += earlier + of_others[buckets + bucket];
         }
         uint32_t const its_tiles = (size + header.tile_rows - 1) / header.tile_rows, its_rows = (size + 15) / 16 * 16;
         uint32_t rows = its_rows, tiles_upto = its_tiles; // inclusive sums over the wavefront, then over wavefronts
@@ -615,12 +600,13 @@ int nk_amd_experts_plan_async(nk_i32_t const *chosen, nk_size_t slots, nk_size_t
     int bits = 0;
     while (experts >> bits) ++bits;
     uint32_t const blocks = slots ? (uint32_t)((slots + kPlanBlockSlots - 1) / kPlanBlockSlots) : 1, lds = (uint32_t)((experts + 1) * 4);
-    uint32_t *const table = slots > kPlanCounted ? (uint32_t *)plan + g.table : nullptr;
+    uint32_t *const table = blocks > 1 ? (uint32_t *)plan + g.table : nullptr;
     if (table) hipLaunchKernelGGL(plan_count_kernel, dim3(blocks), dim3(kPlanThreads), lds, (hipStream_t)stream, chosen, (uint32_t)slots, (uint32_t)experts, table);
-    // Slots that fit one a lane are not followed by three more. A launch that counts goes first where the slots are many (us, with
-    // and without: 2,048 slots 8.2 and 7.5, 4,004 8.5 and 7.3, 8,192 8.3 and 9.5, 32,768 9.4 and 21.9).
+    // Slots that fit one a lane are not followed by three more. (Up to 4,096 slots without the launch that counts, each workgroup
+    // counting all slots: 7.3 us instead of 8.5 by itself, but 11.0 instead of 9.4 where `chosen` is not in the caches any more; eight
+    // slots a lane: 15.5 us for 32,768.)
     auto *const kernel = slots <= kPlanThreads ? plan_kernel<1> : plan_kernel<4>;
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kPlanThreads), lds * (kPlanWaves + 2), (hipStream_t)stream, chosen, (uint32_t)slots, (uint32_t)experts,
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kPlanThreads), lds * kPlanWaves, (hipStream_t)stream, chosen, (uint32_t)slots, (uint32_t)experts,
                        header, (uint32_t)g.offsets, (uint32_t)g.order, (uint32_t)g.place, (uint32_t)g.tiles, bits, table, (uint32_t *)plan);
     hipError_t const e = hipGetLastError();
     return e == hipSuccess ? 0 : mx_fail(e, "plan_kernel");

@@ -251,9 +251,9 @@ def test_experts_products(tokens, top_k, experts, kind, n, k, dtype, out):
     mx.close(got, summed, magnitudes, k, extra)
 
 
-@pytest.mark.parametrize("tokens,top_k,experts,n,k", [(4200, 8, 16, 130, 513), (3000, 6, 40, 77, 1000)])
+@pytest.mark.parametrize("tokens,top_k,experts,n,k", [(4200, 8, 16, 130, 513), (3000, 6, 40, 77, 1000), (4200, 8, 16, 600, 700), (6000, 8, 16, 1100, 200)])
 def test_rows_that_go_to_many(tokens, top_k, experts, n, k):
-    """So many slots that the rows are quantised first and gathered as codes: the same values as one product for each expert."""
+    """Rows that several experts have, some as floats and some quantised first, one tile to a workgroup and several."""
     chosen = torch.from_numpy(routing(tokens, top_k, experts, "some", 3))
     a, stack = normal(tokens, k, torch.bfloat16, 1, 0.2).to(DEV), normal(experts * n, k, torch.float32, 2, 0.2).reshape(experts, n, k).to(DEV)
     got = nk.mx_dots_experts(a, nk.mx_pack(stack), nk.experts_plan(chosen.to(DEV), experts))
