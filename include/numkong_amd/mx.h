@@ -14,8 +14,9 @@
  *  Rows of codes take (depth + 1) / 2 bytes, rows of scales (depth + 31) / 32.
  *
  *  Every call queues its work on `stream` (a hipStream_t, NULL = the default stream), touches device memory only, neither
- *  allocates nor synchronises, may be captured into a HIP graph, and returns 0 or a status that `nk_hip_last_error()`
- *  explains. Strides are in bytes. Sums are held in 32 bits; no result depends on the order in which workgroups run.
+ *  allocates nor synchronises, may be captured into a HIP graph (after one eager call, which loads the kernels), and returns 0
+ *  or a status that `nk_hip_last_error()` explains. Strides are in bytes. Sums are held in 32 bits; no result depends on the
+ *  order in which workgroups run.
  */
 #ifndef NUMKONG_AMD_MX_H
 #define NUMKONG_AMD_MX_H
@@ -39,8 +40,9 @@ NK_DYNAMIC int nk_amd_mx_dequantize_async(nk_dtype_t dtype, void const *codes, n
                                           void const *scales, nk_size_t scales_stride, nk_size_t rows, nk_size_t depth,
                                           void *x, nk_size_t x_stride, void *stream);
 
-/** Bytes of the packed image of `count` matrices of width x depth (0: no such image). The image is this library's own
- *  format (the operand order of the matrix instructions), relocatable, and must be 16-byte aligned. */
+/** Bytes of the packed image of `count` matrices of width x depth (0: no such image; width has to be below 2^31, depth below
+ *  2^25, count below 2^20). The image is this library's own format (the operand order of the matrix instructions),
+ *  relocatable, and must be 16-byte aligned. */
 NK_DYNAMIC nk_size_t nk_amd_mx_packed_size(nk_size_t count, nk_size_t width, nk_size_t depth);
 /** Packs `count` matrices, matrix i at codes + i * codes_matrix and scales + i * scales_matrix bytes. */
 NK_DYNAMIC int nk_amd_mx_pack_async(void const *codes, nk_size_t codes_stride, nk_size_t codes_matrix,
@@ -51,7 +53,8 @@ NK_DYNAMIC int nk_amd_mx_pack_async(void const *codes, nk_size_t codes_stride, n
  *  C[height x width] = A * B^T. A: floats of `a_dtype`, quantised on the way (exactly as nk_amd_mx_quantize_async does), or,
  *  where `a_scales` is not NULL, codes at `a` and scales (then `a_dtype` is not looked at). C: f32, bf16 or f16 by `c_dtype`.
  *  `workspace`: device memory, 256-byte aligned, of nk_amd_mx_dots_workspace_size bytes (which may be 0, then NULL will do);
- *  it belongs to the call until the stream has run it. An image whose header does not say width x depth gives NaNs.
+ *  it belongs to the call until the stream has run it. An image whose header does not say width x depth gives NaNs. A block
+ *  of NaN (scale 255) makes every result NaN that it goes into, also where the other operand's values are zero.
  */
 NK_DYNAMIC nk_size_t nk_amd_mx_dots_workspace_size(nk_size_t height, nk_size_t width, nk_size_t depth, int a_is_codes);
 NK_DYNAMIC int nk_amd_mx_dots_packed_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_stride, void const *a_scales,
@@ -99,7 +102,8 @@ NK_DYNAMIC int nk_amd_experts_plan_async(nk_i32_t const *chosen, nk_size_t slots
  *  y[slot] = A[slot / a_share] * B[expert of slot]^T for every slot, zeros where there is no expert: A has
  *  ceil(slots / a_share) rows (a_share = top_k: a row for each token; 1: a row for each slot). With `weights` (slots, f32)
  *  the `top_k` rows of a token are summed by weight into C[slots / top_k x width] instead, slots without an expert left
- *  out. A, C and workspace as in nk_amd_mx_dots_packed_async; the image holds `experts` matrices.
+ *  out, in 32 bits and in the order of the slots. A, C and workspace as in nk_amd_mx_dots_packed_async; the image holds
+ *  `experts` matrices, and the plan is one of nk_amd_experts_plan_async for these slots and experts.
  */
 NK_DYNAMIC nk_size_t nk_amd_mx_experts_workspace_size(nk_size_t slots, nk_size_t a_share, nk_size_t experts,
                                                       nk_size_t width, nk_size_t depth, int a_is_codes,
