@@ -103,7 +103,7 @@ NK_DYNAMIC int nk_amd_experts_plan_async(nk_i32_t const *chosen, nk_size_t slots
  *  ceil(slots / a_share) rows (a_share = top_k: a row for each token; 1: a row for each slot). With `weights` (slots, f32)
  *  the `top_k` rows of a token are summed by weight into C[slots / top_k x width] instead, slots without an expert left
  *  out, in 32 bits and in the order of the slots. A, C and workspace as in nk_amd_mx_dots_packed_async; the image holds
- *  `experts` matrices, and the plan is one of nk_amd_experts_plan_async for these slots and experts.
+ *  `experts` matrices, and the plan is one of nk_amd_experts_plan_async for these slots and experts (another gives NaNs).
  */
 NK_DYNAMIC nk_size_t nk_amd_mx_experts_workspace_size(nk_size_t slots, nk_size_t a_share, nk_size_t experts,
                                                       nk_size_t width, nk_size_t depth, int a_is_codes,

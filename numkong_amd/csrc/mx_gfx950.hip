@@ -90,8 +90,14 @@ struct StageArgs {
     uint8_t *to, *to_scales;
     uint32_t const *plan; // rows in the plan's order, or NULL
     uint32_t rows, k, supers, order, a_share;
+    uint32_t slots, experts; // that the plan is for
     bool wide;
 };
+/** Is what is at `plan` a plan for so many slots and experts? (One of others has its parts elsewhere, and may end sooner.) */
+__device__ __forceinline__ bool plan_matches(void const *plan, uint32_t slots, uint32_t experts) {
+    PlanHeader const &h = *(PlanHeader const *)plan;
+    return h.magic == kPlanMagic && h.slots == slots && h.experts == experts;
+}
 /** The row of A that row `row` of the fragments is; false where there is none. */
 __device__ __forceinline__ bool source_of(StageArgs const &p, uint32_t row, uint64_t &source) {
     source = row;
@@ -115,7 +121,7 @@ __global__ __launch_bounds__(256) void stage_kernel(StageArgs p) {
     uint32_t const tile = blockIdx.x / p.supers, super = blockIdx.x - tile * p.supers;
     uint32_t const lane = threadIdx.x & 63, u = threadIdx.x >> 6, piece = lane & 15, g = piece >> 2;
     uint32_t const block = (super * 4 + u) * 4 + g, col = block * 32 + (piece & 3) * 8;
-    if (p.plan && tile * 16 >= ((PlanHeader const *)p.plan)->first_zero) return;
+    if (p.plan && (!plan_matches(p.plan, p.slots, p.experts) || tile * 16 >= ((PlanHeader const *)p.plan)->first_zero)) return;
     bool const whole = p.wide && col + 8 <= p.k;
     In const *from[4];
     bool there[4];
@@ -158,7 +164,7 @@ __global__ __launch_bounds__(256) void stage_codes_kernel(StageArgs p) {
     __shared__ __attribute__((aligned(4))) uint8_t bytes[256];
     uint32_t const tile = blockIdx.x / p.supers, super = blockIdx.x - tile * p.supers;
     uint32_t const lane = threadIdx.x & 63, u = threadIdx.x >> 6, r = lane & 15, g = lane >> 4, block = (super * 4 + u) * 4 + g;
-    if (p.plan && tile * 16 >= ((PlanHeader const *)p.plan)->first_zero) return;
+    if (p.plan && (!plan_matches(p.plan, p.slots, p.experts) || tile * 16 >= ((PlanHeader const *)p.plan)->first_zero)) return;
     uint64_t source;
     v4u codes = {0, 0, 0, 0};
     uint32_t scale = 0;
@@ -336,6 +342,11 @@ __global__ __launch_bounds__(256, FM >= 8 ? 1 : 2) void mx_gemm_kernel(MxArgs p)
 
     uint32_t const lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
     uint32_t const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (GROUPED && !plan_matches(p.plan, p.m, p.count)) { // NaNs (sums by weight become that where they are made)
+        for (uint32_t slot = blockIdx.x; !p.sorted && slot < p.m; slot += gridDim.x)
+            for (uint32_t column = threadIdx.x; column < p.n; column += 256) ((Out *)(p.c + slot * p.c_stride))[column] = (Out)__uint_as_float(0x7FC00000u);
+        return;
+    }
     if (GROUPED && !p.sorted) { // rows of no expert are zeros
         PlanHeader const &h = *(PlanHeader const *)p.plan;
         for (uint32_t at = h.first_zero + blockIdx.x; at < h.end_zero; at += gridDim.x) {
@@ -569,6 +580,12 @@ __global__ __launch_bounds__(64 * WAVES, FM >= 4 ? 2 : 4) void mx_few_kernel(MxA
     }
     else {
         tile_m = blockIdx.x / p.tiles_n, tile_n = blockIdx.x - tile_m * p.tiles_n;
+        if (!plan_matches(p.plan, p.m, p.count)) { // NaNs, as in mx_gemm_kernel
+            uint32_t const column = tile_n * NT * 16 + threadIdx.x;
+            if (!p.sorted && threadIdx.x < NT * 16 && column < p.n)
+                for (uint32_t slot = tile_m; slot < p.m; slot += p.tiles_m) ((Out *)(p.c + slot * p.c_stride))[column] = (Out)__uint_as_float(0x7FC00000u);
+            return;
+        }
         PlanHeader const &h = *(PlanHeader const *)p.plan;
         if (tile_m >= h.tile_count + (p.sorted ? 0 : h.zero_tiles)) return;
     }
@@ -688,14 +705,16 @@ __global__ __launch_bounds__(64 * WAVES, FM >= 4 ? 2 : 4) void mx_few_kernel(MxA
 /** out[token] = sum over its slots of weight * row of the plan, slots without an expert left out; a thread for four columns, four
  *  rows under way at a time. Memory bounds it (1001 tokens, 4 of 2050 columns: 7.3 us, 5.6 TB/s). */
 template <class Out>
-__global__ __launch_bounds__(256) void combine_kernel(float const *rows, uint64_t row_values, uint32_t const *plan, uint32_t place,
-                                                      float const *weights, uint32_t top_k, uint32_t tokens, uint32_t n,
-                                                      uint32_t pieces, Out *c, uint64_t c_stride) {
+__global__ __launch_bounds__(256) void combine_kernel(float const *rows, uint64_t row_values, uint32_t const *plan, uint32_t slots,
+                                                      uint32_t experts, uint32_t place, float const *weights, uint32_t top_k,
+                                                      uint32_t tokens, uint32_t n, uint32_t pieces, Out *c, uint64_t c_stride) {
     uint32_t const index = blockIdx.x * 256 + threadIdx.x;
     uint32_t const token = index / pieces, column = (index - token * pieces) * 4;
     if (token >= tokens) return;
-    float sum[4] = {0, 0, 0, 0};
-    for (uint32_t first = 0; first < top_k; first += 4) {
+    bool const good = plan_matches(plan, slots, experts);
+    float const start = good ? 0.0f : __uint_as_float(0x7FC00000u);
+    float sum[4] = {start, start, start, start};
+    for (uint32_t first = 0; good && first < top_k; first += 4) {
         int32_t row[4];
         float weight[4];
         v4f values[4];
@@ -774,12 +793,12 @@ Staging staging_of(uint64_t rows, MxGeometry const &g) {
 }
 /** A into the workspace: rows in order, or the rows of a plan. */
 int stage(int a_dtype, void const *a, uint64_t a_stride, void const *a_scales, uint64_t a_scales_stride, uint32_t rows, uint32_t k,
-          MxGeometry const &g, Staging const &s, uint8_t *to, void const *plan, size_t order, uint32_t a_share, hipStream_t stream) {
+          MxGeometry const &g, Staging const &s, uint8_t *to, void const *plan, size_t order, uint32_t a_share, uint32_t slots, uint32_t experts, hipStream_t stream) {
     uint64_t const grid = (uint64_t)((rows + 15) / 16) * g.supers;
     if (!grid) return 0;
     if (grid > 0x7FFFFFFFull) return mx_fail("mx product: A is too large");
     StageArgs const p = {a, a_stride, (uint8_t const *)a_scales, a_scales_stride, to, to + s.scales_at, (uint32_t const *)plan, rows, k,
-                         g.supers, (uint32_t)order, a_share, aligned(a, a_stride, 16)};
+                         g.supers, (uint32_t)order, a_share, slots, experts, aligned(a, a_stride, 16)};
     if (a_scales) hipLaunchKernelGGL(stage_codes_kernel, dim3((uint32_t)grid), dim3(256), 0, stream, p);
     else
         with_type(a_dtype, [&](auto value) {
@@ -999,7 +1018,7 @@ int nk_amd_mx_dots_packed_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_s
         Staging const s = staging_of(height, g);
         if (s.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < s.bytes))
             return mx_fail("mx_dots_packed: the workspace is too small or not 256-byte aligned");
-        if (int const status = stage(a_dtype, a, a_stride, a_scales, a_scales_stride, p.m, p.k, g, s, (uint8_t *)workspace, nullptr, 0, 1, stream))
+        if (int const status = stage(a_dtype, a, a_stride, a_scales, a_scales_stride, p.m, p.k, g, s, (uint8_t *)workspace, nullptr, 0, 1, 0, 0, stream))
             return status;
         p.a = (uint8_t const *)workspace, p.a_scales = p.a + s.scales_at;
     }
@@ -1046,7 +1065,7 @@ int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_
                 return status;
             a = codes, a_stride = l.codes_stride, a_scales = scales, a_scales_stride = l.codes_scales_stride;
         }
-        if (int const status = stage(a_dtype, a, a_stride, a_scales, a_scales_stride, shape.max_rows, p.k, g, l.staged, (uint8_t *)workspace, plan, shape.order, p.a_share, stream))
+        if (int const status = stage(a_dtype, a, a_stride, a_scales, a_scales_stride, shape.max_rows, p.k, g, l.staged, (uint8_t *)workspace, plan, shape.order, p.a_share, p.m, p.count, stream))
             return status;
         p.a = (uint8_t const *)workspace, p.a_scales = p.a + l.staged.scales_at;
     }
@@ -1066,7 +1085,7 @@ int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_
         int const done = with_type(c_dtype, [&](auto value) {
             typedef decltype(value) Out;
             hipLaunchKernelGGL((combine_kernel<Out>), dim3((uint32_t)((here * pieces + 255) / 256)), dim3(256), 0, stream,
-                               (float const *)sums, l.sums_values, p.plan, place, weights + first * top_k, (uint32_t)top_k, (uint32_t)here,
+                               (float const *)sums, l.sums_values, p.plan, p.m, p.count, place, weights + first * top_k, (uint32_t)top_k, (uint32_t)here,
                                p.n, (uint32_t)pieces, (Out *)((uint8_t *)c + first * c_stride), (uint64_t)c_stride);
             hipError_t const e = hipGetLastError();
             return e == hipSuccess ? 0 : mx_fail(e, "combine_kernel");

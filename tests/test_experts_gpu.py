@@ -265,6 +265,18 @@ def test_rows_that_go_to_many(tokens, top_k, experts, n, k):
     assert not got[((chosen < 0) | (chosen >= experts)).to(DEV)].any()
 
 
+@pytest.mark.parametrize("tokens,experts", [(3, 8), (200, 8), (900, 4)])  # few rows to an expert, some, many
+def test_plan_of_other_sizes_gives_nans(tokens, experts):
+    a, packed = torch.ones((tokens, 64), device=DEV), nk.mx_pack(torch.ones((experts, 80, 64), device=DEV))
+    right = nk.experts_plan(torch.zeros((tokens, 2), dtype=torch.int32, device=DEV), experts)
+    for other in (nk.experts_plan(torch.zeros((tokens + 1, 2), dtype=torch.int32, device=DEV), experts),
+                  nk.experts_plan(torch.zeros((tokens, 2), dtype=torch.int32, device=DEV), experts + 1)):
+        wrong = nk.ExpertsPlan(tokens, 2, experts, other.buffer)
+        assert torch.isnan(nk.mx_dots_experts(a, packed, wrong)).all()
+        assert torch.isnan(nk.mx_dots_experts(a, packed, wrong, torch.ones((tokens, 2), device=DEV))).all()
+    assert (nk.mx_dots_experts(a, packed, right) == 64).all()
+
+
 def test_no_tokens():
     packed = nk.mx_pack(torch.ones((4, 64, 64), device=DEV))
     plan = nk.experts_plan(torch.zeros((0, 2), dtype=torch.int32, device=DEV), 4)
