@@ -15,7 +15,8 @@ ROUTES = [(1, 1, 1, "softmax", False, 1, 1, 1), (5, 8, 2, "softmax", False, 1, 1
           (33, 60, 4, "softmax", False, 1, 1, 1), (7, 64, 6, "softmax", True, 1, 1, 1), (64, 65, 8, "sigmoid", False, 1, 1, 1),
           (100, 128, 8, "softmax", False, 1, 1, 1), (50, 256, 8, "sigmoid", True, 8, 4, 2), (50, 160, 6, "softmax", False, 8, 3, 1),
           (20, 96, 4, "sigmoid", True, 12, 5, 2), (20, 30, 5, "softmax", True, 30, 9, 2), (11, 500, 10, "sigmoid", True, 4, 2, 2),
-          (6, 1000, 64, "softmax", False, 1, 1, 1), (6, 1024, 16, "sigmoid", True, 64, 20, 2), (4099, 72, 3, "softmax", False, 3, 2, 2)]
+          (6, 1000, 64, "softmax", False, 1, 1, 1), (6, 1024, 16, "sigmoid", True, 64, 20, 2), (4099, 72, 3, "softmax", False, 3, 2, 2),
+          (4200, 256, 8, "sigmoid", True, 8, 4, 2), (4100, 200, 4, "softmax", False, 5, 2, 1), (4097, 210, 20, "sigmoid", True, 21, 10, 2)]
 
 
 def logits_of(tokens, experts, dtype, seed):
@@ -99,6 +100,23 @@ def test_masked_logits(score, experts, groups, top_groups):
     assert bool(grad.isfinite().all()) and not grad[0].any() and not grad[logits.isneginf().to(DEV)].any()
 
 
+@pytest.mark.parametrize("experts,groups,top_groups", [(100, 1, 1), (100, 5, 2), (144, 1, 1), (144, 9, 3), (256, 8, 3)])
+def test_many_tokens_choose_as_few(experts, groups, top_groups):
+    """Masks, ties, NaNs and infinities among as many tokens as share wavefronts: chosen as where a token has its own. (Sigmoid
+    scores are those of each logit alone; weights differ by the order of a sum of four.)"""
+    logits = logits_of(32, experts, torch.float32, 8)
+    logits[0], logits[1, 3:], logits[2, :-2], logits[3] = -float("inf"), -float("inf"), -float("inf"), 0.25
+    logits[4, 7], logits[5, 9], logits[6] = float("nan"), float("inf"), torch.finfo(torch.float32).min
+    logits[7:12] = logits[7:12].round()
+    logits = logits.to(DEV)
+    bias = (torch.arange(experts, device=DEV) % 4).float()
+    for of in (None, bias):
+        weights, chosen = nk.experts_route(logits, 4, "sigmoid", of, groups, top_groups, 2)
+        many, many_chosen = nk.experts_route(logits.repeat(160, 1), 4, "sigmoid", of, groups, top_groups, 2)
+        assert torch.equal(many_chosen, chosen.repeat(160, 1))
+        torch.testing.assert_close(many, weights.repeat(160, 1), rtol=2.0**-21, atol=0.0, equal_nan=True)
+
+
 def test_nan_and_infinity_show():
     logits = logits_of(3, 16, torch.float32, 2)
     logits[0, 5], logits[1, 6] = float("nan"), float("inf")
@@ -113,7 +131,8 @@ def test_nan_and_infinity_show():
                          [(1, 4, 2, "softmax", True, torch.float32), (40, 64, 4, "softmax", True, torch.float32),
                           (40, 100, 4, "softmax", False, torch.bfloat16), (33, 256, 8, "sigmoid", True, torch.float32),
                           (33, 130, 8, "sigmoid", False, torch.float16), (9, 1000, 64, "softmax", True, torch.float32),
-                          (5, 300, 1, "sigmoid", False, torch.float32)])
+                          (5, 300, 1, "sigmoid", False, torch.float32), (4200, 100, 4, "softmax", True, torch.float32),
+                          (4200, 160, 20, "sigmoid", True, torch.float32)])
 def test_route_gradient(tokens, experts, top_k, score, renormalize, dtype):
     """Against the formula's gradient in 64 bits, from autograd; padding and missing experts among the rows."""
     logits = logits_of(tokens, experts, dtype, tokens)
