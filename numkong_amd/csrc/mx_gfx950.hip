@@ -282,6 +282,7 @@ struct MxArgs {
     uint64_t a_pitch, c_stride;
     uint32_t m, n, k, steps, supers, tiles, count;
     uint32_t tiles_m, tiles_n; // the grid: tiles of rows, tiles of columns
+    uint32_t band;             // tiles of rows that are walked side by side
     uint32_t order, tile_list; // words into the plan
     uint32_t a_share;          // slots that share a row of A
     uint32_t sorted;           // 1: results in the plan's order of rows (and nothing for rows of no expert), 0: at their slots
@@ -318,8 +319,10 @@ __device__ __forceinline__ bool image_matches(MxArgs const &p) {
  *  have arrived, and everybody says so. Scales come a super ahead.
  *
  *  Workgroups stay: one walks its tiles, and the fetches of the next tile's first steps go out under the last steps of the one
- *  before, so that a tile starts at once. Each of the eight dies gets one stretch of the walk, in bands of some tiles of rows (bf16,
- *  us, bands of 8, 4, 2 and 1: tiles of 256 rows, 8192^3 280, 274, 273, 281; tiles of 128, 8192 x 8192 x 1024 51, 54, 55, 65).
+ *  before, so that a tile starts at once. Each of the eight dies gets one stretch of the walk, in bands of some tiles of rows: low
+ *  bands write whole rows at a time, which memory takes faster (stores alone, 268 MB of f32: bands of 256 rows 45 us, 512 52, 1,024
+ *  60, 2,048 64), high ones read less of B (us, bands of 1, 2, 4 and 8: tiles of 128 rows, bf16 8192 x 8192 x 1024 68, 57, 63, 60, x 4096
+ *  190, 150, 145, 147, f32 8192 x 6656 x 2048 103, 88, 91, 92; tiles of 256, 8192^3 bf16 270, 262, 262, 274, f32 284, 275, 295, 300).
  *
  *  8192^3 with bf16 results takes 241 to 257 us (4.3 to 4.6 PFLOP/s; the matrix instructions alone, on the same random codes, 6.5):
  *  power holds the clock at 1.6 GHz, a step takes 1226 cycles of which 1024 are matrix instructions, a tile's end a tenth of its
@@ -332,7 +335,6 @@ __global__ __launch_bounds__(256, FM >= 8 ? 1 : 2) void mx_gemm_kernel(MxArgs p)
     static_assert(kA % 4 == 0 && kA % kAhead == 0, "whole fetches; operands of A keep their registers from step to step");
     static_assert(kMeet > kFetches && kMeet >= FM, "before a step's meeting: its fetches of A, its scales, B's first half");
     constexpr int kRows = FM * 32, kColumns = 256;
-    constexpr uint32_t kBand = FM >= 8 ? 4 : 8; // tiles of rows that are walked side by side
     constexpr int kPieces = 64 * (int)sizeof(Out) / 16, kEach = 16 / (int)sizeof(Out); // 16-byte pieces of a wavefront's row of C
     __shared__ __attribute__((aligned(1024))) uint8_t ring0[kA * 1024];
     __shared__ __attribute__((aligned(1024))) uint8_t ring1[kA * 1024];
@@ -370,8 +372,8 @@ __global__ __launch_bounds__(256, FM >= 8 ? 1 : 2) void mx_gemm_kernel(MxArgs p)
         uint32_t tile_m;
         if (GROUPED) tile_m = index / p.tiles_n, t.tile_n = index - tile_m * p.tiles_n; // (an expert's tiles side by side)
         else {
-            uint32_t const band = index / (kBand * p.tiles_n), first = band * kBand, at = index - band * kBand * p.tiles_n;
-            uint32_t const high = tiles_m - first < kBand ? tiles_m - first : kBand;
+            uint32_t const band = index / (p.band * p.tiles_n), first = band * p.band, at = index - band * p.band * p.tiles_n;
+            uint32_t const high = tiles_m - first < p.band ? tiles_m - first : p.band;
             t.tile_n = at / high, tile_m = first + at - t.tile_n * high;
         }
         t.rows = row_tile_of(p, tile_m, kRows);
@@ -838,7 +840,7 @@ int launch_few(MxArgs &p, uint32_t max_rows, MxGeometry const &g, hipStream_t st
 }
 template <int FM, class Out, bool GROUPED>
 int launch_gemm(MxArgs &p, hipStream_t stream) {
-    p.tiles_n = (p.tiles + 15) / 16;
+    p.tiles_n = (p.tiles + 15) / 16, p.band = FM >= 8 || p.steps <= 16 ? 2 : 4;
     if (!GROUPED) p.tiles_m = (p.m + 32 * FM - 1) / (32 * FM);
     uint64_t const tiles = (uint64_t)p.tiles_m * p.tiles_n, resident = (uint64_t)compute_unit_count() * (FM >= 8 ? 1 : 2);
     if (tiles > 0x7FFFFFFFull) return mx_fail("mx product: too many tiles");
@@ -855,15 +857,18 @@ int launch_gemm(MxArgs &p, hipStream_t stream) {
  *  compute units idle (us, few rows against many: 128 x 8192 x 8192 19.1 and 27.1, 512 x 2048 x 2048 10.6 and 12.5, 1024 x 1024 x
  *  8192 23.1 and 30.8; at 64 tiles 256 x 8192 x 8192 29.9 and 28.5, 1024 x 2048 x 2048 15.4 and 13.9). A workgroup of few rows
  *  takes one tile of columns while there are fewer than 512 (64 x 2048 x 2048 7.0 us with one, 7.5 with two; 64 x 8192 x 8192
- *  17.0 and 15.0). Tiles of 256 rows from 256 of them on: less of B is read for the same work, the compute units are full. But a
- *  workgroup's results hold up its next tile (stores are waited for in order), and where 16-bit results come every 16 steps or more
- *  often, two workgroups of 128 rows that hide that from each other are faster (8192 x 8192, us, 128 rows and 256: bf16 depth 512
- *  45.3 and 56.0, 1024 62.2 and 69.8, 2048 88.4 and 94.2, 4096 174 and 156; f32 depth 1024 105 and 96).
+ *  17.0 and 15.0). Among many rows tiles of 128, two workgroups to a compute unit, which hide
+ *  each other's ends (a workgroup's results hold up its next tile: stores are waited for in order); of 256 only past a depth of
+ *  6,144 and where they fill the compute units in whole rounds, as less of B is read then (us, 128 rows and 256: bf16 8192 x 8192,
+ *  depth 512 41 and 54, 1,024 57 and 73, 4,096 146 and 151, 6,144 205 and 205, 8,192 265 and 263, 16384 x 8192 x 8192 543 and 522, f32
+ *  8192^3 289 and 273; but 9000 x 9000 x 8192, 6 rounds of 256 rows for 5.06, 327 and 356, 6000 x 6000 x 8192, 3 for 2.25, 164 and 183).
  */
 template <class Out, bool GROUPED>
 int launch_product(MxArgs &p, uint32_t tile_rows, int a_dtype, bool fused, uint32_t fused_rows, MxGeometry const &g, hipStream_t stream) {
     auto const tiles_of = [&](uint64_t rows, uint64_t columns) { return (p.m + rows - 1) / rows * ((p.n + columns - 1) / columns); };
-    uint32_t const rows = GROUPED ? tile_rows : p.m <= 32 || tiles_of(128, 256) < 64 ? (p.m < 64 ? p.m : 64) : tiles_of(256, 256) < 256 || (sizeof(Out) == 2 && g.steps <= 16) ? 128 : 256;
+    uint64_t const large = tiles_of(256, 256), rounds = (large + 255) / 256;
+    bool const whole_rounds = large * 20 >= rounds * 256 * 19;
+    uint32_t const rows = GROUPED ? tile_rows : p.m <= 32 || tiles_of(128, 256) < 64 ? (p.m < 64 ? p.m : 64) : g.steps > 48 && whole_rounds ? 256 : 128;
     if (rows <= 16) {
         constexpr int NT = GROUPED ? 2 : 1; // (experts of 4 tokens, 28 matrices of 2048 x 2048: 13.0 us with two, 14.0 with one)
         if (!fused) return launch_few<1, NT, uint8_t, Out, GROUPED>(p, rows, g, stream);

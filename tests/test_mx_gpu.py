@@ -160,6 +160,26 @@ def test_special_values_stay_in_their_rows(m, n):
     assert (np.abs(got - truth)[~nans] <= mx.sum_bound(k, np.nan_to_num(magnitude))[~nans] + 2.0**-24 * np.abs(truth[~nans])).all()
 
 
+def test_deep_products_in_whole_rounds():
+    """Two tiles of 256 x 256 to a compute unit, the last ones cut on both sides; rows that start anywhere, a NaN among them, a
+    result inside a larger matrix. (The 64-bit products of the plain form's values are made on the GPU.)"""
+    m, n, k = 8100, 4050, 6200
+    a, b = normal(m, k, torch.bfloat16, 1, 0.3), normal(n, k, torch.bfloat16, 2, 0.3)
+    a[4000, 6199], b[77, 0] = float("nan"), float("inf")
+    left, right = torch.from_numpy(mx.rounded(a)).to(DEV), torch.from_numpy(mx.rounded(b)).to(DEV).T.contiguous()
+    truth, magnitude = (left @ right).cpu().numpy(), (left.abs() @ right.abs()).cpu().numpy()
+    packed = nk.mx_pack(b.to(DEV))
+    for out_dtype in FLOATS:
+        store = torch.full((m + 2, n + 9), 77.0, dtype=out_dtype, device=DEV)
+        out = store[1:-1, 3:3 + n]
+        nk.mx_dots_packed(strided(a, 1, 1), packed, out=out)
+        mx.close(out, truth, magnitude, k)
+        again = nk.mx_dots_packed(a.to(DEV), packed, out_dtype=out_dtype)
+        assert torch.equal(again.nan_to_num(0.0), out.nan_to_num(0.0))
+        store[1:-1, 3:3 + n] = 77.0
+        assert bool((store == 77.0).all())
+
+
 def test_scales_of_every_size():
     """Products of scales past the range of 32-bit floats overflow and vanish as the products of the values do."""
     scale_pairs = [(127, 127), (0, 254), (0, 127), (60, 67), (254, 126), (200, 180), (1, 100), (0, 0)]
