@@ -23,7 +23,7 @@ constexpr uint32_t kStretches = sizeof(T) == 4 ? 1 : 2;
  */
 template <class T>
 __global__ __launch_bounds__(256) void quantize_kernel(T const *x, uint64_t x_stride, uint32_t rows, uint32_t k, uint32_t stretches,
-                                                       bool wide, uint8_t *codes, uint64_t codes_stride, bool whole_words,
+                                                       uint8_t *codes, uint64_t codes_stride,
                                                        uint8_t *scales, uint64_t scales_stride) {
     constexpr int N = kEach<T>, kHalves = 8 / N;
     uint32_t const lane = threadIdx.x & 63, first = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kStretches<T>;
@@ -36,8 +36,8 @@ __global__ __launch_bounds__(256) void quantize_kernel(T const *x, uint64_t x_st
         for (int half = 0; half < kHalves; ++half) {
             uint32_t const col = from[t] + half * 256 + lane * N;
             raw[t][half] = v4u {0, 0, 0, 0};
-            if (wide && row[t] < rows && col + N <= k)
-                raw[t][half] = __builtin_nontemporal_load((v4u const *)((T const *)((uint8_t const *)x + row[t] * x_stride) + col));
+            if (row[t] < rows && col + N <= k)
+                raw[t][half] = __builtin_nontemporal_load((v4u_anywhere const *)((T const *)((uint8_t const *)x + row[t] * x_stride) + col));
         }
     }
 #pragma unroll
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(T const *x, uint64_t x_st
         for (int half = 0; half < kHalves; ++half) {
             uint32_t const col = from[t] + half * 256 + lane * N;
             float v[N];
-            if (wide && col + N <= k) widen<T>(raw[t][half], v);
+            if (col + N <= k) widen<T>(raw[t][half], v);
             else load_some((T const *)((uint8_t const *)x + row[t] * x_stride), col, k, v);
             word[half] = quantize_some(v, scale[half]);
         }
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(T const *x, uint64_t x_st
         }
         uint32_t const col = from[t] + at * 8, bytes = col >= k ? 0 : (k - col + 1) / 2;
         uint8_t *to = codes + row[t] * codes_stride + col / 2;
-        if (whole_words && bytes >= 4) *(uint32_t *)to = its_word;
+        if (bytes >= 4) *(u32_anywhere *)to = its_word;
         else
             for (uint32_t i = 0; i < (bytes < 4 ? bytes : 4); ++i) to[i] = (uint8_t)(its_word >> 8 * i);
         if (has_scale && from[t] + block * 32 < k) scales[row[t] * scales_stride + from[t] / 32 + block] = (uint8_t)its_scale;
@@ -71,9 +71,9 @@ __global__ __launch_bounds__(256) void quantize_kernel(T const *x, uint64_t x_st
 }
 
 /** A block's 16 bytes of a row's codes; zeros from column k on. */
-__device__ __forceinline__ v4u load_codes(uint8_t const *row, uint32_t block, uint32_t k, bool wide) {
+__device__ __forceinline__ v4u load_codes(uint8_t const *row, uint32_t block, uint32_t k) {
     v4u word = {0, 0, 0, 0};
-    if (wide && block * 32 + 32 <= k) return *(v4u const *)(row + block * 16);
+    if (block * 32 + 32 <= k) return *(v4u_anywhere const *)(row + block * 16);
     for (uint32_t i = 0; i < 16; ++i) {
         uint32_t const col = block * 32 + 2 * i;
         uint32_t const byte = col + 1 < k ? row[col / 2] : col < k ? row[col / 2] & 15u : 0u;
@@ -91,7 +91,6 @@ struct StageArgs {
     uint32_t const *plan; // rows in the plan's order, or NULL
     uint32_t rows, k, supers, order, a_share;
     uint32_t slots, experts; // that the plan is for
-    bool wide;
 };
 /** Is what is at `plan` a plan for so many slots and experts? (One of others has its parts elsewhere, and may end sooner.) */
 __device__ __forceinline__ bool plan_matches(void const *plan, uint32_t slots, uint32_t experts) {
@@ -122,7 +121,7 @@ __global__ __launch_bounds__(256) void stage_kernel(StageArgs p) {
     uint32_t const lane = threadIdx.x & 63, u = threadIdx.x >> 6, piece = lane & 15, g = piece >> 2;
     uint32_t const block = (super * 4 + u) * 4 + g, col = block * 32 + (piece & 3) * 8;
     if (p.plan && (!plan_matches(p.plan, p.slots, p.experts) || tile * 16 >= ((PlanHeader const *)p.plan)->first_zero)) return;
-    bool const whole = p.wide && col + 8 <= p.k;
+    bool const whole = col + 8 <= p.k;
     In const *from[4];
     bool there[4];
     v4u raw[4][kLoads];
@@ -136,7 +135,7 @@ __global__ __launch_bounds__(256) void stage_kernel(StageArgs p) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) raw[t][i] = ((v4u const *)((there[t] ? from[t] : (In const *)p.a) + col))[i];
+            for (int i = 0; i < kLoads; ++i) raw[t][i] = ((v4u_anywhere const *)((there[t] ? from[t] : (In const *)p.a) + col))[i];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -169,7 +168,7 @@ __global__ __launch_bounds__(256) void stage_codes_kernel(StageArgs p) {
     v4u codes = {0, 0, 0, 0};
     uint32_t scale = 0;
     if (source_of(p, tile * 16 + r, source) && block * 32 < p.k)
-        codes = load_codes((uint8_t const *)p.a + source * p.a_stride, block, p.k, p.wide), scale = p.scales[source * p.scales_stride + block];
+        codes = load_codes((uint8_t const *)p.a + source * p.a_stride, block, p.k), scale = p.scales[source * p.scales_stride + block];
     *(v4u *)(p.to + (((uint64_t)tile * p.supers + super) * 4 + u) * 1024 + lane * 16) = codes;
     bytes[scale_word(r, g) * 4 + u] = (uint8_t)scale;
     __syncthreads();
@@ -182,9 +181,9 @@ __global__ __launch_bounds__(256) void stage_codes_kernel(StageArgs p) {
  *  written past them (8192 x 8192 of f32: 43 us; 56 us through the caches in a kernel that does no more, 43 us past them).
  */
 template <class T>
-__global__ __launch_bounds__(256) void dequantize_kernel(uint8_t const *codes, uint64_t codes_stride, bool whole_words,
+__global__ __launch_bounds__(256) void dequantize_kernel(uint8_t const *codes, uint64_t codes_stride,
                                                          uint8_t const *scales, uint64_t scales_stride, uint32_t rows, uint32_t k,
-                                                         uint32_t stretches, T *x, uint64_t x_stride, bool wide, bool past) {
+                                                         uint32_t stretches, T *x, uint64_t x_stride, bool past) {
     constexpr int N = kEach<T>, kHalves = 8 / N;
     uint32_t const lane = threadIdx.x & 63, first = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kStretches<T>;
     uint32_t row[kStretches<T>], from[kStretches<T>], word[kStretches<T>], scale[kStretches<T>];
@@ -194,7 +193,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(uint8_t const *codes, u
         uint32_t const col = from[t] + lane * 8;
         if (row[t] >= rows || col >= k) continue;
         uint8_t const *its = codes + row[t] * codes_stride + col / 2;
-        if (whole_words && col + 8 <= k) word[t] = *(uint32_t const *)its;
+        if (col + 8 <= k) word[t] = *(u32_anywhere const *)its;
         else
             for (uint32_t i = 0; i < 4; ++i)
                 if (col + 2 * i < k) word[t] |= (uint32_t)its[i] << 8 * i;
@@ -221,7 +220,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(uint8_t const *codes, u
             uint32_t const col = from[t] + half * 256 + lane * N;
             if (col >= k) continue;
             T *to = (T *)((uint8_t *)x + row[t] * x_stride) + col;
-            if (wide && past && col + N <= k) {
+            if (past && col + N <= k) {
                 struct alignas(16) Piece {
                     T x[N];
                 } piece;
@@ -241,7 +240,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(uint8_t const *codes, u
 __global__ __launch_bounds__(256) void mx_pack_kernel(uint8_t const *codes, uint64_t codes_stride, uint64_t codes_matrix,
                                                       uint8_t const *scales, uint64_t scales_stride, uint64_t scales_matrix,
                                                       MxHeader header, uint32_t supers, uint32_t tiles, uint64_t first,
-                                                      uint64_t code_lanes, uint64_t scale_lanes, bool wide, uint8_t *image) {
+                                                      uint64_t code_lanes, uint64_t scale_lanes, uint8_t *image) {
     uint64_t const index = first + (uint64_t)blockIdx.x * 256 + threadIdx.x;
     if (index == 0) *(MxHeader *)image = header;
     uint32_t const lane = index & 63;
@@ -258,7 +257,7 @@ __global__ __launch_bounds__(256) void mx_pack_kernel(uint8_t const *codes, uint
     if (of_codes) {
         uint32_t const block = which * 4 + g;
         v4u word = {0, 0, 0, 0};
-        if (column < header.n && block * 32 < k) word = load_codes(codes + matrix * codes_matrix + column * codes_stride, block, k, wide);
+        if (column < header.n && block * 32 < k) word = load_codes(codes + matrix * codes_matrix + column * codes_stride, block, k);
         *(v4u *)(image + kMxHeaderBytes + index * 16) = word;
         return;
     }
@@ -286,7 +285,6 @@ struct MxArgs {
     uint32_t order, tile_list; // words into the plan
     uint32_t a_share;          // slots that share a row of A
     uint32_t sorted;           // 1: results in the plan's order of rows (and nothing for rows of no expert), 0: at their slots
-    uint32_t a_wide;
 };
 
 /** The rows of one tile. */
@@ -631,7 +629,7 @@ __global__ __launch_bounds__(64 * WAVES, FM >= 4 ? 2 : 4) void mx_few_kernel(MxA
             uint32_t const at = rows.first + row, source = GROUPED ? p.plan[p.order + at] / p.a_share : at;
             In const *from = (In const *)(p.a + source * p.a_pitch);
             float v[N];
-            if (p.a_wide && piece * N + N <= p.k) widen<In>(*(v4u const *)(from + piece * N), v);
+            if (piece * N + N <= p.k) widen<In>(*(v4u_anywhere const *)(from + piece * N), v);
             else load_some(from, piece * N, p.k, v);
             uint32_t scale;
             uint32_t const word = quantize_some(v, scale);
@@ -772,10 +770,9 @@ int launch_quantize(int dtype, void const *x, uint64_t rows, uint64_t k, uint64_
     if (one_row(rows, k, x_stride, element_bytes(dtype), codes_stride, scales_stride)) k *= rows, rows = 1;
     return with_type(dtype, [&](auto value) {
         typedef decltype(value) T;
-        bool const wide = aligned(x, x_stride, 16), whole_words = aligned(codes, codes_stride, 4);
         return by_stretches<T>(rows, k, [&](uint64_t first, uint32_t here, uint32_t stretches, dim3 grid) {
             hipLaunchKernelGGL((quantize_kernel<T>), grid, dim3(256), 0, stream, (T const *)((uint8_t const *)x + first * x_stride), x_stride,
-                               here, (uint32_t)k, stretches, wide, codes + first * codes_stride, codes_stride, whole_words,
+                               here, (uint32_t)k, stretches, codes + first * codes_stride, codes_stride,
                                scales + first * scales_stride, scales_stride);
         });
     });
@@ -800,7 +797,7 @@ int stage(int a_dtype, void const *a, uint64_t a_stride, void const *a_scales, u
     if (!grid) return 0;
     if (grid > 0x7FFFFFFFull) return mx_fail("mx product: A is too large");
     StageArgs const p = {a, a_stride, (uint8_t const *)a_scales, a_scales_stride, to, to + s.scales_at, (uint32_t const *)plan, rows, k,
-                         g.supers, (uint32_t)order, a_share, slots, experts, aligned(a, a_stride, 16)};
+                         g.supers, (uint32_t)order, a_share, slots, experts};
     if (a_scales) hipLaunchKernelGGL(stage_codes_kernel, dim3((uint32_t)grid), dim3(256), 0, stream, p);
     else
         with_type(a_dtype, [&](auto value) {
@@ -954,15 +951,14 @@ int nk_amd_mx_dequantize_async(nk_dtype_t dtype, void const *codes, nk_size_t co
     if (!rows || !depth) return 0;
     if (!x || !codes || !scales) return mx_fail("mx_dequantize: NULL operand");
     if (!aligned(x, x_stride, bytes)) return mx_fail("mx_dequantize: x is not aligned to its elements");
-    bool const past = rows * depth * bytes >= 64ull << 20;
+    bool const past = rows * depth * bytes >= 64ull << 20 && aligned(x, x_stride, 16);
     if (one_row(rows, depth, x_stride, bytes, codes_stride, scales_stride)) depth *= rows, rows = 1;
     return with_type(dtype, [&](auto value) {
         typedef decltype(value) T;
-        bool const wide = aligned(x, x_stride, 16), whole_words = aligned(codes, codes_stride, 4);
         return by_stretches<T>(rows, depth, [&](uint64_t first, uint32_t here, uint32_t stretches, dim3 grid) {
             hipLaunchKernelGGL((dequantize_kernel<T>), grid, dim3(256), 0, (hipStream_t)stream, (uint8_t const *)codes + first * codes_stride,
-                               codes_stride, whole_words, (uint8_t const *)scales + first * scales_stride, scales_stride, here, (uint32_t)depth,
-                               stretches, (T *)((uint8_t *)x + first * x_stride), x_stride, wide, past);
+                               codes_stride, (uint8_t const *)scales + first * scales_stride, scales_stride, here, (uint32_t)depth,
+                               stretches, (T *)((uint8_t *)x + first * x_stride), x_stride, past);
         });
     });
 }
@@ -982,14 +978,13 @@ int nk_amd_mx_pack_async(void const *codes, nk_size_t codes_stride, nk_size_t co
     MxHeader const header = {kMxMagic, 1, (uint32_t)count, (uint32_t)width, (uint32_t)depth, {0, 0, 0}};
     uint64_t const code_lanes = count * (g.code_bytes / 16), scale_lanes = count * (g.scale_bytes / 4);
     uint64_t const total = code_lanes + scale_lanes;
-    bool const wide = aligned(codes, codes_stride | codes_matrix, 16);
     uint64_t const supers = g.supers ? g.supers : 1, tiles = g.tiles ? g.tiles : 1;
     for (uint64_t first = 0; first == 0 || first < total; first += kMostThreads) {
         uint64_t const here = total - first < kMostThreads ? total - first : kMostThreads;
         hipLaunchKernelGGL(mx_pack_kernel, dim3((uint32_t)(here ? (here + 255) / 256 : 1)), dim3(256), 0, (hipStream_t)stream,
                            (uint8_t const *)codes, codes_stride, codes_matrix, (uint8_t const *)scales, scales_stride,
                            scales_matrix, header, (uint32_t)supers, (uint32_t)tiles, first, code_lanes, scale_lanes,
-                           wide, (uint8_t *)packed);
+                           (uint8_t *)packed);
         hipError_t const e = hipGetLastError();
         if (e != hipSuccess) return mx_fail(e, "mx_pack_kernel");
     }
@@ -1018,7 +1013,7 @@ int nk_amd_mx_dots_packed_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_s
     p.image = (uint8_t const *)packed, p.c = (uint8_t *)c, p.c_stride = c_stride;
     p.m = (uint32_t)height, p.n = (uint32_t)width, p.k = (uint32_t)depth, p.count = 1, p.a_share = 1;
     p.steps = g.steps, p.supers = g.supers, p.tiles = g.tiles;
-    if (fused) p.a = (uint8_t const *)a, p.a_pitch = a_stride, p.a_wide = aligned(a, a_stride, 16);
+    if (fused) p.a = (uint8_t const *)a, p.a_pitch = a_stride;
     else {
         Staging const s = staging_of(height, g);
         if (s.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < s.bytes))
@@ -1062,7 +1057,7 @@ int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_
     p.m = (uint32_t)slots, p.n = (uint32_t)width, p.k = (uint32_t)depth, p.count = (uint32_t)experts, p.a_share = (uint32_t)a_share;
     p.steps = g.steps, p.supers = g.supers, p.tiles = g.tiles;
     p.tiles_m = shape.max_tiles, p.order = (uint32_t)shape.order, p.tile_list = (uint32_t)shape.tiles;
-    if (l.fused) p.a = (uint8_t const *)a, p.a_pitch = a_stride, p.a_wide = aligned(a, a_stride, 16);
+    if (l.fused) p.a = (uint8_t const *)a, p.a_pitch = a_stride;
     else {
         if (l.quantised) {
             uint8_t *const codes = (uint8_t *)workspace + l.codes_at, *const scales = (uint8_t *)workspace + l.codes_scales_at;

@@ -121,6 +121,8 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef v4u __attribute__((aligned(1))) v4u_anywhere; // loads and stores of global memory need no alignment
+typedef uint32_t __attribute__((aligned(1))) u32_anywhere;
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -250,10 +252,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(void const *base) {
     return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, 0xFFFFFFFFu, 0x00020000);
 }
 
-/** 16 bytes to any address that is even. */
+/** 16 bytes to any address. */
 __device__ __forceinline__ void store_16(void *to, v4u values) {
-    typedef v4u __attribute__((aligned(2))) anywhere;
-    *(anywhere *)to = values;
+    *(v4u_anywhere *)to = values;
 }
 
 /** What lanes of a wavefront have written to LDS is there for its other lanes. */
