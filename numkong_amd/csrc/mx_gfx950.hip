@@ -324,7 +324,7 @@ __device__ __forceinline__ bool image_matches(MxArgs const &p) {
  *
  *  8192^3 with bf16 results takes 241 to 257 us (4.3 to 4.6 PFLOP/s; the matrix instructions alone, on the same random codes, 6.5):
  *  power holds the clock at 1.6 GHz, a step takes 1226 cycles of which 1024 are matrix instructions, a tile's end a tenth of its
- *  time. Shallow products of f32 results are bound by their stores (8192 x 8191 x 1000: 74 us for 268 MB), experts by both (64 of
+ *  time. Shallow products of f32 results are bound by their stores (8192 x 8191 x 1000: 73 us for 268 MB), experts by both (64 of
  *  512 rows on average, 2048 x 2048: 95 to 104 us for 313 MB).
  */
 template <int FM, class Out, bool GROUPED>
