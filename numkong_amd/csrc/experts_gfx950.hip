@@ -374,6 +374,11 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs p, float 
 
 constexpr int kPlanWaves = 4, kPlanThreads = 64 * kPlanWaves;
 static_assert(kPlanBlockSlots == 4 * kPlanThreads, "what plan_geometry leaves room for");
+/** So many workgroups of plan_kernel add up one another's counts themselves; of more a launch of its own does, whose time grows with the
+ *  slots and not with their square (whole plans, us, by themselves and by that launch: 2^15 slots of 128 experts 10.0 and 11.8, 2^16 11.4 and
+ *  12.4, 2^17 14.4 and 12.7, 2^18 20.2 and 13.7; of 1,024 experts 20.7 and 19.9, 27.5 and 21.3, 41.7 and 22.0, 69.5 and 23.8). 2^20 slots
+ *  take 20 us and 37. */
+constexpr uint32_t kPlanCountBlocks = 64;
 /** Lanes of the wavefront that hold the same bucket, by one ballot for each bit. */
 __device__ __forceinline__ uint64_t same_bucket(uint32_t bucket, int bits, bool active) {
     uint64_t mask = __ballot(active);
@@ -411,17 +416,49 @@ __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(int32_t const 
     for (uint32_t i = threadIdx.x; i < buckets; i += kPlanThreads) table[blockIdx.x * buckets + i] = plan_lds[i];
 }
 
+constexpr uint32_t kScanBuckets = 16, kScanParts = 64, kScanBatch = 8;
+/**
+ *  Of each bucket's counts in `table` the sums over the workgroups before each, and over all of them in the row behind the last, so that a
+ *  workgroup of plan_kernel reads two words for a bucket however many there are. A workgroup takes 16 adjacent buckets; of a
+ *  bucket's column each of 64 threads adds up one stretch, learns from LDS what stands before it, and goes over it again.
+ */
+__global__ __launch_bounds__(kScanBuckets * kScanParts) void plan_scan_kernel(uint32_t buckets, uint32_t blocks, uint32_t *table) {
+    __shared__ uint32_t sums[kScanParts][kScanBuckets];
+    uint32_t const column = threadIdx.x % kScanBuckets, part = threadIdx.x / kScanBuckets, bucket = blockIdx.x * kScanBuckets + column;
+    uint32_t const stretch = (blocks + kScanParts - 1) / kScanParts, from = part * stretch < blocks ? part * stretch : blocks;
+    uint32_t const to = bucket >= buckets ? from : from + stretch < blocks ? from + stretch : blocks;
+    uint32_t sum = 0;
+#pragma unroll 8
+    for (uint32_t at = from; at < to; ++at) sum += table[at * buckets + bucket];
+    sums[part][column] = sum;
+    __syncthreads();
+    uint32_t before = 0;
+    for (uint32_t earlier = 0; earlier < part; ++earlier) before += sums[earlier][column];
+    for (uint32_t at = from; at < to; at += kScanBatch) {
+        uint32_t its[kScanBatch];
+#pragma unroll
+        for (uint32_t i = 0; i < kScanBatch; ++i) its[i] = at + i < to ? table[(at + i) * buckets + bucket] : 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kScanBatch; ++i) {
+            if (at + i < to) table[(at + i) * buckets + bucket] = before;
+            before += its[i];
+        }
+    }
+    if (part == kScanParts - 1 && bucket < buckets) table[blocks * buckets + bucket] = before;
+}
+
 /**
  *  Counting sort of the slots by expert. A wavefront has a stretch of them in registers; it counts them, learns where its slots
  *  of each bucket go (behind those of the wavefronts before it, whose counts are in LDS, and of the workgroups before, in
- *  `table`; NULL where there is one workgroup), and goes over them again in order, so that no atomic decides an order. The first
- *  workgroup also writes the header, the tiles and the slots of rows that stand between experts. Its time is that of a few loads
+ *  `table`; NULL where there is one workgroup), and goes over them again in order, so that no atomic decides an order. `scanned`:
+ *  the table holds sums (plan_scan_kernel), not counts. The first workgroup also writes the header and the slots of rows that
+ *  stand between experts; the tiles are written by all in turn, as one expert may have most of them. Its time is that of a few loads
  *  and LDS round trips one after the other: 32 slots 3.4 us, 1,024 5.3, 4,004 with the launch that counts 8.5, 32,768 9.4.
  */
 template <int BATCH>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(int32_t const *chosen, uint32_t slots, uint32_t experts, PlanHeader header,
                                                             uint32_t offsets, uint32_t order, uint32_t place, uint32_t tiles, int bits,
-                                                            uint32_t const *table, uint32_t *plan) {
+                                                            uint32_t const *table, bool scanned, uint32_t *plan) {
     extern __shared__ uint32_t plan_lds[]; // [wave][bucket] counts, then where the wave's next slot of the bucket goes
     __shared__ uint32_t wave_total[2][kPlanWaves];
     uint32_t const buckets = experts + 1, thread = threadIdx.x, lane = thread & 63;
@@ -442,7 +479,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(int32_t const *chose
         if (bucket < buckets) {
 #pragma unroll
             for (int w = 0; w < kPlanWaves; ++w) here[w] = plan_lds[w * buckets + bucket], size += here[w];
-            if (table) {
+            if (scanned) earlier = table[blockIdx.x * buckets + bucket], size = table[gridDim.x * buckets + bucket];
+            else if (table) {
                 size = 0;
 #pragma unroll 8
                 for (uint32_t block = 0; block < gridDim.x; ++block) {
@@ -470,13 +508,13 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(int32_t const *chose
             uint32_t next = first + earlier;
 #pragma unroll
             for (int w = 0; w < kPlanWaves; ++w) plan_lds[w * buckets + bucket] = next, next += here[w];
+            for (uint32_t t = blockIdx.x; t < its_tiles; t += gridDim.x) {
+                uint32_t const from = first + t * header.tile_rows, to = from + header.tile_rows;
+                PlanTile const tile = {(int32_t)bucket, (int32_t)from, (int32_t)(to < first + size ? to : first + size), 0};
+                *(PlanTile *)(plan + tiles + (first_tile + t) * 4) = tile;
+            }
             if (blockIdx.x == 0) {
                 plan[offsets + bucket] = first;
-                for (uint32_t t = 0; t < its_tiles; ++t) {
-                    uint32_t const from = first + t * header.tile_rows, to = from + header.tile_rows;
-                    PlanTile const tile = {(int32_t)bucket, (int32_t)from, (int32_t)(to < first + size ? to : first + size), 0};
-                    *(PlanTile *)(plan + tiles + (first_tile + t) * 4) = tile;
-                }
                 for (uint32_t at = first + size; at < first + its_rows; ++at) plan[order + at] = 0xFFFFFFFFu;
                 if (bucket == experts) {
                     header.tile_count = first_tile, header.zero_tiles = its_tiles;
@@ -602,12 +640,16 @@ int nk_amd_experts_plan_async(nk_i32_t const *chosen, nk_size_t slots, nk_size_t
     uint32_t const blocks = slots ? (uint32_t)((slots + kPlanBlockSlots - 1) / kPlanBlockSlots) : 1, lds = (uint32_t)((experts + 1) * 4);
     uint32_t *const table = blocks > 1 ? (uint32_t *)plan + g.table : nullptr;
     if (table) hipLaunchKernelGGL(plan_count_kernel, dim3(blocks), dim3(kPlanThreads), lds, (hipStream_t)stream, chosen, (uint32_t)slots, (uint32_t)experts, table);
+    bool const scanned = blocks > kPlanCountBlocks;
+    if (scanned)
+        hipLaunchKernelGGL(plan_scan_kernel, dim3((uint32_t)(experts / kScanBuckets + 1)), dim3(kScanBuckets * kScanParts), 0, (hipStream_t)stream,
+                           (uint32_t)experts + 1, blocks, table);
     // Slots that fit one a lane are not followed by three more. (Up to 4,096 slots without the launch that counts, each workgroup
     // counting all slots: 7.3 us instead of 8.5 by itself, but 11.0 instead of 9.4 where `chosen` is not in the caches any more; eight
     // slots a lane: 15.5 us for 32,768.)
     auto *const kernel = slots <= kPlanThreads ? plan_kernel<1> : plan_kernel<4>;
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kPlanThreads), lds * kPlanWaves, (hipStream_t)stream, chosen, (uint32_t)slots, (uint32_t)experts,
-                       header, (uint32_t)g.offsets, (uint32_t)g.order, (uint32_t)g.place, (uint32_t)g.tiles, bits, table, (uint32_t *)plan);
+                       header, (uint32_t)g.offsets, (uint32_t)g.order, (uint32_t)g.place, (uint32_t)g.tiles, bits, table, scanned, (uint32_t *)plan);
     hipError_t const e = hipGetLastError();
     return e == hipSuccess ? 0 : mx_fail(e, "plan_kernel");
 }

@@ -96,7 +96,7 @@ inline uint32_t plan_tile_rows(size_t slots, size_t experts) {
     size_t const mean = experts ? slots / experts : 0;
     return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
 }
-constexpr size_t kPlanBlockSlots = 1024; // slots of a workgroup that makes the plan; its counts stand behind the tiles
+constexpr size_t kPlanBlockSlots = 1024; // slots of a workgroup that makes the plan; its counts stand behind the tiles, then their sums
 constexpr size_t kMaxExperts = 1024, kMaxTopK = 64, kMaxGroups = 64;
 inline bool plan_geometry(size_t slots, size_t experts, PlanGeometry &g) {
     if (!experts || experts > kMaxExperts || slots >= (1ull << 30)) return false;
@@ -109,7 +109,7 @@ inline bool plan_geometry(size_t slots, size_t experts, PlanGeometry &g) {
     g.place = g.order + g.max_rows;
     g.tiles = (g.place + slots + 3) & ~(size_t)3;
     g.table = g.tiles + (size_t)g.max_tiles * 4;
-    g.total_words = g.table + (slots + kPlanBlockSlots - 1) / kPlanBlockSlots * (experts + 1);
+    g.total_words = g.table + ((slots + kPlanBlockSlots - 1) / kPlanBlockSlots + 1) * (experts + 1);
     return true;
 }
 

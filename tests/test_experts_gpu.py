@@ -234,6 +234,60 @@ def test_plan(tokens, top_k, experts, kind):
     assert tile_count == sum(tile[0] < experts for tile in want)
 
 
+def large_routing(slots, experts, popular):
+    """One expert's share of all slots is `popular`; some slots have no expert."""
+    generator = torch.Generator(device=DEV).manual_seed(slots)
+    chosen = torch.randint(-1, experts, (slots,), dtype=torch.int32, device=DEV, generator=generator)
+    chosen[torch.rand((slots,), device=DEV, generator=generator) < popular] = experts // 2
+    return chosen.reshape(-1, 8)
+
+
+@pytest.mark.parametrize("slots,experts,popular", [(1 << 16, 1024, 0.0), (66 << 10, 100, 0.5), ((1 << 17) + 8, 15, 0.0), (1 << 20, 128, 0.9), (1 << 20, 1024, 0.1),
+                                                   (1 << 27, 8, 0.3)])
+def test_plan_of_many_slots(slots, experts, popular):
+    """As test_plan, by torch's own sort: more workgroups than add up one another's counts, tiles written by several of them."""
+    chosen = large_routing(slots, experts, popular)
+    words = nk.experts_plan(chosen, experts).buffer.view(torch.int32)
+    flat = chosen.reshape(-1)
+    bucket = torch.where((flat >= 0) & (flat < experts), flat, experts)
+    counts = torch.bincount(bucket, minlength=experts + 1)
+    sizes = (counts + 15) // 16 * 16
+    starts = sizes.cumsum(0) - sizes
+    tile_rows, tile_count, zero_tiles, first_zero, end_zero = words[3:8].tolist()
+    assert (first_zero, end_zero) == (int(starts[-1]), int(starts[-1] + counts[-1]))
+    assert torch.equal(words[8:8 + experts + 1], starts.int()) and int(words[9 + experts]) == end_zero
+    by_bucket, slot_at = torch.sort(bucket, stable=True)
+    row_of = starts[by_bucket] + torch.arange(slots, device=DEV) - (counts.cumsum(0) - counts)[by_bucket]
+    order = torch.full((int(sizes.sum()),), -1, dtype=torch.int32, device=DEV)
+    order[row_of] = slot_at.int()
+    place = torch.empty(slots, dtype=torch.int32, device=DEV)
+    place[slot_at] = torch.where(by_bucket < experts, row_of, -1).int()
+    first, room = 8 + (experts + 2 + 3) // 4 * 4, (slots + min(slots, experts + 1) * 15 + 15) // 16 * 16
+    assert torch.equal(words[first:first + len(order)], order)
+    assert torch.equal(words[first + room:first + room + slots], place)
+    tiles = words[(first + room + slots + 3) // 4 * 4:][:4 * (tile_count + zero_tiles)].reshape(-1, 4)
+    of_bucket = (counts + tile_rows - 1) // tile_rows
+    expert = torch.repeat_interleave(torch.arange(experts + 1, device=DEV), of_bucket)
+    row = starts[expert] + tile_rows * (torch.arange(len(expert), device=DEV) - (of_bucket.cumsum(0) - of_bucket)[expert])
+    want = torch.stack([expert, row, torch.minimum(row + tile_rows, (starts + counts)[expert])], 1).int()
+    assert torch.equal(tiles[:, :3], want) and tile_count == int(of_bucket[:-1].sum())
+
+
+def test_a_plan_takes_time_by_its_slots():
+    """32 times the slots: about 32 times the work, where a thousand times would be work that grows with their square."""
+    def milliseconds(slots):
+        chosen = large_routing(slots, 8, 0.9)
+        nk.experts_plan(chosen, 8)
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        nk.experts_plan(chosen, 8)
+        end.record()
+        end.synchronize()
+        return start.elapsed_time(end)
+
+    assert milliseconds(1 << 27) < 4 * 32 * milliseconds(1 << 22)
+
+
 @pytest.mark.parametrize("tokens,top_k,experts,kind", CASES)
 @pytest.mark.parametrize("n,k,dtype,out", [(130, 200, torch.bfloat16, torch.bfloat16), (64, 513, torch.float32, torch.float32), (77, 33, torch.float16, torch.float16)])
 def test_experts_products(tokens, top_k, experts, kind, n, k, dtype, out):
