@@ -595,13 +595,18 @@ int nk_amd_experts_route_async(nk_dtype_t dtype, void const *logits, nk_size_t l
     if ((size_t)how->top_groups * (experts / how->groups) < top_k) return mx_fail("experts_route: the groups that stay hold fewer than top_k experts");
     if (!tokens) return 0;
     if (!weights || !chosen) return mx_fail("experts_route: NULL operand");
-    RouteArgs const p = {logits, logits_stride, (uint32_t)tokens, (uint32_t)experts, (uint32_t)top_k, bias, *how, weights, chosen};
     return with_row<false>(dtype, tokens <= (experts > 128 ? 4096 : 2048), experts, [&](auto value, auto lanes, auto per_lane) {
         typedef decltype(value) T;
         constexpr int L = decltype(lanes)::value, J = decltype(per_lane)::value;
-        hipLaunchKernelGGL((route_kernel<T, L, J>), dim3((uint32_t)((tokens + 256 / L - 1) / (256 / L))), dim3(256), 0, (hipStream_t)stream, p);
-        hipError_t const e = hipGetLastError();
-        return e == hipSuccess ? 0 : mx_fail(e, "route_kernel");
+        for (uint64_t first = 0; first < tokens; first += kMostThreads / L) {
+            uint64_t const here = tokens - first < kMostThreads / L ? tokens - first : kMostThreads / L;
+            RouteArgs const p = {(uint8_t const *)logits + first * logits_stride, logits_stride, (uint32_t)here, (uint32_t)experts, (uint32_t)top_k,
+                                 bias, *how, weights + first * top_k, chosen + first * top_k};
+            hipLaunchKernelGGL((route_kernel<T, L, J>), dim3((uint32_t)((here + 256 / L - 1) / (256 / L))), dim3(256), 0, (hipStream_t)stream, p);
+            hipError_t const e = hipGetLastError();
+            if (e != hipSuccess) return mx_fail(e, "route_kernel");
+        }
+        return 0;
     });
 }
 
@@ -613,14 +618,19 @@ int nk_amd_experts_route_backward_async(nk_dtype_t dtype, void const *logits, nk
     if (!chosen || !grad_weights || !grad_logits) return mx_fail("experts_route_backward: NULL operand");
     int const bytes = dtype == nk_f32_k ? 4 : 2;
     if (((uintptr_t)grad_logits | grad_stride) & (bytes - 1)) return mx_fail("experts_route_backward: grad_logits is not aligned to its elements");
-    RouteArgs const p = {logits, logits_stride, (uint32_t)tokens, (uint32_t)experts, (uint32_t)top_k, nullptr, *how, nullptr, (int32_t *)chosen};
     return with_row<true>(dtype, tokens <= 4096, experts, [&](auto value, auto lanes, auto per_lane) {
         typedef decltype(value) T;
         constexpr int L = decltype(lanes)::value, J = decltype(per_lane)::value;
-        hipLaunchKernelGGL((route_backward_kernel<T, L, J>), dim3((uint32_t)((tokens + 256 / L - 1) / (256 / L))), dim3(256), 0,
-                           (hipStream_t)stream, p, grad_weights, (T *)grad_logits, (uint64_t)grad_stride);
-        hipError_t const e = hipGetLastError();
-        return e == hipSuccess ? 0 : mx_fail(e, "route_backward_kernel");
+        for (uint64_t first = 0; first < tokens; first += kMostThreads / L) {
+            uint64_t const here = tokens - first < kMostThreads / L ? tokens - first : kMostThreads / L;
+            RouteArgs const p = {(uint8_t const *)logits + first * logits_stride, logits_stride, (uint32_t)here, (uint32_t)experts, (uint32_t)top_k,
+                                 nullptr, *how, nullptr, (int32_t *)chosen + first * top_k};
+            hipLaunchKernelGGL((route_backward_kernel<T, L, J>), dim3((uint32_t)((here + 256 / L - 1) / (256 / L))), dim3(256), 0,
+                               (hipStream_t)stream, p, grad_weights + first * top_k, (T *)((uint8_t *)grad_logits + first * grad_stride), (uint64_t)grad_stride);
+            hipError_t const e = hipGetLastError();
+            if (e != hipSuccess) return mx_fail(e, "route_backward_kernel");
+        }
+        return 0;
     });
 }
 

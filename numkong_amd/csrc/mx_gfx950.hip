@@ -91,6 +91,7 @@ struct StageArgs {
     uint32_t const *plan; // rows in the plan's order, or NULL
     uint32_t rows, k, supers, order, a_share;
     uint32_t slots, experts; // that the plan is for
+    uint32_t first;          // workgroups of the launches before
 };
 /** Is what is at `plan` a plan for so many slots and experts? (One of others has its parts elsewhere, and may end sooner.) */
 __device__ __forceinline__ bool plan_matches(void const *plan, uint32_t slots, uint32_t experts) {
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(256) void stage_kernel(StageArgs p) {
     __shared__ __attribute__((aligned(16))) uint32_t words[4][256];
     __shared__ __attribute__((aligned(4))) uint8_t bytes[256];
     constexpr int kLoads = sizeof(In) / 2; // 16-byte loads of a lane's eight values
-    uint32_t const tile = blockIdx.x / p.supers, super = blockIdx.x - tile * p.supers;
+    uint32_t const index = p.first + blockIdx.x, tile = index / p.supers, super = index - tile * p.supers;
     uint32_t const lane = threadIdx.x & 63, u = threadIdx.x >> 6, piece = lane & 15, g = piece >> 2;
     uint32_t const block = (super * 4 + u) * 4 + g, col = block * 32 + (piece & 3) * 8;
     if (p.plan && (!plan_matches(p.plan, p.slots, p.experts) || tile * 16 >= ((PlanHeader const *)p.plan)->first_zero)) return;
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(256) void stage_kernel(StageArgs p) {
 /** The same from codes: a lane's 16 bytes of a row are its 16 bytes of the fragment. */
 __global__ __launch_bounds__(256) void stage_codes_kernel(StageArgs p) {
     __shared__ __attribute__((aligned(4))) uint8_t bytes[256];
-    uint32_t const tile = blockIdx.x / p.supers, super = blockIdx.x - tile * p.supers;
+    uint32_t const index = p.first + blockIdx.x, tile = index / p.supers, super = index - tile * p.supers;
     uint32_t const lane = threadIdx.x & 63, u = threadIdx.x >> 6, r = lane & 15, g = lane >> 4, block = (super * 4 + u) * 4 + g;
     if (p.plan && (!plan_matches(p.plan, p.slots, p.experts) || tile * 16 >= ((PlanHeader const *)p.plan)->first_zero)) return;
     uint64_t source;
@@ -281,6 +282,7 @@ struct MxArgs {
     uint64_t a_pitch, c_stride;
     uint32_t m, n, k, steps, supers, tiles, count;
     uint32_t tiles_m, tiles_n; // the grid: tiles of rows, tiles of columns
+    uint32_t first_n;          // tiles of columns of the launches before (products of few rows)
     uint32_t band;             // tiles of rows that are walked side by side
     uint32_t order, tile_list; // words into the plan
     uint32_t a_share;          // slots that share a row of A
@@ -577,9 +579,10 @@ __global__ __launch_bounds__(64 * WAVES, FM >= 4 ? 2 : 4) void mx_few_kernel(MxA
         uint32_t const index = blockIdx.x >> 3, column = index / p.tiles_m;
         tile_m = index - column * p.tiles_m, tile_n = column * 8 + (blockIdx.x & 7);
         if (tile_n >= p.tiles_n) return;
+        tile_n += p.first_n;
     }
     else {
-        tile_m = blockIdx.x / p.tiles_n, tile_n = blockIdx.x - tile_m * p.tiles_n;
+        tile_m = blockIdx.x / p.tiles_n, tile_n = p.first_n + blockIdx.x - tile_m * p.tiles_n;
         if (!plan_matches(p.plan, p.m, p.count)) { // NaNs, as in mx_gemm_kernel
             uint32_t const column = tile_n * NT * 16 + threadIdx.x;
             if (!p.sorted && threadIdx.x < NT * 16 && column < p.n)
@@ -738,7 +741,6 @@ __global__ __launch_bounds__(256) void combine_kernel(float const *rows, uint64_
 
 int element_bytes(int dtype) { return dtype == nk_f32_k ? 4 : dtype == nk_bf16_k || dtype == nk_f16_k ? 2 : 0; }
 bool aligned(void const *ptr, uint64_t stride, uint64_t to) { return !(((uintptr_t)ptr | stride) & (to - 1)); }
-constexpr uint64_t kMostThreads = 1ull << 31;
 
 /** Calls `f` with a value of the element type's C++ type. */
 template <class F>
@@ -793,19 +795,28 @@ Staging staging_of(uint64_t rows, MxGeometry const &g) {
 /** A into the workspace: rows in order, or the rows of a plan. */
 int stage(int a_dtype, void const *a, uint64_t a_stride, void const *a_scales, uint64_t a_scales_stride, uint32_t rows, uint32_t k,
           MxGeometry const &g, Staging const &s, uint8_t *to, void const *plan, size_t order, uint32_t a_share, uint32_t slots, uint32_t experts, hipStream_t stream) {
-    uint64_t const grid = (uint64_t)((rows + 15) / 16) * g.supers;
-    if (!grid) return 0;
-    if (grid > 0x7FFFFFFFull) return mx_fail("mx product: A is too large");
-    StageArgs const p = {a, a_stride, (uint8_t const *)a_scales, a_scales_stride, to, to + s.scales_at, (uint32_t const *)plan, rows, k,
-                         g.supers, (uint32_t)order, a_share, slots, experts};
-    if (a_scales) hipLaunchKernelGGL(stage_codes_kernel, dim3((uint32_t)grid), dim3(256), 0, stream, p);
-    else
-        with_type(a_dtype, [&](auto value) {
-            hipLaunchKernelGGL(stage_kernel<decltype(value)>, dim3((uint32_t)grid), dim3(256), 0, stream, p);
-            return 0;
-        });
-    hipError_t const e = hipGetLastError();
-    return e == hipSuccess ? 0 : mx_fail(e, "stage_kernel");
+    uint64_t const total = (uint64_t)((rows + 15) / 16) * g.supers;
+    StageArgs p = {a, a_stride, (uint8_t const *)a_scales, a_scales_stride, to, to + s.scales_at, (uint32_t const *)plan, rows, k,
+                   g.supers, (uint32_t)order, a_share, slots, experts, 0};
+    for (uint64_t first = 0; first < total; first += kMostThreads / 256) {
+        dim3 const grid((uint32_t)(total - first < kMostThreads / 256 ? total - first : kMostThreads / 256));
+        p.first = (uint32_t)first;
+        if (a_scales) hipLaunchKernelGGL(stage_codes_kernel, grid, dim3(256), 0, stream, p);
+        else
+            with_type(a_dtype, [&](auto value) {
+                hipLaunchKernelGGL(stage_kernel<decltype(value)>, grid, dim3(256), 0, stream, p);
+                return 0;
+            });
+        hipError_t const e = hipGetLastError();
+        if (e != hipSuccess) return mx_fail(e, "stage_kernel");
+    }
+    return 0;
+}
+/** Fragments of A and tiles of C are counted in 32 bits: looked at before anything is queued. `row_tiles`: of 128 rows, or of a plan. */
+int check_size(uint64_t rows, uint64_t row_tiles, uint64_t n, MxGeometry const &g) {
+    if ((rows + 15) / 16 * g.supers > 0x7FFFFFFFull) return mx_fail("mx product: A is too large");
+    if (row_tiles * ((n + 255) / 256) > 0x7FFFFFFFull) return mx_fail("mx product: too many tiles");
+    return 0;
 }
 
 /**
@@ -821,15 +832,19 @@ bool fuses(uint64_t rows, uint64_t values, MxGeometry const &g) {
 
 template <int WAVES, int FM, int NT, class In, class Out, bool GROUPED>
 int launch_few_of(MxArgs &p, uint32_t max_rows, MxGeometry const &g, hipStream_t stream) {
-    p.tiles_n = (p.tiles + NT - 1) / NT;
-    if (!GROUPED) p.tiles_m = (p.m + 16 * FM - 1) / (16 * FM);
-    uint64_t const grid = (uint64_t)p.tiles_m * (GROUPED ? p.tiles_n : (p.tiles_n + 7) / 8 * 8);
-    if (grid > 0x7FFFFFFFull) return mx_fail("mx product: too many tiles");
     uint32_t lds = WAVES * FM * NT * 1024;
     if (sizeof(In) != 1 && fused_bytes(max_rows, g) > lds) lds = fused_bytes(max_rows, g);
-    hipLaunchKernelGGL((mx_few_kernel<WAVES, FM, NT, In, Out, GROUPED>), dim3((uint32_t)grid), dim3(64 * WAVES), lds, stream, p);
-    hipError_t const e = hipGetLastError();
-    return e == hipSuccess ? 0 : mx_fail(e, "mx_few_kernel");
+    if (!GROUPED) p.tiles_m = (p.m + 16 * FM - 1) / (16 * FM);
+    // tiles of columns of one launch (tiles of rows are few thousands at most, see launch_product and plan_tile_rows)
+    uint32_t const tiles_n = (p.tiles + NT - 1) / NT, slab = (uint32_t)(kMostThreads / (64 * WAVES) / p.tiles_m) / 8 * 8;
+    for (p.first_n = 0; p.first_n < tiles_n; p.first_n += slab) {
+        p.tiles_n = tiles_n - p.first_n < slab ? tiles_n - p.first_n : slab;
+        uint32_t const grid = p.tiles_m * (GROUPED ? p.tiles_n : (p.tiles_n + 7) / 8 * 8);
+        hipLaunchKernelGGL((mx_few_kernel<WAVES, FM, NT, In, Out, GROUPED>), dim3(grid), dim3(64 * WAVES), lds, stream, p);
+        hipError_t const e = hipGetLastError();
+        if (e != hipSuccess) return mx_fail(e, "mx_few_kernel");
+    }
+    return 0;
 }
 template <int FM, int NT, class In, class Out, bool GROUPED>
 int launch_few(MxArgs &p, uint32_t max_rows, MxGeometry const &g, hipStream_t stream) {
@@ -840,7 +855,6 @@ int launch_gemm(MxArgs &p, hipStream_t stream) {
     p.tiles_n = (p.tiles + 15) / 16, p.band = FM >= 8 || p.steps <= 16 ? 2 : 4;
     if (!GROUPED) p.tiles_m = (p.m + 32 * FM - 1) / (32 * FM);
     uint64_t const tiles = (uint64_t)p.tiles_m * p.tiles_n, resident = (uint64_t)compute_unit_count() * (FM >= 8 ? 1 : 2);
-    if (tiles > 0x7FFFFFFFull) return mx_fail("mx product: too many tiles");
     if (!resident) return mx_fail("mx product: no GPU");
     uint64_t const grid = ((tiles < resident ? tiles : resident) + 7) / 8 * 8;
     hipLaunchKernelGGL((mx_gemm_kernel<FM, Out, GROUPED>), dim3((uint32_t)grid), dim3(256), 0, stream, p);
@@ -1005,6 +1019,7 @@ int nk_amd_mx_dots_packed_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_s
     hipStream_t const stream = (hipStream_t)stream_;
     if (height >= (1ull << 31) || !mx_geometry(1, width, depth, g)) return mx_fail("mx_dots_packed: unsupported dimensions");
     if (!height || !width) return 0;
+    if (int const status = check_size(height, (height + 127) / 128, width, g)) return status;
     if (int const status = depth ? check_a(a_dtype, a, a_scales, a_stride) : 0) return status;
     if (int const status = check_c(c_dtype, c, c_stride)) return status;
     if (!packed || ((uintptr_t)packed & 15)) return mx_fail("mx_dots_packed: the image has to be 16-byte aligned");
@@ -1046,6 +1061,7 @@ int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_
     if (!mx_geometry(experts, width, depth, g) || !plan_geometry(slots, experts, shape)) return mx_fail("mx_dots_experts: unsupported dimensions");
     if (!a_share || !top_k || slots % top_k || slots % a_share) return mx_fail("mx_dots_experts: slots have to be whole rows of top_k and of a_share");
     if (!slots || !width) return 0;
+    if (int const status = check_size(shape.max_rows, shape.max_tiles, width, g)) return status;
     if (int const status = depth ? check_a(a_dtype, a, a_scales, a_stride) : 0) return status;
     if (int const status = check_c(c_dtype, c, c_stride)) return status;
     if (!packed || ((uintptr_t)packed & 15) || !plan || ((uintptr_t)plan & 15)) return mx_fail("mx_dots_experts: image and plan have to be 16-byte aligned");

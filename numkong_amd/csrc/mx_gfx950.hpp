@@ -42,6 +42,9 @@
 
 namespace nk_gfx950 {
 
+/** Threads of one launch: HIP takes fewer than 2^32. What needs more is queued in several. */
+constexpr uint64_t kMostThreads = 1ull << 31;
+
 /** The text that nk_hip_last_error() gives on this thread; both return a status for the caller to hand on. */
 int mx_fail(hipError_t status, char const *what);
 int mx_fail(char const *what);

@@ -182,6 +182,25 @@ def test_route_gradient_by_differences(score, renormalize):
     assert (np.abs(got - want) <= allowed).all()
 
 
+def test_more_tokens_than_one_launch_takes():
+    """2^26 rows of logits, a wavefront each: the choices and the gradients of those at the ends of the launches and between are
+    those of the same rows alone, bit for bit."""
+    tokens, experts, top_k = (1 << 26) + 37, 257, 2
+    rows = torch.tensor([0, 1, (1 << 25) - 1, 1 << 25, (1 << 25) + 1, (1 << 26) - 1, 1 << 26, tokens - 1], device=DEV)
+    logits = torch.zeros((tokens, experts), dtype=torch.bfloat16, device=DEV)
+    logits[rows] = logits_of(len(rows), experts, torch.bfloat16, 1).to(DEV)
+    grad = torch.zeros((tokens, top_k), device=DEV)
+    grad[rows] = normal(len(rows), top_k, torch.float32, 2, 0.0).to(DEV)
+    weights, chosen = nk.experts_route(logits, top_k)
+    few, few_chosen = nk.experts_route(logits[rows], top_k)
+    assert torch.equal(weights[rows], few) and torch.equal(chosen[rows], few_chosen)
+    assert int((chosen != torch.arange(top_k, device=DEV)).any(1).sum()) <= len(rows)  # (equal logits: the first two)
+    got = nk.experts_route_backward(grad, logits, chosen)
+    assert torch.equal(got[rows], nk.experts_route_backward(grad[rows], logits[rows], few_chosen))
+    del logits, got
+    torch.cuda.empty_cache()
+
+
 # ---- the plan and the products ---------------------------------------------------------------------------------------
 
 def routing(tokens, top_k, experts, kind, seed=0):

@@ -114,6 +114,18 @@ def test_experts_products_refuse():
             assert "workspace" in refused(*call(weights=weights, workspace=workspace, room=room))
 
 
+def test_products_refuse_before_anything_is_queued():
+    """What is too large for the kernels' own counts: no launch for A's rows goes before the refusal."""
+    most = (1 << 31) - 1
+    call = lambda height, width, depth: ("mx_dots_packed_async", BF16, SOME, 2 * depth, None, 0, SOME, F32, SOME, 4 * width,  # noqa: E731
+                                         height, width, depth, SOME, 1 << 62, None)
+    assert "too many tiles" in refused(*call(most, most, 32)) and "too large" in refused(*call(most, 100, 1 << 20))
+    slots = 1 << 29  # (rows that eight slots share would be quantised first)
+    call = lambda width, depth: ("mx_dots_experts_async", BF16, SOME, 2 * depth, None, 0, 8, SOME, SOME, slots, 8, 8, None, F32, SOME, 4 * width,  # noqa: E731
+                                 width, depth, SOME, 1 << 62, None)
+    assert "too large" in refused(*call(100, 1 << 16)) and "too many tiles" in refused(*call(most, 256))
+
+
 def test_routing_refuses():
     def how(groups=1, top_groups=1, group_top=1):
         return ctypes.byref(binding._Route(0, 1, 1.0, groups, top_groups, group_top))
