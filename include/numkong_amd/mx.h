@@ -69,14 +69,15 @@ typedef struct {
     float scale;      /* and multiplied by this */
     int groups;       /* experts stand in so many groups of equal size (1: no groups) */
     int top_groups;   /* of which so many stay, those whose */
-    int group_top;    /* best so many (1 or 2) selection scores have the largest sum */
+    int group_top;    /* best so many (1 or 2) selection scores have the largest sum; a masked expert adds nothing to it */
 } nk_amd_route_t;
 
 /**
  *  For each of `tokens` rows of logits (f32, bf16 or f16) the `top_k` experts of largest selection score, in descending
  *  order, ties to the lowest index: `chosen` (tokens x top_k, i32), and their weights (tokens x top_k, f32). The selection
  *  score is the logit, or score + bias[expert] (f32) where a bias is given; weights never contain the bias. A logit of
- *  -inf is never chosen: where a row has too few others, the expert is -1 and its weight 0. A NaN ranks above all numbers.
+ *  -inf is never chosen: where a row (the groups of it that stay) has too few others, the expert is -1 and its weight 0. Groups
+ *  with an expert that can be chosen stand before those without. A NaN ranks above all numbers.
  *  At most 1024 experts, top_k at most 64, 64 groups.
  */
 NK_DYNAMIC int nk_amd_experts_route_async(nk_dtype_t dtype, void const *logits, nk_size_t logits_stride,

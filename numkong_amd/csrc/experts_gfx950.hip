@@ -227,7 +227,11 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
     if (p.how.groups > 1) {
         uint32_t const groups = (uint32_t)p.how.groups, size = p.experts / groups, lanes = size / J;
         bool const two = p.how.group_top == 2 && size > 1;
-        auto const group_key = [&](uint32_t first, uint32_t second) { return two ? key_of(number_of(first) + number_of(second)) : first; };
+        // (a masked expert adds nothing to its group, and a group with one that can be chosen stands before those without, also where
+        // a sum of the lowest numbers overflows: what cannot be chosen never keeps out what can)
+        auto const group_key = [&](uint32_t first, uint32_t second) {
+            return two && second > kMaskedKey ? larger(key_of(number_of(first) + number_of(second)), kMaskedKey + 1) : first;
+        };
         auto const best_two = [&](uint32_t lanes, uint32_t &first, uint32_t &second) __attribute__((always_inline)) { // of adjacent lanes, in all
             reduce_steps(lanes, [&](auto step) __attribute__((always_inline)) {
                 uint32_t const other = across<decltype(step)::value>(first), next = across<decltype(step)::value>(second);

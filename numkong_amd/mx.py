@@ -403,7 +403,8 @@ def experts_route(logits, top_k: int, score: str = "softmax", bias=None, groups:
     (float32, one for each expert) where a bias is given; the weights are the scores themselves, divided by their sum over
     the chosen where ``renormalize`` is set, times ``scale``. With ``groups`` > 1 the experts stand in groups of equal size, of
     which the ``top_groups`` stay whose ``group_top`` (1 or 2) best selection scores have the largest sum (without a bias:
-    the sum of logits). A logit of -inf is never chosen; a row with too few others gets expert -1 with weight 0."""
+    the sum of logits; the sum of scores that a bias of zeros gives is another). A logit of -inf is never chosen and adds
+    nothing to its group; a row with too few others in the groups that stay gets expert -1 with weight 0."""
     if _CALLS is not None:
         if (made := _CALLS.route(logits, top_k, bias, _SCORES.get(score), bool(renormalize), scale, groups, top_groups, group_top)) is not None:
             return made

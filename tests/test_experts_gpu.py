@@ -100,6 +100,58 @@ def test_masked_logits(score, experts, groups, top_groups):
     assert bool(grad.isfinite().all()) and not grad[0].any() and not grad[logits.isneginf().to(DEV)].any()
 
 
+def choice_of_two(selection, groups, top_groups):
+    """64-bit selection scores where groups are picked by the sum of their best two; of one that can be chosen, by that one."""
+    inside = selection.reshape(len(selection), groups, -1)
+    best = np.sort(inside, 2)[:, :, ::-1]
+    low = float(torch.finfo(torch.float32).min)
+    second = np.where(np.isneginf(best[:, :, 1]), 0.0, best[:, :, 1])
+    of_group = np.where(np.isneginf(best[:, :, 0]), -np.inf, np.maximum(best[:, :, 0] + second, low))
+    order = np.argsort(-of_group, axis=1, kind="stable")
+    keep = np.zeros_like(of_group, dtype=bool)
+    np.put_along_axis(keep, order[:, :top_groups], True, 1)
+    return np.where(keep[:, :, None], inside, -np.inf).reshape(selection.shape)
+
+
+@pytest.mark.parametrize("tokens", [40, 4200])  # a wavefront for a token, and 16 lanes
+@pytest.mark.parametrize("experts,groups,top_groups", [(64, 8, 4), (64, 8, 1), (30, 5, 2), (100, 5, 2), (144, 9, 3), (256, 8, 3), (512, 64, 20), (1000, 50, 7)])
+def test_masked_experts_in_groups(tokens, experts, groups, top_groups):
+    """Whatever is masked, the groups that stay are those that have something to choose, by two best of it. Logits are whole
+    numbers, scores with a bias ones and quarters: sums of two are exact, and ties go to the lowest."""
+    generator = torch.Generator().manual_seed(experts + groups)
+    logits = torch.randint(-20, 21, (tokens, experts), generator=generator).float()
+    masked = torch.rand((tokens, experts), generator=generator) < torch.rand((tokens, 1), generator=generator) ** 0.2
+    logits[masked] = -float("inf")
+    size = experts // groups
+    logits[0], logits[0, -4] = -float("inf"), 3.0  # a single expert, in the last group
+    logits[1], logits[1, -size:] = -float("inf"), torch.finfo(torch.float32).min  # lowest numbers are numbers, their sum as well
+    logits[2], logits[2, -1], logits[2, 0] = -float("inf"), -20.0, -19.0
+    logits[3] = -float("inf")
+    logits[4], logits[4, -2] = -float("inf"), float("inf")
+    logits[4, -size - 1] = 5.0
+    bias = torch.randint(-3, 4, (experts,), generator=generator) / 4
+    for score, of in (("softmax", None), ("sigmoid", bias)):
+        x = logits if of is None else torch.where(logits.isneginf(), logits, 60.0)
+        selection = x.double().numpy() if of is None else np.where(np.isneginf(x.numpy()), -np.inf, 1.0 + bias.double().numpy())
+        selection = choice_of_two(selection, groups, top_groups)
+        order = np.argsort(-selection, axis=1, kind="stable")[:, :4]
+        there = ~np.isneginf(np.take_along_axis(selection, order, 1))
+        weights, chosen = nk.experts_route(x.to(DEV), 4, score, None if of is None else of.to(DEV), groups, top_groups, 2)
+        np.testing.assert_array_equal(chosen.cpu().numpy(), np.where(there, order, -1))
+        assert (weights.cpu().numpy()[~there] == 0).all()
+        assert chosen[0].tolist() == [experts - 4, -1, -1, -1] and int(chosen[1, 0]) >= experts - size and int(chosen[4, 0]) >= 0
+
+
+def test_groups_by_scores():
+    """Groups by the sum of two scores, not of two logits, are what a bias of zeros gives."""
+    logits = torch.tensor([[6.0, -6.0, 0.1, 0.1], [0.0, 9.0, 4.0, 4.5], [-3.0, 2.0, 0.0, 0.0]])
+    s = torch.sigmoid(logits.double()).reshape(3, 2, 2).sum(2)
+    _, chosen = nk.experts_route(logits.to(DEV), 2, "sigmoid", torch.zeros(4, device=DEV), 2, 1, 2)
+    assert torch.equal(chosen.cpu() // 2, s.argmax(1, keepdim=True).expand(3, 2))
+    _, chosen = nk.experts_route(logits.to(DEV), 2, "sigmoid", None, 2, 1, 2)
+    assert torch.equal(chosen.cpu() // 2, logits.reshape(3, 2, 2).sum(2).argmax(1, keepdim=True).expand(3, 2))
+
+
 @pytest.mark.parametrize("experts,groups,top_groups", [(100, 1, 1), (100, 5, 2), (144, 1, 1), (144, 9, 3), (256, 8, 3)])
 def test_many_tokens_choose_as_few(experts, groups, top_groups):
     """Masks, ties, NaNs and infinities among as many tokens as share wavefronts: chosen as where a token has its own. (Sigmoid
