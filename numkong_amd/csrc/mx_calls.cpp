@@ -35,6 +35,7 @@ struct Library {
     decltype(&nk_amd_mx_dots_experts_async) experts;
 };
 Library library;
+decltype(&nk_amd_mx_packed_size) packed_size;
 
 PyObject *bind(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
     if (count != (Py_ssize_t)(sizeof(Library) / sizeof(void *))) {
@@ -51,6 +52,13 @@ PyObject *bind(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
     }
     memcpy(&library, addresses, sizeof(library));
     Py_RETURN_NONE;
+}
+
+PyObject *bind_packed_size(PyObject *, PyObject *address) {
+    packed_size = (decltype(packed_size))PyLong_AsVoidPtr(address);
+    if (packed_size) Py_RETURN_NONE;
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "the address is NULL");
+    return nullptr;
 }
 
 /** Other threads of Python may run while the work is queued. */
@@ -169,7 +177,7 @@ PyObject *dots(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
     at::Tensor const *const image = tensor_of(arguments[3], 1, home);
     at::ScalarType const type = ((THPDtype *)arguments[6])->scalar_type;
     nk_dtype_t const dtype = code_of(type);
-    if (!image || !dtype) Py_RETURN_NONE;
+    if (!image || !dtype || image->nbytes() < packed_size(1, width, depth)) Py_RETURN_NONE;
     at::Tensor c, workspace;
     int status;
     {
@@ -291,7 +299,9 @@ PyObject *experts(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
     at::ScalarType const type = ((THPDtype *)arguments[12])->scalar_type;
     nk_dtype_t const dtype = code_of(type);
     int64_t const slots = tokens * top_k, rows = a.t->size(0);
-    if (!image || !plan_ || !dtype || (rows != tokens && rows != slots)) Py_RETURN_NONE;
+    if (!image || !plan_ || !dtype || (rows != tokens && rows != slots) || image->nbytes() < packed_size(matrices, width, depth) ||
+        plan_->nbytes() < library.plan_size(slots, matrices))
+        Py_RETURN_NONE;
     if (arguments[11] != Py_None) {
         weights = tensor_of(arguments[11], 2, home);
         if (!weights || weights->scalar_type() != at::kFloat || weights->size(0) != tokens || weights->size(1) != top_k || !weights->is_contiguous())
@@ -316,7 +326,7 @@ PyObject *experts(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
 }
 
 #define CALL(name) {#name, (PyCFunction)(void (*)())name, METH_FASTCALL, nullptr}
-PyMethodDef calls[] = {CALL(bind), CALL(quantize), CALL(dequantize), CALL(dots), CALL(route), CALL(route_backward), CALL(plan), CALL(experts),
+PyMethodDef calls[] = {CALL(bind), {"bind_packed_size", bind_packed_size, METH_O, nullptr}, CALL(quantize), CALL(dequantize), CALL(dots), CALL(route), CALL(route_backward), CALL(plan), CALL(experts),
                        {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mx_calls", nullptr, -1, calls, nullptr, nullptr, nullptr, nullptr};
 

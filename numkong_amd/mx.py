@@ -71,6 +71,7 @@ def _library():
             _mx_calls.bind(*(ctypes.cast(getattr(lib, "nk_amd_" + name), ctypes.c_void_p).value for name in (
                 "mx_quantize_async", "mx_dequantize_async", "mx_dots_workspace_size", "mx_dots_packed_async", "experts_route_async",
                 "experts_route_backward_async", "experts_plan_size", "experts_plan_async", "mx_experts_workspace_size", "mx_dots_experts_async")))
+            _mx_calls.bind_packed_size(ctypes.cast(lib.nk_amd_mx_packed_size, ctypes.c_void_p).value)
         _CALLS = _mx_calls
     return _LIB
 
@@ -175,6 +176,12 @@ def _check_host_out(out, shape, dtype):
             raise TypeError(f"out must have dtype {dtype}")
         if t.is_cuda:
             raise ValueError("out is in GPU memory, the operands in host memory")
+
+
+def _check_room(buffer, needed: int, what: str) -> None:
+    """What a kernel finds its way in by sizes alone has to be as large as these say."""
+    if buffer.nbytes < needed or not buffer.is_contiguous():
+        raise ValueError(f"{what} has to be {needed} adjacent bytes for these sizes, got {buffer.nbytes}")
 
 
 def _out_dtype(out, out_dtype):
@@ -371,6 +378,7 @@ def mx_dots_packed(a, packed: MxPackedMatrix, out=None, out_dtype=None):
     if index != _device():
         with torch.cuda.device(index):
             return mx_dots_packed(a, packed, out, out_dtype)
+    _check_room(packed.buffer, lib.nk_amd_mx_packed_size(1, width, depth), "the packed image")
     result = _result(torch, out, (height, width), out_dtype, t)
     needed = lib.nk_amd_mx_dots_workspace_size(height, width, depth, scales is not None)
     workspace = torch.empty_strided((needed,), (1,), dtype=torch.uint8, device=t.device) if needed else None
@@ -539,6 +547,8 @@ def mx_dots_experts(a, packed: MxPackedMatrix, plan: ExpertsPlan, weights=None, 
     if index != _device():
         with torch.cuda.device(index):
             return mx_dots_experts(a, packed, plan, weights, out, out_dtype)
+    _check_room(packed.buffer, lib.nk_amd_mx_packed_size(plan.experts, width, depth), "the packed image")
+    _check_room(plan.buffer, lib.nk_amd_experts_plan_size(slots, plan.experts), "the plan")
     result = _result(torch, out, shape, out_dtype, t)
     if weights is not None:
         weights, stride = weights.contiguous(), _row_bytes(result)

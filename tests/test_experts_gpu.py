@@ -421,6 +421,37 @@ def test_plan_of_other_sizes_gives_nans(tokens, experts):
     assert (nk.mx_dots_experts(a, packed, right) == 64).all()
 
 
+@pytest.mark.parametrize("short_way", [True, False])
+def test_images_and_plans_are_as_large_as_their_sizes_say(monkeypatch, short_way):
+    """Parts of an image or a plan, and buffers that are not in one piece, are refused before a kernel looks for the rest."""
+    from numkong_amd import mx as binding
+
+    a, packed, stack = torch.ones((6, 64), device=DEV), nk.mx_pack(torch.ones((80, 64), device=DEV)), nk.mx_pack(torch.ones((8, 80, 64), device=DEV))
+    plan = nk.experts_plan(torch.zeros((6, 2), dtype=torch.int32, device=DEV), 8)
+    if not short_way:
+        monkeypatch.setattr(binding, "_CALLS", None)
+
+    def parts(buffer):
+        twice = torch.zeros(2 * buffer.numel(), dtype=torch.uint8, device=DEV)
+        return buffer[:0], buffer[:1], buffer[:-1], buffer[:64].clone(), twice[::2]
+
+    for part in parts(packed.buffer):
+        with pytest.raises(ValueError, match="packed image"):
+            nk.mx_dots_packed(a, nk.MxPackedMatrix(1, 80, 64, part))
+    with pytest.raises(ValueError, match="packed image"):
+        nk.mx_dots_packed(a, nk.MxPackedMatrix(1, 1 << 30, 64, packed.buffer))
+    for weights in (None, torch.ones((6, 2), device=DEV)):
+        for part in parts(stack.buffer):
+            with pytest.raises(ValueError, match="packed image"):
+                nk.mx_dots_experts(a, nk.MxPackedMatrix(8, 80, 64, part), plan, weights)
+        for part in parts(plan.buffer):
+            with pytest.raises(ValueError, match="the plan"):
+                nk.mx_dots_experts(a, stack, nk.ExpertsPlan(6, 2, 8, part), weights)
+        larger = [torch.cat([one, one.new_zeros(100)]) for one in (stack.buffer, plan.buffer)]
+        got = nk.mx_dots_experts(a, nk.MxPackedMatrix(8, 80, 64, larger[0]), nk.ExpertsPlan(6, 2, 8, larger[1]), weights)
+        assert bool((got == (64 if weights is None else 128)).all())
+
+
 def test_no_tokens():
     packed = nk.mx_pack(torch.ones((4, 64, 64), device=DEV))
     plan = nk.experts_plan(torch.zeros((0, 2), dtype=torch.int32, device=DEV), 4)
