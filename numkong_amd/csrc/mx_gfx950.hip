@@ -282,7 +282,6 @@ struct MxArgs {
     uint64_t a_pitch, c_stride;
     uint32_t m, n, k, steps, supers, tiles, count;
     uint32_t tiles_m, tiles_n; // the grid: tiles of rows, tiles of columns
-    uint32_t first_n;          // tiles of columns of the launches before (products of few rows)
     uint32_t band;             // tiles of rows that are walked side by side
     uint32_t order, tile_list; // words into the plan
     uint32_t a_share;          // slots that share a row of A
@@ -579,10 +578,9 @@ __global__ __launch_bounds__(64 * WAVES, FM >= 4 ? 2 : 4) void mx_few_kernel(MxA
         uint32_t const index = blockIdx.x >> 3, column = index / p.tiles_m;
         tile_m = index - column * p.tiles_m, tile_n = column * 8 + (blockIdx.x & 7);
         if (tile_n >= p.tiles_n) return;
-        tile_n += p.first_n;
     }
     else {
-        tile_m = blockIdx.x / p.tiles_n, tile_n = p.first_n + blockIdx.x - tile_m * p.tiles_n;
+        tile_m = blockIdx.x / p.tiles_n, tile_n = blockIdx.x - tile_m * p.tiles_n;
         if (!plan_matches(p.plan, p.m, p.count)) { // NaNs, as in mx_gemm_kernel
             uint32_t const column = tile_n * NT * 16 + threadIdx.x;
             if (!p.sorted && threadIdx.x < NT * 16 && column < p.n)
@@ -825,6 +823,10 @@ int check_size(uint64_t rows, uint64_t row_tiles, uint64_t n, MxGeometry const &
  *  `values`: of A, as many as a workgroup is expected to have; `rows`: the most that it may have, which have to fit.
  */
 constexpr uint32_t kFusedBytes = 64 * 1024, kFusedValues = 16 * 1024;
+/** Does a launch take all tiles of a product of few rows, at 512 threads for 16 columns of a tile of rows? Where it does not (2^27 columns, 2^15 of
+ *  a thousand experts) the kernel for many rows has the work, whose workgroups stay, and A is staged for it. (The kernel for few rows in
+ *  several launches, each told where its columns begin: 1 x 8192 x 8192 8.9 us instead of 8.6.) */
+bool launches_few(uint64_t row_tiles, uint64_t n) { return row_tiles * ((n + 15) / 16 + 7) * 512 < 1ull << 32; }
 uint32_t fused_bytes(uint32_t rows, MxGeometry const &g) { return rows * (g.steps * 64 + 16) + rows * g.steps * 4; }
 bool fuses(uint64_t rows, uint64_t values, MxGeometry const &g) {
     return rows <= 16 && values <= kFusedValues && (uint64_t)rows * (g.steps * 68 + 16) <= kFusedBytes;
@@ -832,19 +834,14 @@ bool fuses(uint64_t rows, uint64_t values, MxGeometry const &g) {
 
 template <int WAVES, int FM, int NT, class In, class Out, bool GROUPED>
 int launch_few_of(MxArgs &p, uint32_t max_rows, MxGeometry const &g, hipStream_t stream) {
+    p.tiles_n = (p.tiles + NT - 1) / NT;
+    if (!GROUPED) p.tiles_m = (p.m + 16 * FM - 1) / (16 * FM);
+    uint32_t const grid = p.tiles_m * (GROUPED ? p.tiles_n : (p.tiles_n + 7) / 8 * 8); // (launches_few)
     uint32_t lds = WAVES * FM * NT * 1024;
     if (sizeof(In) != 1 && fused_bytes(max_rows, g) > lds) lds = fused_bytes(max_rows, g);
-    if (!GROUPED) p.tiles_m = (p.m + 16 * FM - 1) / (16 * FM);
-    // tiles of columns of one launch (tiles of rows are few thousands at most, see launch_product and plan_tile_rows)
-    uint32_t const tiles_n = (p.tiles + NT - 1) / NT, slab = (uint32_t)(kMostThreads / (64 * WAVES) / p.tiles_m) / 8 * 8;
-    for (p.first_n = 0; p.first_n < tiles_n; p.first_n += slab) {
-        p.tiles_n = tiles_n - p.first_n < slab ? tiles_n - p.first_n : slab;
-        uint32_t const grid = p.tiles_m * (GROUPED ? p.tiles_n : (p.tiles_n + 7) / 8 * 8);
-        hipLaunchKernelGGL((mx_few_kernel<WAVES, FM, NT, In, Out, GROUPED>), dim3(grid), dim3(64 * WAVES), lds, stream, p);
-        hipError_t const e = hipGetLastError();
-        if (e != hipSuccess) return mx_fail(e, "mx_few_kernel");
-    }
-    return 0;
+    hipLaunchKernelGGL((mx_few_kernel<WAVES, FM, NT, In, Out, GROUPED>), dim3(grid), dim3(64 * WAVES), lds, stream, p);
+    hipError_t const e = hipGetLastError();
+    return e == hipSuccess ? 0 : mx_fail(e, "mx_few_kernel");
 }
 template <int FM, int NT, class In, class Out, bool GROUPED>
 int launch_few(MxArgs &p, uint32_t max_rows, MxGeometry const &g, hipStream_t stream) {
@@ -875,11 +872,12 @@ int launch_gemm(MxArgs &p, hipStream_t stream) {
  *  8192^3 289 and 273; but 9000 x 9000 x 8192, 6 rounds of 256 rows for 5.06, 327 and 356, 6000 x 6000 x 8192, 3 for 2.25, 164 and 183).
  */
 template <class Out, bool GROUPED>
-int launch_product(MxArgs &p, uint32_t tile_rows, int a_dtype, bool fused, uint32_t fused_rows, MxGeometry const &g, hipStream_t stream) {
+int launch_product(MxArgs &p, bool few, uint32_t tile_rows, int a_dtype, bool fused, uint32_t fused_rows, MxGeometry const &g, hipStream_t stream) {
     auto const tiles_of = [&](uint64_t rows, uint64_t columns) { return (p.m + rows - 1) / rows * ((p.n + columns - 1) / columns); };
     uint64_t const large = tiles_of(256, 256), rounds = (large + 255) / 256;
     bool const whole_rounds = large * 20 >= rounds * 256 * 19;
-    uint32_t const rows = GROUPED ? tile_rows : p.m <= 32 || tiles_of(128, 256) < 64 ? (p.m < 64 ? p.m : 64) : g.steps > 48 && whole_rounds ? 256 : 128;
+    bool const small = p.m <= 32 || tiles_of(128, 256) < 64;
+    uint32_t const rows = GROUPED ? (few ? tile_rows : 128) : few && small ? (p.m < 64 ? p.m : 64) : g.steps > 48 && whole_rounds ? 256 : 128;
     if (rows <= 16) {
         constexpr int NT = GROUPED ? 2 : 1; // (experts of 4 tokens, 28 matrices of 2048 x 2048: 13.0 us with two, 14.0 with one)
         if (!fused) return launch_few<1, NT, uint8_t, Out, GROUPED>(p, rows, g, stream);
@@ -914,12 +912,13 @@ struct ExpertsLayout {
     Staging staged;
     uint64_t codes_at, codes_stride, codes_scales_at, codes_scales_stride; // A's rows as codes, where they are quantised first
     uint64_t sums_at, sums_values, bytes; // rows of the plan before they are summed: values a row
-    bool fused, quantised;
+    bool few, fused, quantised;
 };
 ExpertsLayout experts_layout(PlanGeometry const &shape, uint64_t slots, uint64_t a_share, uint64_t experts, uint64_t n, uint64_t k,
                              MxGeometry const &g, bool a_is_codes, bool weighted) {
     ExpertsLayout l = {};
-    l.fused = !a_is_codes && shape.tile_rows == 16 && fuses(16, (slots / experts + 1) * k, g);
+    l.few = launches_few(shape.max_tiles, n);
+    l.fused = l.few && !a_is_codes && shape.tile_rows == 16 && fuses(16, (slots / experts + 1) * k, g);
     if (!l.fused) l.staged = staging_of(shape.max_rows, g);
     uint64_t at = l.staged.bytes;
     // Rows that go to several experts are quantised once and gathered as codes, where that is worth a launch more (32,768 slots
@@ -1008,7 +1007,7 @@ int nk_amd_mx_pack_async(void const *codes, nk_size_t codes_stride, nk_size_t co
 nk_size_t nk_amd_mx_dots_workspace_size(nk_size_t height, nk_size_t width, nk_size_t depth, int a_is_codes) {
     MxGeometry g;
     if (!height || !width || height >= (1ull << 31) || !mx_geometry(1, width, depth, g)) return 0;
-    return !a_is_codes && fuses(height, height * depth, g) ? 0 : staging_of(height, g).bytes;
+    return !a_is_codes && launches_few((height + 63) / 64, width) && fuses(height, height * depth, g) ? 0 : staging_of(height, g).bytes;
 }
 
 int nk_amd_mx_dots_packed_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_stride, void const *a_scales,
@@ -1023,7 +1022,7 @@ int nk_amd_mx_dots_packed_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_s
     if (int const status = depth ? check_a(a_dtype, a, a_scales, a_stride) : 0) return status;
     if (int const status = check_c(c_dtype, c, c_stride)) return status;
     if (!packed || ((uintptr_t)packed & 15)) return mx_fail("mx_dots_packed: the image has to be 16-byte aligned");
-    bool const fused = !a_scales && fuses(height, height * depth, g);
+    bool const few = launches_few((height + 63) / 64, width), fused = few && !a_scales && fuses(height, height * depth, g);
     MxArgs p = {};
     p.image = (uint8_t const *)packed, p.c = (uint8_t *)c, p.c_stride = c_stride;
     p.m = (uint32_t)height, p.n = (uint32_t)width, p.k = (uint32_t)depth, p.count = 1, p.a_share = 1;
@@ -1038,7 +1037,7 @@ int nk_amd_mx_dots_packed_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_s
         p.a = (uint8_t const *)workspace, p.a_scales = p.a + s.scales_at;
     }
     return with_type(c_dtype, [&](auto value) {
-        return launch_product<decltype(value), false>(p, 0, a_dtype, fused, p.m, g, stream);
+        return launch_product<decltype(value), false>(p, few, 0, a_dtype, fused, p.m, g, stream);
     });
 }
 
@@ -1090,7 +1089,7 @@ int nk_amd_mx_dots_experts_async(nk_dtype_t a_dtype, void const *a, nk_size_t a_
     if (weights) p.sorted = 1, p.c = sums, p.c_stride = l.sums_values * 4;
     else p.c = (uint8_t *)c, p.c_stride = c_stride;
     int const status = with_type(product_dtype, [&](auto value) {
-        return launch_product<decltype(value), true>(p, shape.tile_rows, a_dtype, l.fused, 16, g, stream);
+        return launch_product<decltype(value), true>(p, l.few, shape.tile_rows, a_dtype, l.fused, 16, g, stream);
     });
     if (status || !weights) return status;
     uint64_t const tokens = slots / top_k, pieces = (width + 3) / 4;
