@@ -459,10 +459,10 @@ __global__ __launch_bounds__(kScanBuckets * kScanParts) void plan_scan_kernel(ui
  *  stand between experts; the tiles are written by all in turn, as one expert may have most of them. Its time is that of a few loads
  *  and LDS round trips one after the other: 32 slots 3.4 us, 1,024 5.3, 4,004 with the launch that counts 8.5, 32,768 9.4.
  */
-template <int BATCH>
+template <int BATCH, bool SCANNED>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(int32_t const *chosen, uint32_t slots, uint32_t experts, PlanHeader header,
                                                             uint32_t offsets, uint32_t order, uint32_t place, uint32_t tiles, int bits,
-                                                            uint32_t const *table, bool scanned, uint32_t *plan) {
+                                                            uint32_t const *table, uint32_t blocks, uint32_t *plan) {
     extern __shared__ uint32_t plan_lds[]; // [wave][bucket] counts, then where the wave's next slot of the bucket goes
     __shared__ uint32_t wave_total[2][kPlanWaves];
     uint32_t const buckets = experts + 1, thread = threadIdx.x, lane = thread & 63;
@@ -483,11 +483,11 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(int32_t const *chose
         if (bucket < buckets) {
 #pragma unroll
             for (int w = 0; w < kPlanWaves; ++w) here[w] = plan_lds[w * buckets + bucket], size += here[w];
-            if (scanned) earlier = table[blockIdx.x * buckets + bucket], size = table[gridDim.x * buckets + bucket];
+            if (SCANNED) earlier = table[blockIdx.x * buckets + bucket], size = table[blocks * buckets + bucket];
             else if (table) {
                 size = 0;
 #pragma unroll 8
-                for (uint32_t block = 0; block < gridDim.x; ++block) {
+                for (uint32_t block = 0; block < blocks; ++block) {
                     uint32_t const its = table[block * buckets + bucket];
                     size += its, earlier += block < blockIdx.x ? its : 0;
                 }
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(int32_t const *chose
             uint32_t next = first + earlier;
 #pragma unroll
             for (int w = 0; w < kPlanWaves; ++w) plan_lds[w * buckets + bucket] = next, next += here[w];
-            for (uint32_t t = blockIdx.x; t < its_tiles; t += gridDim.x) {
+            for (uint32_t t = blockIdx.x; t < its_tiles; t += blocks) {
                 uint32_t const from = first + t * header.tile_rows, to = from + header.tile_rows;
                 PlanTile const tile = {(int32_t)bucket, (int32_t)from, (int32_t)(to < first + size ? to : first + size), 0};
                 *(PlanTile *)(plan + tiles + (first_tile + t) * 4) = tile;
@@ -661,9 +661,9 @@ int nk_amd_experts_plan_async(nk_i32_t const *chosen, nk_size_t slots, nk_size_t
     // Slots that fit one a lane are not followed by three more. (Up to 4,096 slots without the launch that counts, each workgroup
     // counting all slots: 7.3 us instead of 8.5 by itself, but 11.0 instead of 9.4 where `chosen` is not in the caches any more; eight
     // slots a lane: 15.5 us for 32,768.)
-    auto *const kernel = slots <= kPlanThreads ? plan_kernel<1> : plan_kernel<4>;
+    auto *const kernel = slots <= kPlanThreads ? plan_kernel<1, false> : scanned ? plan_kernel<4, true> : plan_kernel<4, false>;
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kPlanThreads), lds * kPlanWaves, (hipStream_t)stream, chosen, (uint32_t)slots, (uint32_t)experts,
-                       header, (uint32_t)g.offsets, (uint32_t)g.order, (uint32_t)g.place, (uint32_t)g.tiles, bits, table, scanned, (uint32_t *)plan);
+                       header, (uint32_t)g.offsets, (uint32_t)g.order, (uint32_t)g.place, (uint32_t)g.tiles, bits, table, blocks, (uint32_t *)plan);
     hipError_t const e = hipGetLastError();
     return e == hipSuccess ? 0 : mx_fail(e, "plan_kernel");
 }
