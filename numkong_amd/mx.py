@@ -163,6 +163,8 @@ def _result(torch, out, shape, dtype, like):
         raise ValueError(f"out is on {t.device}, the operands on {like.device}")
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError("out rows must be contiguous")
+    if t.dim() == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError("out rows share memory")
     return t
 
 

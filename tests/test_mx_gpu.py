@@ -145,6 +145,23 @@ def test_product_of_views(m, n):
         assert bool((store == 77.0).all())
 
 
+def test_results_whose_rows_share_memory_are_refused():
+    a, packed, matrix = torch.ones((4, 64), device=DEV), nk.mx_pack(torch.ones((8, 64), device=DEV)), nk.mx_quantize(torch.ones((4, 64), device=DEV))
+    stack, plan = nk.mx_pack(torch.ones((2, 8, 64), device=DEV)), nk.experts_plan(torch.zeros((4, 1), dtype=torch.int32, device=DEV), 2)
+    weights = torch.ones((4, 1), device=DEV)
+    row = torch.zeros(100, device=DEV)
+    for step in (0, 1, 7):
+        out = row.as_strided((4, 8), (step, 1))
+        with pytest.raises(ValueError, match="share memory"):
+            nk.mx_dots_packed(a, packed, out=out)
+        with pytest.raises(ValueError, match="share memory"):
+            nk.mx_dots_experts(a, stack, plan, weights, out=out)
+        with pytest.raises(ValueError, match="share memory"):
+            nk.mx_dequantize(matrix, out=row.as_strided((4, 64), (step, 1)))
+    out = row.as_strided((4, 8), (8, 1))
+    assert bool((nk.mx_dots_packed(a, packed, out=out) == 64).all()) and bool((nk.mx_dots_packed(a[:1], packed, out=row.as_strided((1, 8), (0, 1))) == 64).all())
+
+
 @pytest.mark.parametrize("m,n", [(1, 90), (20, 90), (70, 90), (260, 90), (1100, 2100), (2100, 8200)])
 def test_special_values_stay_in_their_rows(m, n):
     k = 200
