@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
@@ -101,13 +102,16 @@ at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type, at::Tensor const &l
 }
 void *stream_of(Home const &home) { return (void *)c10::hip::getCurrentHIPStream((c10::DeviceIndex)home.index).stream(); }
 
+/** Does autograd follow it? Then mx.py says what becomes of the gradient. */
+bool tracked(at::Tensor const &t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+
 /** What a product's call says of A: a float matrix, or codes and scales. */
 struct Left {
     at::Tensor const *t = nullptr, *scales = nullptr;
     int64_t depth = 0;
     nk_dtype_t dtype = nk_dtype_t(0);
     bool found(PyObject *a, PyObject *its_scales, PyObject *its_depth, Home &home) {
-        if (!(t = tensor_of(a, 2, home))) return false;
+        if (!(t = tensor_of(a, 2, home)) || tracked(*t)) return false;
         if (its_scales == Py_None) {
             depth = t->size(1), dtype = code_of(t->scalar_type());
             return dtype != 0;
@@ -215,7 +219,7 @@ PyObject *route(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
     nk_dtype_t const dtype = logits ? code_of(logits->scalar_type()) : nk_dtype_t(0);
     int64_t top_k;
     nk_amd_route_t how;
-    if (!dtype || !natural(arguments[1], top_k) || !route_of(arguments + 3, true, how)) Py_RETURN_NONE;
+    if (!dtype || tracked(*logits) || !natural(arguments[1], top_k) || !route_of(arguments + 3, true, how)) Py_RETURN_NONE;
     int64_t const tokens = logits->size(0), experts = logits->size(1);
     if (arguments[2] != Py_None) {
         bias = tensor_of(arguments[2], 1, home);
@@ -304,7 +308,8 @@ PyObject *experts(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
         Py_RETURN_NONE;
     if (arguments[11] != Py_None) {
         weights = tensor_of(arguments[11], 2, home);
-        if (!weights || weights->scalar_type() != at::kFloat || weights->size(0) != tokens || weights->size(1) != top_k || !weights->is_contiguous())
+        if (!weights || weights->scalar_type() != at::kFloat || weights->size(0) != tokens || weights->size(1) != top_k || !weights->is_contiguous() ||
+            tracked(*weights))
             Py_RETURN_NONE;
     }
     at::Tensor y, workspace;

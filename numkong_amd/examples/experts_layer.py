@@ -35,30 +35,13 @@ class ExpertsLayer:
         return self.experts(x, self.scores(x))
 
 
-class RouteWeights(torch.autograd.Function):
-    """``experts_route`` for autograd: weights with a gradient, experts without."""
-
-    @staticmethod
-    def forward(ctx, logits, top_k, score):
-        weights, chosen = nk.experts_route(logits, top_k, score)
-        ctx.save_for_backward(logits, chosen)
-        ctx.score = score
-        ctx.mark_non_differentiable(chosen)
-        return weights, chosen
-
-    @staticmethod
-    def backward(ctx, grad_weights, _):
-        logits, chosen = ctx.saved_tensors
-        return nk.experts_route_backward(grad_weights, logits, chosen, ctx.score), None, None
-
-
 def train_router(x, wanted, experts: int, top_k: int, steps: int, rate: float = 0.5):
     """Teaches a router to give the weight of each token to its `wanted` expert; (first loss, last loss)."""
     router = torch.zeros((x.shape[1], experts), device=x.device, requires_grad=True)
     losses = []
     for _ in range(steps):
         logits = x @ router
-        weights, chosen = RouteWeights.apply(logits, top_k, "softmax")
+        weights, chosen = nk.experts_route(logits, top_k)  # (weights have a gradient)
         hit = chosen == wanted[:, None]
         # a token whose expert is not among the chosen pulls it up through the scores of all
         loss = ((1 - (weights * hit).sum(1)) * hit.any(1)).mean() + torch.nn.functional.cross_entropy(logits, wanted) * 0.5

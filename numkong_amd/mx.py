@@ -109,6 +109,54 @@ def _row_bytes(t) -> int:
     return (t.stride(0) if rows > 1 else columns) * t.itemsize
 
 
+_ROUTE = _PRODUCT = None  # what autograd knows of the calls below (torch's classes, made when the first is needed)
+
+
+def _autograd():
+    global _ROUTE, _PRODUCT
+    if _ROUTE is None:
+        import torch
+
+        class Route(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, logits, top_k, score, bias, groups, top_groups, group_top, renormalize, scale):
+                weights, experts = experts_route(logits, top_k, score, bias, groups, top_groups, group_top, renormalize, scale)
+                ctx.save_for_backward(logits, experts)
+                ctx.kind = score, renormalize, scale
+                ctx.mark_non_differentiable(experts)
+                return weights, experts
+
+            @staticmethod
+            @torch.autograd.function.once_differentiable
+            def backward(ctx, grad_weights, _):
+                return (experts_route_backward(grad_weights, *ctx.saved_tensors, *ctx.kind), *[None] * 8)
+
+        class Product(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, what, product, *operands):
+                ctx.what = what
+                return product()
+
+            @staticmethod
+            def backward(ctx, _):
+                raise NumKongAmdError(f"{ctx.what} has no gradient: detach its operands, or call it under torch.no_grad()")
+
+        _PRODUCT, _ROUTE = Product, Route
+
+
+def _tracked(torch, *operands) -> bool:
+    """Does autograd follow one of the operands?"""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands)
+
+
+def _without_gradient(what: str, out, product, *operands):
+    """The result of a product for autograd, which says so when a gradient is asked for that there is none of."""
+    if out is not None:
+        raise NumKongAmdError(f"{what} with out= takes no operands that require a gradient")
+    _autograd()
+    return _PRODUCT.apply(what, product, *operands)
+
+
 def _home(*operands):
     """The index of the GPU that the operands are on, None where all are in host memory."""
     home, host = None, False
@@ -263,7 +311,7 @@ class MxPackedMatrix:
 def mx_quantize(x) -> MxMatrix:
     """The rows of ``x`` (float32, bfloat16 or float16) as 4-bit codes with a scale for each 32 values: the power of two
     that brings the block's largest magnitude into [4, 8); codes to nearest, ties to even, stopping at 6. A block that holds a
-    NaN or an infinity becomes NaN."""
+    NaN or an infinity becomes NaN. Codes and scales are whole numbers, which no gradient passes."""
     if _CALLS is not None and (made := _CALLS.quantize(x)) is not None:
         return MxMatrix._made(*made, x.shape[1])
     lib, torch, dtype_codes = _LIB or _library()
@@ -355,7 +403,8 @@ def _left_operand(a, dtype_codes):
 
 def mx_dots_packed(a, packed: MxPackedMatrix, out=None, out_dtype=None):
     """``C[height x width] = a @ B.T`` with 4-bit operands and 32-bit sums. ``a``: floats, quantised on the way exactly as
-    ``mx_quantize`` does, or an MxMatrix; the result is float32 (default), bfloat16 or float16 (``out_dtype``, or ``out``'s)."""
+    ``mx_quantize`` does, or an MxMatrix; the result is float32 (default), bfloat16 or float16 (``out_dtype``, or ``out``'s).
+    There is no gradient: a backward pass through the result raises."""
     lib, torch, dtype_codes = _LIB or _library()
     if _CALLS is not None and out is None and type(packed) is MxPackedMatrix and packed.count == 1:
         values, scales, depth = (a.codes, a.scales, a.depth) if type(a) is MxMatrix else (a, None, None)
@@ -377,6 +426,8 @@ def mx_dots_packed(a, packed: MxPackedMatrix, out=None, out_dtype=None):
     index = t.get_device()
     if packed.buffer.get_device() != index:
         raise ValueError(f"a is on {t.device}, packed on {packed.buffer.device}")
+    if _tracked(torch, t):
+        return _without_gradient("mx_dots_packed", out, lambda: mx_dots_packed(a, packed, None, out_dtype), t)
     if index != _device():
         with torch.cuda.device(index):
             return mx_dots_packed(a, packed, out, out_dtype)
@@ -414,7 +465,9 @@ def experts_route(logits, top_k: int, score: str = "softmax", bias=None, groups:
     the chosen where ``renormalize`` is set, times ``scale``. With ``groups`` > 1 the experts stand in groups of equal size, of
     which the ``top_groups`` stay whose ``group_top`` (1 or 2) best selection scores have the largest sum (without a bias:
     the sum of logits; the sum of scores that a bias of zeros gives is another). A logit of -inf is never chosen and adds
-    nothing to its group; a row with too few others in the groups that stay gets expert -1 with weight 0."""
+    nothing to its group; a row with too few others in the groups that stay gets expert -1 with weight 0.
+
+    The weights have a gradient for ``logits`` (``experts_route_backward``), which autograd follows; none for ``bias``."""
     if _CALLS is not None:
         if (made := _CALLS.route(logits, top_k, bias, _SCORES.get(score), bool(renormalize), scale, groups, top_groups, group_top)) is not None:
             return made
@@ -431,6 +484,9 @@ def experts_route(logits, top_k: int, score: str = "softmax", bias=None, groups:
     if index is None:
         found = experts_route(_to_gpu(t), top_k, score, _to_gpu(bias), groups, top_groups, group_top, renormalize, scale)
         return tuple(_to_host(one, _is_numpy(logits)) for one in found)
+    if _tracked(torch, t):
+        _autograd()
+        return _ROUTE.apply(t, top_k, score, bias, groups, top_groups, group_top, renormalize, scale)
     if index != _device():
         with torch.cuda.device(index):
             return experts_route(t, top_k, score, bias, groups, top_groups, group_top, renormalize, scale)
@@ -511,7 +567,7 @@ def mx_dots_experts(a, packed: MxPackedMatrix, plan: ExpertsPlan, weights=None, 
     """``y[token, i] = B[expert i of the token] @ a[token]`` (tokens x top_k x width), zeros where a slot has no expert. ``a``
     has a row for each token, or one for each slot (tokens * top_k rows); floats or an MxMatrix as in ``mx_dots_packed``.
     With ``weights`` (tokens x top_k, float32) the rows of a token are summed by weight instead: tokens x width, slots without
-    an expert left out."""
+    an expert left out. There is no gradient: a backward pass through the result raises."""
     lib, torch, dtype_codes = _LIB or _library()
     if _CALLS is not None and out is None and type(packed) is MxPackedMatrix and type(plan) is ExpertsPlan:
         values, scales, depth = (a.codes, a.scales, a.depth) if type(a) is MxMatrix else (a, None, None)
@@ -546,6 +602,8 @@ def mx_dots_experts(a, packed: MxPackedMatrix, plan: ExpertsPlan, weights=None, 
     for buffer, what in ((packed.buffer, "packed"), (plan.buffer, "plan")):
         if buffer.get_device() != index:
             raise ValueError(f"a is on {t.device}, {what} on {buffer.device}")
+    if _tracked(torch, t, weights):
+        return _without_gradient("mx_dots_experts", out, lambda: mx_dots_experts(a, packed, plan, weights, None, out_dtype), t, weights)
     if index != _device():
         with torch.cuda.device(index):
             return mx_dots_experts(a, packed, plan, weights, out, out_dtype)

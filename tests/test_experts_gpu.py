@@ -253,6 +253,61 @@ def test_more_tokens_than_one_launch_takes():
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("short_way", [True, False])
+@pytest.mark.parametrize("score,biased,groups,renormalize,dtype", [("softmax", False, 1, True, torch.float32), ("sigmoid", True, 4, True, torch.bfloat16),
+                                                                   ("sigmoid", False, 1, False, torch.float16), ("softmax", True, 2, False, torch.float32)])
+def test_autograd_follows_the_weights(monkeypatch, score, biased, groups, renormalize, dtype, short_way):
+    """Weights that a loss is made of hand their gradient on to whatever made the logits, by experts_route_backward."""
+    from numkong_amd import mx as binding
+
+    if not short_way:
+        monkeypatch.setattr(binding, "_CALLS", None)
+    source, grad = logits_of(30, 24, torch.float32, 1).to(DEV).requires_grad_(), normal(30, 3, torch.float32, 2, 0.0).to(DEV)
+    bias = torch.rand(24, device=DEV).requires_grad_() if biased else None
+    kind = dict(bias=bias, groups=groups, top_groups=max(1, groups // 2), group_top=2 if groups > 1 else 1)
+    logits = (2 * source).to(dtype)
+    weights, chosen = nk.experts_route(logits, 3, score, renormalize=renormalize, scale=1.5, **kind)
+    with torch.no_grad():
+        plain, plain_chosen = nk.experts_route(logits, 3, score, renormalize=renormalize, scale=1.5, **kind)
+    assert weights.requires_grad and not chosen.requires_grad and not plain.requires_grad
+    assert torch.equal(weights, plain) and torch.equal(chosen, plain_chosen)
+    (weights * grad).sum().backward()
+    want = nk.experts_route_backward(grad, logits.detach(), chosen, score, renormalize, 1.5)
+    assert torch.equal(source.grad, 2 * want.float()) and (not biased or bias.grad is None)
+    again = nk.experts_route(logits.detach().requires_grad_(), 3, score)[0].sum()  # (its gradient is one number for all)
+    again.backward()
+    host = logits.detach().cpu().requires_grad_()
+    (nk.experts_route(host, 3, score, renormalize=renormalize, scale=1.5, **{**kind, "bias": bias.detach().cpu() if biased else None})[0] * grad.cpu()).sum().backward()
+    assert torch.equal(host.grad, want.cpu())
+    leaf = logits.detach().requires_grad_()
+    first, = torch.autograd.grad(nk.experts_route(leaf, 3, score)[0].square().sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        first.sum().backward()
+
+
+@pytest.mark.parametrize("short_way", [True, False])
+def test_products_say_that_they_have_no_gradient(monkeypatch, short_way):
+    from numkong_amd import mx as binding
+
+    if not short_way:
+        monkeypatch.setattr(binding, "_CALLS", None)
+    a, packed, stack = normal(6, 64, torch.float32, 1).to(DEV), nk.mx_pack(torch.ones((8, 64), device=DEV)), nk.mx_pack(torch.ones((4, 8, 64), device=DEV))
+    plan, weights = nk.experts_plan(torch.zeros((6, 2), dtype=torch.int32, device=DEV), 4), torch.rand((6, 2), device=DEV)
+    leaf, weight = a.clone().requires_grad_(), weights.clone().requires_grad_()
+    for name, tracked, plain in (("mx_dots_packed", lambda **o: nk.mx_dots_packed(leaf, packed, **o), lambda: nk.mx_dots_packed(a, packed)),
+                                 ("mx_dots_experts", lambda **o: nk.mx_dots_experts(leaf, stack, plan, **o), lambda: nk.mx_dots_experts(a, stack, plan)),
+                                 ("mx_dots_experts", lambda **o: nk.mx_dots_experts(a, stack, plan, weight, **o), lambda: nk.mx_dots_experts(a, stack, plan, weights))):
+        want, got = plain(), tracked()
+        assert torch.equal(got, want) and got.requires_grad and not want.requires_grad
+        with pytest.raises(nk.NumKongAmdError, match=name + " has no gradient"):
+            got.sum().backward()
+        with pytest.raises(nk.NumKongAmdError, match="out="):
+            tracked(out=torch.empty_like(want))
+        with torch.no_grad():
+            assert not tracked().requires_grad and torch.equal(tracked(out=torch.empty_like(want)), want)
+    assert leaf.grad is None and weight.grad is None
+
+
 # ---- the plan and the products ---------------------------------------------------------------------------------------
 
 def routing(tokens, top_k, experts, kind, seed=0):
