@@ -205,9 +205,9 @@ bool route_of(PyObject *const *arguments, bool groups, nk_amd_route_t &how) {
     if (!natural(arguments[0], sigmoid) || !PyBool_Check(arguments[1]) || !PyFloat_CheckExact(arguments[2])) return false;
     for (int i = 0; groups && i < 3; ++i)
         if (!natural(arguments[3 + i], numbers[i]) || numbers[i] > 1024) return false;
-    double const scale = PyFloat_AS_DOUBLE(arguments[2]);
+    float const scale = (float)PyFloat_AS_DOUBLE(arguments[2]);
     if (!std::isfinite(scale)) return false;
-    how = {(int)sigmoid, arguments[1] == Py_True, (float)scale, (int)numbers[0], (int)numbers[1], (int)numbers[2]};
+    how = {(int)sigmoid, arguments[1] == Py_True, scale, (int)numbers[0], (int)numbers[1], (int)numbers[2]};
     return true;
 }
 

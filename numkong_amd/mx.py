@@ -450,8 +450,10 @@ _SCORES = {"softmax": 0, "sigmoid": 1}
 def _route_kind(score, renormalize, scale, groups=1, top_groups=1, group_top=1):
     if score not in _SCORES:
         raise ValueError(f"score must be one of {sorted(_SCORES)}, got {score!r}")
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    if not math.isfinite(ctypes.c_float(scale).value):
+        raise ValueError("scale must be a finite 32-bit number")
+    if any(not -(1 << 31) <= number < 1 << 31 for number in (groups, top_groups, group_top)):  # (ctypes would keep their low bits)
+        raise ValueError("groups, top_groups and group_top must be 32-bit numbers")
     return _Route(_SCORES[score], int(bool(renormalize)), scale, groups, top_groups, group_top)
 
 
@@ -548,7 +550,7 @@ def experts_plan(chosen, experts: int) -> ExpertsPlan:
     if chosen.dim() != 2 or chosen.dtype != torch.int32:
         raise ValueError("chosen must be a tokens x top_k matrix of int32")
     tokens, top_k = chosen.shape
-    size = lib.nk_amd_experts_plan_size(tokens * top_k, experts) if experts > 0 else 0
+    size = lib.nk_amd_experts_plan_size(tokens * top_k, experts) if 0 < experts < 1 << 32 else 0
     if size == 0:
         raise ValueError("a plan is for 1 to 1024 experts and fewer than 2^30 slots")
     if not chosen.is_cuda:

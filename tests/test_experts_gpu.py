@@ -169,6 +169,23 @@ def test_many_tokens_choose_as_few(experts, groups, top_groups):
         torch.testing.assert_close(many, weights.repeat(160, 1), rtol=2.0**-21, atol=0.0, equal_nan=True)
 
 
+@pytest.mark.parametrize("short_way", [True, False])
+def test_what_routing_refuses(monkeypatch, short_way):
+    """By both ways."""
+    from numkong_amd import mx as binding
+
+    if not short_way:
+        monkeypatch.setattr(binding, "_CALLS", None)
+    logits = torch.zeros((1000, 64), device=DEV)
+    for scale in (1e39, -float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="finite"):
+            nk.experts_route(logits, 2, scale=scale)
+    with pytest.raises(ValueError, match="32-bit"):
+        nk.experts_route(logits, 2, groups=(1 << 32) + 1)
+    with pytest.raises(nk.NumKongAmdError, match="groups"):
+        nk.experts_route(logits, 2, groups=-1)
+
+
 def test_nan_and_infinity_show():
     logits = logits_of(3, 16, torch.float32, 2)
     logits[0, 5], logits[1, 6] = float("nan"), float("inf")

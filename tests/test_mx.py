@@ -236,6 +236,20 @@ def test_wrong_shapes_and_values(call):
         call()
 
 
+@pytest.mark.parametrize("call", [
+    lambda: nk.experts_route(torch.zeros((4, 64)), 2, scale=1e39),
+    lambda: nk.experts_route(torch.zeros((4, 64)), 2, groups=(1 << 32) + 1),
+    lambda: nk.experts_route(torch.zeros((4, 64)), 2, groups=4, top_groups=(1 << 32) + 1),
+    lambda: nk.experts_route(torch.zeros((4, 64)), 2, group_top=-(1 << 32) + 1),
+    lambda: nk.experts_route_backward(torch.zeros((4, 2)), torch.zeros((4, 64)), torch.zeros((4, 2), dtype=torch.int32), scale=-1e39),
+    lambda: nk.experts_plan(torch.zeros((4, 2), dtype=torch.int32), (1 << 64) + 8),
+])
+def test_numbers_that_the_library_cannot_hold(call):
+    """Refused, and not taken for what is left of them in 32 or 64 bits."""
+    with pytest.raises(ValueError):
+        call()
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="there is a GPU")
 @pytest.mark.parametrize("call", [
     lambda: nk.mx_quantize(torch.zeros((4, 64))), lambda: nk.mx_quantize(np.zeros((4, 64), np.float32)), lambda: nk.mx_dequantize(codes()),
