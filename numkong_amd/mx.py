@@ -492,6 +492,8 @@ def experts_route(logits, top_k: int, score: str = "softmax", bias=None, groups:
     if index != _device():
         with torch.cuda.device(index):
             return experts_route(t, top_k, score, bias, groups, top_groups, group_top, renormalize, scale)
+    # (no token: the library looks at the rest before room is made for results that are refused)
+    _check(lib.nk_amd_experts_route_async(dtype_codes[t.dtype], None, 0, 0, experts, top_k, None, how, None, None, None), "experts_route")
     device = t.device
     weights, chosen = _new(torch, tokens, top_k, torch.float32, device), _new(torch, tokens, top_k, torch.int32, device)
     _check(lib.nk_amd_experts_route_async(dtype_codes[t.dtype], t.data_ptr(), _row_bytes(t), tokens, experts, top_k,

@@ -171,12 +171,15 @@ def test_many_tokens_choose_as_few(experts, groups, top_groups):
 
 @pytest.mark.parametrize("short_way", [True, False])
 def test_what_routing_refuses(monkeypatch, short_way):
-    """By both ways."""
+    """Before room is made for it, and by both ways."""
     from numkong_amd import mx as binding
 
     if not short_way:
         monkeypatch.setattr(binding, "_CALLS", None)
     logits = torch.zeros((1000, 64), device=DEV)
+    for top_k in (0, 65, 1 << 40, -1):
+        with pytest.raises(nk.NumKongAmdError, match="1 to 1024 experts"):
+            nk.experts_route(logits, top_k)
     for scale in (1e39, -float("inf"), float("nan")):
         with pytest.raises(ValueError, match="finite"):
             nk.experts_route(logits, 2, scale=scale)
