@@ -370,7 +370,8 @@ def mx_pack(b) -> MxPackedMatrix:
     if not isinstance(b, MxMatrix):
         b = _tensor(b, "b")
         b = _floats(b, "b", 3 if b.dim() == 3 else 2)
-        flat = mx_quantize((b if b.is_cuda else _to_gpu(b)).reshape(-1, b.shape[-1]) if b.dim() == 3 else b if b.is_cuda else _to_gpu(b))
+        rows = b if b.is_cuda else _to_gpu(b)
+        flat = mx_quantize(rows.flatten(0, 1) if b.dim() == 3 else rows)
         b = MxMatrix(flat.codes.reshape(*b.shape[:-1], flat.codes.shape[-1]), flat.scales.reshape(*b.shape[:-1], flat.scales.shape[-1]), b.shape[-1])
     b = _matrix_of(b, "b")
     if not b.codes.is_cuda:

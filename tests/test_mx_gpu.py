@@ -216,6 +216,18 @@ def test_no_depth_and_no_rows():
         assert got.shape == (m, n) and not got.any()
 
 
+@pytest.mark.parametrize("shape", [(3, 4, 0), (0, 4, 64), (3, 0, 64), (0, 0, 0)])
+def test_stacks_of_nothing(shape):
+    packed = nk.mx_pack(torch.ones(shape, device=DEV))
+    assert (packed.count, packed.width, packed.depth) == shape
+    if shape[0]:
+        plan = nk.experts_plan(torch.zeros((5, 2), dtype=torch.int32, device=DEV), shape[0])
+        got = nk.mx_dots_experts(torch.ones((5, shape[2]), device=DEV), packed, plan)
+        assert got.shape == (5, 2, shape[1]) and not got.any()
+        got = nk.mx_dots_experts(torch.ones((5, shape[2]), device=DEV), packed, plan, torch.ones((5, 2), device=DEV))
+        assert got.shape == (5, shape[1]) and not got.any()
+
+
 def test_image_of_other_sizes_gives_nans():
     lib = nk.library()
     packed = nk.mx_pack(torch.ones((64, 256), device=DEV))
