@@ -16,8 +16,8 @@
  *  Every call queues its work on `stream` (a hipStream_t, NULL = the default stream), touches device memory only, neither
  *  allocates nor synchronises, may be captured into a HIP graph (after one eager call, which loads the kernels), and returns 0
  *  or a status that `nk_hip_last_error()` explains. Strides are in bytes; results share memory neither with one another's rows nor
- *  with operands. Sums are held in 32 bits; no result depends on the
- *  order in which workgroups run.
+ *  with operands. Sums are held in 32 bits (of products below 2^-149 nothing may be left); no result depends on the order in which
+ *  workgroups run.
  */
 #ifndef NUMKONG_AMD_MX_H
 #define NUMKONG_AMD_MX_H

@@ -527,6 +527,25 @@ def test_images_and_plans_are_as_large_as_their_sizes_say(monkeypatch, short_way
         assert bool((got == (64 if weights is None else 128)).all())
 
 
+@pytest.mark.parametrize("tokens,experts", [(3, 8), (200, 8), (900, 4)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_no_depth_and_other_images(tokens, experts, dtype):
+    """Few rows to an expert, some, many; some without an expert, the sums by weight as well."""
+    chosen = torch.from_numpy(routing(tokens, 2, experts, "some", 1)).to(DEV)
+    there = (chosen >= 0) & (chosen < experts)
+    plan, weights = nk.experts_plan(chosen, experts), torch.ones((tokens, 2), device=DEV)
+    empty = nk.mx_pack(torch.ones((experts, 300, 0), device=DEV))
+    other = nk.MxPackedMatrix(experts, 300, 60, nk.mx_pack(torch.ones((experts, 300, 64), device=DEV)).buffer)
+    for k, packed in ((0, empty), (60, other)):
+        a = torch.ones((tokens, k), device=DEV)
+        rows = nk.mx_dots_experts(a, packed, plan, out_dtype=dtype)
+        sums = nk.mx_dots_experts(a, packed, plan, weights, out_dtype=dtype)
+        if k:
+            assert bool(rows[there].isnan().all()) and bool(sums[there.any(1)].isnan().all()) and not sums[~there.any(1)].any()
+        else:
+            assert rows.shape == (tokens, 2, 300) and not rows.any() and not sums.any()
+
+
 def test_no_tokens():
     packed = nk.mx_pack(torch.ones((4, 64, 64), device=DEV))
     plan = nk.experts_plan(torch.zeros((0, 2), dtype=torch.int32, device=DEV), 4)

@@ -106,6 +106,26 @@ def test_dequantize_rows_of_any_kind(depth, pad):
     np.testing.assert_array_equal(out.cpu().numpy(), mx.values(codes, scales).astype(np.float32))
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows,depth,pad", [(8192, 4096, 0), (8300, 4093, 3), (8300, 4090, 22)])
+def test_dequantize_past_the_caches(dtype, rows, depth, pad):
+    """64 MiB and more at addresses of 16 bytes: rows in one piece, cut, and apart; nothing beside them written."""
+    generator = torch.Generator(device=DEV).manual_seed(depth)
+    codes = torch.randint(0, 256, (rows, depth // 2 + depth % 2), dtype=torch.uint8, device=DEV, generator=generator)
+    scales = torch.randint(115, 135, (rows, (depth + 31) // 32), dtype=torch.uint8, device=DEV, generator=generator)
+    scales[77, 5] = 255
+    store = torch.full((rows, depth + pad), 77.0, dtype=dtype, device=DEV)
+    out = store[:, :depth]
+    assert out.data_ptr() % 16 == 0 and out.stride(0) * out.itemsize % 16 == 0 and rows * depth * out.itemsize >= 64 << 20
+    nk.mx_dequantize(nk.MxMatrix(codes, scales, depth), dtype, out)
+    one_each = torch.stack([codes & 15, codes >> 4], -1).flatten(1)[:, :depth]
+    powers = torch.exp2(scales.double() - 127).masked_fill(scales == 255, float("nan"))
+    want = (torch.tensor(mx.GRID, device=DEV)[one_each.long()] * powers.repeat_interleave(32, 1)[:, :depth]).to(dtype)
+    torch.testing.assert_close(out, want, rtol=0.0, atol=0.0, equal_nan=True)
+    out.fill_(77.0)
+    assert bool((store == 77.0).all())
+
+
 def product_of(a, b):
     left, right = mx.rounded(a), mx.rounded(b)
     return left @ right.T, np.abs(left) @ np.abs(right).T
@@ -208,6 +228,43 @@ def test_scales_of_every_size():
         with np.errstate(over="ignore"):
             want = float(np.float32(32 * 2.0 ** (left + right - 254)))
         assert got == want, (left, right)
+
+
+@pytest.mark.parametrize("m,n", [(8, 40), (30, 700), (64, 700), (1100, 2100)])
+def test_scales_of_every_pair(m, n):
+    """The same of all pairs of some scales, in each kernel's instruction; the blocks of a row differ, and one is left of each sum:
+    32 equal products, whose sums in 32 bits are exact in any order unless a product is below the smallest number, 2^-149; then
+    each of 32 additions may be off by half of that."""
+    some = np.array([0, 1, 2, 60, 67, 100, 126, 127, 128, 180, 200, 252, 253, 254], dtype=np.int64)
+    left, right = some[np.arange(m) * 5 % len(some)], some[np.arange(n) * 3 % len(some)]
+    codes, scales = np.zeros((m, 640), dtype=np.uint8), np.full((m, 20), 127, dtype=np.uint8)
+    block = np.arange(m) * 7 % 20
+    for row in range(m):
+        codes[row, 32 * block[row]:32 * block[row] + 32] = 2  # ones
+        scales[row, block[row]] = left[row]
+    b_codes, b_scales = np.full((n, 640), 2, dtype=np.uint8), np.repeat(right.astype(np.uint8)[:, None], 20, 1)
+    make = lambda c, e: nk.MxMatrix(torch.from_numpy(mx.packed(c)).to(DEV), torch.from_numpy(e).to(DEV), 640)  # noqa: E731
+    got = nk.mx_dots_packed(make(codes, scales), nk.mx_pack(make(b_codes, b_scales))).cpu().numpy()
+    power = (left[:, None] + right[None, :] - 254).astype(np.float64)
+    with np.errstate(over="ignore"):
+        want = (32 * 2.0 ** power).astype(np.float32)
+    held = power >= -149
+    np.testing.assert_array_equal(got[held], want[held])
+    assert (np.abs(got.astype(np.float64) - 32 * 2.0 ** power)[~held] <= 32 * 2.0**-150).all()
+
+
+@pytest.mark.parametrize("out", FLOATS)
+@pytest.mark.parametrize("m,n", [(40, 700), (1100, 2100), (2100, 8200)])
+def test_no_depth_and_other_images_of_many_rows(m, n, out):
+    """Zeros where there is nothing to add up, NaNs where the image is one of something else, and nothing beside them."""
+    for k, packed, right in ((0, nk.mx_pack(torch.ones((n, 0), device=DEV)), 0.0),
+                             (200, nk.MxPackedMatrix(1, n, 200, nk.mx_pack(torch.ones((n, 256), device=DEV)).buffer), float("nan"))):
+        store = torch.full((m + 2, n + 9), 77.0, dtype=out, device=DEV)
+        view = store[1:-1, 3:3 + n]
+        nk.mx_dots_packed(torch.ones((m, k), device=DEV), packed, out=view)
+        assert torch.equal(view.isnan(), torch.full_like(view, right).isnan()) and not view.nan_to_num(0.0).any()
+        view.fill_(77.0)
+        assert bool((store == 77.0).all())
 
 
 def test_no_depth_and_no_rows():
