@@ -874,10 +874,12 @@ int launch_gemm(MxArgs &p, hipStream_t stream) {
 template <class Out, bool GROUPED>
 int launch_product(MxArgs &p, bool few, uint32_t tile_rows, int a_dtype, bool fused, uint32_t fused_rows, MxGeometry const &g, hipStream_t stream) {
     auto const tiles_of = [&](uint64_t rows, uint64_t columns) { return (p.m + rows - 1) / rows * ((p.n + columns - 1) / columns); };
-    uint64_t const large = tiles_of(256, 256), rounds = (large + 255) / 256;
-    bool const whole_rounds = large * 20 >= rounds * 256 * 19;
+    auto const whole_rounds = [&] { // (within a twentieth)
+        uint64_t const large = tiles_of(256, 256), units = (uint64_t)compute_unit_count();
+        return units && large * 20 >= (large + units - 1) / units * units * 19;
+    };
     bool const small = p.m <= 32 || tiles_of(128, 256) < 64;
-    uint32_t const rows = GROUPED ? (few ? tile_rows : 128) : few && small ? (p.m < 64 ? p.m : 64) : g.steps > 48 && whole_rounds ? 256 : 128;
+    uint32_t const rows = GROUPED ? (few ? tile_rows : 128) : few && small ? (p.m < 64 ? p.m : 64) : g.steps > 48 && whole_rounds() ? 256 : 128;
     if (rows <= 16) {
         constexpr int NT = GROUPED ? 2 : 1; // (experts of 4 tokens, 28 matrices of 2048 x 2048: 13.0 us with two, 14.0 with one)
         if (!fused) return launch_few<1, NT, uint8_t, Out, GROUPED>(p, rows, g, stream);
