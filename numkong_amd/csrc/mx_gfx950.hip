@@ -879,7 +879,7 @@ int launch_product(MxArgs &p, bool few, uint32_t tile_rows, int a_dtype, bool fu
         return units && large * 20 >= (large + units - 1) / units * units * 19;
     };
     bool const small = p.m <= 32 || tiles_of(128, 256) < 64;
-    uint32_t const rows = GROUPED ? (few ? tile_rows : 128) : few && small ? (p.m < 64 ? p.m : 64) : g.steps > 48 && whole_rounds() ? 256 : 128;
+    uint32_t const rows = GROUPED ? (few ? tile_rows : 128) : few && small ? (p.m < 64 ? p.m : 64) : g.steps > 48 && g.steps < kMxMaxDepth / 128 && whole_rounds() ? 256 : 128;
     if (rows <= 16) {
         constexpr int NT = GROUPED ? 2 : 1; // (experts of 4 tokens, 28 matrices of 2048 x 2048: 13.0 us with two, 14.0 with one)
         if (!fused) return launch_few<1, NT, uint8_t, Out, GROUPED>(p, rows, g, stream);

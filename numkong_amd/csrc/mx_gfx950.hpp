@@ -56,7 +56,8 @@ struct MxHeader {
     uint32_t magic, version, count, n, k, reserved[3];
 };
 
-/** Depths of products: below 2^25, so that eight tiles of the image, and 256 rows of A, lie within 32-bit offsets. */
+/** Depths of products: below 2^25, so that eight tiles of the image, and 128 rows of A, lie within 32-bit offsets; 256 rows but at the last
+ *  128 depths, where their last bytes are the 2^32nd, which a buffer does not reach (buffer_of). */
 constexpr uint64_t kMxMaxDepth = 1ull << 25;
 
 struct MxGeometry {
