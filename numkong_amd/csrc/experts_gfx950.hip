@@ -197,7 +197,7 @@ struct RouteArgs {
  *  lowest is the lowest expert. A choice is a maximum over each lane's keys and over the lanes; the lane that holds it takes it
  *  out and notes it. What bounds this is the number of instructions, which 16 lanes to a token share among four of them, and for few
  *  tokens the time that they take one after the other (with_row). 16,384 tokens of 256 experts, sigmoid and bias, 4 of 8 groups,
- *  8 chosen: 14 us, at 3 us for the traffic; 8192 tokens of 128 experts, 8 chosen: 5.7 us. Groups of whole lanes are found in
+ *  8 chosen: 14.6 us, at 3 us for the traffic; 8192 tokens of 128 experts, 8 chosen: 5.5 us. Groups of whole lanes are found in
  *  registers, others through LDS (the same 16,384 tokens through LDS, a lane for four groups: 23.6 us).
  */
 template <class T, int L, int J>
@@ -327,7 +327,8 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
 /**
  *  With s the scores, S the chosen, D = sum_S s + 1e-20:  ds_j = scale (g_j - sum_S g s / D) / D where weights are
  *  renormalised, scale g_j where not, 0 outside S; then dl_j = ds_j s_j (1 - s_j) for sigmoid scores, and
- *  dl_i = s_i (ds_i - sum_S ds s) for softmax.
+ *  dl_i = s_i (ds_i - sum_S ds s) for softmax. Not its bytes bound it (8192 tokens of 128 experts in bf16: 5.7 us for 4.2 MB) but one
+ *  token's work after the other: two wavefronts to a SIMD, 711 vector instructions in each, 57 % of whose time is waiting for loads and LDS.
  */
 template <class T, int L, int J>
 __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs p, float const *grad, T *out, uint64_t out_stride) {
@@ -457,7 +458,8 @@ __global__ __launch_bounds__(kScanBuckets * kScanParts) void plan_scan_kernel(ui
  *  `table`; NULL where there is one workgroup), and goes over them again in order, so that no atomic decides an order. `scanned`:
  *  the table holds sums (plan_scan_kernel), not counts. The first workgroup also writes the header and the slots of rows that
  *  stand between experts; the tiles are written by all in turn, as one expert may have most of them. Its time is that of a few loads
- *  and LDS round trips one after the other: 32 slots 3.4 us, 1,024 5.3, 4,004 with the launch that counts 8.5, 32,768 9.4.
+ *  and LDS round trips one after the other: 32 slots 3.6 us, 1,024 5.5, 4,004 6.1 and the launch that counts 2.0, 32,768 7.3 and 2.6,
+ *  2^20 11.1, 3.7 and the sums 6.5 (back to back 8.4, 9.6 and 20).
  */
 template <int BATCH, bool SCANNED>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(int32_t const *chosen, uint32_t slots, uint32_t experts, PlanHeader header,

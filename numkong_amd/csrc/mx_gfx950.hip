@@ -18,7 +18,7 @@ constexpr uint32_t kStretches = sizeof(T) == 4 ? 1 : 2;
 /**
  *  16 bytes of x a load, side by side over the wavefront, past the caches (x is read once); codes leave a word a lane. A lane's
  *  load of f32 is half a word of codes, so the two halves of a stretch are exchanged between neighbours. What bounds it is
- *  memory: 8192 x 8192 of f32, 268 MB in and 36 MB out, take 51 us. (Eight values a lane, loads of 32 bytes apart: 52 us in a
+ *  memory: 8192 x 8192 of f32, 268 MB in and 36 MB out, take 49 us. (Eight values a lane, loads of 32 bytes apart: 52 us in a
  *  kernel that does no more; such halves, through the caches: 52 us; past them: 47 us.)
  */
 template <class T>
@@ -237,7 +237,8 @@ __global__ __launch_bounds__(256) void dequantize_kernel(uint8_t const *codes, u
 // ---- packing ------------------------------------------------------------------------------------------------------
 
 /** One thread for 16 bytes of a tile's codes or for a word of its scales; the header by the first workgroup. Memory bounds it
- *  (8192 x 8192: 15.5 us, 4.6 TB/s read and written), and it runs once for a matrix. */
+ *  (8192 x 8192: 14.8 us, 4.8 TB/s read and written; 32 matrices of 2050 x 1000, whose rows end inside a block that is fetched by
+ *  bytes: 17.4 us, 4.1 TB/s), and it runs once for a matrix. */
 __global__ __launch_bounds__(256) void mx_pack_kernel(uint8_t const *codes, uint64_t codes_stride, uint64_t codes_matrix,
                                                       uint8_t const *scales, uint64_t scales_stride, uint64_t scales_matrix,
                                                       MxHeader header, uint32_t supers, uint32_t tiles, uint64_t first,
@@ -323,10 +324,11 @@ __device__ __forceinline__ bool image_matches(MxArgs const &p) {
  *  60, 2,048 64), high ones read less of B (us, bands of 1, 2, 4 and 8: tiles of 128 rows, bf16 8192 x 8192 x 1024 68, 57, 63, 60, x 4096
  *  190, 150, 145, 147, f32 8192 x 6656 x 2048 103, 88, 91, 92; tiles of 256, 8192^3 bf16 270, 262, 262, 274, f32 284, 275, 295, 300).
  *
- *  8192^3 with bf16 results takes 241 to 257 us (4.3 to 4.6 PFLOP/s; the matrix instructions alone, on the same random codes, 6.5):
+ *  8192^3 with bf16 results takes 260 to 265 us (4.2 PFLOP/s; on other days from 246; the matrix instructions alone, on such codes, 6.5):
  *  power holds the clock at 1.6 GHz, a step takes 1226 cycles of which 1024 are matrix instructions, a tile's end a tenth of its
- *  time. Shallow products of f32 results are bound by their stores (8192 x 8191 x 1000: 73 us for 268 MB), experts by both (64 of
- *  512 rows on average, 2048 x 2048: 95 to 104 us for 313 MB).
+ *  time. (Among the others are moves of scalar registers, of which the bases of two tiles and the choices between them take more than
+ *  there are: the compiler keeps 55 to 98 of them in lanes of vector registers.) Shallow products of f32 results are bound by their stores
+ *  (8192 x 8191 x 1000: 74 to 79 us for 268 MB), experts by both (64 of 512 rows on average, 2048 x 2048: 99 to 107 us for 313 MB).
  */
 template <int FM, class Out, bool GROUPED>
 __global__ __launch_bounds__(256, FM >= 8 ? 1 : 2) void mx_gemm_kernel(MxArgs p) {
@@ -565,9 +567,10 @@ __global__ __launch_bounds__(256, FM >= 8 ? 1 : 2) void mx_gemm_kernel(MxArgs p)
 /**
  *  The product for few rows: the stream of B is the work, so a workgroup takes 16 NT columns and its wavefronts the supers of
  *  the depth in turn, B straight into registers, and their sums meet in LDS. In: the type of A's values, which the workgroup
- *  quantises into LDS itself (one launch, and A is read by all lanes), or `uint8_t`: A is staged already. B's first loads are
- *  on their way while A is quantised. 1 x 8192 against 8192 columns: 7.4 us, 4.8 TB/s of the image; 64 rows 11.2 us; 32 slots of 29
- *  experts, 2048 x 2048: 12.2 us, 5.3 TB/s.
+ *  quantises into LDS itself (one launch, and A is read by all lanes), or `uint8_t`: A is staged already, and goes into registers.
+ *  B's first loads are on their way while A is quantised. 1 x 8192 against 8192 columns: 8.8 us, 4.1 TB/s of the image; 64 rows 12.1 us,
+ *  as each of 256 workgroups reads all of A (278 KB, 71 MB out of the L2s beside 36 MB of image: 107 MB of requests were counted); 32 slots of 29
+ *  experts, 2048 x 2048: 14.3 us, 4.5 TB/s.
  */
 template <int WAVES, int FM, int NT, class In, class Out, bool GROUPED>
 __global__ __launch_bounds__(64 * WAVES, FM >= 4 ? 2 : 4) void mx_few_kernel(MxArgs p) {
@@ -704,7 +707,7 @@ __global__ __launch_bounds__(64 * WAVES, FM >= 4 ? 2 : 4) void mx_few_kernel(MxA
 }
 
 /** out[token] = sum over its slots of weight * row of the plan, slots without an expert left out; a thread for four columns, four
- *  rows under way at a time. Memory bounds it (1001 tokens, 4 of 2050 columns: 7.3 us, 5.6 TB/s). */
+ *  rows under way at a time. Memory bounds it (1001 tokens, 4 of 2050 columns: 8.0 us, 5.1 TB/s). */
 template <class Out>
 __global__ __launch_bounds__(256) void combine_kernel(float const *rows, uint64_t row_values, uint32_t const *plan, uint32_t slots,
                                                       uint32_t experts, uint32_t place, float const *weights, uint32_t top_k,
