@@ -100,58 +100,6 @@ def test_masked_logits(score, experts, groups, top_groups):
     assert bool(grad.isfinite().all()) and not grad[0].any() and not grad[logits.isneginf().to(DEV)].any()
 
 
-def choice_of_two(selection, groups, top_groups):
-    """64-bit selection scores where groups are picked by the sum of their best two; of one that can be chosen, by that one."""
-    inside = selection.reshape(len(selection), groups, -1)
-    best = np.sort(inside, 2)[:, :, ::-1]
-    low = float(torch.finfo(torch.float32).min)
-    second = np.where(np.isneginf(best[:, :, 1]), 0.0, best[:, :, 1])
-    of_group = np.where(np.isneginf(best[:, :, 0]), -np.inf, np.maximum(best[:, :, 0] + second, low))
-    order = np.argsort(-of_group, axis=1, kind="stable")
-    keep = np.zeros_like(of_group, dtype=bool)
-    np.put_along_axis(keep, order[:, :top_groups], True, 1)
-    return np.where(keep[:, :, None], inside, -np.inf).reshape(selection.shape)
-
-
-@pytest.mark.parametrize("tokens", [40, 4200])  # a wavefront for a token, and 16 lanes
-@pytest.mark.parametrize("experts,groups,top_groups", [(64, 8, 4), (64, 8, 1), (30, 5, 2), (100, 5, 2), (144, 9, 3), (256, 8, 3), (512, 64, 20), (1000, 50, 7)])
-def test_masked_experts_in_groups(tokens, experts, groups, top_groups):
-    """Whatever is masked, the groups that stay are those that have something to choose, by two best of it. Logits are whole
-    numbers, scores with a bias ones and quarters: sums of two are exact, and ties go to the lowest."""
-    generator = torch.Generator().manual_seed(experts + groups)
-    logits = torch.randint(-20, 21, (tokens, experts), generator=generator).float()
-    masked = torch.rand((tokens, experts), generator=generator) < torch.rand((tokens, 1), generator=generator) ** 0.2
-    logits[masked] = -float("inf")
-    size = experts // groups
-    logits[0], logits[0, -4] = -float("inf"), 3.0  # a single expert, in the last group
-    logits[1], logits[1, -size:] = -float("inf"), torch.finfo(torch.float32).min  # lowest numbers are numbers, their sum as well
-    logits[2], logits[2, -1], logits[2, 0] = -float("inf"), -20.0, -19.0
-    logits[3] = -float("inf")
-    logits[4], logits[4, -2] = -float("inf"), float("inf")
-    logits[4, -size - 1] = 5.0
-    bias = torch.randint(-3, 4, (experts,), generator=generator) / 4
-    for score, of in (("softmax", None), ("sigmoid", bias)):
-        x = logits if of is None else torch.where(logits.isneginf(), logits, 60.0)
-        selection = x.double().numpy() if of is None else np.where(np.isneginf(x.numpy()), -np.inf, 1.0 + bias.double().numpy())
-        selection = choice_of_two(selection, groups, top_groups)
-        order = np.argsort(-selection, axis=1, kind="stable")[:, :4]
-        there = ~np.isneginf(np.take_along_axis(selection, order, 1))
-        weights, chosen = nk.experts_route(x.to(DEV), 4, score, None if of is None else of.to(DEV), groups, top_groups, 2)
-        np.testing.assert_array_equal(chosen.cpu().numpy(), np.where(there, order, -1))
-        assert (weights.cpu().numpy()[~there] == 0).all()
-        assert chosen[0].tolist() == [experts - 4, -1, -1, -1] and int(chosen[1, 0]) >= experts - size and int(chosen[4, 0]) >= 0
-
-
-def test_groups_by_scores():
-    """Groups by the sum of two scores, not of two logits, are what a bias of zeros gives."""
-    logits = torch.tensor([[6.0, -6.0, 0.1, 0.1], [0.0, 9.0, 4.0, 4.5], [-3.0, 2.0, 0.0, 0.0]])
-    s = torch.sigmoid(logits.double()).reshape(3, 2, 2).sum(2)
-    _, chosen = nk.experts_route(logits.to(DEV), 2, "sigmoid", torch.zeros(4, device=DEV), 2, 1, 2)
-    assert torch.equal(chosen.cpu() // 2, s.argmax(1, keepdim=True).expand(3, 2))
-    _, chosen = nk.experts_route(logits.to(DEV), 2, "sigmoid", None, 2, 1, 2)
-    assert torch.equal(chosen.cpu() // 2, logits.reshape(3, 2, 2).sum(2).argmax(1, keepdim=True).expand(3, 2))
-
-
 @pytest.mark.parametrize("experts,groups,top_groups", [(100, 1, 1), (100, 5, 2), (144, 1, 1), (144, 9, 3), (256, 8, 3)])
 def test_many_tokens_choose_as_few(experts, groups, top_groups):
     """Masks, ties, NaNs and infinities among as many tokens as share wavefronts: chosen as where a token has its own. (Sigmoid
@@ -167,26 +115,6 @@ def test_many_tokens_choose_as_few(experts, groups, top_groups):
         many, many_chosen = nk.experts_route(logits.repeat(160, 1), 4, "sigmoid", of, groups, top_groups, 2)
         assert torch.equal(many_chosen, chosen.repeat(160, 1))
         torch.testing.assert_close(many, weights.repeat(160, 1), rtol=2.0**-21, atol=0.0, equal_nan=True)
-
-
-@pytest.mark.parametrize("short_way", [True, False])
-def test_what_routing_refuses(monkeypatch, short_way):
-    """Before room is made for it, and by both ways."""
-    from numkong_amd import mx as binding
-
-    if not short_way:
-        monkeypatch.setattr(binding, "_CALLS", None)
-    logits = torch.zeros((1000, 64), device=DEV)
-    for top_k in (0, 65, 1 << 40, -1):
-        with pytest.raises(nk.NumKongAmdError, match="1 to 1024 experts"):
-            nk.experts_route(logits, top_k)
-    for scale in (1e39, -float("inf"), float("nan")):
-        with pytest.raises(ValueError, match="finite"):
-            nk.experts_route(logits, 2, scale=scale)
-    with pytest.raises(ValueError, match="32-bit"):
-        nk.experts_route(logits, 2, groups=(1 << 32) + 1)
-    with pytest.raises(nk.NumKongAmdError, match="groups"):
-        nk.experts_route(logits, 2, groups=-1)
 
 
 def test_nan_and_infinity_show():
@@ -254,80 +182,6 @@ def test_route_gradient_by_differences(score, renormalize):
     assert (np.abs(got - want) <= allowed).all()
 
 
-def test_more_tokens_than_one_launch_takes():
-    """2^26 rows of logits, a wavefront each: the choices and the gradients of those at the ends of the launches and between are
-    those of the same rows alone, bit for bit."""
-    tokens, experts, top_k = (1 << 26) + 37, 257, 2
-    rows = torch.tensor([0, 1, (1 << 25) - 1, 1 << 25, (1 << 25) + 1, (1 << 26) - 1, 1 << 26, tokens - 1], device=DEV)
-    logits = torch.zeros((tokens, experts), dtype=torch.bfloat16, device=DEV)
-    logits[rows] = logits_of(len(rows), experts, torch.bfloat16, 1).to(DEV)
-    grad = torch.zeros((tokens, top_k), device=DEV)
-    grad[rows] = normal(len(rows), top_k, torch.float32, 2, 0.0).to(DEV)
-    weights, chosen = nk.experts_route(logits, top_k)
-    few, few_chosen = nk.experts_route(logits[rows], top_k)
-    assert torch.equal(weights[rows], few) and torch.equal(chosen[rows], few_chosen)
-    assert int((chosen != torch.arange(top_k, device=DEV)).any(1).sum()) <= len(rows)  # (equal logits: the first two)
-    got = nk.experts_route_backward(grad, logits, chosen)
-    assert torch.equal(got[rows], nk.experts_route_backward(grad[rows], logits[rows], few_chosen))
-    del logits, got
-    torch.cuda.empty_cache()
-
-
-@pytest.mark.parametrize("short_way", [True, False])
-@pytest.mark.parametrize("score,biased,groups,renormalize,dtype", [("softmax", False, 1, True, torch.float32), ("sigmoid", True, 4, True, torch.bfloat16),
-                                                                   ("sigmoid", False, 1, False, torch.float16), ("softmax", True, 2, False, torch.float32)])
-def test_autograd_follows_the_weights(monkeypatch, score, biased, groups, renormalize, dtype, short_way):
-    """Weights that a loss is made of hand their gradient on to whatever made the logits, by experts_route_backward."""
-    from numkong_amd import mx as binding
-
-    if not short_way:
-        monkeypatch.setattr(binding, "_CALLS", None)
-    source, grad = logits_of(30, 24, torch.float32, 1).to(DEV).requires_grad_(), normal(30, 3, torch.float32, 2, 0.0).to(DEV)
-    bias = torch.rand(24, device=DEV).requires_grad_() if biased else None
-    kind = dict(bias=bias, groups=groups, top_groups=max(1, groups // 2), group_top=2 if groups > 1 else 1)
-    logits = (2 * source).to(dtype)
-    weights, chosen = nk.experts_route(logits, 3, score, renormalize=renormalize, scale=1.5, **kind)
-    with torch.no_grad():
-        plain, plain_chosen = nk.experts_route(logits, 3, score, renormalize=renormalize, scale=1.5, **kind)
-    assert weights.requires_grad and not chosen.requires_grad and not plain.requires_grad
-    assert torch.equal(weights, plain) and torch.equal(chosen, plain_chosen)
-    (weights * grad).sum().backward()
-    want = nk.experts_route_backward(grad, logits.detach(), chosen, score, renormalize, 1.5)
-    assert torch.equal(source.grad, 2 * want.float()) and (not biased or bias.grad is None)
-    again = nk.experts_route(logits.detach().requires_grad_(), 3, score)[0].sum()  # (its gradient is one number for all)
-    again.backward()
-    host = logits.detach().cpu().requires_grad_()
-    (nk.experts_route(host, 3, score, renormalize=renormalize, scale=1.5, **{**kind, "bias": bias.detach().cpu() if biased else None})[0] * grad.cpu()).sum().backward()
-    assert torch.equal(host.grad, want.cpu())
-    leaf = logits.detach().requires_grad_()
-    first, = torch.autograd.grad(nk.experts_route(leaf, 3, score)[0].square().sum(), leaf, create_graph=True)
-    with pytest.raises(RuntimeError):
-        first.sum().backward()
-
-
-@pytest.mark.parametrize("short_way", [True, False])
-def test_products_say_that_they_have_no_gradient(monkeypatch, short_way):
-    from numkong_amd import mx as binding
-
-    if not short_way:
-        monkeypatch.setattr(binding, "_CALLS", None)
-    a, packed, stack = normal(6, 64, torch.float32, 1).to(DEV), nk.mx_pack(torch.ones((8, 64), device=DEV)), nk.mx_pack(torch.ones((4, 8, 64), device=DEV))
-    plan, weights = nk.experts_plan(torch.zeros((6, 2), dtype=torch.int32, device=DEV), 4), torch.rand((6, 2), device=DEV)
-    leaf, weight = a.clone().requires_grad_(), weights.clone().requires_grad_()
-    for name, tracked, plain in (("mx_dots_packed", lambda **o: nk.mx_dots_packed(leaf, packed, **o), lambda: nk.mx_dots_packed(a, packed)),
-                                 ("mx_dots_experts", lambda **o: nk.mx_dots_experts(leaf, stack, plan, **o), lambda: nk.mx_dots_experts(a, stack, plan)),
-                                 ("mx_dots_experts", lambda **o: nk.mx_dots_experts(a, stack, plan, weight, **o), lambda: nk.mx_dots_experts(a, stack, plan, weights))):
-        want, got = plain(), tracked()
-        assert torch.equal(got, want) and got.requires_grad and not want.requires_grad
-        with pytest.raises(nk.NumKongAmdError, match=name + " has no gradient"):
-            got.sum().backward()
-        with pytest.raises(nk.NumKongAmdError, match="out="):
-            tracked(out=torch.empty_like(want))
-        with torch.no_grad():
-            assert not tracked().requires_grad and torch.equal(tracked(out=torch.empty_like(want)), want)
-    assert leaf.grad is None and weight.grad is None
-
-
 # ---- the plan and the products ---------------------------------------------------------------------------------------
 
 def routing(tokens, top_k, experts, kind, seed=0):
@@ -378,60 +232,6 @@ def test_plan(tokens, top_k, experts, kind):
             for e in range(experts + 1) for row in range(0, counts[e], tile_rows)]
     np.testing.assert_array_equal(tiles[:, :3], np.array(want).reshape(-1, 3))
     assert tile_count == sum(tile[0] < experts for tile in want)
-
-
-def large_routing(slots, experts, popular):
-    """One expert's share of all slots is `popular`; some slots have no expert."""
-    generator = torch.Generator(device=DEV).manual_seed(slots)
-    chosen = torch.randint(-1, experts, (slots,), dtype=torch.int32, device=DEV, generator=generator)
-    chosen[torch.rand((slots,), device=DEV, generator=generator) < popular] = experts // 2
-    return chosen.reshape(-1, 8)
-
-
-@pytest.mark.parametrize("slots,experts,popular", [(1 << 16, 1024, 0.0), (66 << 10, 100, 0.5), ((1 << 17) + 8, 15, 0.0), (1 << 20, 128, 0.9), (1 << 20, 1024, 0.1),
-                                                   (1 << 27, 8, 0.3)])
-def test_plan_of_many_slots(slots, experts, popular):
-    """As test_plan, by torch's own sort: more workgroups than add up one another's counts, tiles written by several of them."""
-    chosen = large_routing(slots, experts, popular)
-    words = nk.experts_plan(chosen, experts).buffer.view(torch.int32)
-    flat = chosen.reshape(-1)
-    bucket = torch.where((flat >= 0) & (flat < experts), flat, experts)
-    counts = torch.bincount(bucket, minlength=experts + 1)
-    sizes = (counts + 15) // 16 * 16
-    starts = sizes.cumsum(0) - sizes
-    tile_rows, tile_count, zero_tiles, first_zero, end_zero = words[3:8].tolist()
-    assert (first_zero, end_zero) == (int(starts[-1]), int(starts[-1] + counts[-1]))
-    assert torch.equal(words[8:8 + experts + 1], starts.int()) and int(words[9 + experts]) == end_zero
-    by_bucket, slot_at = torch.sort(bucket, stable=True)
-    row_of = starts[by_bucket] + torch.arange(slots, device=DEV) - (counts.cumsum(0) - counts)[by_bucket]
-    order = torch.full((int(sizes.sum()),), -1, dtype=torch.int32, device=DEV)
-    order[row_of] = slot_at.int()
-    place = torch.empty(slots, dtype=torch.int32, device=DEV)
-    place[slot_at] = torch.where(by_bucket < experts, row_of, -1).int()
-    first, room = 8 + (experts + 2 + 3) // 4 * 4, (slots + min(slots, experts + 1) * 15 + 15) // 16 * 16
-    assert torch.equal(words[first:first + len(order)], order)
-    assert torch.equal(words[first + room:first + room + slots], place)
-    tiles = words[(first + room + slots + 3) // 4 * 4:][:4 * (tile_count + zero_tiles)].reshape(-1, 4)
-    of_bucket = (counts + tile_rows - 1) // tile_rows
-    expert = torch.repeat_interleave(torch.arange(experts + 1, device=DEV), of_bucket)
-    row = starts[expert] + tile_rows * (torch.arange(len(expert), device=DEV) - (of_bucket.cumsum(0) - of_bucket)[expert])
-    want = torch.stack([expert, row, torch.minimum(row + tile_rows, (starts + counts)[expert])], 1).int()
-    assert torch.equal(tiles[:, :3], want) and tile_count == int(of_bucket[:-1].sum())
-
-
-def test_a_plan_takes_time_by_its_slots():
-    """32 times the slots: about 32 times the work, where a thousand times would be work that grows with their square."""
-    def milliseconds(slots):
-        chosen = large_routing(slots, 8, 0.9)
-        nk.experts_plan(chosen, 8)
-        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-        start.record()
-        nk.experts_plan(chosen, 8)
-        end.record()
-        end.synchronize()
-        return start.elapsed_time(end)
-
-    assert milliseconds(1 << 27) < 4 * 32 * milliseconds(1 << 22)
 
 
 @pytest.mark.parametrize("tokens,top_k,experts,kind", CASES)
@@ -494,56 +294,6 @@ def test_plan_of_other_sizes_gives_nans(tokens, experts):
         assert torch.isnan(nk.mx_dots_experts(a, packed, wrong)).all()
         assert torch.isnan(nk.mx_dots_experts(a, packed, wrong, torch.ones((tokens, 2), device=DEV))).all()
     assert (nk.mx_dots_experts(a, packed, right) == 64).all()
-
-
-@pytest.mark.parametrize("short_way", [True, False])
-def test_images_and_plans_are_as_large_as_their_sizes_say(monkeypatch, short_way):
-    """Parts of an image or a plan, and buffers that are not in one piece, are refused before a kernel looks for the rest."""
-    from numkong_amd import mx as binding
-
-    a, packed, stack = torch.ones((6, 64), device=DEV), nk.mx_pack(torch.ones((80, 64), device=DEV)), nk.mx_pack(torch.ones((8, 80, 64), device=DEV))
-    plan = nk.experts_plan(torch.zeros((6, 2), dtype=torch.int32, device=DEV), 8)
-    if not short_way:
-        monkeypatch.setattr(binding, "_CALLS", None)
-
-    def parts(buffer):
-        twice = torch.zeros(2 * buffer.numel(), dtype=torch.uint8, device=DEV)
-        return buffer[:0], buffer[:1], buffer[:-1], buffer[:64].clone(), twice[::2]
-
-    for part in parts(packed.buffer):
-        with pytest.raises(ValueError, match="packed image"):
-            nk.mx_dots_packed(a, nk.MxPackedMatrix(1, 80, 64, part))
-    with pytest.raises(ValueError, match="packed image"):
-        nk.mx_dots_packed(a, nk.MxPackedMatrix(1, 1 << 30, 64, packed.buffer))
-    for weights in (None, torch.ones((6, 2), device=DEV)):
-        for part in parts(stack.buffer):
-            with pytest.raises(ValueError, match="packed image"):
-                nk.mx_dots_experts(a, nk.MxPackedMatrix(8, 80, 64, part), plan, weights)
-        for part in parts(plan.buffer):
-            with pytest.raises(ValueError, match="the plan"):
-                nk.mx_dots_experts(a, stack, nk.ExpertsPlan(6, 2, 8, part), weights)
-        larger = [torch.cat([one, one.new_zeros(100)]) for one in (stack.buffer, plan.buffer)]
-        got = nk.mx_dots_experts(a, nk.MxPackedMatrix(8, 80, 64, larger[0]), nk.ExpertsPlan(6, 2, 8, larger[1]), weights)
-        assert bool((got == (64 if weights is None else 128)).all())
-
-
-@pytest.mark.parametrize("tokens,experts", [(3, 8), (200, 8), (900, 4)])
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_no_depth_and_other_images(tokens, experts, dtype):
-    """Few rows to an expert, some, many; some without an expert, the sums by weight as well."""
-    chosen = torch.from_numpy(routing(tokens, 2, experts, "some", 1)).to(DEV)
-    there = (chosen >= 0) & (chosen < experts)
-    plan, weights = nk.experts_plan(chosen, experts), torch.ones((tokens, 2), device=DEV)
-    empty = nk.mx_pack(torch.ones((experts, 300, 0), device=DEV))
-    other = nk.MxPackedMatrix(experts, 300, 60, nk.mx_pack(torch.ones((experts, 300, 64), device=DEV)).buffer)
-    for k, packed in ((0, empty), (60, other)):
-        a = torch.ones((tokens, k), device=DEV)
-        rows = nk.mx_dots_experts(a, packed, plan, out_dtype=dtype)
-        sums = nk.mx_dots_experts(a, packed, plan, weights, out_dtype=dtype)
-        if k:
-            assert bool(rows[there].isnan().all()) and bool(sums[there.any(1)].isnan().all()) and not sums[~there.any(1)].any()
-        else:
-            assert rows.shape == (tokens, 2, 300) and not rows.any() and not sums.any()
 
 
 def test_no_tokens():

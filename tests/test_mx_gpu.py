@@ -358,42 +358,3 @@ def test_offsets_past_32_bits():
     truth, magnitude = left @ picked.T, np.abs(left) @ np.abs(picked).T
     mx.close(nk.mx_dots_packed(small.to(DEV), nk.mx_pack(matrix))[:, rows], truth, magnitude, k)
     mx.close(nk.mx_dots_packed(matrix, nk.mx_pack(small.to(DEV)))[rows].T, truth, magnitude, k)
-
-
-def test_more_rows_than_one_launch_takes():
-    """2^28 rows of A, as floats and as codes: quantised pairs of values give sums that 32 bits hold."""
-    rows, k, n = (1 << 28) + 37, 2, 3
-    generator = torch.Generator(device=DEV).manual_seed(1)
-    a = torch.randint(-40, 41, (rows, k), device=DEV, generator=generator, dtype=torch.int8).to(torch.bfloat16)
-    b = torch.tensor([[1.0, -3.0], [0.5, 6.0], [4.0, 1.5]], device=DEV)
-    packed, codes = nk.mx_pack(b), nk.mx_quantize(a)
-    values = nk.mx_dequantize(codes)
-    for left in (a, codes):
-        got = nk.mx_dots_packed(left, packed)
-        for column in range(n):
-            assert torch.equal(got[:, column], values[:, 0] * b[column, 0] + values[:, 1] * b[column, 1])
-        del got
-    torch.cuda.empty_cache()
-
-
-def test_more_columns_than_one_launch_takes():
-    """A matrix of 2^28 columns against one row, and as an expert's against two: sums of quarters below 2^13, which 32 bits hold."""
-    n, k = (1 << 28) + 100, 32
-    generator = torch.Generator(device=DEV).manual_seed(2)
-    codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device=DEV, generator=generator)
-    matrix = nk.MxMatrix(codes, torch.full((n, 1), 127, dtype=torch.uint8, device=DEV), k)
-    a = normal(2, k, torch.float32, 3).to(DEV)
-    left = nk.mx_dequantize(nk.mx_quantize(a))
-    packed = nk.mx_pack(matrix)
-    one = nk.mx_dots_packed(a[:1], packed)
-    for first in (0, (1 << 26) - 500, (1 << 27) - 500, (1 << 27) + 12345, n - 1000):
-        part = nk.MxMatrix(codes[first:first + 1000], matrix.scales[first:first + 1000], k)
-        assert torch.equal(one[:, first:first + 1000], left[:1] @ nk.mx_dequantize(part).T.contiguous()), first
-    chosen = torch.zeros((2, 1), dtype=torch.int32, device=DEV)
-    both = nk.mx_dots_experts(a, nk.MxPackedMatrix(1, n, k, packed.buffer), nk.experts_plan(chosen, 1))
-    assert torch.equal(both[0], one)
-    for first in (0, (1 << 26) - 500, (1 << 27) - 500, (1 << 27) + 12345, n - 1000):
-        part = nk.MxMatrix(codes[first:first + 1000], matrix.scales[first:first + 1000], k)
-        assert torch.equal(both[1:, 0, first:first + 1000], left[1:] @ nk.mx_dequantize(part).T.contiguous()), first
-    del one, both, packed, codes, matrix
-    torch.cuda.empty_cache()
