@@ -190,7 +190,7 @@ def _to_host(result, as_numpy: bool, out=None):
     if out is not None:
         _tensor(out, "out").copy_(result)
         return out
-    return result.cpu().numpy() if as_numpy else result.cpu()
+    return result.detach().cpu().numpy() if as_numpy else result.cpu()
 
 
 def _new(torch, rows, columns, dtype, device):

@@ -136,6 +136,8 @@ def test_products_say_that_they_have_no_gradient(monkeypatch, short_way):
         with torch.no_grad():
             assert not tracked().requires_grad and torch.equal(tracked(out=torch.empty_like(want)), want)
     assert leaf.grad is None and weight.grad is None
+    array = nk.mx_dots_experts(a.cpu().numpy(), stack, plan, weights.cpu().requires_grad_())  # (an array holds no gradient)
+    np.testing.assert_array_equal(array, nk.mx_dots_experts(a, stack, plan, weights).cpu().numpy())
 
 
 @pytest.mark.parametrize("short_way", [True, False])
