@@ -105,6 +105,9 @@ void *stream_of(Home const &home) { return (void *)c10::hip::getCurrentHIPStream
 /** Does autograd follow it? Then mx.py says what becomes of the gradient. */
 bool tracked(at::Tensor const &t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
 
+/** Is the buffer as large as its sizes say (0: there are no such sizes)? */
+bool holds(at::Tensor const &buffer, nk_size_t needed) { return needed && buffer.nbytes() >= needed; }
+
 /** What a product's call says of A: a float matrix, or codes and scales. */
 struct Left {
     at::Tensor const *t = nullptr, *scales = nullptr;
@@ -181,7 +184,7 @@ PyObject *dots(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
     at::Tensor const *const image = tensor_of(arguments[3], 1, home);
     at::ScalarType const type = ((THPDtype *)arguments[6])->scalar_type;
     nk_dtype_t const dtype = code_of(type);
-    if (!image || !dtype || image->nbytes() < packed_size(1, width, depth)) Py_RETURN_NONE;
+    if (!image || !dtype || !holds(*image, packed_size(1, width, depth))) Py_RETURN_NONE;
     at::Tensor c, workspace;
     int status;
     {
@@ -303,8 +306,8 @@ PyObject *experts(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
     at::ScalarType const type = ((THPDtype *)arguments[12])->scalar_type;
     nk_dtype_t const dtype = code_of(type);
     int64_t const slots = tokens * top_k, rows = a.t->size(0);
-    if (!image || !plan_ || !dtype || (rows != tokens && rows != slots) || image->nbytes() < packed_size(matrices, width, depth) ||
-        plan_->nbytes() < library.plan_size(slots, matrices))
+    if (!image || !plan_ || !dtype || (rows != tokens && rows != slots) || !holds(*image, packed_size(matrices, width, depth)) ||
+        !holds(*plan_, library.plan_size(slots, matrices)))
         Py_RETURN_NONE;
     if (arguments[11] != Py_None) {
         weights = tensor_of(arguments[11], 2, home);

@@ -230,6 +230,8 @@ def _check_host_out(out, shape, dtype):
 
 def _check_room(buffer, needed: int, what: str) -> None:
     """What a kernel finds its way in by sizes alone has to be as large as these say."""
+    if not needed:
+        raise ValueError(f"{what} is of sizes that are not supported")
     if buffer.nbytes < needed or not buffer.is_contiguous():
         raise ValueError(f"{what} has to be {needed} adjacent bytes for these sizes, got {buffer.nbytes}")
 

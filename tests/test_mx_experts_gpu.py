@@ -157,8 +157,9 @@ def test_images_and_plans_are_as_large_as_their_sizes_say(monkeypatch, short_way
     for part in parts(packed.buffer):
         with pytest.raises(ValueError, match="packed image"):
             nk.mx_dots_packed(a, nk.MxPackedMatrix(1, 80, 64, part))
-    with pytest.raises(ValueError, match="packed image"):
-        nk.mx_dots_packed(a, nk.MxPackedMatrix(1, 1 << 30, 64, packed.buffer))
+    for width in (1 << 30, 1 << 31, 1 << 40):
+        with pytest.raises(ValueError, match="packed image"):
+            nk.mx_dots_packed(a, nk.MxPackedMatrix(1, width, 64, packed.buffer))
     for weights in (None, torch.ones((6, 2), device=DEV)):
         for part in parts(stack.buffer):
             with pytest.raises(ValueError, match="packed image"):
