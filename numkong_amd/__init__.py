@@ -22,6 +22,18 @@ from .api import (  # noqa: F401
     library,
     library_path,
 )
+from .dense import (  # noqa: F401
+    Mx8Matrix,
+    gated_linear,
+    gated_linear_backward,
+    linear,
+    linear_backward,
+    mx8_dequantize,
+    mx8_quantize,
+    rms_norm,
+    rms_norm_backward,
+    rms_norm_mx8,
+)
 from .mx import (  # noqa: F401
     ExpertsPlan,
     MxMatrix,

@@ -1,0 +1,148 @@
+/**
+ *  @brief What the norm's and the dense products' kernels share: 8-bit blocks, activations, values of any float type.
+ *  @file numkong_amd/csrc/dense_gfx950.hpp
+ */
+#ifndef NUMKONG_AMD_DENSE_GFX950_HPP
+#define NUMKONG_AMD_DENSE_GFX950_HPP
+
+#include "mx_gfx950.hpp"
+#include "numkong_amd/dense.h"
+
+namespace nk_gfx950 {
+
+/** Bytes of a value of a float type; 0: it is none. */
+inline int float_bytes(int dtype) { return dtype == nk_f32_k ? 4 : dtype == nk_bf16_k || dtype == nk_f16_k ? 2 : 0; }
+inline bool aligned_to(void const *p, uint64_t stride, uint64_t bytes) { return !((uintptr_t)p % bytes) && !(stride % bytes); }
+
+/** A value of a float type that the host names: 0 f32, 1 bf16, 2 f16 (a branch that all lanes take alike). */
+enum Kind : uint32_t { kF32 = 0, kBF16 = 1, kF16 = 2 };
+inline Kind kind_of(int dtype) { return dtype == nk_bf16_k ? kBF16 : dtype == nk_f16_k ? kF16 : kF32; }
+__host__ __device__ inline uint32_t bytes_of(uint32_t kind) { return kind == kF32 ? 4 : 2; }
+
+/** Eight adjacent values of a row from column `col` on; zeros from column `k` on. */
+template <class T>
+__device__ __forceinline__ void load_8(T const *row, uint32_t col, uint32_t k, float (&v)[8]) {
+    if (col + 8 <= k) {
+        if constexpr (sizeof(T) == 4) {
+            v4u const low = *(v4u_anywhere const *)(row + col), high = *(v4u_anywhere const *)(row + col + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(low[i]), v[4 + i] = __uint_as_float(high[i]);
+        } else widen<T>(*(v4u_anywhere const *)(row + col), v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = col + i < k ? (float)row[col + i] : 0.0f;
+}
+__device__ __forceinline__ void load_8(uint32_t kind, void const *row, uint32_t col, uint32_t k, float (&v)[8]) {
+    if (kind == kF32) load_8((float const *)row, col, k, v);
+    else if (kind == kBF16) load_8((__bf16 const *)row, col, k, v);
+    else load_8((_Float16 const *)row, col, k, v);
+}
+/** `count` (up to 8) adjacent results at column `col` of a row. */
+__device__ __forceinline__ void store_8(uint32_t kind, void *row, uint32_t col, float const (&v)[8], uint32_t count) {
+    if (kind == kF32) store_some((float *)row + col, v, count);
+    else if (kind == kBF16) store_some((__bf16 *)row + col, v, count);
+    else store_some((_Float16 *)row + col, v, count);
+}
+__device__ __forceinline__ float load_1(uint32_t kind, void const *row, uint64_t col) {
+    return kind == kF32 ? ((float const *)row)[col] : kind == kBF16 ? (float)((__bf16 const *)row)[col] : (float)((_Float16 const *)row)[col];
+}
+__device__ __forceinline__ void store_1(uint32_t kind, void *row, uint64_t col, float v) {
+    if (kind == kF32) ((float *)row)[col] = v;
+    else if (kind == kBF16) ((__bf16 *)row)[col] = (__bf16)v;
+    else ((_Float16 *)row)[col] = (_Float16)v;
+}
+
+/**
+ *  A lane's eight values of a block of 32, which four adjacent lanes hold, to e4m3 codes (the first in the lowest byte) and the
+ *  block's scale byte. The scale is the smallest power of two that keeps the largest magnitude within 448 = 1.75 x 2^8: its exponent
+ *  field less 8, and one more where the mantissa is above 0.75; none is below 2^-127. Nothing saturates then, and the
+ *  conversion, which divides by the scale, rounds to nearest even. A NaN or an infinity has the largest field and decides
+ *  for its block.
+ */
+__device__ __forceinline__ v2u quantize_8(float const (&v)[8], uint32_t &scale) {
+    uint32_t largest = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        uint32_t const magnitude = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+        largest = largest > magnitude ? largest : magnitude;
+    }
+    largest = block_max<4>(largest);
+    uint32_t const field = largest >> 23, above = (largest & 0x7FFFFFu) > 0x600000u;
+    scale = field == 255 ? 255 : field + above > 8 ? field + above - 8 : 0;
+    v2u codes = {0, 0};
+#ifdef NK_MX_DEVICE_BUILTINS
+    typedef short v2s __attribute__((ext_vector_type(2)));
+    float const power = __uint_as_float(scale ? scale << 23 : 0x00400000u);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        v2s word = {0, 0};
+        word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(word, v[4 * i], v[4 * i + 1], power, false);
+        word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(word, v[4 * i + 2], v[4 * i + 3], power, true);
+        codes[i] = field == 255 ? 0u : __builtin_bit_cast(uint32_t, word);
+    }
+#endif
+    return codes;
+}
+/** `count` (up to 8) codes to any address. */
+__device__ __forceinline__ void store_codes(uint8_t *to, v2u codes, uint32_t count) {
+    if (count >= 8) {
+        typedef v2u __attribute__((aligned(1))) v2u_anywhere;
+        *(v2u_anywhere *)to = codes;
+        return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i)
+        if (i < count) to[i] = (uint8_t)(codes[i / 4] >> 8 * (i % 4));
+}
+
+/** The four values of a word of e4m3 codes. */
+__device__ __forceinline__ void widen_e4m3(uint32_t word, float (&v)[4]) {
+#ifdef NK_MX_DEVICE_BUILTINS
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    v2f const low = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, false), high = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, true);
+    v[0] = low[0], v[1] = low[1], v[2] = high[0], v[3] = high[1];
+#endif
+}
+/** The power of two of a scale byte. */
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+    return byte == 255 ? __builtin_nanf("") : __uint_as_float(byte ? byte << 23 : 0x00400000u);
+}
+
+/**
+ *  Activations and their slopes, in 32 bits. Silu is x / (1 + e^-x): where e^-x overflows x is below -88 and the result rounds to -0.
+ *  The tanh of gelu_tanh is written as 1 - 2 / (1 + e^2z), so 0.5 x (1 + tanh z) = x - x / (1 + e^2z), without cancellation
+ *  that a negative z would bring.
+ */
+__device__ __forceinline__ float activate(uint32_t kind, float x) {
+    switch (kind) {
+    case nk_amd_relu: return x > 0 ? x : x != x ? x : 0.0f;
+    case nk_amd_silu: return x == -__builtin_inff() ? -0.0f : x / (1.0f + expf(-x));
+    case nk_amd_gelu: return x == -__builtin_inff() ? -0.0f : 0.5f * x * erfcf(-0.70710678118654752f * x);
+    case nk_amd_gelu_tanh: {
+        float const z = 1.5957691216057308f * (x + 0.044715f * x * x * x); // twice the argument of tanh
+        return x == -__builtin_inff() ? -0.0f : x / (1.0f + expf(-z));
+    }
+    default: return x;
+    }
+}
+__device__ __forceinline__ float slope(uint32_t kind, float x) {
+    if (fabsf(x) > 110.0f) return kind && x < 0 ? 0.0f : 1.0f; // (the limits, which infinities and overflows would miss)
+    switch (kind) {
+    case nk_amd_relu: return x > 0 ? 1.0f : 0.0f;
+    case nk_amd_silu: {
+        float const s = 1.0f / (1.0f + expf(-x));
+        return s + s * (x * (1.0f - s));
+    }
+    case nk_amd_gelu: return 0.5f * erfcf(-0.70710678118654752f * x) + x * (0.39894228040143268f * expf(-0.5f * x * x));
+    case nk_amd_gelu_tanh: {
+        float const z = 1.5957691216057308f * (x + 0.044715f * x * x * x), s = 1.0f / (1.0f + expf(-z));
+        return s + s * (x * (1.0f - s)) * (1.5957691216057308f * (1.0f + 0.134145f * x * x));
+    }
+    default: return 1.0f;
+    }
+}
+
+} // namespace nk_gfx950
+
+#endif // NUMKONG_AMD_DENSE_GFX950_HPP
