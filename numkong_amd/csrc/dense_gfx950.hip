@@ -8,118 +8,373 @@
  *
  *  and gated, with q = A W_up^T and C = f(p) q:  d = g q f'(p), e = g f(p);  of A: d W + e W_up;  of W: d^T A;  of W_up: e^T A.
  */
-#include "dense_gfx950.hpp"
+#include "dense_tiles_gfx950.hpp"
 
 namespace nk_gfx950 {
 
-int launch_mx8_quantize(uint32_t kind, void const *x, uint64_t x_stride, uint64_t rows, uint64_t k, uint8_t *codes, uint64_t codes_stride,
-                        uint8_t *scales, uint64_t scales_stride, hipStream_t stream); // norm_gfx950.hip
+int launch_mx8_quantize(uint32_t kind, void const *x, uint64_t x_stride, uint64_t rows, uint64_t k, uint64_t stored, uint8_t *codes, uint64_t codes_stride,
+                        uint8_t *scales, uint64_t scales_stride, uint32_t *words, uint64_t pitch, hipStream_t stream); // norm_gfx950.hip
 int launch_column_sum(float const *values, uint64_t rows, uint64_t k, uint32_t kind, void *out, hipStream_t stream);
 
 namespace {
 
-/** What becomes of a product's sums. */
-struct Epilogue {
-    void const *bias;
-    uint8_t const *residual;
-    uint8_t *c;
-    float *pre, *pre_up;
-    uint64_t residual_stride, c_stride, pre_stride;
-    uint32_t bias_kind, residual_kind, c_kind, activation;
-};
-__device__ __forceinline__ void finish_one(Epilogue const &e, uint64_t row, uint32_t col, float p, float q, bool gated) {
-    if (e.bias) p += load_1(e.bias_kind, e.bias, col);
-    if (e.pre) {
-        *((float *)((uint8_t *)e.pre + row * e.pre_stride) + col) = p;
-        if (gated) *((float *)((uint8_t *)e.pre_up + row * e.pre_stride) + col) = q;
-    }
-    float v = activate(e.activation, p);
-    if (gated) v *= q;
-    if (e.residual) v += load_1(e.residual_kind, e.residual + row * e.residual_stride, col);
-    store_1(e.c_kind, e.c + row * e.c_stride, col, v);
+inline uint64_t up_to(uint64_t n, uint64_t step) { return (n + step - 1) / step * step; }
+
+/** Up to 16 bytes of a row of `bytes` from `at` on, wherever they lie; zeros behind the end. */
+__device__ __forceinline__ v4u load_piece(uint8_t const *row, uint32_t at, uint32_t bytes) {
+    if (at + 16 <= bytes) return *(v4u_anywhere const *)(row + at);
+    v4u piece = {0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i)
+        if (at + i < bytes) piece[i / 4] |= (uint32_t)row[at + i] << 8 * (i % 4);
+    return piece;
 }
 
-/** An operand: rows of the result (or columns) by `row` bytes, the depth by `step` bytes; with scales mx8. */
-struct Side {
+// ---- operands as the tiles take them -------------------------------------------------------------------------------
+
+/** Rows of `bytes` to where they are 16-byte aligned, zeros up to the next multiple of 16: a thread for 16 bytes. */
+__global__ __launch_bounds__(256) void realign_kernel(uint8_t const *from, uint64_t from_stride, uint64_t pieces, uint32_t each, uint32_t bytes, uint8_t *to, uint64_t to_stride) {
+    uint64_t const at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= pieces) return;
+    uint64_t const row = at / each;
+    uint32_t const piece = (uint32_t)(at - row * each);
+    *(v4u *)(to + row * to_stride + piece * 16) = load_piece(from + row * from_stride, piece * 16, bytes);
+}
+int launch_realign(uint8_t const *from, uint64_t from_stride, uint64_t rows, uint64_t bytes, uint8_t *to, uint64_t to_stride, hipStream_t stream) {
+    uint64_t const each = (bytes + 15) / 16, most = kMostThreads / each; // rows of a launch
+    for (uint64_t first = 0; first < rows; first += most) {
+        uint64_t const here = rows - first < most ? rows - first : most;
+        hipLaunchKernelGGL(realign_kernel, dim3((uint32_t)((here * each + 255) / 256)), dim3(256), 0, stream, from + first * from_stride, from_stride, here * each, (uint32_t)each, (uint32_t)bytes,
+                           to + first * to_stride, to_stride);
+        hipError_t const e = hipGetLastError();
+        if (e != hipSuccess) return mx_fail(e, "realign_kernel");
+    }
+    return 0;
+}
+
+struct WordsArgs {
+    uint8_t const *scales[2];
+    uint64_t stride[2];
+    uint32_t *words[2];
+    uint32_t rows, blocks, stages, pitch;
+};
+/** Scales as the tiles read them, words of four blocks by stage and row (zeros where there is no block): 32 rows times 32 stages a workgroup, through LDS, as
+ *  rows are read and written along different axes. */
+__global__ __launch_bounds__(256) void scale_words_kernel(WordsArgs p) {
+    __shared__ uint32_t tile[32][33];
+    int const which = blockIdx.z;
+    uint32_t const row0 = blockIdx.x * 32, stage0 = blockIdx.y * 32, x = threadIdx.x % 32;
+#pragma unroll
+    for (uint32_t y = threadIdx.x / 32; y < 32; y += 8) {
+        uint32_t const row = row0 + y, block = (stage0 + x) * 4;
+        uint32_t word = 0;
+        if (row < p.rows && block < p.blocks) {
+            uint8_t const *const at = p.scales[which] + row * p.stride[which] + block;
+            if (block + 4 <= p.blocks) word = *(u32_anywhere const *)at;
+            else
+                for (uint32_t i = 0; i < p.blocks - block; ++i) word |= (uint32_t)at[i] << 8 * i;
+        }
+        tile[y][x] = word;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t y = threadIdx.x / 32; y < 32; y += 8)
+        if (stage0 + y < p.stages) p.words[which][(uint64_t)(stage0 + y) * p.pitch + row0 + x] = tile[x][y];
+}
+
+/** Sums of the splits, in their order, and what follows: eight adjacent results a thread. */
+template <bool GATED>
+__global__ __launch_bounds__(256) void join_kernel(float const *partial, uint32_t splits, uint32_t m, uint32_t n, Epilogue e) {
+    uint32_t const each = (n + 7) / 8;
+    uint64_t const at = (uint64_t)blockIdx.x * 256 + threadIdx.x, row = at / each, plane = (uint64_t)m * n;
+    if (row >= m) return;
+    uint32_t const col = (uint32_t)(at - row * each) * 8;
+    float v[8] = {}, q[8] = {};
+    for (uint32_t i = 0; i < splits; ++i) {
+        float part[8];
+        load_8(partial + i * plane * (GATED ? 2 : 1) + row * n, col, n, part);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += part[j];
+        if constexpr (GATED) {
+            load_8(partial + (2 * i + 1) * plane + row * n, col, n, part);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[j] += part[j];
+        }
+    }
+    finish_8<GATED>(e, row, col, n, v, q);
+}
+
+// ---- few rows ------------------------------------------------------------------------------------------------------
+
+struct FewSide {
     uint8_t const *values;
-    uint64_t row, step;
+    uint64_t stride;
     uint8_t const *scales;
     uint64_t scales_stride;
 };
-template <class T>
-__device__ __forceinline__ T value_of(Side const &s, uint64_t row, uint32_t k) {
-    uint8_t const *const at = s.values + row * s.row + k * s.step;
-    if (!s.scales) return *(T const *)at;
-    float four[4];
-    widen_e4m3(*at, four);
-    return (T)(four[0] * scale_of(s.scales[row * s.scales_stride + k / 32]));
-}
-
-struct SimpleArgs {
-    Side a[2], b[2]; // of sums over two depths: both pairs; gated: the second b
-    uint32_t m, n, k, pairs;
+struct FewArgs {
+    FewSide a, b[2];
+    uint32_t m, n, bytes; // bytes of a row
+    uint32_t first;       // of the launch's blocks of columns
     Epilogue e;
 };
+/** c += x y for 16 rows of each and 64 bytes of depth of 16-bit values. */
 template <class T>
-struct Vector8;
-template <>
-struct Vector8<__bf16> {
-    typedef __bf16 type __attribute__((ext_vector_type(8)));
-};
-template <>
-struct Vector8<_Float16> {
-    typedef _Float16 type __attribute__((ext_vector_type(8)));
-};
-template <class T>
-__device__ __forceinline__ v16f multiply(typename Vector8<T>::type a, typename Vector8<T>::type b, v16f c) {
+__device__ __forceinline__ v4f multiply_16(v4u x, v4u y, v4f c) {
 #ifdef NK_MX_DEVICE_BUILTINS
-    if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, x), __builtin_bit_cast(v8bf, y), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, y), c, 0, 0, 0);
+#else
+    return c;
+#endif
+}
+/** 128 8-bit values; a lane's scales. */
+__device__ __forceinline__ v4f multiply_16(v4u const (&x)[2], v4u const (&y)[2], v4f c, uint32_t x_scale, uint32_t y_scale) {
+#ifdef NK_MX_DEVICE_BUILTINS
+    v8i const p = {(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3], (int)x[1][0], (int)x[1][1], (int)x[1][2], (int)x[1][3]};
+    v8i const q = {(int)y[0][0], (int)y[0][1], (int)y[0][2], (int)y[0][3], (int)y[1][0], (int)y[1][1], (int)y[1][2], (int)y[1][3]};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(p, q, c, 0, 0, 0, (int)x_scale, 0, (int)y_scale);
 #else
     return c;
 #endif
 }
 
-/** The plainest form: 64 x 64 results a workgroup, 32 x 32 a wavefront, operands one value at a time into LDS. */
-template <class T, bool GATED>
-__global__ __launch_bounds__(256) void simple_kernel(SimpleArgs p) {
-    typedef typename Vector8<T>::type V;
-    __shared__ __attribute__((aligned(16))) T as[64][40], bs[GATED ? 2 : 1][64][40];
-    uint32_t const row0 = blockIdx.y * 64, col0 = blockIdx.x * 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    v16f sum = {}, sum_up = {};
-    for (uint32_t pair = 0; pair < p.pairs; ++pair)
-        for (uint32_t k0 = 0; k0 < p.k; k0 += 32) {
-            __syncthreads();
-            for (uint32_t i = threadIdx.x; i < 64 * 32; i += 256) {
-                uint32_t const row = i / 32, k = i % 32;
-                as[row][k] = row0 + row < p.m && k0 + k < p.k ? value_of<T>(p.a[pair], row0 + row, k0 + k) : (T)0;
-                bool const there = col0 + row < p.n && k0 + k < p.k;
-                bs[0][row][k] = there ? value_of<T>(p.b[pair], col0 + row, k0 + k) : (T)0;
-                if (GATED) bs[GATED][row][k] = there ? value_of<T>(p.b[1], col0 + row, k0 + k) : (T)0;
-            }
-            __syncthreads();
-            for (uint32_t k = 0; k < 32; k += 16) {
-                uint32_t const at = k + 8 * (lane / 32), row = (wave & 1) * 32 + lane % 32, col = (wave >> 1) * 32 + lane % 32;
-                V const a = *(V const *)&as[row][at];
-                sum = multiply<T>(a, *(V const *)&bs[0][col][at], sum);
-                if (GATED) sum_up = multiply<T>(a, *(V const *)&bs[GATED][col][at], sum_up);
+/**
+ *  Up to 16 MB rows: the stream of the matrix is what bounds it. A workgroup has 16 NB columns (of both matrices, where gated); its wavefronts take every
+ *  WAVES-th 256 bytes of depth, and their sums are joined at the end in their order. Each wavefront reads whole 256-byte pieces of rows, at any
+ *  alignment, two pieces ahead, and turns them to fragments through LDS of its own (16-byte piece p of row r at p ^ r), without a barrier.
+ */
+template <class T, int MB, int NB, bool GATED, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void few_kernel(FewArgs p) {
+    constexpr bool kScaled = __is_same(T, Mx8);
+    constexpr int kMatrices = GATED ? 2 : 1, kBlocks = NB * kMatrices, kSteps = kScaled ? 2 : 4;
+    __shared__ __attribute__((aligned(1024))) uint8_t rooms[WAVES][(kBlocks + MB) * 4096];
+    uint32_t const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, r4 = l / 16, piece = l % 16;
+    uint32_t const col0 = (p.first + blockIdx.x) * 16 * NB, row0 = blockIdx.y * 16 * MB, rows = p.m - row0, chunks = (p.bytes + 255) / 256;
+    uint8_t *const room = rooms[wave];
+
+    uint8_t const *w_rows[kBlocks][4], *a_rows[MB][4]; // rows past the end are the last one again: their results are dropped
+    uint8_t const *w_scales[kBlocks], *a_scales[MB];
+    uint32_t const blocks = (p.bytes + 31) / 32;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+        FewSide const &side = p.b[b / NB];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t const col = col0 + b % NB * 16 + i * 4 + r4;
+            w_rows[b][i] = side.values + (col < p.n ? col : p.n - 1) * side.stride;
+        }
+        uint32_t const col = col0 + b % NB * 16 + l % 16;
+        w_scales[b] = side.scales + (col < p.n ? col : p.n - 1) * side.scales_stride;
+    }
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t const row = b * 16 + i * 4 + r4;
+            a_rows[b][i] = p.a.values + (row0 + (row < rows ? row : rows - 1)) * p.a.stride;
+        }
+        uint32_t const row = b * 16 + l % 16;
+        a_scales[b] = p.a.scales + (row0 + (row < rows ? row : rows - 1)) * p.a.scales_stride;
+    }
+
+    v4f sum[kBlocks][MB] = {};
+    v4u w[2][kBlocks][4], a[2][MB][4] = {};
+    uint32_t w_scale[2][kBlocks][2], a_scale[2][MB][2];
+    auto const load = [&](auto slot, uint32_t c) {
+        constexpr int kSlot = decltype(slot)::value;
+        uint32_t const at = c * 256 + piece * 16;
+        if constexpr (kScaled) { // the lane's blocks: those of its quarter of the wavefront
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                uint32_t const block = c * 8 + s * 4 + r4;
+                bool const there = block < blocks;
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) w_scale[kSlot][b][s] = there ? w_scales[b][block] : 0;
+#pragma unroll
+                for (int b = 0; b < MB; ++b) a_scale[kSlot][b][s] = there ? a_scales[b][block] : 0;
             }
         }
-    for (uint32_t i = 0; i < 16; ++i) {
-        uint32_t const row = row0 + (wave & 1) * 32 + i % 4 + 8 * (i / 4) + 4 * (lane / 32), col = col0 + (wave >> 1) * 32 + lane % 32;
-        if (row < p.m && col < p.n) finish_one(p.e, row, col, sum[i], sum_up[i], GATED);
+        if ((c + 1) * 256 <= p.bytes) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[kSlot][b][i] = *(v4u_anywhere const *)(w_rows[b][i] + at);
+#pragma unroll
+            for (int b = 0; b < MB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (b * 16 + i * 4 < rows) a[kSlot][b][i] = *(v4u_anywhere const *)(a_rows[b][i] + at);
+        } else {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[kSlot][b][i] = load_piece(w_rows[b][i], at, p.bytes);
+#pragma unroll
+            for (int b = 0; b < MB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (b * 16 + i * 4 < rows) a[kSlot][b][i] = load_piece(a_rows[b][i], at, p.bytes);
+        }
+    };
+    auto const fragment = [&](int b, int at) { return *(v4u const *)(room + b * 4096 + l % 16 * 256 + (((uint32_t)at) ^ (l % 16)) * 16); };
+    auto const step = [&](auto slot, uint32_t c) {
+        constexpr int kSlot = decltype(slot)::value;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t const r = i * 4 + r4, to = r * 256 + (piece ^ r) * 16;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) *(v4u *)(room + b * 4096 + to) = w[kSlot][b][i];
+#pragma unroll
+            for (int b = 0; b < MB; ++b) *(v4u *)(room + (kBlocks + b) * 4096 + to) = a[kSlot][b][i];
+        }
+        uint32_t ws[kBlocks][2], as[MB][2];
+        if constexpr (kScaled) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) ws[b][s] = w_scale[kSlot][b][s];
+#pragma unroll
+                for (int b = 0; b < MB; ++b) as[b][s] = a_scale[kSlot][b][s];
+            }
+        }
+        if (c + 2 * WAVES < chunks) load(slot, c + 2 * WAVES);
+        wave_fence();
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            if constexpr (kScaled) { // of the 128 values at 128 s a lane has 16 of the first 64 and as many of the second
+                int const first = 8 * s + r4;
+                v4u x[kBlocks][2], y[MB][2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b) x[b][h] = fragment(b, first + 4 * h);
+#pragma unroll
+                    for (int b = 0; b < MB; ++b) y[b][h] = fragment(kBlocks + b, first + 4 * h);
+                }
+#pragma unroll
+                for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                    for (int j = 0; j < MB; ++j) sum[i][j] = multiply_16(x[i], y[j], sum[i][j], ws[i][s], as[j][s]);
+            } else {
+                v4u x[kBlocks], y[MB];
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) x[b] = fragment(b, 4 * s + r4);
+#pragma unroll
+                for (int b = 0; b < MB; ++b) y[b] = fragment(kBlocks + b, 4 * s + r4);
+#pragma unroll
+                for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                    for (int j = 0; j < MB; ++j) sum[i][j] = multiply_16<T>(x[i], y[j], sum[i][j]);
+            }
+        }
+        wave_fence();
+    };
+    if (wave < chunks) load(Number<0>(), wave);
+    if (wave + WAVES < chunks) load(Number<1>(), wave + WAVES);
+    for (uint32_t c = wave; c < chunks; c += 2 * WAVES) {
+        step(Number<0>(), c);
+        if (c + WAVES < chunks) step(Number<1>(), c + WAVES);
+    }
+
+    // sums of the wavefronts: [matrix][row][column], a lane has four columns of a row
+    constexpr uint32_t kPitch = 16 * NB + 4, kRoom = kMatrices * MB * 16 * kPitch;
+    static_assert(kRoom * 4 <= sizeof(rooms[0]), "sums have to fit the wavefront's room");
+    wave_fence();
+    float *const mine = (float *)room;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) *(v4f *)(mine + ((b / NB * MB + i) * 16 + l % 16) * kPitch + b % NB * 16 + r4 * 4) = sum[b][i];
+    __syncthreads();
+    for (uint32_t t = threadIdx.x; t < MB * 16 * NB * 2; t += 64 * WAVES) {
+        uint32_t const r = t / (NB * 2), c = t % (NB * 2) * 8;
+        if (r >= rows || col0 + c >= p.n) continue;
+        float v[8] = {}, q[8] = {};
+        for (int i = 0; i < WAVES; ++i) {
+            float const *const its = (float const *)rooms[i] + r * kPitch + c;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] += its[j];
+                if (GATED) q[j] += its[MB * 16 * kPitch + j];
+            }
+        }
+        finish_8<GATED>(p.e, row0 + r, col0 + c, p.n, v, q);
     }
 }
-template <class T>
-int launch_simple(SimpleArgs const &p, bool gated, hipStream_t stream) {
-    dim3 const grid((p.n + 63) / 64, (p.m + 63) / 64);
-    if (gated) hipLaunchKernelGGL((simple_kernel<T, true>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((simple_kernel<T, false>), grid, dim3(256), 0, stream, p);
-    hipError_t const e = hipGetLastError();
-    return e == hipSuccess ? 0 : mx_fail(e, "simple_kernel");
+template <class T, int MB, int NB, bool GATED, int WAVES>
+int launch_few(FewArgs p, hipStream_t stream) {
+    uint32_t const high = (p.m + 16 * MB - 1) / (16 * MB), blocks = (p.n + 16 * NB - 1) / (16 * NB);
+    uint64_t const most = kMostThreads / (64 * WAVES) / high; // blocks of a launch
+    for (uint64_t first = 0; first < blocks; first += most) {
+        p.first = (uint32_t)first;
+        hipLaunchKernelGGL((few_kernel<T, MB, NB, GATED, WAVES>), dim3((uint32_t)(blocks - first < most ? blocks - first : most), high), dim3(64 * WAVES), 0, stream, p);
+        hipError_t const e = hipGetLastError();
+        if (e != hipSuccess) return mx_fail(e, "few_kernel");
+    }
+    return 0;
 }
-int launch_simple(int dtype, SimpleArgs const &p, bool gated, hipStream_t stream) {
-    return dtype == nk_f16_k ? launch_simple<_Float16>(p, gated, stream) : launch_simple<__bf16>(p, gated, stream);
+template <class T>
+int launch_few_of(FewArgs const &p, bool gated, hipStream_t stream) {
+    if (p.m <= 16) return gated ? launch_few<T, 1, 1, true, 4>(p, stream) : launch_few<T, 1, 1, false, 8>(p, stream);
+    if (p.m <= 32) return gated ? launch_few<T, 2, 1, true, 4>(p, stream) : launch_few<T, 2, 1, false, 8>(p, stream);
+    return gated ? launch_few<T, 4, 1, true, 4>(p, stream) : launch_few<T, 4, 1, false, 4>(p, stream);
+}
+constexpr uint64_t kFewRows = 64;
+
+// ---- tiles ---------------------------------------------------------------------------------------------------------
+
+struct TilePlan {
+    int shape;
+    uint32_t splits, split_stages;
+};
+/** The shape of tiles and the splits of the depth that take the least time by a simple account, in cycles of a compute unit. */
+TilePlan tile_plan(uint64_t m, uint64_t n, uint64_t stages, bool gated) {
+    static constexpr double kStage[3] = {330, 750, 2300}, kEnds[3] = {2500, 3500, 9000}; // of a stage of a workgroup, of its beginning and end
+    uint64_t const units = (uint64_t)compute_unit_count();
+    TilePlan best = {0, 1, (uint32_t)stages};
+    double least = 1e300;
+    for (int shape = 0; shape < 3; ++shape) {
+        uint64_t const rows = 64u << shape, columns = gated ? (shape == 2 ? 128 : 64) : rows;
+        uint64_t const tiles = ((m + rows - 1) / rows) * ((n + columns - 1) / columns);
+        double const stage = gated && shape == 0 ? 500 : kStage[shape];
+        for (uint64_t splits = 1; splits <= 16; splits *= 2) {
+            if (splits > 1 && (stages < splits * 4 || tiles * splits > units * 4)) break;
+            uint64_t const each = (stages + splits - 1) / splits, even = splits > 1 ? up_to(each, 2) : each, there = stages ? (stages + even - 1) / even : 1;
+            uint64_t const rounds = (tiles * there + units - 1) / units;
+            double const joined = there > 1 ? 8000 + (double)m * n * (gated ? 2 : 1) * (there + 1) * 4 / 2500 : 0; // (a launch; 2500 bytes a cycle)
+            double const time = rounds * (stage * even + kEnds[shape]) + joined;
+            if (time < least) least = time, best = {shape, (uint32_t)there, (uint32_t)(stages ? even : 0)};
+        }
+    }
+    return best;
+}
+/** Are there more results than the tiles of one launch make? */
+bool too_many(TilePlan const &t, uint64_t m, uint64_t n, bool gated) {
+    uint64_t const rows = 64u << t.shape, columns = gated ? (t.shape == 2 ? 128 : 64) : rows;
+    return ((m + rows - 1) / rows) * ((n + columns - 1) / columns) * t.splits * 256 >= (1ull << 32);
+}
+uint64_t partial_bytes(TilePlan const &t, uint64_t m, uint64_t n, bool gated) { return t.splits > 1 ? up_to(t.splits * m * n * (gated ? 8 : 4), 256) : 0; }
+
+/** Queues the tiles of a product (extents, depths and operands are in `p`) and what joins their splits. */
+int launch_tiles(int dtype, TileForm form, TilePlan const &t, TileArgs p, float *partial, hipStream_t stream) {
+    form.shape = t.shape;
+    p.splits = t.splits, p.split_stages = t.split_stages, p.partial = partial;
+    uint32_t const rows = 64u << t.shape, columns = form.gated ? (t.shape == 2 ? 128 : 64) : rows;
+    p.tiles_m = (p.m + rows - 1) / rows, p.tiles_n = (p.n + columns - 1) / columns;
+    if (int const status = dtype == nk_bf16_k ? launch_tiles_bf16(form, p, stream) : dtype == nk_f16_k ? launch_tiles_f16(form, p, stream) : launch_tiles_mx8(form, p, stream)) return status;
+    if (t.splits == 1) return 0;
+    uint64_t const eights = (uint64_t)p.m * ((p.n + 7) / 8);
+    dim3 const grid((uint32_t)((eights + 255) / 256));
+    if (form.gated) hipLaunchKernelGGL(join_kernel<true>, grid, dim3(256), 0, stream, partial, p.splits, p.m, p.n, p.e);
+    else hipLaunchKernelGGL(join_kernel<false>, grid, dim3(256), 0, stream, partial, p.splits, p.m, p.n, p.e);
+    hipError_t const e = hipGetLastError();
+    return e == hipSuccess ? 0 : mx_fail(e, "join_kernel");
+}
+
+/** Can the tiles read these rows in place? `along`: the depth runs along them. */
+bool in_place(void const *values, uint64_t stride, uint64_t bytes, bool along) {
+    return !((uintptr_t)values & 3) && !(stride & 3) && stride <= kTileStride && (!along || bytes % 16 == 0);
 }
 
 // ---- the gradient of the sums --------------------------------------------------------------------------------------
@@ -170,7 +425,6 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs p) {
 }
 
 constexpr uint64_t kMaxDepth = 1ull << 22, kMaxRows = 1ull << 31;
-inline uint64_t up_to(uint64_t n, uint64_t step) { return (n + step - 1) / step * step; }
 
 // ---- what calls ask for --------------------------------------------------------------------------------------------
 
@@ -203,36 +457,86 @@ int check_workspace(char const *what, void const *workspace, uint64_t bytes, uin
     return needed && (!workspace || ((uintptr_t)workspace & 255) || bytes < needed) ? mx_fail(what) : 0;
 }
 
-/** Where a product's workspace has A's codes, if they are made on the way. */
+/** Where a product's workspace has what it makes of its operands. */
 struct LinearLayout {
-    uint64_t codes_stride, scales_stride, scales_at, bytes;
-    bool quantises;
+    bool few, quantises, moves_a, moves_w, moves_up; // A's codes are made; rows are moved to where the tiles can read them
+    uint64_t codes_stride, moved_stride;
+    uint64_t scales_stride, scales_at; // A's scales as bytes (few rows)
+    uint64_t a_pitch, w_pitch, a_words_at, w_words_at, up_words_at;
+    uint64_t a_at, w_at, up_at, partial_at, bytes;
+    uint64_t stages;
+    TilePlan tiles;
 };
 LinearLayout linear_layout(nk_amd_linear_t const *l) {
     LinearLayout y = {};
-    y.quantises = l->w_dtype == nk_e4m3_k && l->a_dtype != nk_e4m3_k && l->height && l->width && l->depth;
-    if (!y.quantises) return y;
-    y.codes_stride = up_to(l->depth, 128), y.scales_stride = y.codes_stride / 32;
-    y.scales_at = up_to(l->height * y.codes_stride, 256);
-    y.bytes = up_to(y.scales_at + l->height * y.scales_stride, 256);
-    return y;
+    if (!l->height || !l->width) return y;
+    bool const mx8 = l->w_dtype == nk_e4m3_k;
+    uint64_t const bytes = l->depth * (mx8 ? 1 : 2);
+    uint64_t end = 0;
+    auto const room = [&](uint64_t size) { uint64_t const at = end; return end += up_to(size, 256), at; };
+    y.quantises = mx8 && l->a_dtype != nk_e4m3_k && l->depth;
+    y.codes_stride = up_to(l->depth, 128), y.moved_stride = up_to(bytes, 128);
+    y.few = l->height <= kFewRows;
+    if (y.quantises) y.a_at = room(l->height * y.codes_stride);
+    if (y.few) {
+        y.scales_stride = y.codes_stride / 32;
+        if (y.quantises) y.scales_at = room(l->height * y.scales_stride);
+        return y.bytes = end, y;
+    }
+    y.stages = (bytes + 127) / 128;
+    y.moves_a = !y.quantises && bytes && !in_place(l->a, l->a_stride, bytes, true);
+    y.moves_w = bytes && !in_place(l->w, l->w_stride, bytes, true);
+    y.moves_up = l->gated && bytes && !in_place(l->w_up, l->w_up_stride, bytes, true);
+    if (y.moves_a) y.a_at = room(l->height * y.moved_stride);
+    if (y.moves_w) y.w_at = room(l->width * y.moved_stride);
+    if (y.moves_up) y.up_at = room(l->width * y.moved_stride);
+    if (mx8) {
+        y.a_pitch = up_to(l->height, 256), y.w_pitch = up_to(l->width, 256);
+        y.a_words_at = room(y.stages * y.a_pitch * 4), y.w_words_at = room(y.stages * y.w_pitch * 4);
+        if (l->gated) y.up_words_at = room(y.stages * y.w_pitch * 4);
+    }
+    y.tiles = tile_plan(l->height, l->width, y.stages, l->gated);
+    y.partial_at = room(partial_bytes(y.tiles, l->height, l->width, l->gated));
+    return y.bytes = end, y;
+}
+/** Queues the scales of `count` matrices as words. */
+int launch_scale_words(WordsArgs const &p, uint32_t count, hipStream_t stream) {
+    hipLaunchKernelGGL(scale_words_kernel, dim3(p.pitch / 32, (p.stages + 31) / 32, count), dim3(256), 0, stream, p);
+    hipError_t const e = hipGetLastError();
+    return e == hipSuccess ? 0 : mx_fail(e, "scale_words_kernel");
 }
 
-/** Where a backward pass's workspace has d (and e behind it in each row), and the sums of d. */
+/** Where a backward pass's workspace has d (and e behind it in each row), the sums of d, operands moved to where the tiles can read them, and splits. */
 struct BackwardLayout {
-    uint64_t padded, d_stride, partial_at, partials, rows_each, bytes;
-    bool writes_d, sums;
+    uint64_t padded, d_stride, column_sums_at, partials, rows_each, bytes;
+    bool writes_d, sums, moves_a, moves_w, moves_up;
+    uint64_t moved_stride, a_at, w_at, up_at, partial_at;
+    uint64_t stages, first_stages; // of the depth of A's gradient
+    TilePlan of_a, of_w;
 };
 BackwardLayout backward_layout(nk_amd_linear_backward_t const *l) {
     BackwardLayout y = {};
-    bool const gated = l->gated, products = l->grad_a || l->grad_w || l->grad_w_up;
-    y.writes_d = products && (gated || l->activation || l->grad_dtype != l->dtype);
+    uint64_t end = 0;
+    auto const room = [&](uint64_t size) { uint64_t const at = end; return end += up_to(size, 256), at; };
+    bool const gated = l->gated, some = l->height && l->width, of_a = l->grad_a && some && l->depth, of_w = (l->grad_w || l->grad_w_up) && some && l->depth;
+    y.writes_d = (of_a || of_w) && (gated || l->activation || l->grad_dtype != l->dtype || !in_place(l->grad, l->grad_stride, l->width * 2, true));
     y.sums = l->grad_bias != nullptr;
     y.padded = up_to(l->width, 64), y.d_stride = y.padded * 2 * (gated ? 2 : 1);
     y.rows_each = l->height <= 1u << 21 ? 64 : 128, y.partials = (l->height + y.rows_each - 1) / y.rows_each;
-    y.partial_at = y.writes_d ? up_to(l->height * y.d_stride, 256) : 0;
-    y.bytes = y.partial_at + (y.sums ? up_to(y.partials * l->width * 4, 256) : 0);
-    return y;
+    if (y.writes_d) room(l->height * y.d_stride); // (at 0)
+    if (y.sums) y.column_sums_at = room(y.partials * l->width * 4);
+    y.moved_stride = up_to(l->depth * 2, 128);
+    y.moves_a = of_w && !in_place(l->a, l->a_stride, 0, false);
+    y.moves_w = of_a && !in_place(l->w, l->w_stride, 0, false);
+    y.moves_up = gated && of_a && !in_place(l->w_up, l->w_up_stride, 0, false);
+    if (y.moves_a) y.a_at = room(l->height * y.moved_stride);
+    if (y.moves_w) y.w_at = room(l->width * y.moved_stride);
+    if (y.moves_up) y.up_at = room(l->width * y.moved_stride);
+    y.first_stages = y.padded / 64, y.stages = y.first_stages * (gated ? 2 : 1);
+    y.of_a = tile_plan(l->height, l->depth, y.stages, false), y.of_w = tile_plan(l->width, l->depth, (l->height + 63) / 64, false);
+    uint64_t const a_bytes = of_a ? partial_bytes(y.of_a, l->height, l->depth, false) : 0, w_bytes = of_w ? partial_bytes(y.of_w, l->width, l->depth, false) : 0;
+    y.partial_at = room(a_bytes > w_bytes ? a_bytes : w_bytes);
+    return y.bytes = end, y;
 }
 int check_backward(nk_amd_linear_backward_t const *l) {
     if (!l) return mx_fail("linear_backward: NULL operand");
@@ -258,27 +562,61 @@ nk_size_t nk_amd_linear_workspace_size(nk_amd_linear_t const *l) {
     return check_linear(l) ? 0 : linear_layout(l).bytes;
 }
 
-int nk_amd_linear_async(nk_amd_linear_t const *l, void *workspace, nk_size_t workspace_bytes, void *stream) {
+int nk_amd_linear_async(nk_amd_linear_t const *l, void *workspace, nk_size_t workspace_bytes, void *raw_stream) {
     if (int const status = check_linear(l)) return status;
     if (!l->height || !l->width) return 0;
     if (int const status = check_linear_operands(l)) return status;
     LinearLayout const y = linear_layout(l);
     if (check_workspace("linear: the workspace is too small or not 256-byte aligned", workspace, workspace_bytes, y.bytes)) return -1;
+    if (!y.few && too_many(y.tiles, l->height, l->width, l->gated)) return mx_fail("linear: more results than one launch makes");
     bool const mx8 = l->w_dtype == nk_e4m3_k, gated = l->gated;
-    uint64_t const bytes = mx8 ? 1 : 2;
-    SimpleArgs p = {};
-    p.m = (uint32_t)l->height, p.n = (uint32_t)l->width, p.k = (uint32_t)l->depth, p.pairs = 1;
-    p.a[0] = {(uint8_t const *)l->a, l->a_stride, bytes, (uint8_t const *)(mx8 ? l->a_scales : nullptr), l->a_scales_stride};
-    if (y.quantises) {
-        uint8_t *const codes = (uint8_t *)workspace, *const scales = codes + y.scales_at;
-        if (int const status = launch_mx8_quantize(kind_of(l->a_dtype), l->a, l->a_stride, l->height, l->depth, codes, y.codes_stride, scales, y.scales_stride, (hipStream_t)stream)) return status;
-        p.a[0] = {codes, y.codes_stride, bytes, scales, y.scales_stride};
+    hipStream_t const stream = (hipStream_t)raw_stream;
+    uint8_t *const room = (uint8_t *)workspace;
+    uint64_t const bytes = l->depth * (mx8 ? 1 : 2);
+    Epilogue const e = {l->bias, (uint8_t const *)l->residual, (uint8_t *)l->c, l->pre, l->pre_up, l->residual_stride, l->c_stride, l->pre_stride, kind_of(l->bias_dtype),
+                        kind_of(l->residual_dtype), kind_of(l->c_dtype), (uint32_t)l->activation};
+    if (y.quantises)
+        if (int const status = launch_mx8_quantize(kind_of(l->a_dtype), l->a, l->a_stride, l->height, l->depth, up_to(l->depth, 16), room + y.a_at, y.codes_stride, y.few ? room + y.scales_at : nullptr,
+                                                   y.scales_stride, y.few ? nullptr : (uint32_t *)(room + y.a_words_at), y.a_pitch, stream)) return status;
+    if (y.few) {
+        FewArgs p = {};
+        p.m = (uint32_t)l->height, p.n = (uint32_t)l->width, p.bytes = (uint32_t)bytes, p.e = e;
+        p.a = {(uint8_t const *)l->a, l->a_stride, (uint8_t const *)l->a_scales, l->a_scales_stride};
+        if (y.quantises) p.a = {room + y.a_at, y.codes_stride, room + y.scales_at, y.scales_stride};
+        p.b[0] = {(uint8_t const *)l->w, l->w_stride, (uint8_t const *)l->w_scales, l->w_scales_stride};
+        p.b[1] = {(uint8_t const *)l->w_up, l->w_up_stride, (uint8_t const *)l->w_up_scales, l->w_up_scales_stride};
+        return mx8 ? launch_few_of<Mx8>(p, gated, stream) : l->w_dtype == nk_f16_k ? launch_few_of<_Float16>(p, gated, stream) : launch_few_of<__bf16>(p, gated, stream);
     }
-    p.b[0] = {(uint8_t const *)l->w, l->w_stride, bytes, (uint8_t const *)(mx8 ? l->w_scales : nullptr), l->w_scales_stride};
-    p.b[1] = {(uint8_t const *)l->w_up, l->w_up_stride, bytes, (uint8_t const *)(mx8 ? l->w_up_scales : nullptr), l->w_up_scales_stride};
-    p.e = {l->bias, (uint8_t const *)l->residual, (uint8_t *)l->c, l->pre, l->pre_up, l->residual_stride, l->c_stride, l->pre_stride, kind_of(l->bias_dtype),
-           kind_of(l->residual_dtype), kind_of(l->c_dtype), (uint32_t)l->activation};
-    return launch_simple(l->w_dtype, p, gated, (hipStream_t)stream);
+    TileArgs p = {};
+    p.m = (uint32_t)l->height, p.n = (uint32_t)l->width, p.stages = p.first_stages = (uint32_t)y.stages, p.e = e;
+    uint32_t const k = (uint32_t)(up_to(bytes, 16) / (mx8 ? 1 : 2)); // (what is moved or quantised ends with zeros)
+    p.a.extent = p.m, p.b.extent = p.n, p.a.k = p.b.k = k;
+    p.a.pitch = (uint32_t)y.a_pitch, p.b.pitch = (uint32_t)y.w_pitch;
+    p.a.values[0] = (uint8_t const *)l->a, p.a.stride[0] = l->a_stride;
+    p.b.values[0] = (uint8_t const *)l->w, p.b.stride[0] = l->w_stride;
+    p.b.values[1] = (uint8_t const *)l->w_up, p.b.stride[1] = l->w_up_stride;
+    if (y.quantises) p.a.values[0] = room + y.a_at, p.a.stride[0] = y.codes_stride;
+    auto const move = [&](TileSide &side, int which, uint64_t rows, uint64_t at) {
+        int const status = launch_realign(side.values[which], side.stride[which], rows, bytes, room + at, y.moved_stride, stream);
+        side.values[which] = room + at, side.stride[which] = y.moved_stride;
+        return status;
+    };
+    if (y.moves_a)
+        if (int const status = move(p.a, 0, l->height, y.a_at)) return status;
+    if (y.moves_w)
+        if (int const status = move(p.b, 0, l->width, y.w_at)) return status;
+    if (y.moves_up)
+        if (int const status = move(p.b, 1, l->width, y.up_at)) return status;
+    if (mx8 && y.stages) {
+        p.a.scales[0] = (uint32_t *)(room + y.a_words_at), p.b.scales[0] = (uint32_t *)(room + y.w_words_at), p.b.scales[1] = (uint32_t *)(room + y.up_words_at);
+        uint32_t const blocks = (uint32_t)((l->depth + 31) / 32);
+        WordsArgs const of_w = {{(uint8_t const *)l->w_scales, (uint8_t const *)l->w_up_scales}, {l->w_scales_stride, l->w_up_scales_stride}, {(uint32_t *)p.b.scales[0], (uint32_t *)p.b.scales[1]}, p.n, blocks, p.stages, p.b.pitch};
+        if (int const status = launch_scale_words(of_w, gated ? 2 : 1, stream)) return status;
+        WordsArgs const of_a = {{(uint8_t const *)l->a_scales}, {l->a_scales_stride}, {(uint32_t *)p.a.scales[0]}, p.m, blocks, p.stages, p.a.pitch};
+        if (!y.quantises)
+            if (int const status = launch_scale_words(of_a, 1, stream)) return status;
+    }
+    return launch_tiles(l->w_dtype, {0, false, false, gated}, y.tiles, p, (float *)(room + y.partial_at), stream);
 }
 
 nk_size_t nk_amd_linear_backward_workspace_size(nk_amd_linear_backward_t const *l) {
@@ -301,10 +639,12 @@ int nk_amd_linear_backward_async(nk_amd_linear_backward_t const *l, void *worksp
     }
     BackwardLayout const y = backward_layout(l);
     if (check_workspace("linear_backward: the workspace is too small or not 256-byte aligned", workspace, workspace_bytes, y.bytes)) return -1;
+    if ((l->grad_a && too_many(y.of_a, l->height, l->depth, false)) || ((l->grad_w || l->grad_w_up) && too_many(y.of_w, l->width, l->depth, false)))
+        return mx_fail("linear_backward: more results than one launch makes");
     uint8_t *const d = (uint8_t *)workspace;
-    float *const partial = (float *)(d + y.partial_at);
+    float *const column_sums = (float *)(d + y.column_sums_at), *const partial = (float *)(d + y.partial_at);
     if (some && (y.writes_d || y.sums)) {
-        SlopeArgs const s = {(uint8_t const *)l->grad, gated || l->activation ? l->pre : nullptr, l->pre_up, y.writes_d ? d : nullptr, y.sums ? partial : nullptr, l->grad_stride,
+        SlopeArgs const s = {(uint8_t const *)l->grad, gated || l->activation ? l->pre : nullptr, l->pre_up, y.writes_d ? d : nullptr, y.sums ? column_sums : nullptr, l->grad_stride,
                              l->pre_stride, y.d_stride, (uint32_t)l->height, (uint32_t)l->width, (uint32_t)y.padded, (uint32_t)y.padded, kind_of(l->grad_dtype), (uint32_t)l->activation,
                              (uint32_t)y.rows_each, gated};
         dim3 const grid((uint32_t)((y.padded + 511) / 512), (uint32_t)y.partials);
@@ -314,26 +654,52 @@ int nk_amd_linear_backward_async(nk_amd_linear_backward_t const *l, void *worksp
         if (e != hipSuccess) return mx_fail(e, "slope_kernel");
     }
     if (y.sums && l->width)
-        if (int const status = launch_column_sum(partial, y.partials, l->width, kind_of(l->bias_dtype), l->grad_bias, stream)) return status;
+        if (int const status = launch_column_sum(column_sums, y.partials, l->width, kind_of(l->bias_dtype), l->grad_bias, stream)) return status;
     uint8_t const *const of_p = y.writes_d ? d : (uint8_t const *)l->grad, *const of_q = d + y.padded * 2;
     uint64_t const d_stride = y.writes_d ? y.d_stride : l->grad_stride;
     auto const kind = kind_of(l->dtype);
-    if (l->grad_a && l->height && l->depth) { // rows of d times columns of W
-        SimpleArgs p = {};
-        p.m = (uint32_t)l->height, p.n = (uint32_t)l->depth, p.k = (uint32_t)l->width, p.pairs = gated ? 2 : 1;
-        p.a[0] = {of_p, d_stride, 2, nullptr, 0}, p.a[1] = {of_q, d_stride, 2, nullptr, 0};
-        p.b[0] = {(uint8_t const *)l->w, 2, l->w_stride, nullptr, 0}, p.b[1] = {(uint8_t const *)l->w_up, 2, l->w_up_stride, nullptr, 0};
+    if (!some || !l->depth) { // gradients of empty sums
+        for (int i = 0; i < 3; ++i) {
+            uint64_t const rows = i ? l->width : l->height, stride = i == 0 ? l->grad_a_stride : i == 1 ? l->grad_w_stride : l->grad_w_up_stride;
+            void *const to = i == 0 ? l->grad_a : i == 1 ? l->grad_w : l->grad_w_up;
+            if (!to || !rows || !l->depth) continue;
+            FewArgs p = {}; // (no depth: zeros)
+            p.m = (uint32_t)rows, p.n = (uint32_t)l->depth;
+            p.e.c = (uint8_t *)to, p.e.c_stride = stride, p.e.c_kind = kind;
+            if (int const status = launch_few<__bf16, 4, 1, false, 4>(p, stream)) return status;
+        }
+        return 0;
+    }
+    uint8_t const *a = (uint8_t const *)l->a, *w[2] = {(uint8_t const *)l->w, (uint8_t const *)l->w_up};
+    uint64_t a_stride = l->a_stride, w_stride[2] = {l->w_stride, l->w_up_stride};
+    auto const move = [&](uint8_t const *&values, uint64_t &stride, uint64_t rows, uint64_t at) {
+        int const status = launch_realign(values, stride, rows, l->depth * 2, d + at, y.moved_stride, stream);
+        values = d + at, stride = y.moved_stride;
+        return status;
+    };
+    if (y.moves_a)
+        if (int const status = move(a, a_stride, l->height, y.a_at)) return status;
+    if (y.moves_w)
+        if (int const status = move(w[0], w_stride[0], l->width, y.w_at)) return status;
+    if (y.moves_up)
+        if (int const status = move(w[1], w_stride[1], l->width, y.up_at)) return status;
+    if (l->grad_a) { // rows of d times columns of W
+        TileArgs p = {};
+        p.m = (uint32_t)l->height, p.n = (uint32_t)l->depth, p.stages = (uint32_t)y.stages, p.first_stages = (uint32_t)y.first_stages;
+        p.a.values[0] = of_p, p.a.stride[0] = d_stride, p.a.extent = p.m, p.a.k = (uint32_t)(y.writes_d ? y.d_stride / 2 : l->width);
+        p.b = {{w[0], w[1]}, {w_stride[0], w_stride[1]}, {}, 0, p.n, (uint32_t)l->width};
         p.e.c = (uint8_t *)l->grad_a, p.e.c_stride = l->grad_a_stride, p.e.c_kind = kind;
-        if (int const status = launch_simple(l->dtype, p, false, stream)) return status;
+        if (int const status = launch_tiles(l->dtype, {0, false, true, false}, y.of_a, p, partial, stream)) return status;
     }
     for (int i = 0; i < 2; ++i) { // columns of d times columns of A
         void *const to = i ? l->grad_w_up : l->grad_w;
-        if (!to || !l->width || !l->depth) continue;
-        SimpleArgs p = {};
-        p.m = (uint32_t)l->width, p.n = (uint32_t)l->depth, p.k = (uint32_t)l->height, p.pairs = 1;
-        p.a[0] = {i ? of_q : of_p, 2, d_stride, nullptr, 0}, p.b[0] = {(uint8_t const *)l->a, 2, l->a_stride, nullptr, 0};
+        if (!to) continue;
+        TileArgs p = {};
+        p.m = (uint32_t)l->width, p.n = (uint32_t)l->depth, p.stages = p.first_stages = (uint32_t)((l->height + 63) / 64);
+        p.a = {{i ? of_q : of_p}, {d_stride}, {}, 0, p.m, (uint32_t)l->height};
+        p.b = {{a}, {a_stride}, {}, 0, p.n, (uint32_t)l->height};
         p.e.c = (uint8_t *)to, p.e.c_stride = i ? l->grad_w_up_stride : l->grad_w_stride, p.e.c_kind = kind;
-        if (int const status = launch_simple(l->dtype, p, false, stream)) return status;
+        if (int const status = launch_tiles(l->dtype, {0, true, true, false}, y.of_w, p, partial, stream)) return status;
     }
     return 0;
 }
