@@ -402,10 +402,16 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs p) {
             load_8(p.grad_kind, p.grad + row * p.grad_stride, col, p.n, g);
             if (p.pre) load_8((float const *)((uint8_t const *)p.pre + row * p.pre_stride), col, p.n, x);
             if (p.gated) load_8((float const *)((uint8_t const *)p.pre_up + row * p.pre_stride), col, p.n, up);
+            if (p.gated) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) e[j] = x[j];
+                activate_8(p.activation, e);
+            }
+            if (p.pre) slope_8(p.activation, x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                d[j] = p.pre ? g[j] * slope(p.activation, x[j]) : g[j];
-                if (p.gated) d[j] *= up[j], e[j] = g[j] * activate(p.activation, x[j]);
+                d[j] = p.pre ? g[j] * x[j] : g[j];
+                if (p.gated) d[j] *= up[j], e[j] *= g[j];
                 sum[j] += d[j];
             }
             if (p.d) {

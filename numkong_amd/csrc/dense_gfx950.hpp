@@ -110,37 +110,90 @@ __device__ __forceinline__ float scale_of(uint32_t byte) {
 }
 
 /**
- *  Activations and their slopes, in 32 bits. Silu is x / (1 + e^-x): where e^-x overflows x is below -88 and the result rounds to -0.
- *  The tanh of gelu_tanh is written as 1 - 2 / (1 + e^2z), so 0.5 x (1 + tanh z) = x - x / (1 + e^2z), without cancellation
- *  that a negative z would bring.
+ *  Activations and their slopes in 32 bits, off by a few units in the last place. The sigmoid is 1 / (1 + e^-x) by the part's own 2^x and reciprocal
+ *  (one unit each; the library's forms cost three times the instructions, and tiles would wait for them: f16 8192 x 8191 x 1000 with relu in a
+ *  switch for each value and these took 60 us more). The tanh of gelu_tanh is written as 1 - 2 / (1 + e^2z), so that 0.5 x (1 + tanh z) = x / (1 + e^-2z).
+ *  Gelu: with h = erfc(|x| / sqrt 2) / 2 it is x - x h, or x h below zero, and h = e^(-x^2/2) t P(t), t = 1 / (1 + 0.35 |x|): P is fitted
+ *  to that quotient over all |x| <= 16 by least squares weighted towards the largest relative error (8 degrees, 5 units of 2^-24 with its
+ *  evaluation). What is beyond +-16 (+-110 for slopes) is at its limit.
  */
-__device__ __forceinline__ float activate(uint32_t kind, float x) {
+__device__ __forceinline__ float power_of_2(float x) {
+#ifdef NK_MX_DEVICE_BUILTINS
+    return __builtin_amdgcn_exp2f(x);
+#else
+    return x;
+#endif
+}
+__device__ __forceinline__ float reciprocal(float x) {
+#ifdef NK_MX_DEVICE_BUILTINS
+    return __builtin_amdgcn_rcpf(x);
+#else
+    return x;
+#endif
+}
+constexpr float kLog2E = 1.4426950408889634f;
+/** erfc(|x| / sqrt 2) / 2 and e^(-x^2/2), |x| <= 16. */
+__device__ __forceinline__ float half_erfc(float x, float &bell) {
+    float const square = x * x, rest = __builtin_fmaf(x, x, -square);
+    float const power = square * (-0.5f * kLog2E); // (its rounding, and those of the square and the constant, would be 18 units at x = 5)
+    float const lost = __builtin_fmaf(square, -0.5f * kLog2E, -power) + __builtin_fmaf(rest, -0.5f * kLog2E, square * -9.6298e-9f);
+    bell = power_of_2(power);
+    bell = __builtin_fmaf(bell, lost * 0.69314718f, bell);
+    float const t = reciprocal(__builtin_fmaf(0.35f, fabsf(x), 1.0f));
+    float h = -0.0291648954f;
+    h = __builtin_fmaf(h, t, 0.144065633f), h = __builtin_fmaf(h, t, -0.255912066f), h = __builtin_fmaf(h, t, 0.159404889f), h = __builtin_fmaf(h, t, -0.0232723057f);
+    h = __builtin_fmaf(h, t, 0.105578497f), h = __builtin_fmaf(h, t, 0.11981453f), h = __builtin_fmaf(h, t, 0.139864475f), h = __builtin_fmaf(h, t, 0.139621243f);
+    return h * t * bell;
+}
+/** e^-z of gelu_tanh's sigmoid. */
+__device__ __forceinline__ float gelu_tanh_power(float x) { return power_of_2(x * __builtin_fmaf(x * x, -0.044715f * 1.5957691216057308f * kLog2E, -1.5957691216057308f * kLog2E)); }
+__device__ __forceinline__ float within(float x, float limit) { return x > limit ? limit : x < -limit ? -limit : x; } // (NaN stays)
+
+__device__ __forceinline__ float relu(float x) { return x < 0 ? 0.0f : x; }
+__device__ __forceinline__ float silu(float x) { return x < -128.0f ? -0.0f : x * reciprocal(1.0f + power_of_2(x * -kLog2E)); }
+__device__ __forceinline__ float gelu(float x) {
+    float bell;
+    float const near = within(x, 16.0f);
+    return relu(x) - fabsf(near) * half_erfc(near, bell);
+}
+__device__ __forceinline__ float gelu_tanh(float x) { return x < -128.0f ? -0.0f : x * reciprocal(1.0f + gelu_tanh_power(x)); }
+
+__device__ __forceinline__ float relu_slope(float x) { return x > 0 ? 1.0f : 0.0f; }
+__device__ __forceinline__ float silu_slope(float x) {
+    float const e = power_of_2(within(x, 80.0f) * -kLog2E), s = reciprocal(1.0f + e);
+    return fabsf(x) > 80.0f ? relu_slope(x) : __builtin_fmaf(x * e * s, s, s);
+}
+__device__ __forceinline__ float gelu_slope(float x) {
+    float bell;
+    float const near = within(x, 16.0f), h = half_erfc(near, bell);
+    return __builtin_fmaf(near * 0.39894228040143268f, bell, x < 0 ? h : 1.0f - h);
+}
+__device__ __forceinline__ float gelu_tanh_slope(float x) {
+    float const near = within(x, 9.0f), e = gelu_tanh_power(near), s = reciprocal(1.0f + e);
+    float const bend = near * __builtin_fmaf(near * near, 0.134145f * 1.5957691216057308f, 1.5957691216057308f);
+    return fabsf(x) > 9.0f ? relu_slope(x) : __builtin_fmaf(bend * e * s, s, s);
+}
+/** Eight values at once: one branch, which all lanes take alike. */
+__device__ __forceinline__ void activate_8(uint32_t kind, float (&x)[8]) {
+#define NK_EACH(f)                                                                                                                                             \
+    _Pragma("unroll") for (int i = 0; i < 8; ++i) x[i] = f(x[i]);                                                                                               \
+    break
     switch (kind) {
-    case nk_amd_relu: return x > 0 ? x : x != x ? x : 0.0f;
-    case nk_amd_silu: return x == -__builtin_inff() ? -0.0f : x / (1.0f + expf(-x));
-    case nk_amd_gelu: return x == -__builtin_inff() ? -0.0f : 0.5f * x * erfcf(-0.70710678118654752f * x);
-    case nk_amd_gelu_tanh: {
-        float const z = 1.5957691216057308f * (x + 0.044715f * x * x * x); // twice the argument of tanh
-        return x == -__builtin_inff() ? -0.0f : x / (1.0f + expf(-z));
-    }
-    default: return x;
+    case nk_amd_relu: NK_EACH(relu);
+    case nk_amd_silu: NK_EACH(silu);
+    case nk_amd_gelu: NK_EACH(gelu);
+    case nk_amd_gelu_tanh: NK_EACH(gelu_tanh);
     }
 }
-__device__ __forceinline__ float slope(uint32_t kind, float x) {
-    if (fabsf(x) > 110.0f) return kind && x < 0 ? 0.0f : 1.0f; // (the limits, which infinities and overflows would miss)
+__device__ __forceinline__ void slope_8(uint32_t kind, float (&x)[8]) {
     switch (kind) {
-    case nk_amd_relu: return x > 0 ? 1.0f : 0.0f;
-    case nk_amd_silu: {
-        float const s = 1.0f / (1.0f + expf(-x));
-        return s + s * (x * (1.0f - s));
+    case nk_amd_no_activation: NK_EACH([](float) { return 1.0f; });
+    case nk_amd_relu: NK_EACH(relu_slope);
+    case nk_amd_silu: NK_EACH(silu_slope);
+    case nk_amd_gelu: NK_EACH(gelu_slope);
+    case nk_amd_gelu_tanh: NK_EACH(gelu_tanh_slope);
     }
-    case nk_amd_gelu: return 0.5f * erfcf(-0.70710678118654752f * x) + x * (0.39894228040143268f * expf(-0.5f * x * x));
-    case nk_amd_gelu_tanh: {
-        float const z = 1.5957691216057308f * (x + 0.044715f * x * x * x), s = 1.0f / (1.0f + expf(-z));
-        return s + s * (x * (1.0f - s)) * (1.5957691216057308f * (1.0f + 0.134145f * x * x));
-    }
-    default: return 1.0f;
-    }
+#undef NK_EACH
 }
 
 } // namespace nk_gfx950

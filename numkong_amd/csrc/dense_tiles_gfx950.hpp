@@ -187,13 +187,11 @@ struct Bringer {
     }
 };
 
-/** Eight adjacent results of a row from their sums; `q`: gated, the other product's. */
+/** Eight adjacent results of a row from their sums; `q`: gated, the other product's; `bias` and `r` are looked at only where there are such. */
 template <bool GATED>
-__device__ __forceinline__ void finish_8(Epilogue const &e, uint64_t row, uint32_t col, uint32_t n, float (&p)[8], float const (&q)[8]) {
+__device__ __forceinline__ void finish_8(Epilogue const &e, uint64_t row, uint32_t col, uint32_t n, float (&p)[8], float const (&q)[8], float const (&bias)[8], float const (&r)[8]) {
     uint32_t const count = n - col;
-    if (e.bias) {
-        float bias[8];
-        load_8(e.bias_kind, e.bias, col, n, bias);
+    if (!GATED && e.bias) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] += bias[i];
     }
@@ -201,21 +199,24 @@ __device__ __forceinline__ void finish_8(Epilogue const &e, uint64_t row, uint32
         store_some((float *)((uint8_t *)e.pre + row * e.pre_stride) + col, p, count);
         if (GATED) store_some((float *)((uint8_t *)e.pre_up + row * e.pre_stride) + col, q, count);
     }
-    if (e.activation) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = activate(e.activation, p[i]);
-    }
+    activate_8(e.activation, p);
     if constexpr (GATED) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] *= q[i];
     }
-    if (e.residual) {
-        float r[8];
-        load_8(e.residual_kind, e.residual + row * e.residual_stride, col, n, r);
+    if (!GATED && e.residual) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] += r[i];
     }
     store_8(e.c_kind, e.c + row * e.c_stride, col, p, count);
+}
+/** The same, with what it needs of the bias and the residual. */
+template <bool GATED>
+__device__ __forceinline__ void finish_8(Epilogue const &e, uint64_t row, uint32_t col, uint32_t n, float (&p)[8], float const (&q)[8]) {
+    float bias[8], r[8];
+    if (!GATED && e.bias) load_8(e.bias_kind, e.bias, col, n, bias);
+    if (!GATED && e.residual) load_8(e.residual_kind, e.residual + row * e.residual_stride, col, n, r);
+    finish_8<GATED>(e, row, col, n, p, q, bias, r);
 }
 
 /** Nothing that reads or writes LDS moves across; what this wavefront has begun to load into LDS, and read from it, is there. */
@@ -293,6 +294,21 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void tile_kernel(TileArgs
                 else sum[i][j] = multiply_32<T>(y[kFrom][j][0], x[kFrom][i][0], sum[i][j]);
             }
     };
+    // The instructions of a step in turn, reads (and what brings the next stage) between the products: left to itself, the compiler puts each read
+    // right before the product that waits for it.
+    auto const in_turn = [&](auto brings) {
+#ifdef NK_MX_DEVICE_BUILTINS
+        constexpr int kReads = kParts * (WM * (A_COLUMNS ? 2 : 1) + WN * (B_COLUMNS ? 2 : 1)), kLoads = decltype(brings)::value ? A::kLoads + B::kLoads : 0;
+        constexpr int kAll = kReads | kLoads | WM * WN, kTurns = kAll % 8 == 0 ? 8 : kAll % 4 == 0 ? 4 : kAll % 2 == 0 ? 2 : 1; // (divides all three)
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, kReads / kTurns, 0);
+            if constexpr (kLoads > 0) __builtin_amdgcn_sched_group_barrier(0x10, kLoads / kTurns, 0);
+            __builtin_amdgcn_sched_group_barrier(0x8, WM * WN / kTurns, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#endif
+    };
     auto const stage = [&](uint8_t *at_a, uint8_t *at_b, uint8_t *next_a, uint8_t *next_b, uint32_t s, auto slot) {
         if constexpr (kScaled) { // (a step's two blocks are bytes 0 and 1, then 2 and 3; the lane's half of the wavefront says which of the two)
             constexpr int kSlot = decltype(slot)::value;
@@ -303,16 +319,20 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void tile_kernel(TileArgs
         }
         read(1, at_a, at_b, 1);
         multiply(Number<0>());
+        in_turn(Number<0>());
         if constexpr (kSteps == 4) {
             read(0, at_a, at_b, 2);
             multiply(Number<1>());
+            in_turn(Number<0>());
             read(1, at_a, at_b, 3);
             multiply(Number<0>());
+            in_turn(Number<0>());
         }
         arrive_and_meet();
-        bring(at_a, at_b, s + 2, slot);
         read(0, next_a, next_b, 0);
+        bring(at_a, at_b, s + 2, slot);
         multiply(Number<1>());
+        in_turn(Number<1>());
     };
 
     if (begin < end) {
@@ -326,42 +346,67 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void tile_kernel(TileArgs
         }
     }
 
-    // 32 rows at a time through LDS, each wavefront in an array of its own: piece p (four results) of row r at p ^ r
+    // 64 rows at a time (32, if there are no more) through LDS, each wavefront in an array of its own: piece p (four results) of row r at p ^ r.
+    // A lane has the same columns in all of them; four rows' residuals are asked for before the first is needed.
     __syncthreads();
+    constexpr int kHigh = WM < 2 ? WM : 2;
     constexpr uint32_t kWidth = WN * 32, kPieces = kWidth / 4;
     float *const room = (float *)(wave == 0 ? a0 : wave == 1 ? a1 : wave == 2 ? b0 : b1);
     constexpr uint32_t kOut = GATED ? kWidth / 2 : kWidth, kLanes = kOut / 8; // results of a row, lanes that finish them
-#pragma unroll
-    for (int i = 0; i < WM; ++i) {
-        if (row0 + a_begin + i * 32 >= p.m) break;
+    constexpr uint32_t kTurns = kHigh * kLanes / 2, kAhead = kTurns < 4 ? kTurns : 4;
+    uint32_t const c = l % kLanes * 8, col = col0 + (GATED ? b_begin / 2 : b_begin) + c, piece = (GATED ? c / 32 * 64 + c % 32 : c) / 4;
+    bool const last = p.splits == 1;
+    float bias[8];
+    if (!GATED && last && p.e.bias && col < p.n) load_8(p.e.bias_kind, p.e.bias, col, p.n, bias);
+    auto const put = [&](int i, auto from) {
+        constexpr int kFrom = decltype(from)::value;
         uint32_t const r = l % 32;
 #pragma unroll
         for (int j = 0; j < WN; ++j)
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-                *(v4f *)(room + r * kWidth + ((j * 8 + t * 2 + l / 32) ^ (r % kPieces)) * 4) = v4f {sum[i][j][4 * t], sum[i][j][4 * t + 1], sum[i][j][4 * t + 2], sum[i][j][4 * t + 3]};
+                *(v4f *)(room + (i * 32 + r) * kWidth + ((j * 8 + t * 2 + l / 32) ^ (r % kPieces)) * 4) =
+                    v4f {sum[kFrom][j][4 * t], sum[kFrom][j][4 * t + 1], sum[kFrom][j][4 * t + 2], sum[kFrom][j][4 * t + 3]};
+    };
+#pragma unroll 1
+    for (uint32_t part = 0; part < WM / kHigh; ++part) {
+        uint32_t const first = row0 + a_begin + part * kHigh * 32;
+        if (first >= p.m) break;
+        if (part == 0) {
+            put(0, Number<0>());
+            if constexpr (kHigh > 1) put(1, Number<1>());
+        } else if constexpr (WM > 2) put(0, Number<2>()), put(1, Number<3>());
         wave_fence();
 #pragma unroll 1
-        for (uint32_t turn = 0; turn < kLanes / 2; ++turn) {
-            uint32_t const r = turn * (64 / kLanes) + l / kLanes, c = l % kLanes * 8;
-            uint32_t const row = row0 + a_begin + i * 32 + r, col = col0 + (GATED ? b_begin / 2 : b_begin) + c;
-            uint32_t const piece = (GATED ? c / 32 * 64 + c % 32 : c) / 4;
-            float v[8], q[8] = {};
+        for (uint32_t turn = 0; turn < kTurns; turn += kAhead) {
+            float rest[kAhead][8];
+            if (!GATED && last && p.e.residual) {
 #pragma unroll
-            for (uint32_t t = 0; t < 2; ++t) {
-                v4f const four = *(v4f const *)(room + r * kWidth + ((piece + t) ^ (r % kPieces)) * 4);
-                v[4 * t] = four[0], v[4 * t + 1] = four[1], v[4 * t + 2] = four[2], v[4 * t + 3] = four[3];
-                if constexpr (GATED) {
-                    v4f const its = *(v4f const *)(room + r * kWidth + ((piece + 8 + t) ^ (r % kPieces)) * 4);
-                    q[4 * t] = its[0], q[4 * t + 1] = its[1], q[4 * t + 2] = its[2], q[4 * t + 3] = its[3];
+                for (uint32_t i = 0; i < kAhead; ++i) {
+                    uint32_t const row = first + (turn + i) * (64 / kLanes) + l / kLanes;
+                    if (row < p.m && col < p.n) load_8(p.e.residual_kind, p.e.residual + row * p.e.residual_stride, col, p.n, rest[i]);
                 }
             }
-            if (row >= p.m || col >= p.n) continue;
-            if (p.splits > 1) {
-                float *const to = p.partial + ((uint64_t)split * (GATED ? 2 : 1) * p.m + row) * p.n + col;
-                store_some(to, v, p.n - col);
-                if (GATED) store_some(to + (uint64_t)p.m * p.n, q, p.n - col);
-            } else finish_8<GATED>(p.e, row, col, p.n, v, q);
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; ++i) {
+                uint32_t const r = (turn + i) * (64 / kLanes) + l / kLanes, row = first + r;
+                float v[8], q[8] = {};
+#pragma unroll
+                for (uint32_t t = 0; t < 2; ++t) {
+                    v4f const four = *(v4f const *)(room + r * kWidth + ((piece + t) ^ (r % kPieces)) * 4);
+                    v[4 * t] = four[0], v[4 * t + 1] = four[1], v[4 * t + 2] = four[2], v[4 * t + 3] = four[3];
+                    if constexpr (GATED) {
+                        v4f const its = *(v4f const *)(room + r * kWidth + ((piece + 8 + t) ^ (r % kPieces)) * 4);
+                        q[4 * t] = its[0], q[4 * t + 1] = its[1], q[4 * t + 2] = its[2], q[4 * t + 3] = its[3];
+                    }
+                }
+                if (row >= p.m || col >= p.n) continue;
+                if (!last) {
+                    float *const to = p.partial + ((uint64_t)split * (GATED ? 2 : 1) * p.m + row) * p.n + col;
+                    store_some(to, v, p.n - col);
+                    if (GATED) store_some(to + (uint64_t)p.m * p.n, q, p.n - col);
+                } else finish_8<GATED>(p.e, row, col, p.n, v, q, bias, rest[i]);
+            }
         }
         wave_fence();
     }
