@@ -89,19 +89,19 @@ __global__ __launch_bounds__(256) void join_kernel(float const *partial, uint32_
     uint64_t const at = (uint64_t)blockIdx.x * 256 + threadIdx.x, row = at / each, plane = (uint64_t)m * n;
     if (row >= m) return;
     uint32_t const col = (uint32_t)(at - row * each) * 8;
-    float v[8] = {}, q[8] = {};
+    float v[1][8] = {}, q[1][8] = {};
     for (uint32_t i = 0; i < splits; ++i) {
         float part[8];
-        load_8(partial + i * plane * (GATED ? 2 : 1) + row * n, col, n, part);
+        load_adjacent(partial + i * plane * (GATED ? 2 : 1) + row * n, col, n, part);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += part[j];
+        for (int j = 0; j < 8; ++j) v[0][j] += part[j];
         if constexpr (GATED) {
-            load_8(partial + (2 * i + 1) * plane + row * n, col, n, part);
+            load_adjacent(partial + (2 * i + 1) * plane + row * n, col, n, part);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] += part[j];
+            for (int j = 0; j < 8; ++j) q[0][j] += part[j];
         }
     }
-    finish_8<GATED>(e, row, col, n, v, q);
+    finish<GATED>(e, (uint32_t)row, m, col, n, v, q);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------
@@ -290,16 +290,16 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(FewArgs p) {
     for (uint32_t t = threadIdx.x; t < MB * 16 * NB * 2; t += 64 * WAVES) {
         uint32_t const r = t / (NB * 2), c = t % (NB * 2) * 8;
         if (r >= rows || col0 + c >= p.n) continue;
-        float v[8] = {}, q[8] = {};
+        float v[1][8] = {}, q[1][8] = {};
         for (int i = 0; i < WAVES; ++i) {
             float const *const its = (float const *)rooms[i] + r * kPitch + c;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                v[j] += its[j];
-                if (GATED) q[j] += its[MB * 16 * kPitch + j];
+                v[0][j] += its[j];
+                if (GATED) q[0][j] += its[MB * 16 * kPitch + j];
             }
         }
-        finish_8<GATED>(p.e, row0 + r, col0 + c, p.n, v, q);
+        finish<GATED>(p.e, row0 + r, p.m, col0 + c, p.n, v, q);
     }
 }
 template <class T, int MB, int NB, bool GATED, int WAVES>
@@ -317,10 +317,9 @@ int launch_few(FewArgs p, hipStream_t stream) {
 template <class T>
 int launch_few_of(FewArgs const &p, bool gated, hipStream_t stream) {
     if (p.m <= 16) return gated ? launch_few<T, 1, 1, true, 4>(p, stream) : launch_few<T, 1, 1, false, 8>(p, stream);
-    if (p.m <= 32) return gated ? launch_few<T, 2, 1, true, 4>(p, stream) : launch_few<T, 2, 1, false, 8>(p, stream);
-    return gated ? launch_few<T, 4, 1, true, 4>(p, stream) : launch_few<T, 4, 1, false, 4>(p, stream);
+    return gated ? launch_few<T, 2, 1, true, 4>(p, stream) : launch_few<T, 2, 1, false, 8>(p, stream);
 }
-constexpr uint64_t kFewRows = 64;
+constexpr uint64_t kFewRows = 32; // (48 x 8192 x 8192 bf16 took 76 us in such a kernel; tiles take 64 rows in 28)
 
 // ---- tiles ---------------------------------------------------------------------------------------------------------
 
@@ -328,23 +327,30 @@ struct TilePlan {
     int shape;
     uint32_t splits, split_stages;
 };
-/** The shape of tiles and the splits of the depth that take the least time by a simple account, in cycles of a compute unit. */
+/**
+ *  The shape of tiles and the splits of the depth that take the least time by a simple account, in microseconds of a compute unit, from what was
+ *  measured with bf16: a stage of a workgroup that is alone (512 x 4096 x 4096 and 64 x 8192 x 8192), one among as many as fit (8192 x 8192 by depths of 64 to
+ *  4096), what a tile's beginning and end add, and a launch and the partial sums' way through memory where there are splits. It is within a
+ *  sixth of the times of ten products between 64 x 8192 x 8192 and 4096 x 4096 x 1024.
+ */
 TilePlan tile_plan(uint64_t m, uint64_t n, uint64_t stages, bool gated) {
-    static constexpr double kStage[3] = {330, 750, 2300}, kEnds[3] = {2500, 3500, 9000}; // of a stage of a workgroup, of its beginning and end
+    static constexpr double kAlone[3] = {0.45, 0.57, 1.48}, kEach[3] = {0.173, 0.442, 1.48}, kEnds[3] = {0.8, 2.5, 13.5};
+    static constexpr uint64_t kResident[3] = {4, 2, 1};
     uint64_t const units = (uint64_t)compute_unit_count();
     TilePlan best = {0, 1, (uint32_t)stages};
     double least = 1e300;
     for (int shape = 0; shape < 3; ++shape) {
         uint64_t const rows = 64u << shape, columns = gated ? (shape == 2 ? 128 : 64) : rows;
         uint64_t const tiles = ((m + rows - 1) / rows) * ((n + columns - 1) / columns);
-        double const stage = gated && shape == 0 ? 500 : kStage[shape];
+        double const each = gated && shape == 0 ? 0.3 : kEach[shape];
+        auto const together = [&](uint64_t workgroups) { return workgroups * each > kAlone[shape] ? workgroups * each : workgroups ? kAlone[shape] : 0.0; };
         for (uint64_t splits = 1; splits <= 16; splits *= 2) {
             if (splits > 1 && (stages < splits * 4 || tiles * splits > units * 4)) break;
-            uint64_t const each = (stages + splits - 1) / splits, even = splits > 1 ? up_to(each, 2) : each, there = stages ? (stages + even - 1) / even : 1;
-            uint64_t const rounds = (tiles * there + units - 1) / units;
-            double const joined = there > 1 ? 8000 + (double)m * n * (gated ? 2 : 1) * (there + 1) * 4 / 2500 : 0; // (a launch; 2500 bytes a cycle)
-            double const time = rounds * (stage * even + kEnds[shape]) + joined;
-            if (time < least) least = time, best = {shape, (uint32_t)there, (uint32_t)(stages ? even : 0)};
+            uint64_t const some = (stages + splits - 1) / splits, its = splits > 1 ? up_to(some, 2) : some, there = stages ? (stages + its - 1) / its : 1;
+            uint64_t const on_unit = (tiles * there + units - 1) / units;
+            double const joined = there > 1 ? 4 + (double)m * n * (gated ? 2 : 1) * (there + 1) * 4 / 3e6 : 0;
+            double const time = its * (on_unit / kResident[shape] * together(kResident[shape]) + together(on_unit % kResident[shape])) + on_unit * kEnds[shape] + joined;
+            if (time < least) least = time, best = {shape, (uint32_t)there, (uint32_t)its};
         }
     }
     return best;
@@ -398,26 +404,26 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs p) {
         for (uint32_t i = threadIdx.x >> 6; i < p.rows_each; i += 4) {
             uint64_t const row = (uint64_t)blockIdx.y * p.rows_each + i;
             if (row >= p.m) break;
-            float g[8], x[8], up[8], d[8], e[8];
-            load_8(p.grad_kind, p.grad + row * p.grad_stride, col, p.n, g);
-            if (p.pre) load_8((float const *)((uint8_t const *)p.pre + row * p.pre_stride), col, p.n, x);
-            if (p.gated) load_8((float const *)((uint8_t const *)p.pre_up + row * p.pre_stride), col, p.n, up);
+            float g[8], x[1][8], up[8], d[8], e[1][8];
+            load_adjacent(p.grad_kind, p.grad + row * p.grad_stride, col, p.n, g);
+            if (p.pre) load_adjacent((float const *)((uint8_t const *)p.pre + row * p.pre_stride), col, p.n, x[0]);
             if (p.gated) {
+                load_adjacent((float const *)((uint8_t const *)p.pre_up + row * p.pre_stride), col, p.n, up);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] = x[j];
-                activate_8(p.activation, e);
+                for (int j = 0; j < 8; ++j) e[0][j] = x[0][j];
+                activate(p.activation, e);
             }
-            if (p.pre) slope_8(p.activation, x);
+            if (p.pre) slope(p.activation, x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                d[j] = p.pre ? g[j] * x[j] : g[j];
-                if (p.gated) d[j] *= up[j], e[j] *= g[j];
+                d[j] = p.pre ? g[j] * x[0][j] : g[j];
+                if (p.gated) d[j] *= up[j], e[0][j] *= g[j];
                 sum[j] += d[j];
             }
             if (p.d) {
                 T *const to = (T *)(p.d + row * p.d_stride) + col;
                 store_some(to, d, p.padded - col);
-                if (p.gated) store_some(to + p.up_at, e, p.padded - col);
+                if (p.gated) store_some(to + p.up_at, e[0], p.padded - col);
             }
         }
     if (!p.partial) return;
@@ -672,7 +678,7 @@ int nk_amd_linear_backward_async(nk_amd_linear_backward_t const *l, void *worksp
             FewArgs p = {}; // (no depth: zeros)
             p.m = (uint32_t)rows, p.n = (uint32_t)l->depth;
             p.e.c = (uint8_t *)to, p.e.c_stride = stride, p.e.c_kind = kind;
-            if (int const status = launch_few<__bf16, 4, 1, false, 4>(p, stream)) return status;
+            if (int const status = launch_few<__bf16, 2, 1, false, 8>(p, stream)) return status;
         }
         return 0;
     }

@@ -21,7 +21,7 @@ __host__ __device__ inline uint32_t bytes_of(uint32_t kind) { return kind == kF3
 
 /** Eight adjacent values of a row from column `col` on; zeros from column `k` on. */
 template <class T>
-__device__ __forceinline__ void load_8(T const *row, uint32_t col, uint32_t k, float (&v)[8]) {
+__device__ __forceinline__ void load_adjacent(T const *row, uint32_t col, uint32_t k, float (&v)[8]) {
     if (col + 8 <= k) {
         if constexpr (sizeof(T) == 4) {
             v4u const low = *(v4u_anywhere const *)(row + col), high = *(v4u_anywhere const *)(row + col + 4);
@@ -33,10 +33,32 @@ __device__ __forceinline__ void load_8(T const *row, uint32_t col, uint32_t k, f
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = col + i < k ? (float)row[col + i] : 0.0f;
 }
-__device__ __forceinline__ void load_8(uint32_t kind, void const *row, uint32_t col, uint32_t k, float (&v)[8]) {
-    if (kind == kF32) load_8((float const *)row, col, k, v);
-    else if (kind == kBF16) load_8((__bf16 const *)row, col, k, v);
-    else load_8((_Float16 const *)row, col, k, v);
+/** Four likewise. */
+template <class T>
+__device__ __forceinline__ void load_adjacent(T const *row, uint32_t col, uint32_t k, float (&v)[4]) {
+    if (col + 4 <= k) {
+        if constexpr (sizeof(T) == 4) {
+            v4u const words = *(v4u_anywhere const *)(row + col);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(words[i]);
+        } else {
+            typedef v2u __attribute__((aligned(1))) v2u_anywhere;
+            v2u const words = *(v2u_anywhere const *)(row + col);
+            float both[8];
+            widen<T>(v4u {words[0], words[1], 0, 0}, both);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = both[i];
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = col + i < k ? (float)row[col + i] : 0.0f;
+}
+template <int V>
+__device__ __forceinline__ void load_adjacent(uint32_t kind, void const *row, uint32_t col, uint32_t k, float (&v)[V]) {
+    if (kind == kF32) load_adjacent((float const *)row, col, k, v);
+    else if (kind == kBF16) load_adjacent((__bf16 const *)row, col, k, v);
+    else load_adjacent((_Float16 const *)row, col, k, v);
 }
 /** `count` (up to 8) adjacent results at column `col` of a row. */
 __device__ __forceinline__ void store_8(uint32_t kind, void *row, uint32_t col, float const (&v)[8], uint32_t count) {
@@ -173,10 +195,11 @@ __device__ __forceinline__ float gelu_tanh_slope(float x) {
     float const bend = near * __builtin_fmaf(near * near, 0.134145f * 1.5957691216057308f, 1.5957691216057308f);
     return fabsf(x) > 9.0f ? relu_slope(x) : __builtin_fmaf(bend * e * s, s, s);
 }
-/** Eight values at once: one branch, which all lanes take alike. */
-__device__ __forceinline__ void activate_8(uint32_t kind, float (&x)[8]) {
+/** Many values at once: one branch, which all lanes take alike. (A branch for each eight costs a wavefront that is alone more than their products.) */
+template <int N, int V>
+__device__ __forceinline__ void activate(uint32_t kind, float (&x)[N][V]) {
 #define NK_EACH(f)                                                                                                                                             \
-    _Pragma("unroll") for (int i = 0; i < 8; ++i) x[i] = f(x[i]);                                                                                               \
+    _Pragma("unroll") for (int i = 0; i < N * V; ++i) x[i / V][i % V] = f(x[i / V][i % V]);                                                                      \
     break
     switch (kind) {
     case nk_amd_relu: NK_EACH(relu);
@@ -185,7 +208,8 @@ __device__ __forceinline__ void activate_8(uint32_t kind, float (&x)[8]) {
     case nk_amd_gelu_tanh: NK_EACH(gelu_tanh);
     }
 }
-__device__ __forceinline__ void slope_8(uint32_t kind, float (&x)[8]) {
+template <int N, int V>
+__device__ __forceinline__ void slope(uint32_t kind, float (&x)[N][V]) {
     switch (kind) {
     case nk_amd_no_activation: NK_EACH([](float) { return 1.0f; });
     case nk_amd_relu: NK_EACH(relu_slope);

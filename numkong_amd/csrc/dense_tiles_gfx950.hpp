@@ -187,36 +187,82 @@ struct Bringer {
     }
 };
 
-/** Eight adjacent results of a row from their sums; `q`: gated, the other product's; `bias` and `r` are looked at only where there are such. */
-template <bool GATED>
-__device__ __forceinline__ void finish_8(Epilogue const &e, uint64_t row, uint32_t col, uint32_t n, float (&p)[8], float const (&q)[8], float const (&bias)[8], float const (&r)[8]) {
-    uint32_t const count = n - col;
+template <class T>
+struct Bytes {
+    typedef uint8_t type;
+};
+template <class T>
+struct Bytes<T const> {
+    typedef uint8_t const type;
+};
+/** Where N rows of V adjacent results lie: row `row + i step` of the matrix for i < N, of which the lane's own part, `lane` rows and `col` columns further on,
+ *  is added last: all else is the same in all lanes. WHOLE: all of them are within m x n. */
+template <int N, int V, bool WHOLE>
+struct Rows {
+    uint32_t row, step, m, lane, col, n;
+    template <class T>
+    __device__ __forceinline__ T *at(T *base, uint64_t stride, uint64_t of_lane, int i) const {
+        typedef typename Bytes<T>::type B;
+        return (T *)((B *)base + (uint64_t)(row + i * step) * stride + of_lane);
+    }
+    template <class T>
+    __device__ __forceinline__ uint64_t of_lane(T const *, uint64_t stride) const { return lane * stride + (uint64_t)col * sizeof(T); }
+    __device__ __forceinline__ bool inside(int i) const { return WHOLE || (row + i * step + lane < m && col < n); }
+    __device__ __forceinline__ uint32_t end() const { return WHOLE ? ~0u : n - col; }
+    template <class T>
+    __device__ __forceinline__ void store(T *base, uint64_t stride, float const (&v)[N][V]) const {
+        uint64_t const its = of_lane(base, stride);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (inside(i)) store_some(at(base, stride, its, i), v[i], end());
+    }
+    template <class T>
+    __device__ __forceinline__ void load(T const *base, uint64_t stride, float (&v)[N][V]) const {
+        uint64_t const its = of_lane(base, stride);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (inside(i)) load_adjacent(at(base, stride, its, i), 0, end(), v[i]);
+    }
+};
+/** N rows of V adjacent results from their sums; `q`: gated, the other product's. `bias` and `rest`, the residual, are looked at only where there are such. */
+template <bool GATED, int N, int V, bool WHOLE>
+__device__ __forceinline__ void finish(Epilogue const &e, Rows<N, V, WHOLE> const &rows, float (&p)[N][V], float const (&q)[N][V], float const (&bias)[V], float const (&rest)[N][V]) {
     if (!GATED && e.bias) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] += bias[i];
+        for (int i = 0; i < N * V; ++i) p[i / V][i % V] += bias[i % V];
     }
     if (e.pre) {
-        store_some((float *)((uint8_t *)e.pre + row * e.pre_stride) + col, p, count);
-        if (GATED) store_some((float *)((uint8_t *)e.pre_up + row * e.pre_stride) + col, q, count);
+        rows.store(e.pre, e.pre_stride, p);
+        if (GATED) rows.store(e.pre_up, e.pre_stride, q);
     }
-    activate_8(e.activation, p);
+    activate(e.activation, p);
     if constexpr (GATED) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] *= q[i];
+        for (int i = 0; i < N * V; ++i) p[i / V][i % V] *= q[i / V][i % V];
     }
     if (!GATED && e.residual) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] += r[i];
+        for (int i = 0; i < N * V; ++i) p[i / V][i % V] += rest[i / V][i % V];
     }
-    store_8(e.c_kind, e.c + row * e.c_stride, col, p, count);
+    if (e.c_kind == kF32) rows.store((float *)e.c, e.c_stride, p);
+    else if (e.c_kind == kBF16) rows.store((__bf16 *)e.c, e.c_stride, p);
+    else rows.store((_Float16 *)e.c, e.c_stride, p);
 }
-/** The same, with what it needs of the bias and the residual. */
+/** A residual's. */
+template <int N, int V, bool WHOLE>
+__device__ __forceinline__ void load_rest(Epilogue const &e, Rows<N, V, WHOLE> const &rows, float (&rest)[N][V]) {
+    if (e.residual_kind == kF32) rows.load((float const *)e.residual, e.residual_stride, rest);
+    else if (e.residual_kind == kBF16) rows.load((__bf16 const *)e.residual, e.residual_stride, rest);
+    else rows.load((_Float16 const *)e.residual, e.residual_stride, rest);
+}
+/** `finish` of one row with what it needs of the bias and the residual. */
 template <bool GATED>
-__device__ __forceinline__ void finish_8(Epilogue const &e, uint64_t row, uint32_t col, uint32_t n, float (&p)[8], float const (&q)[8]) {
-    float bias[8], r[8];
-    if (!GATED && e.bias) load_8(e.bias_kind, e.bias, col, n, bias);
-    if (!GATED && e.residual) load_8(e.residual_kind, e.residual + row * e.residual_stride, col, n, r);
-    finish_8<GATED>(e, row, col, n, p, q, bias, r);
+__device__ __forceinline__ void finish(Epilogue const &e, uint32_t row, uint32_t m, uint32_t col, uint32_t n, float (&p)[1][8], float const (&q)[1][8]) {
+    Rows<1, 8, false> const rows = {0, 0, m, row, col, n};
+    float bias[8], rest[1][8];
+    if (!GATED && e.bias) load_adjacent(e.bias_kind, e.bias, col, n, bias);
+    if (!GATED && e.residual) load_rest(e, rows, rest);
+    finish<GATED>(e, rows, p, q, bias, rest);
 }
 
 /** Nothing that reads or writes LDS moves across; what this wavefront has begun to load into LDS, and read from it, is there. */
@@ -346,18 +392,15 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void tile_kernel(TileArgs
         }
     }
 
-    // 64 rows at a time (32, if there are no more) through LDS, each wavefront in an array of its own: piece p (four results) of row r at p ^ r.
-    // A lane has the same columns in all of them; four rows' residuals are asked for before the first is needed.
+    // 64 rows at a time (32, if there are no more) through LDS, each wavefront in an array of its own: piece p (four results) of row r at p ^ r. A lane
+    // has the same columns in all of them: eight, or four where results of 32 bits are written, in whole lines then (8192 x 8192 x 64 to f32: 82 us, and
+    // 93 with eight, two stores with gaps; to bf16 72 and 57). Four or eight rows are finished at a time, their residuals asked for before.
     __syncthreads();
     constexpr int kHigh = WM < 2 ? WM : 2;
-    constexpr uint32_t kWidth = WN * 32, kPieces = kWidth / 4;
+    constexpr uint32_t kWidth = WN * 32, kPieces = kWidth / 4, kOut = GATED ? kWidth / 2 : kWidth; // kOut: results of a row
     float *const room = (float *)(wave == 0 ? a0 : wave == 1 ? a1 : wave == 2 ? b0 : b1);
-    constexpr uint32_t kOut = GATED ? kWidth / 2 : kWidth, kLanes = kOut / 8; // results of a row, lanes that finish them
-    constexpr uint32_t kTurns = kHigh * kLanes / 2, kAhead = kTurns < 4 ? kTurns : 4;
-    uint32_t const c = l % kLanes * 8, col = col0 + (GATED ? b_begin / 2 : b_begin) + c, piece = (GATED ? c / 32 * 64 + c % 32 : c) / 4;
+    uint32_t const out0 = col0 + (GATED ? b_begin / 2 : b_begin);
     bool const last = p.splits == 1;
-    float bias[8];
-    if (!GATED && last && p.e.bias && col < p.n) load_8(p.e.bias_kind, p.e.bias, col, p.n, bias);
     auto const put = [&](int i, auto from) {
         constexpr int kFrom = decltype(from)::value;
         uint32_t const r = l % 32;
@@ -368,47 +411,56 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void tile_kernel(TileArgs
                 *(v4f *)(room + (i * 32 + r) * kWidth + ((j * 8 + t * 2 + l / 32) ^ (r % kPieces)) * 4) =
                     v4f {sum[kFrom][j][4 * t], sum[kFrom][j][4 * t + 1], sum[kFrom][j][4 * t + 2], sum[kFrom][j][4 * t + 3]};
     };
-#pragma unroll 1
-    for (uint32_t part = 0; part < WM / kHigh; ++part) {
-        uint32_t const first = row0 + a_begin + part * kHigh * 32;
-        if (first >= p.m) break;
-        if (part == 0) {
-            put(0, Number<0>());
-            if constexpr (kHigh > 1) put(1, Number<1>());
-        } else if constexpr (WM > 2) put(0, Number<2>()), put(1, Number<3>());
-        wave_fence();
+    auto const finish_part = [&](auto values, auto whole, uint32_t first) __attribute__((always_inline)) {
+        constexpr int V = decltype(values)::value;
+        constexpr bool kWhole = decltype(whole)::value != 0;
+        constexpr uint32_t kLanes = kOut / V, kStep = 64 / kLanes, kTurns = kHigh * 32 / kStep, kAhead = !kWhole ? 1 : kTurns < 16 / V ? kTurns : 16 / V;
+        uint32_t const c = l % kLanes * V, col = out0 + c, piece = (GATED ? c / 32 * 64 + c % 32 : c) / 4;
+        float bias[V];
+        if (!GATED && last && p.e.bias && (kWhole || col < p.n)) load_adjacent(p.e.bias_kind, p.e.bias, col, p.n, bias);
 #pragma unroll 1
         for (uint32_t turn = 0; turn < kTurns; turn += kAhead) {
-            float rest[kAhead][8];
-            if (!GATED && last && p.e.residual) {
-#pragma unroll
-                for (uint32_t i = 0; i < kAhead; ++i) {
-                    uint32_t const row = first + (turn + i) * (64 / kLanes) + l / kLanes;
-                    if (row < p.m && col < p.n) load_8(p.e.residual_kind, p.e.residual + row * p.e.residual_stride, col, p.n, rest[i]);
-                }
-            }
+            Rows<kAhead, V, kWhole> const rows = {first + turn * kStep, kStep, p.m, l / kLanes, col, p.n};
+            float rest[kAhead][V], v[kAhead][V], q[kAhead][V];
+            if (!GATED && last && p.e.residual) load_rest(p.e, rows, rest);
 #pragma unroll
             for (uint32_t i = 0; i < kAhead; ++i) {
-                uint32_t const r = (turn + i) * (64 / kLanes) + l / kLanes, row = first + r;
-                float v[8], q[8] = {};
+                uint32_t const r = turn * kStep + l / kLanes + i * kStep;
 #pragma unroll
-                for (uint32_t t = 0; t < 2; ++t) {
+                for (uint32_t t = 0; t < V / 4; ++t) {
                     v4f const four = *(v4f const *)(room + r * kWidth + ((piece + t) ^ (r % kPieces)) * 4);
-                    v[4 * t] = four[0], v[4 * t + 1] = four[1], v[4 * t + 2] = four[2], v[4 * t + 3] = four[3];
+                    v[i][4 * t] = four[0], v[i][4 * t + 1] = four[1], v[i][4 * t + 2] = four[2], v[i][4 * t + 3] = four[3];
                     if constexpr (GATED) {
                         v4f const its = *(v4f const *)(room + r * kWidth + ((piece + 8 + t) ^ (r % kPieces)) * 4);
-                        q[4 * t] = its[0], q[4 * t + 1] = its[1], q[4 * t + 2] = its[2], q[4 * t + 3] = its[3];
+                        q[i][4 * t] = its[0], q[i][4 * t + 1] = its[1], q[i][4 * t + 2] = its[2], q[i][4 * t + 3] = its[3];
                     }
                 }
-                if (row >= p.m || col >= p.n) continue;
-                if (!last) {
-                    float *const to = p.partial + ((uint64_t)split * (GATED ? 2 : 1) * p.m + row) * p.n + col;
-                    store_some(to, v, p.n - col);
-                    if (GATED) store_some(to + (uint64_t)p.m * p.n, q, p.n - col);
-                } else finish_8<GATED>(p.e, row, col, p.n, v, q, bias, rest[i]);
+            }
+            if (last) finish<GATED>(p.e, rows, v, q, bias, rest);
+            else {
+                float *const to = p.partial + (uint64_t)split * (GATED ? 2 : 1) * p.m * p.n;
+                rows.store(to, (uint64_t)p.n * 4, v);
+                if (GATED) rows.store(to + (uint64_t)p.m * p.n, (uint64_t)p.n * 4, q);
             }
         }
+    };
+    auto const finish_rows = [&](uint32_t first) __attribute__((always_inline)) {
         wave_fence();
+        bool const whole = first + kHigh * 32 <= p.m && out0 + kOut <= p.n;
+        if (!whole) finish_part(Number<4>(), Number<0>(), first);
+        else if (!last || p.e.pre || p.e.c_kind == kF32) finish_part(Number<4>(), Number<1>(), first);
+        else finish_part(Number<8>(), Number<1>(), first);
+        wave_fence();
+    };
+    uint32_t const first = row0 + a_begin;
+    if (first >= p.m) return;
+    put(0, Number<0>());
+    if constexpr (kHigh > 1) put(1, Number<1>());
+    finish_rows(first);
+    if constexpr (WM > kHigh) {
+        if (first + kHigh * 32 >= p.m) return;
+        put(0, Number<2>()), put(1, Number<3>());
+        finish_rows(first + kHigh * 32);
     }
 }
 

@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void mx8_quantize_kernel(uint32_t kind, uint8_
     uint32_t const col = (uint32_t)(at - row * each) * 512 + (threadIdx.x & 63) * 8;
     float v[8];
     uint32_t scale;
-    load_8(kind, x + row * x_stride, col, k, v);
+    load_adjacent(kind, x + row * x_stride, col, k, v);
     v2u const code = quantize_8(v, scale);
     if (words) {
         uint32_t word = scale << (threadIdx.x & 12) * 2;
@@ -139,10 +139,10 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs p) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         uint32_t const col = (i * blockDim.x + threadIdx.x) * 8;
-        load_8((T const *)(p.x + row * p.x_stride), col, p.k, t[i]);
+        load_adjacent((T const *)(p.x + row * p.x_stride), col, p.k, t[i]);
         if (p.residual) {
             float r[8];
-            load_8((T const *)(p.residual + row * p.residual_stride), col, p.k, r);
+            load_adjacent((T const *)(p.residual + row * p.residual_stride), col, p.k, r);
 #pragma unroll
             for (int j = 0; j < 8; ++j) t[i][j] = (float)(T)(t[i][j] + r[j]);
             if (col < p.k) store_some((T *)(p.total + row * p.total_stride) + col, t[i], p.k - col);
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs p) {
     for (int i = 0; i < P; ++i) {
         uint32_t const col = (i * blockDim.x + threadIdx.x) * 8;
         float w[8], y[8];
-        if (p.weight) load_8(p.weight_kind, p.weight, col, p.k, w);
+        if (p.weight) load_adjacent(p.weight_kind, p.weight, col, p.k, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             Wide const v = p.weight ? (Wide)t[i][j] * scale * (Wide)w[j] : (Wide)t[i][j] * scale;
@@ -197,10 +197,10 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(NormBackwardArg
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             uint32_t const col = (i * blockDim.x + threadIdx.x) * 8;
-            load_8((T const *)(p.total + row * p.total_stride), col, p.k, t[i]);
-            load_8(p.grad_kind, p.grad + row * p.grad_stride, col, p.k, g[i]);
+            load_adjacent((T const *)(p.total + row * p.total_stride), col, p.k, t[i]);
+            load_adjacent(p.grad_kind, p.grad + row * p.grad_stride, col, p.k, g[i]);
             float w[8];
-            if (p.weight) load_8(p.weight_kind, p.weight, col, p.k, w);
+            if (p.weight) load_adjacent(p.weight_kind, p.weight, col, p.k, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 square += t[i][j] * t[i][j];
@@ -214,8 +214,8 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(NormBackwardArg
             uint32_t const col = (i * blockDim.x + threadIdx.x) * 8;
             if (col >= p.k) continue;
             float w[8], of_x[8];
-            if (p.weight) load_8(p.weight_kind, p.weight, col, p.k, w);
-            if (p.grad_total) load_8((T const *)(p.grad_total + row * p.grad_total_stride), col, p.k, of_x);
+            if (p.weight) load_adjacent(p.weight_kind, p.weight, col, p.k, w);
+            if (p.grad_total) load_adjacent((T const *)(p.grad_total + row * p.grad_total_stride), col, p.k, of_x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float const v = scale * ((p.weight ? g[i][j] * w[j] : g[i][j]) - t[i][j] * shift);
