@@ -336,7 +336,7 @@ struct TilePlan {
 TilePlan tile_plan(uint64_t m, uint64_t n, uint64_t stages, bool gated) {
     static constexpr double kAlone[3] = {0.45, 0.57, 1.48}, kEach[3] = {0.173, 0.442, 1.48}, kEnds[3] = {0.8, 2.5, 13.5};
     static constexpr uint64_t kResident[3] = {4, 2, 1};
-    uint64_t const units = (uint64_t)compute_unit_count();
+    uint64_t const found = (uint64_t)compute_unit_count(), units = found ? found : 256; // (a size may be asked for where there is no GPU)
     TilePlan best = {0, 1, (uint32_t)stages};
     double least = 1e300;
     for (int shape = 0; shape < 3; ++shape) {

@@ -51,15 +51,16 @@ class _LinearBackward(ctypes.Structure):
 
 
 _LIB = None
+_CALLS = None  # csrc/dense_calls.cpp: the calls in their ordinary form; each gives None for what is to go the general way below
 
 
 def _library():
     """The shared library with the entry points of dense.h bound, the torch module, and the codes of its float types."""
-    global _LIB
+    global _LIB, _CALLS
     if _LIB is None:
         lib, torch, codes = mx._library()
         of = ctypes.POINTER
-        for name, result, arguments in (
+        functions = (
             ("mx8_quantize_async", _i32, [_i32, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _vp]),
             ("mx8_dequantize_async", _i32, [_i32, _vp, _sz, _vp, _sz, _sz, _sz, _vp, _sz, _vp]),
             ("rms_norm_async", _i32, [of(_RmsNorm), _vp]),
@@ -69,10 +70,18 @@ def _library():
             ("linear_async", _i32, [of(_Linear), _vp, _sz, _vp]),
             ("linear_backward_workspace_size", _sz, [of(_LinearBackward)]),
             ("linear_backward_async", _i32, [of(_LinearBackward), _vp, _sz, _vp]),
-        ):
+        )
+        for name, result, arguments in functions:
             function = getattr(lib, "nk_amd_" + name)
             function.restype, function.argtypes = result, arguments
         _LIB = lib, torch, codes
+        try:
+            from .lib import _dense_calls
+        except ImportError:  # built for another torch, or not at all
+            _dense_calls = None
+        else:
+            _dense_calls.bind(*(ctypes.cast(getattr(lib, "nk_amd_" + name), _vp).value for name, *_ in functions))
+        _CALLS = _dense_calls
     return _LIB
 
 
@@ -152,13 +161,18 @@ class Mx8Matrix:
         return self.codes.get_device()
 
     @classmethod
+    def _made(cls, codes, scales):
+        """One whose parts are known to be right."""
+        matrix = cls.__new__(cls)
+        matrix.codes, matrix.scales = codes, scales
+        return matrix
+
+    @classmethod
     def _empty(cls, torch, rows: int, depth: int, device):
         """Room for one; rows start where the products can read them in place."""
         blocks = (depth + BLOCK - 1) // BLOCK
-        matrix = cls.__new__(cls)
-        matrix.codes = torch.empty_strided((rows, depth), (max((depth + 15) // 16 * 16, 1), 1), dtype=torch.float8_e4m3fn, device=device)
-        matrix.scales = torch.empty_strided((rows, blocks), (max((blocks + 3) // 4 * 4, 1), 1), dtype=torch.uint8, device=device)
-        return matrix
+        return cls._made(torch.empty_strided((rows, depth), (max((depth + 15) // 16 * 16, 1), 1), dtype=torch.float8_e4m3fn, device=device),
+                         torch.empty_strided((rows, blocks), (max((blocks + 3) // 4 * 4, 1), 1), dtype=torch.uint8, device=device))
 
     def cpu(self) -> "Mx8Matrix":
         return Mx8Matrix(self.codes.cpu().contiguous(), self.scales.cpu().contiguous())
@@ -172,6 +186,8 @@ def mx8_quantize(x) -> Mx8Matrix:
     (not below 2^-127) that keeps the block's largest magnitude within 448; codes to nearest, ties to even. A block that holds a NaN
     or an infinity becomes NaN. Codes and scales are numbers that no gradient passes."""
     lib, torch, dtype_codes = _library()
+    if _CALLS is not None and (made := _CALLS.quantize(x)) is not None:
+        return Mx8Matrix._made(*made)
     t = _floats(x, "x")
     if not t.is_cuda:
         return mx8_quantize(_to_gpu(t)).cpu()
@@ -192,6 +208,8 @@ def mx8_dequantize(matrix: Mx8Matrix, dtype=None, out=None):
     lib, torch, dtype_codes = _library()
     if not isinstance(matrix, Mx8Matrix):
         raise TypeError("matrix must be an Mx8Matrix")
+    if _CALLS is not None and out is None and (made := _CALLS.dequantize(matrix.codes, matrix.scales, dtype)) is not None:
+        return made
     dtype = mx._out_dtype(out, dtype)
     if not matrix.is_cuda:
         _check_host_out(out, matrix.shape, dtype)
@@ -315,7 +333,9 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-6, out_dtype=None):
     returned. ``x`` and ``residual``: rows x depth of one float type, depth at most 32768; ``weight``: depth values of any.
 
     The results have gradients (``rms_norm_backward``), which autograd follows."""
-    lib, torch, dtype_codes = _library()
+    lib, torch, dtype_codes = _LIB or _library()
+    if _CALLS is not None and (made := _CALLS.norm(x, weight, residual, eps, out_dtype, False)) is not None:
+        return made[0] if residual is None else (made[0], made[2])
     t, weight, residual, eps = _norm_operands(x, weight, residual, eps)
     out_dtype = t.dtype if out_dtype is None else mx._out_dtype(None, out_dtype)
     index = _home(t, weight, residual)
@@ -336,7 +356,10 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-6, out_dtype=None):
 def rms_norm_mx8(x, weight=None, residual=None, eps: float = 1e-6):
     """``rms_norm`` with ``y`` as an ``Mx8Matrix``: the codes and scales of the exact values, not of values that were rounded before.
     There is no gradient: operands that require one are refused while autograd records."""
-    lib, torch, dtype_codes = _library()
+    lib, torch, dtype_codes = _LIB or _library()
+    if _CALLS is not None and (made := _CALLS.norm(x, weight, residual, eps, None, True)) is not None:
+        y = Mx8Matrix._made(*made[:2])
+        return y if residual is None else (y, made[2])
     t, weight, residual, eps = _norm_operands(x, weight, residual, eps)
     index = _home(t, weight, residual)
     if _tracked(torch, t, weight, residual):
@@ -356,7 +379,9 @@ def rms_norm_backward(grad, total, weight=None, grad_total=None, eps: float = 1e
     """The gradients ``(of x, of weight)`` from ``grad``, that of ``y``: ``total`` is what was normed (``x``, or the sum that ``rms_norm``
     returned), ``grad_total`` the gradient that the sum has got from elsewhere. That of the residual is that of ``x``. The second is
     None without a ``weight``, or where it is not needed."""
-    lib, torch, dtype_codes = _library()
+    lib, torch, dtype_codes = _LIB or _library()
+    if _CALLS is not None and (made := _CALLS.norm_backward(grad, total, weight, grad_total, eps, need_weight)) is not None:
+        return made
     t, g = _floats(total, "total"), _floats(grad, "grad")
     weight, eps = _vector(weight, t.shape[1], "weight"), _eps(eps)
     if g.shape != t.shape:
@@ -439,6 +464,11 @@ def _operand(m, codes):
     return codes[m.dtype], m.data_ptr(), _row_bytes(m), None, 0
 
 
+def _parts(m):
+    """An operand and its scales, if it has any."""
+    return (m.codes, m.scales) if type(m) is Mx8Matrix else (m, None)
+
+
 def _multiply(a, w, w_up, bias, activation, residual, out, out_dtype, sums, where):
     """Queues a product of operands on the current GPU: (result, [sums])."""
     lib, torch, dtype_codes = _library()
@@ -472,7 +502,10 @@ def linear(a, w, bias=None, activation=None, residual=None, out=None, out_dtype=
 
     16-bit products have gradients for ``a``, ``w``, ``bias`` and ``residual``, which autograd follows; 8-bit ones have none and refuse
     operands that require one while autograd records. With ``sums`` the result is ``(y, a @ w.T + bias)``, as ``linear_backward`` takes them."""
-    lib, torch, dtype_codes = _library()
+    lib, torch, dtype_codes = _LIB or _library()
+    if _CALLS is not None and out is None:
+        if (made := _CALLS.linear(*_parts(a), *_parts(w), None, None, bias, ACTIVATIONS.get(activation), residual, out_dtype, sums)) is not None:
+            return made[:2] if sums else made[0]
     w = _matrix(w, "w")
     t = _left(a, w)
     height, width, code = t.shape[0], w.shape[0], _activation(activation)
@@ -505,7 +538,10 @@ def linear(a, w, bias=None, activation=None, residual=None, out=None, out_dtype=
 def gated_linear(a, w_gate, w_up, activation="silu", out=None, out_dtype=None, sums: bool = False):
     """``activation(a @ w_gate.T) * (a @ w_up.T)``, both products in one kernel. Operands, types and gradients as in ``linear``; the two
     matrices have one type and shape. With ``sums`` the result is ``(y, a @ w_gate.T, a @ w_up.T)``, as ``gated_linear_backward`` takes them."""
-    lib, torch, dtype_codes = _library()
+    lib, torch, dtype_codes = _LIB or _library()
+    if _CALLS is not None and out is None and w_up is not None:
+        if (made := _CALLS.linear(*_parts(a), *_parts(w_gate), *_parts(w_up), None, ACTIVATIONS.get(activation), None, out_dtype, sums)) is not None:
+            return made if sums else made[0]
     gate, up = _matrix(w_gate, "w_gate"), _matrix(w_up, "w_up")
     if gate.shape != up.shape or isinstance(gate, Mx8Matrix) != isinstance(up, Mx8Matrix) or getattr(gate, "dtype", None) != getattr(up, "dtype", None):
         raise ValueError("w_gate and w_up must have the same shape and type")
@@ -534,7 +570,10 @@ def gated_linear(a, w_gate, w_up, activation="silu", out=None, out_dtype=None, s
 
 def _backward(grad, a, w, w_up, sums, activation, need_a, need_w, need_up, bias_dtype, where):
     """(of a, of w, of w_up, of the bias): the gradients of either product, None where one is not needed."""
-    lib, torch, dtype_codes = _library()
+    lib, torch, dtype_codes = _LIB or _library()
+    if _CALLS is not None and len(sums) <= 2:
+        if (made := _CALLS.linear_backward(grad, a, w, w_up, *sums, *[None] * (2 - len(sums)), ACTIVATIONS.get(activation), need_a, need_w, need_up, bias_dtype)) is not None:
+            return made
     names = ("w", None) if w_up is None else ("w_gate", "w_up")
     w, w_up = _matrix(w, names[0]), None if w_up is None else _matrix(w_up, names[1])
     if isinstance(a, Mx8Matrix) or isinstance(w, Mx8Matrix) or isinstance(w_up, Mx8Matrix):
