@@ -185,47 +185,123 @@ struct NormBackwardArgs {
     float eps;
 };
 
-/** A workgroup for every gridDim.x-th row, its part of the weight's gradient in registers until the last. */
-template <class T, int P>
+/** Eight adjacent values as they lie in memory, so that a row can be on its way while the one before is worked on; HALF: of 16 bits for certain. */
+template <bool HALF>
+struct Raw {
+    v4u low, high; // (high: of f32 only)
+    __device__ __forceinline__ void load(uint32_t kind, uint8_t const *row, uint32_t col, uint32_t k) {
+        uint32_t const size = HALF ? 2 : bytes_of(kind);
+        uint8_t const *const at = row + (uint64_t)col * size;
+        if (col + 8 <= k) {
+            low = *(v4u_anywhere const *)at;
+            if (size == 4) high = *(v4u_anywhere const *)(at + 16);
+            return;
+        }
+        low = high = v4u {0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+            if (col + i < k) {
+                if (size == 4) (i < 4 ? low : high)[i % 4] = ((uint32_t const *)at)[i];
+                else low[i / 2] |= (uint32_t)((uint16_t const *)at)[i] << 16 * (i % 2);
+            }
+    }
+    __device__ __forceinline__ void widen_to(uint32_t kind, float (&v)[8]) const {
+        if (!HALF && kind == kF32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(low[i]), v[4 + i] = __uint_as_float(high[i]);
+        } else if (kind == kBF16) widen<__bf16>(low, v);
+        else widen<_Float16>(low, v);
+    }
+};
+
+/**
+ *  Threads (x) share a row, rows (y) a workgroup, as forward; a workgroup has every gridDim.x-th of such groups and keeps its part of the weight's
+ *  gradient in registers until the last. Rows of at most 8192 values of 16 bits (HALF: all operands) are asked for before the one before is worked on; of others
+ *  two do not fit the registers. Memory is what bounds it (8192 x 4096 bf16
+ *  with the total's gradient: 62 us without the weight's, 113 with it, when rows were loaded in turn and 1024 parts added up by 128 workgroups).
+ */
+template <class T, int P, bool HALF>
 __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(NormBackwardArgs p) {
-    __shared__ float sums[2][16], products[2][16];
+    constexpr uint32_t kKind = sizeof(T) == 4 ? kF32 : __is_same(T, __bf16) ? kBF16 : kF16;
+    __shared__ float sums[2][16][2];
+    extern __shared__ float parts[]; // rows of a workgroup but the first: theirs of the weight's gradient
     float of_weight[P][8] = {};
-    uint32_t turn = 0;
-    for (uint64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) { // (two sets of sums: no wavefront writes what another still reads)
-        float t[P][8], g[P][8];
+    constexpr bool kAhead = HALF && P == 1;
+    Raw<HALF> w, ahead[3];
+    auto const load_weight = [&](uint32_t col) { if (p.weight) w.load(p.weight_kind, (uint8_t const *)p.weight, col, p.k); };
+    auto const load_row = [&](uint64_t row, uint32_t col, Raw<HALF> (&raw)[3], bool rest) { // total, gradient, the total's gradient
+        raw[0].load(kKind, p.total + row * p.total_stride, col, p.k);
+        raw[1].load(p.grad_kind, p.grad + row * p.grad_stride, col, p.k);
+        if (rest && p.grad_total) raw[2].load(kKind, p.grad_total + row * p.grad_total_stride, col, p.k);
+    };
+    if (P == 1) load_weight(threadIdx.x * 8); // (of longer rows it comes out of the caches each time, and so do their values for the second loop)
+    uint64_t const step = (uint64_t)gridDim.x * blockDim.y;
+    uint64_t row = (uint64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    if (kAhead && row < p.rows) load_row(row, threadIdx.x * 8, ahead, true);
+    for (uint32_t turn = 0; row < p.rows; row += step, turn ^= 1) { // (two sets of sums: no wavefront writes what another still reads)
         float square = 0, inner = 0;
+        Raw<HALF> now[3];
+        if (P == 1) {
+            if (kAhead) now[0] = ahead[0], now[1] = ahead[1], now[2] = ahead[2];
+            else load_row(row, threadIdx.x * 8, now, true);
+        }
+        if (kAhead && row + step < p.rows) load_row(row + step, threadIdx.x * 8, ahead, true);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             uint32_t const col = (i * blockDim.x + threadIdx.x) * 8;
-            load_adjacent((T const *)(p.total + row * p.total_stride), col, p.k, t[i]);
-            load_adjacent(p.grad_kind, p.grad + row * p.grad_stride, col, p.k, g[i]);
-            float w[8];
-            if (p.weight) load_adjacent(p.weight_kind, p.weight, col, p.k, w);
+            float x[8], y[8], z[8];
+            if (P > 1) load_weight(col), load_row(row, col, now, false);
+            now[0].widen_to(kKind, x), now[1].widen_to(p.grad_kind, y);
+            if (p.weight) w.widen_to(p.weight_kind, z);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                square += t[i][j] * t[i][j];
-                inner += (p.weight ? g[i][j] * w[j] : g[i][j]) * t[i][j];
+                square += x[j] * x[j];
+                inner += (p.weight ? y[j] * z[j] : y[j]) * x[j];
             }
         }
-        square = row_sum(square, sums[turn]), inner = row_sum(inner, products[turn]);
+#pragma unroll
+        for (int half = 32; half; half >>= 1) square += __shfl_xor(square, half), inner += __shfl_xor(inner, half);
+        if (blockDim.x > 64) { // (then the workgroup has one row, and all its threads are here)
+            if (!(threadIdx.x & 63)) sums[turn][threadIdx.x >> 6][0] = square, sums[turn][threadIdx.x >> 6][1] = inner;
+            __syncthreads();
+            square = sums[turn][0][0], inner = sums[turn][0][1];
+            for (uint32_t i = 1; i < blockDim.x / 64; ++i) square += sums[turn][i][0], inner += sums[turn][i][1];
+        }
         float const scale = 1.0f / sqrtf(square / (float)p.k + p.eps), shift = inner / (float)p.k * scale * scale;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             uint32_t const col = (i * blockDim.x + threadIdx.x) * 8;
-            if (col >= p.k) continue;
-            float w[8], of_x[8];
-            if (p.weight) load_adjacent(p.weight_kind, p.weight, col, p.k, w);
-            if (p.grad_total) load_adjacent((T const *)(p.grad_total + row * p.grad_total_stride), col, p.k, of_x);
+            float x[8], y[8], z[8], of_x[8];
+            if (P > 1) load_weight(col), load_row(row, col, now, true);
+            now[0].widen_to(kKind, x), now[1].widen_to(p.grad_kind, y);
+            if (p.weight) w.widen_to(p.weight_kind, z);
+            if (p.grad_total) now[2].widen_to(kKind, of_x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                float const v = scale * ((p.weight ? g[i][j] * w[j] : g[i][j]) - t[i][j] * shift);
+                float const v = scale * ((p.weight ? y[j] * z[j] : y[j]) - x[j] * shift);
                 of_x[j] = p.grad_total ? of_x[j] + v : v;
-                of_weight[i][j] += g[i][j] * (t[i][j] * scale);
+                of_weight[i][j] += y[j] * (x[j] * scale);
             }
-            store_some((T *)(p.grad_x + row * p.grad_x_stride) + col, of_x, p.k - col);
+            if (col < p.k) store_some((T *)(p.grad_x + row * p.grad_x_stride) + col, of_x, p.k - col);
         }
     }
     if (!p.partial) return;
+    if (blockDim.y > 1) { // rows of at most 1024 values: those of the workgroup are added up in their order
+        uint32_t const width = blockDim.x * 8 * P;
+        if (threadIdx.y) {
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) parts[(threadIdx.y - 1) * width + (i * blockDim.x + threadIdx.x) * 8 + j] = of_weight[i][j];
+        }
+        __syncthreads();
+        if (threadIdx.y) return;
+        for (uint32_t y = 1; y < blockDim.y; ++y)
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) of_weight[i][j] += parts[(y - 1) * width + (i * blockDim.x + threadIdx.x) * 8 + j];
+    }
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         uint32_t const col = (i * blockDim.x + threadIdx.x) * 8;
@@ -233,17 +309,20 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(NormBackwardArg
     }
 }
 
-/** out[col] = the sum over `rows` rows of 32-bit values: eight wavefront halves take every eighth row of 32 columns each. */
-__global__ __launch_bounds__(256) void column_sum_kernel(float const *values, uint32_t rows, uint32_t k, uint32_t kind, void *out) {
-    __shared__ float sums[8][32];
-    uint32_t const col = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
+/** out[col] = the sum over `rows` rows of 32-bit values: 32 halves of wavefronts take every 32nd row of 32 columns each. */
+__global__ __launch_bounds__(1024) void column_sum_kernel(float const *values, uint32_t rows, uint32_t k, uint32_t kind, void *out) {
+    __shared__ float sums[32][33];
+    uint32_t const x = threadIdx.x & 31, col = blockIdx.x * 32 + x, part = threadIdx.x >> 5;
     float sum = 0;
-    if (col < k)
-        for (uint32_t row = part; row < rows; row += 8) sum += values[(uint64_t)row * k + col];
-    sums[part][threadIdx.x & 31] = sum;
+    if (col < k) {
+#pragma unroll 4
+        for (uint32_t row = part; row < rows; row += 32) sum += values[(uint64_t)row * k + col];
+    }
+    sums[part][x] = sum;
     __syncthreads();
     if (part || col >= k) return;
-    for (int i = 1; i < 8; ++i) sum += sums[i][threadIdx.x];
+#pragma unroll 8
+    for (int i = 1; i < 32; ++i) sum += sums[i][x];
     store_1(kind, out, col, sum);
 }
 
@@ -272,7 +351,12 @@ int with_float(int dtype, Call call) {
     return dtype == nk_f32_k ? call(float()) : dtype == nk_bf16_k ? call(__bf16()) : call(_Float16());
 }
 
-uint32_t norm_backward_workgroups(uint64_t rows) { return (uint32_t)(rows < 1024 ? rows : 1024); }
+/** Workgroups of a backward pass: what 1024 threads a compute unit are, or groups of rows, if there are fewer. */
+uint32_t norm_backward_workgroups(uint64_t rows, uint64_t k) {
+    NormShape const shape = norm_shape(k);
+    uint64_t const groups = (rows + shape.rows - 1) / shape.rows, most = 256 * 1024 / (shape.threads * shape.rows);
+    return (uint32_t)(groups < most ? groups : most);
+}
 
 } // namespace
 
@@ -287,7 +371,7 @@ int launch_mx8_quantize(uint32_t kind, void const *x, uint64_t x_stride, uint64_
 }
 
 int launch_column_sum(float const *values, uint64_t rows, uint64_t k, uint32_t kind, void *out, hipStream_t stream) {
-    hipLaunchKernelGGL(column_sum_kernel, dim3((uint32_t)((k + 31) / 32)), dim3(256), 0, stream, values, (uint32_t)rows, (uint32_t)k, kind, out);
+    hipLaunchKernelGGL(column_sum_kernel, dim3((uint32_t)((k + 31) / 32)), dim3(1024), 0, stream, values, (uint32_t)rows, (uint32_t)k, kind, out);
     hipError_t const e = hipGetLastError();
     return e == hipSuccess ? 0 : mx_fail(e, "column_sum_kernel");
 }
@@ -359,7 +443,7 @@ int nk_amd_rms_norm_async(nk_amd_rms_norm_t const *n, void *stream) {
 
 nk_size_t nk_amd_rms_norm_backward_workspace_size(nk_amd_rms_norm_backward_t const *n) {
     if (!n || !n->grad_weight || n->rows >= (1ull << 31) || n->depth > kMaxNormDepth) return 0;
-    return (norm_backward_workgroups(n->rows) * n->depth * 4 + 255) / 256 * 256;
+    return (norm_backward_workgroups(n->rows, n->depth) * n->depth * 4 + 255) / 256 * 256;
 }
 
 int nk_amd_rms_norm_backward_async(nk_amd_rms_norm_backward_t const *n, void *workspace, nk_size_t workspace_bytes, void *stream) {
@@ -377,7 +461,7 @@ int nk_amd_rms_norm_backward_async(nk_amd_rms_norm_backward_t const *n, void *wo
     nk_size_t const needed = nk_amd_rms_norm_backward_workspace_size(n);
     if (needed && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < needed)) return mx_fail("rms_norm_backward: the workspace is too small or not 256-byte aligned");
     NormShape const shape = norm_shape(n->depth);
-    uint32_t const workgroups = norm_backward_workgroups(n->rows);
+    uint32_t const workgroups = norm_backward_workgroups(n->rows, n->depth);
     NormBackwardArgs const p = {(uint8_t const *)n->total, (uint8_t const *)n->grad, (uint8_t const *)n->grad_total, (uint8_t *)n->grad_x, n->total_stride, n->grad_stride,
                                 n->grad_total_stride, n->grad_x_stride, n->weight, n->grad_weight ? (float *)workspace : nullptr, n->rows, (uint32_t)n->depth,
                                 kind_of(n->weight_dtype), kind_of(n->grad_dtype), n->eps};
@@ -385,7 +469,12 @@ int nk_amd_rms_norm_backward_async(nk_amd_rms_norm_backward_t const *n, void *wo
         int const status = with_float(n->dtype, [&](auto value) {
             typedef decltype(value) T;
             return with_passes(shape.passes, [&](auto number) {
-                hipLaunchKernelGGL((rms_norm_backward_kernel<T, decltype(number)::value>), dim3(workgroups), dim3(shape.threads), 0, (hipStream_t)stream, p);
+                constexpr int P = decltype(number)::value;
+                dim3 const grid(workgroups), block(shape.threads, shape.rows);
+                uint32_t const room = (shape.rows - 1) * shape.threads * shape.passes * 32;
+                bool const half = sizeof(T) == 2 && grad_bytes == 2 && (!n->weight || weight_bytes == 2);
+                if (half) hipLaunchKernelGGL((rms_norm_backward_kernel<T, P, sizeof(T) == 2>), grid, block, room, (hipStream_t)stream, p);
+                else hipLaunchKernelGGL((rms_norm_backward_kernel<T, P, false>), grid, block, room, (hipStream_t)stream, p);
                 hipError_t const e = hipGetLastError();
                 return e == hipSuccess ? 0 : mx_fail(e, "rms_norm_backward_kernel");
             });
