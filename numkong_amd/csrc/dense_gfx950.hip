@@ -12,18 +12,25 @@
 
 namespace nk_gfx950 {
 
-int launch_mx8_quantize(uint32_t kind, void const *x, uint64_t x_stride, uint64_t rows, uint64_t k, uint64_t stored, uint8_t *codes, uint64_t codes_stride,
-                        uint8_t *scales, uint64_t scales_stride, uint32_t *words, uint64_t pitch, hipStream_t stream); // norm_gfx950.hip
 int launch_column_sum(float const *values, uint64_t rows, uint64_t k, uint32_t kind, void *out, hipStream_t stream);
 
 namespace {
 
 inline uint64_t up_to(uint64_t n, uint64_t step) { return (n + step - 1) / step * step; }
 
-/** Up to 16 bytes of a row of `bytes` from `at` on, wherever they lie; zeros behind the end. */
+/** Up to 16 bytes of a row of `bytes` from `at` on, wherever they lie; zeros behind the end. (The row's last piece is its last 16 bytes, shifted: byte by
+ *  byte, 1 x 8192 x 1000 in 8 bits took 12 us, and 5.6 with twice the bytes and no such piece.) */
 __device__ __forceinline__ v4u load_piece(uint8_t const *row, uint32_t at, uint32_t bytes) {
     if (at + 16 <= bytes) return *(v4u_anywhere const *)(row + at);
     v4u piece = {0, 0, 0, 0};
+    if (at >= bytes) return piece;
+    if (bytes >= 16) {
+        v4u const last = *(v4u_anywhere const *)(row + bytes - 16);
+        uint32_t const gone = (at + 16 - bytes) * 8; // bits: 8 to 120
+        uint64_t const low = last[0] | (uint64_t)last[1] << 32, high = last[2] | (uint64_t)last[3] << 32;
+        uint64_t const first = gone < 64 ? low >> gone | high << (64 - gone) : high >> (gone - 64), second = gone < 64 ? high >> gone : 0;
+        return v4u {(uint32_t)first, (uint32_t)(first >> 32), (uint32_t)second, (uint32_t)(second >> 32)};
+    }
 #pragma unroll
     for (uint32_t i = 0; i < 16; ++i)
         if (at + i < bytes) piece[i / 4] |= (uint32_t)row[at + i] << 8 * (i % 4);
@@ -33,53 +40,89 @@ __device__ __forceinline__ v4u load_piece(uint8_t const *row, uint32_t at, uint3
 // ---- operands as the tiles take them -------------------------------------------------------------------------------
 
 /** Rows of `bytes` to where they are 16-byte aligned, zeros up to the next multiple of 16: a thread for 16 bytes. */
-__global__ __launch_bounds__(256) void realign_kernel(uint8_t const *from, uint64_t from_stride, uint64_t pieces, uint32_t each, uint32_t bytes, uint8_t *to, uint64_t to_stride) {
-    uint64_t const at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= pieces) return;
-    uint64_t const row = at / each;
-    uint32_t const piece = (uint32_t)(at - row * each);
-    *(v4u *)(to + row * to_stride + piece * 16) = load_piece(from + row * from_stride, piece * 16, bytes);
-}
-int launch_realign(uint8_t const *from, uint64_t from_stride, uint64_t rows, uint64_t bytes, uint8_t *to, uint64_t to_stride, hipStream_t stream) {
-    uint64_t const each = (bytes + 15) / 16, most = kMostThreads / each; // rows of a launch
-    for (uint64_t first = 0; first < rows; first += most) {
-        uint64_t const here = rows - first < most ? rows - first : most;
-        hipLaunchKernelGGL(realign_kernel, dim3((uint32_t)((here * each + 255) / 256)), dim3(256), 0, stream, from + first * from_stride, from_stride, here * each, (uint32_t)each, (uint32_t)bytes,
-                           to + first * to_stride, to_stride);
-        hipError_t const e = hipGetLastError();
-        if (e != hipSuccess) return mx_fail(e, "realign_kernel");
-    }
-    return 0;
+struct MoveArgs {
+    uint8_t const *from;
+    uint64_t from_stride, pieces; // rows times `each`
+    uint8_t *to;
+    uint64_t to_stride;
+    uint32_t each, bytes;
+};
+__device__ __forceinline__ void move_rows(MoveArgs const &p, uint64_t block) {
+    uint64_t const at = block * 256 + threadIdx.x;
+    if (at >= p.pieces) return;
+    uint64_t const row = at / p.each;
+    uint32_t const piece = (uint32_t)(at - row * p.each);
+    *(v4u *)(p.to + row * p.to_stride + piece * 16) = load_piece(p.from + row * p.from_stride, piece * 16, p.bytes);
 }
 
-struct WordsArgs {
-    uint8_t const *scales[2];
-    uint64_t stride[2];
-    uint32_t *words[2];
-    uint32_t rows, blocks, stages, pitch;
-};
 /** Scales as the tiles read them, words of four blocks by stage and row (zeros where there is no block): 32 rows times 32 stages a workgroup, through LDS, as
  *  rows are read and written along different axes. */
-__global__ __launch_bounds__(256) void scale_words_kernel(WordsArgs p) {
-    __shared__ uint32_t tile[32][33];
-    int const which = blockIdx.z;
-    uint32_t const row0 = blockIdx.x * 32, stage0 = blockIdx.y * 32, x = threadIdx.x % 32;
+struct WordsArgs {
+    uint8_t const *scales;
+    uint64_t stride;
+    uint32_t *words;
+    uint32_t rows, blocks, stages, pitch;
+};
+__device__ __forceinline__ void scale_words(WordsArgs const &p, uint64_t block, uint32_t (&tile)[32][33]) {
+    uint32_t const high = p.pitch / 32, row0 = (uint32_t)(block % high) * 32, stage0 = (uint32_t)(block / high) * 32, x = threadIdx.x % 32;
 #pragma unroll
     for (uint32_t y = threadIdx.x / 32; y < 32; y += 8) {
-        uint32_t const row = row0 + y, block = (stage0 + x) * 4;
+        uint32_t const row = row0 + y, at = (stage0 + x) * 4;
         uint32_t word = 0;
-        if (row < p.rows && block < p.blocks) {
-            uint8_t const *const at = p.scales[which] + row * p.stride[which] + block;
-            if (block + 4 <= p.blocks) word = *(u32_anywhere const *)at;
+        if (row < p.rows && at < p.blocks) {
+            uint8_t const *const from = p.scales + row * p.stride + at;
+            if (at + 4 <= p.blocks) word = *(u32_anywhere const *)from;
             else
-                for (uint32_t i = 0; i < p.blocks - block; ++i) word |= (uint32_t)at[i] << 8 * i;
+                for (uint32_t i = 0; i < p.blocks - at; ++i) word |= (uint32_t)from[i] << 8 * i;
         }
         tile[y][x] = word;
     }
     __syncthreads();
 #pragma unroll
     for (uint32_t y = threadIdx.x / 32; y < 32; y += 8)
-        if (stage0 + y < p.stages) p.words[which][(uint64_t)(stage0 + y) * p.pitch + row0 + x] = tile[x][y];
+        if (stage0 + y < p.stages) p.words[(uint64_t)(stage0 + y) * p.pitch + row0 + x] = tile[x][y];
+}
+
+/** What is made of a product's operands before it: every job in one launch, as each by itself takes 3 us of a small product's 14. */
+struct Preparation {
+    QuantizeArgs quantize;
+    MoveArgs move[3];
+    WordsArgs words[3];
+    uint64_t ends[7]; // the first workgroup behind each job's
+    uint64_t first;   // of the launch
+    int moves, scaled;
+    void add(QuantizeArgs const &q) { quantize = q; }
+    void add(uint8_t const *from, uint64_t from_stride, uint64_t rows, uint64_t bytes, uint8_t *to, uint64_t to_stride) {
+        uint64_t const each = (bytes + 15) / 16;
+        move[moves++] = {from, from_stride, rows * each, to, to_stride, (uint32_t)each, (uint32_t)bytes};
+    }
+    void add(WordsArgs const &w) { words[scaled++] = w; }
+};
+__global__ __launch_bounds__(256) void prepare_kernel(Preparation p) {
+    __shared__ uint32_t tile[32][33];
+    uint64_t const block = p.first + blockIdx.x;
+    if (block < p.ends[0]) return quantize_stretches(p.quantize, block);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        if (block < p.ends[1 + i]) return move_rows(p.move[i], block - p.ends[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        if (block < p.ends[4 + i]) return scale_words(p.words[i], block - p.ends[3 + i], tile);
+    }
+}
+int launch_preparation(Preparation &p, hipStream_t stream) {
+    uint64_t end = 0;
+    p.ends[0] = end += (p.quantize.stretches + 3) / 4;
+    for (int i = 0; i < 3; ++i) p.ends[1 + i] = end += (p.move[i].pieces + 255) / 256;
+    for (int i = 0; i < 3; ++i) p.ends[4 + i] = end += (uint64_t)(p.words[i].pitch / 32) * ((p.words[i].stages + 31) / 32);
+    for (p.first = 0; p.first < end; p.first += kMostThreads / 256) {
+        uint64_t const here = end - p.first < kMostThreads / 256 ? end - p.first : kMostThreads / 256;
+        hipLaunchKernelGGL(prepare_kernel, dim3((uint32_t)here), dim3(256), 0, stream, p);
+        hipError_t const e = hipGetLastError();
+        if (e != hipSuccess) return mx_fail(e, "prepare_kernel");
+    }
+    return 0;
 }
 
 /** Sums of the splits, in their order, and what follows: eight adjacent results a thread. */
@@ -511,13 +554,6 @@ LinearLayout linear_layout(nk_amd_linear_t const *l) {
     y.partial_at = room(partial_bytes(y.tiles, l->height, l->width, l->gated));
     return y.bytes = end, y;
 }
-/** Queues the scales of `count` matrices as words. */
-int launch_scale_words(WordsArgs const &p, uint32_t count, hipStream_t stream) {
-    hipLaunchKernelGGL(scale_words_kernel, dim3(p.pitch / 32, (p.stages + 31) / 32, count), dim3(256), 0, stream, p);
-    hipError_t const e = hipGetLastError();
-    return e == hipSuccess ? 0 : mx_fail(e, "scale_words_kernel");
-}
-
 /** Where a backward pass's workspace has d (and e behind it in each row), the sums of d, operands moved to where the tiles can read them, and splits. */
 struct BackwardLayout {
     uint64_t padded, d_stride, column_sums_at, partials, rows_each, bytes;
@@ -587,9 +623,12 @@ int nk_amd_linear_async(nk_amd_linear_t const *l, void *workspace, nk_size_t wor
     uint64_t const bytes = l->depth * (mx8 ? 1 : 2);
     Epilogue const e = {l->bias, (uint8_t const *)l->residual, (uint8_t *)l->c, l->pre, l->pre_up, l->residual_stride, l->c_stride, l->pre_stride, kind_of(l->bias_dtype),
                         kind_of(l->residual_dtype), kind_of(l->c_dtype), (uint32_t)l->activation};
-    if (y.quantises)
-        if (int const status = launch_mx8_quantize(kind_of(l->a_dtype), l->a, l->a_stride, l->height, l->depth, up_to(l->depth, 16), room + y.a_at, y.codes_stride, y.few ? room + y.scales_at : nullptr,
-                                                   y.scales_stride, y.few ? nullptr : (uint32_t *)(room + y.a_words_at), y.a_pitch, stream)) return status;
+    Preparation before = {};
+    if (y.quantises) {
+        uint64_t const each = (l->depth + 511) / 512;
+        before.add(QuantizeArgs {(uint8_t const *)l->a, l->a_stride, l->height * each, room + y.a_at, y.few ? room + y.scales_at : nullptr, y.codes_stride, y.scales_stride,
+                    y.few ? nullptr : (uint32_t *)(room + y.a_words_at), y.a_pitch, kind_of(l->a_dtype), (uint32_t)each, (uint32_t)l->depth, (uint32_t)up_to(l->depth, 16)});
+    }
     if (y.few) {
         FewArgs p = {};
         p.m = (uint32_t)l->height, p.n = (uint32_t)l->width, p.bytes = (uint32_t)bytes, p.e = e;
@@ -597,6 +636,7 @@ int nk_amd_linear_async(nk_amd_linear_t const *l, void *workspace, nk_size_t wor
         if (y.quantises) p.a = {room + y.a_at, y.codes_stride, room + y.scales_at, y.scales_stride};
         p.b[0] = {(uint8_t const *)l->w, l->w_stride, (uint8_t const *)l->w_scales, l->w_scales_stride};
         p.b[1] = {(uint8_t const *)l->w_up, l->w_up_stride, (uint8_t const *)l->w_up_scales, l->w_up_scales_stride};
+        if (int const status = launch_preparation(before, stream)) return status;
         return mx8 ? launch_few_of<Mx8>(p, gated, stream) : l->w_dtype == nk_f16_k ? launch_few_of<_Float16>(p, gated, stream) : launch_few_of<__bf16>(p, gated, stream);
     }
     TileArgs p = {};
@@ -609,25 +649,20 @@ int nk_amd_linear_async(nk_amd_linear_t const *l, void *workspace, nk_size_t wor
     p.b.values[1] = (uint8_t const *)l->w_up, p.b.stride[1] = l->w_up_stride;
     if (y.quantises) p.a.values[0] = room + y.a_at, p.a.stride[0] = y.codes_stride;
     auto const move = [&](TileSide &side, int which, uint64_t rows, uint64_t at) {
-        int const status = launch_realign(side.values[which], side.stride[which], rows, bytes, room + at, y.moved_stride, stream);
+        before.add(side.values[which], side.stride[which], rows, bytes, room + at, y.moved_stride);
         side.values[which] = room + at, side.stride[which] = y.moved_stride;
-        return status;
     };
-    if (y.moves_a)
-        if (int const status = move(p.a, 0, l->height, y.a_at)) return status;
-    if (y.moves_w)
-        if (int const status = move(p.b, 0, l->width, y.w_at)) return status;
-    if (y.moves_up)
-        if (int const status = move(p.b, 1, l->width, y.up_at)) return status;
+    if (y.moves_a) move(p.a, 0, l->height, y.a_at);
+    if (y.moves_w) move(p.b, 0, l->width, y.w_at);
+    if (y.moves_up) move(p.b, 1, l->width, y.up_at);
     if (mx8 && y.stages) {
         p.a.scales[0] = (uint32_t *)(room + y.a_words_at), p.b.scales[0] = (uint32_t *)(room + y.w_words_at), p.b.scales[1] = (uint32_t *)(room + y.up_words_at);
         uint32_t const blocks = (uint32_t)((l->depth + 31) / 32);
-        WordsArgs const of_w = {{(uint8_t const *)l->w_scales, (uint8_t const *)l->w_up_scales}, {l->w_scales_stride, l->w_up_scales_stride}, {(uint32_t *)p.b.scales[0], (uint32_t *)p.b.scales[1]}, p.n, blocks, p.stages, p.b.pitch};
-        if (int const status = launch_scale_words(of_w, gated ? 2 : 1, stream)) return status;
-        WordsArgs const of_a = {{(uint8_t const *)l->a_scales}, {l->a_scales_stride}, {(uint32_t *)p.a.scales[0]}, p.m, blocks, p.stages, p.a.pitch};
-        if (!y.quantises)
-            if (int const status = launch_scale_words(of_a, 1, stream)) return status;
+        before.add(WordsArgs {(uint8_t const *)l->w_scales, l->w_scales_stride, (uint32_t *)p.b.scales[0], p.n, blocks, p.stages, p.b.pitch});
+        if (gated) before.add(WordsArgs {(uint8_t const *)l->w_up_scales, l->w_up_scales_stride, (uint32_t *)p.b.scales[1], p.n, blocks, p.stages, p.b.pitch});
+        if (!y.quantises) before.add(WordsArgs {(uint8_t const *)l->a_scales, l->a_scales_stride, (uint32_t *)p.a.scales[0], p.m, blocks, p.stages, p.a.pitch});
     }
+    if (int const status = launch_preparation(before, stream)) return status;
     return launch_tiles(l->w_dtype, {0, false, false, gated}, y.tiles, p, (float *)(room + y.partial_at), stream);
 }
 
@@ -684,17 +719,15 @@ int nk_amd_linear_backward_async(nk_amd_linear_backward_t const *l, void *worksp
     }
     uint8_t const *a = (uint8_t const *)l->a, *w[2] = {(uint8_t const *)l->w, (uint8_t const *)l->w_up};
     uint64_t a_stride = l->a_stride, w_stride[2] = {l->w_stride, l->w_up_stride};
+    Preparation before = {};
     auto const move = [&](uint8_t const *&values, uint64_t &stride, uint64_t rows, uint64_t at) {
-        int const status = launch_realign(values, stride, rows, l->depth * 2, d + at, y.moved_stride, stream);
+        before.add(values, stride, rows, l->depth * 2, d + at, y.moved_stride);
         values = d + at, stride = y.moved_stride;
-        return status;
     };
-    if (y.moves_a)
-        if (int const status = move(a, a_stride, l->height, y.a_at)) return status;
-    if (y.moves_w)
-        if (int const status = move(w[0], w_stride[0], l->width, y.w_at)) return status;
-    if (y.moves_up)
-        if (int const status = move(w[1], w_stride[1], l->width, y.up_at)) return status;
+    if (y.moves_a) move(a, a_stride, l->height, y.a_at);
+    if (y.moves_w) move(w[0], w_stride[0], l->width, y.w_at);
+    if (y.moves_up) move(w[1], w_stride[1], l->width, y.up_at);
+    if (int const status = launch_preparation(before, stream)) return status;
     if (l->grad_a) { // rows of d times columns of W
         TileArgs p = {};
         p.m = (uint32_t)l->height, p.n = (uint32_t)l->depth, p.stages = (uint32_t)y.stages, p.first_stages = (uint32_t)y.first_stages;

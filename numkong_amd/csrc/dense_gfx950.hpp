@@ -118,6 +118,36 @@ __device__ __forceinline__ void store_codes(uint8_t *to, v2u codes, uint32_t cou
         if (i < count) to[i] = (uint8_t)(codes[i / 4] >> 8 * (i % 4));
 }
 
+/** Rows to codes and scales: bytes, or words of four blocks, [word of the row][pitch rows]. */
+struct QuantizeArgs {
+    uint8_t const *x;
+    uint64_t x_stride, stretches; // stretches: rows times `each`
+    uint8_t *codes, *scales;      // scales or words: NULL, if it is the other
+    uint64_t codes_stride, scales_stride;
+    uint32_t *words;
+    uint64_t pitch;
+    uint32_t kind, each, k, stored; // each: 512 values, of a row; codes are written up to `stored`, zeros from k on
+};
+/** Four of the stretches, a wavefront each: eight values a lane, four lanes to a block. Memory is what bounds it (16384 x 8192 bf16 71 us, 5.7 TB/s). */
+__device__ __forceinline__ void quantize_stretches(QuantizeArgs const &p, uint64_t four) {
+    uint64_t const at = four * 4 + (threadIdx.x >> 6);
+    if (at >= p.stretches) return;
+    uint64_t const row = at / p.each;
+    uint32_t const col = (uint32_t)(at - row * p.each) * 512 + (threadIdx.x & 63) * 8;
+    float v[8];
+    uint32_t scale;
+    load_adjacent(p.kind, p.x + row * p.x_stride, col, p.k, v);
+    v2u const code = quantize_8(v, scale);
+    if (p.words) {
+        uint32_t word = scale << (threadIdx.x & 12) * 2;
+        word |= __shfl_xor(word, 4);
+        word |= __shfl_xor(word, 8);
+        if (!(threadIdx.x & 15) && col < p.k) p.words[col / 128 * p.pitch + row] = word;
+    }
+    if (col < p.stored) store_codes(p.codes + row * p.codes_stride + col, code, p.stored - col);
+    if (p.scales && !(threadIdx.x & 3) && col < p.k) p.scales[row * p.scales_stride + col / 32] = (uint8_t)scale;
+}
+
 /** The four values of a word of e4m3 codes. */
 __device__ __forceinline__ void widen_e4m3(uint32_t word, float (&v)[4]) {
 #ifdef NK_MX_DEVICE_BUILTINS

@@ -224,6 +224,34 @@ struct Rows {
             if (inside(i)) load_adjacent(at(base, stride, its, i), 0, end(), v[i]);
     }
 };
+/** V adjacent values of a residual as they lie in memory. */
+template <int V>
+struct RawPiece {
+    v4u words[V / 4];
+    __device__ __forceinline__ void load(uint32_t kind, uint8_t const *at) {
+        if (kind == kF32) {
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) words[i] = *(v4u_anywhere const *)(at + 16 * i);
+        } else if constexpr (V == 8) words[0] = *(v4u_anywhere const *)at;
+        else {
+            typedef v2u __attribute__((aligned(1))) v2u_anywhere;
+            v2u const half = *(v2u_anywhere const *)at;
+            words[0] = v4u {half[0], half[1], 0, 0};
+        }
+    }
+    __device__ __forceinline__ void widen_to(uint32_t kind, float (&v)[V]) const {
+        if (kind == kF32) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = __uint_as_float(words[i / 4][i % 4]);
+            return;
+        }
+        float all[8];
+        if (kind == kBF16) widen<__bf16>(words[0], all);
+        else widen<_Float16>(words[0], all);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = all[i];
+    }
+};
 /** N rows of V adjacent results from their sums; `q`: gated, the other product's. `bias` and `rest`, the residual, are looked at only where there are such. */
 template <bool GATED, int N, int V, bool WHOLE>
 __device__ __forceinline__ void finish(Epilogue const &e, Rows<N, V, WHOLE> const &rows, float (&p)[N][V], float const (&q)[N][V], float const (&bias)[V], float const (&rest)[N][V]) {
@@ -393,8 +421,9 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void tile_kernel(TileArgs
     }
 
     // 64 rows at a time (32, if there are no more) through LDS, each wavefront in an array of its own: piece p (four results) of row r at p ^ r. A lane
-    // has the same columns in all of them: eight, or four where results of 32 bits are written, in whole lines then (8192 x 8192 x 64 to f32: 82 us, and
-    // 93 with eight, two stores with gaps; to bf16 72 and 57). Four or eight rows are finished at a time, their residuals asked for before.
+    // has the same columns in all of them: eight, or four where C is of 32 bits and so written in whole lines (8192 x 8192 x 64 to f32: 82 us, and
+    // 93 with eight, two stores with gaps; to bf16 72 and 57; with the sums for the gradients beside bf16 eight again, 8192 x 4096 x 4096 282 and 328).
+    // Two or four rows are finished at a time.
     __syncthreads();
     constexpr int kHigh = WM < 2 ? WM : 2;
     constexpr uint32_t kWidth = WN * 32, kPieces = kWidth / 4, kOut = GATED ? kWidth / 2 : kWidth; // kOut: results of a row
@@ -411,18 +440,45 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void tile_kernel(TileArgs
                 *(v4f *)(room + (i * 32 + r) * kWidth + ((j * 8 + t * 2 + l / 32) ^ (r % kPieces)) * 4) =
                     v4f {sum[kFrom][j][4 * t], sum[kFrom][j][4 * t + 1], sum[kFrom][j][4 * t + 2], sum[kFrom][j][4 * t + 3]};
     };
-    auto const finish_part = [&](auto values, auto whole, uint32_t first) __attribute__((always_inline)) {
+    auto const finish_part = [&](auto values, auto whole, auto part, uint32_t first) __attribute__((always_inline)) {
         constexpr int V = decltype(values)::value;
         constexpr bool kWhole = decltype(whole)::value != 0;
         constexpr uint32_t kLanes = kOut / V, kStep = 64 / kLanes, kTurns = kHigh * 32 / kStep, kAhead = !kWhole ? 1 : kTurns < 16 / V ? kTurns : 16 / V;
         uint32_t const c = l % kLanes * V, col = out0 + c, piece = (GATED ? c / 32 * 64 + c % 32 : c) / 4;
         float bias[V];
         if (!GATED && last && p.e.bias && (kWhole || col < p.n)) load_adjacent(p.e.bias_kind, p.e.bias, col, p.n, bias);
+        // Of whole tiles the residual is asked for before the sums are put down, eight groups of rows (of 32-bit results four) ahead.
+        bool const rests = !GATED && last && p.e.residual;
+        constexpr int kRing = !kWhole || GATED ? 1 : V == 8 ? 8 : 4;
+        RawPiece<V> ring[kRing][kAhead];
+        auto const ask = [&](uint32_t turn, RawPiece<V> (&to)[kAhead]) {
+            uint64_t const of_lane = l / kLanes * p.e.residual_stride + (uint64_t)col * bytes_of(p.e.residual_kind);
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; ++i) to[i].load(p.e.residual_kind, p.e.residual + (uint64_t)(first + (turn + i) * kStep) * p.e.residual_stride + of_lane);
+        };
+        if (kRing > 1 && rests) {
+#pragma unroll
+            for (int i = 0; i < kRing; ++i)
+                if (i * kAhead < kTurns) ask(i * kAhead, ring[i]);
+        }
+        put(0, Number<decltype(part)::value * kHigh>());
+        if constexpr (kHigh > 1) put(1, Number<decltype(part)::value * kHigh + 1>());
+        wave_fence();
 #pragma unroll 1
         for (uint32_t turn = 0; turn < kTurns; turn += kAhead) {
             Rows<kAhead, V, kWhole> const rows = {first + turn * kStep, kStep, p.m, l / kLanes, col, p.n};
             float rest[kAhead][V], v[kAhead][V], q[kAhead][V];
-            if (!GATED && last && p.e.residual) load_rest(p.e, rows, rest);
+            if (rests) {
+                if constexpr (kRing > 1) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kAhead; ++i) {
+                        ring[0][i].widen_to(p.e.residual_kind, rest[i]);
+#pragma unroll
+                        for (int j = 0; j + 1 < kRing; ++j) ring[j][i] = ring[j + 1][i];
+                    }
+                    if (turn + kRing * kAhead < kTurns) ask(turn + kRing * kAhead, ring[kRing - 1]);
+                } else load_rest(p.e, rows, rest);
+            }
 #pragma unroll
             for (uint32_t i = 0; i < kAhead; ++i) {
                 uint32_t const r = turn * kStep + l / kLanes + i * kStep;
@@ -444,23 +500,18 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void tile_kernel(TileArgs
             }
         }
     };
-    auto const finish_rows = [&](uint32_t first) __attribute__((always_inline)) {
-        wave_fence();
+    auto const finish_rows = [&](auto part, uint32_t first) __attribute__((always_inline)) {
         bool const whole = first + kHigh * 32 <= p.m && out0 + kOut <= p.n;
-        if (!whole) finish_part(Number<4>(), Number<0>(), first);
-        else if (!last || p.e.pre || p.e.c_kind == kF32) finish_part(Number<4>(), Number<1>(), first);
-        else finish_part(Number<8>(), Number<1>(), first);
+        if (!whole) finish_part(Number<4>(), Number<0>(), part, first);
+        else if (!last || p.e.c_kind == kF32) finish_part(Number<4>(), Number<1>(), part, first);
+        else finish_part(Number<8>(), Number<1>(), part, first);
         wave_fence();
     };
     uint32_t const first = row0 + a_begin;
     if (first >= p.m) return;
-    put(0, Number<0>());
-    if constexpr (kHigh > 1) put(1, Number<1>());
-    finish_rows(first);
+    finish_rows(Number<0>(), first);
     if constexpr (WM > kHigh) {
-        if (first + kHigh * 32 >= p.m) return;
-        put(0, Number<2>()), put(1, Number<3>());
-        finish_rows(first + kHigh * 32);
+        if (first + kHigh * 32 < p.m) finish_rows(Number<1>(), first + kHigh * 32);
     }
 }
 

@@ -24,29 +24,7 @@ int in_pieces(uint64_t rows, uint64_t threads, char const *what, Launch launch) 
 
 // ---- 8-bit blocks --------------------------------------------------------------------------------------------------
 
-/**
- *  A wavefront for 512 adjacent values of a row, eight a lane, four lanes to a block. Memory is what bounds it. Codes are written up to
- *  `stored` (zeros from `k` on); scales as bytes, or as words of four blocks, [word of the row][pitch rows].
- */
-__global__ __launch_bounds__(256) void mx8_quantize_kernel(uint32_t kind, uint8_t const *x, uint64_t x_stride, uint64_t stretches, uint32_t each, uint32_t k, uint32_t stored,
-                                                           uint8_t *codes, uint64_t codes_stride, uint8_t *scales, uint64_t scales_stride, uint32_t *words, uint64_t pitch) {
-    uint64_t const at = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= stretches) return;
-    uint64_t const row = at / each;
-    uint32_t const col = (uint32_t)(at - row * each) * 512 + (threadIdx.x & 63) * 8;
-    float v[8];
-    uint32_t scale;
-    load_adjacent(kind, x + row * x_stride, col, k, v);
-    v2u const code = quantize_8(v, scale);
-    if (words) {
-        uint32_t word = scale << (threadIdx.x & 12) * 2;
-        word |= __shfl_xor(word, 4);
-        word |= __shfl_xor(word, 8);
-        if (!(threadIdx.x & 15) && col < k) words[col / 128 * pitch + row] = word;
-    }
-    if (col < stored) store_codes(codes + row * codes_stride + col, code, stored - col);
-    if (scales && !(threadIdx.x & 3) && col < k) scales[row * scales_stride + col / 32] = (uint8_t)scale;
-}
+__global__ __launch_bounds__(256) void mx8_quantize_kernel(QuantizeArgs p) { quantize_stretches(p, blockIdx.x); }
 
 __global__ __launch_bounds__(256) void mx8_dequantize_kernel(uint8_t const *codes, uint64_t codes_stride, uint8_t const *scales, uint64_t scales_stride,
                                                              uint64_t stretches, uint32_t each, uint32_t k, uint32_t kind, uint8_t *x, uint64_t x_stride) {
@@ -360,16 +338,6 @@ uint32_t norm_backward_workgroups(uint64_t rows, uint64_t k) {
 
 } // namespace
 
-int launch_mx8_quantize(uint32_t kind, void const *x, uint64_t x_stride, uint64_t rows, uint64_t k, uint64_t stored, uint8_t *codes, uint64_t codes_stride,
-                        uint8_t *scales, uint64_t scales_stride, uint32_t *words, uint64_t pitch, hipStream_t stream) {
-    uint64_t const each = (k + 511) / 512;
-    return in_pieces(rows, each * 64, "mx8_quantize_kernel", [&](uint64_t first, uint64_t here) {
-        hipLaunchKernelGGL(mx8_quantize_kernel, dim3((uint32_t)((here * each + 3) / 4)), dim3(256), 0, stream, kind, (uint8_t const *)x + first * x_stride, x_stride, here * each,
-                           (uint32_t)each, (uint32_t)k, (uint32_t)stored, codes + first * codes_stride, codes_stride, scales ? scales + first * scales_stride : nullptr, scales_stride,
-                           words ? words + first : nullptr, pitch);
-    });
-}
-
 int launch_column_sum(float const *values, uint64_t rows, uint64_t k, uint32_t kind, void *out, hipStream_t stream) {
     hipLaunchKernelGGL(column_sum_kernel, dim3((uint32_t)((k + 31) / 32)), dim3(1024), 0, stream, values, (uint32_t)rows, (uint32_t)k, kind, out);
     hipError_t const e = hipGetLastError();
@@ -390,7 +358,12 @@ int nk_amd_mx8_quantize_async(nk_dtype_t dtype, void const *x, nk_size_t rows, n
     if (!rows || !depth) return 0;
     if (!x || !codes || !scales) return mx_fail("mx8_quantize: NULL operand");
     if (!aligned_to(x, x_stride, bytes)) return mx_fail("mx8_quantize: x is not aligned to its elements");
-    return launch_mx8_quantize(kind_of(dtype), x, x_stride, rows, depth, depth, (uint8_t *)codes, codes_stride, (uint8_t *)scales, scales_stride, nullptr, 0, (hipStream_t)stream);
+    uint64_t const each = (depth + 511) / 512;
+    return in_pieces(rows, each * 64, "mx8_quantize_kernel", [&](uint64_t first, uint64_t here) {
+        QuantizeArgs const p = {(uint8_t const *)x + first * x_stride, x_stride, here * each, (uint8_t *)codes + first * codes_stride, (uint8_t *)scales + first * scales_stride, codes_stride,
+                                scales_stride, nullptr, 0, kind_of(dtype), (uint32_t)each, (uint32_t)depth, (uint32_t)depth};
+        hipLaunchKernelGGL(mx8_quantize_kernel, dim3((uint32_t)((here * each + 3) / 4)), dim3(256), 0, (hipStream_t)stream, p);
+    });
 }
 
 int nk_amd_mx8_dequantize_async(nk_dtype_t dtype, void const *codes, nk_size_t codes_stride, void const *scales, nk_size_t scales_stride,
