@@ -3,11 +3,16 @@
  *  @file numkong_amd/csrc/dense_calls.cpp
  *
  *  As mx_calls.cpp: every function returns None for what it does not take, or what the library refuses, and dense.py goes its general way then.
- *  (Through ctypes a product of one token takes 11 us of the host, a norm 10; its kernel may be shorter.)
+ *  (Through ctypes a product of one token takes 11 us of the host, a norm 10; its kernel may be shorter.) Operands that autograd follows are taken as well;
+ *  what the backward passes do is what dense.py's do. (In Python a small norm with its gradients took 90 us of the host.)
  */
 #include "torch_calls.hpp"
 
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include "numkong_amd/dense.h"
+#include "numkong_amd/hip_abi.h"
 
 namespace {
 
@@ -21,6 +26,7 @@ struct Library {
     decltype(&nk_amd_linear_async) linear;
     decltype(&nk_amd_linear_backward_workspace_size) linear_backward_room;
     decltype(&nk_amd_linear_backward_async) linear_backward;
+    decltype(&nk_hip_last_error) last_error;
 };
 Library library;
 
@@ -46,8 +52,11 @@ bool floats(PyObject *argument, int64_t dims, Home &home, at::Tensor const *&t) 
     t = nullptr;
     if (argument == Py_None) return true;
     t = tensor_of(argument, dims, home);
-    return t && code_of(t->scalar_type()) && !tracked(*t);
+    return t && code_of(t->scalar_type());
 }
+/** Does autograd follow one of them? */
+template <class... Tensors>
+bool followed(Tensors... t) { return ((t && tracked(*t)) || ...); }
 nk_dtype_t dtype_of(at::Tensor const *t) { return t ? code_of(t->scalar_type()) : nk_dtype_t(0); }
 void *data_of(at::Tensor const *t) { return t ? t->data_ptr() : nullptr; }
 nk_size_t stride_of(at::Tensor const *t) { return t ? row_bytes(*t) : 0; }
@@ -75,7 +84,7 @@ struct Matrix {
     at::Tensor const *t = nullptr, *scales = nullptr;
     bool found(PyObject *values, PyObject *its_scales, Home &home) {
         if (!(t = tensor_of(values, 2, home))) return false;
-        if (its_scales == Py_None) return code_of(t->scalar_type()) && !tracked(*t);
+        if (its_scales == Py_None) return code_of(t->scalar_type());
         scales = tensor_of(its_scales, 2, home);
         return scales && t->scalar_type() == at::kFloat8_e4m3fn && scales->scalar_type() == at::kByte && scales->size(0) == t->size(0) &&
                scales->size(1) == (t->size(1) + 31) / 32;
@@ -125,6 +134,83 @@ PyObject *dequantize(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
+void *stream_on(at::Tensor const &t) { return (void *)c10::hip::getCurrentHIPStream((c10::DeviceIndex)t.get_device()).stream(); }
+typedef std::optional<at::Tensor> Maybe;
+at::Tensor const *present(at::Tensor const &t) { return t.defined() ? &t : nullptr; }
+at::Tensor const *present(Maybe const &t) { return t ? &*t : nullptr; }
+Maybe maybe(at::Tensor const *t) { return t ? Maybe(*t) : Maybe(); }
+/** Is a gradient of input `i` asked for? (Autograd counts those that there are.) */
+bool needs(torch::autograd::AutogradContext *ctx, int64_t i) {
+    int64_t const there = ctx->saved_data["there"].toInt();
+    return there >> i & 1 && ctx->needs_input_grad((size_t)__builtin_popcountll((uint64_t)there & ((1ull << i) - 1)));
+}
+void check(int status, char const *where) { TORCH_CHECK(!status, where, ": ", library.last_error()); }
+/** A gradient as the kernels read it: autograd hands on expanded and transposed ones too. */
+at::Tensor rows_of(at::Tensor const &t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
+/** Gradients that no gradient passes: asked for one, they say so. */
+torch::autograd::variable_list once(torch::autograd::variable_list found) {
+    if (!c10::GradMode::is_enabled()) return found;
+    torch::autograd::variable_list there;
+    for (auto const &t : found)
+        if (t.defined()) there.push_back(t.detach().set_requires_grad(true));
+    auto const error = std::make_shared<torch::autograd::DelayedError>("the gradients of the dense operators have no gradients of their own", (int)there.size());
+    if (there.empty()) return found;
+    there = (*error)(std::move(there));
+    size_t next = 0;
+    for (auto &t : found)
+        if (t.defined()) t = there[next++];
+    return found;
+}
+
+int run_norm(at::Tensor const &x, at::Tensor const *weight, at::Tensor const *residual, float eps, at::ScalarType type, bool mx8, at::Tensor &y, at::Tensor &scales, at::Tensor &total) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    int64_t const rows = x.size(0), depth = x.size(1);
+    if (mx8) y = strided(rows, depth, 16, at::kFloat8_e4m3fn, x), scales = strided(rows, (depth + 31) / 32, 4, at::kByte, x);
+    else y = fresh({rows, depth}, type, x);
+    if (residual) total = fresh({rows, depth}, x.scalar_type(), x);
+    nk_amd_rms_norm_t const n = {(nk_size_t)rows, (nk_size_t)depth, eps, dtype_of(&x), x.data_ptr(), row_bytes(x), data_of(residual),
+                                 stride_of(residual), residual ? total.data_ptr() : nullptr, residual ? row_bytes(total) : 0, dtype_of(weight), data_of(weight),
+                                 mx8 ? nk_e4m3_k : code_of(type), y.data_ptr(), row_bytes(y), mx8 ? scales.data_ptr() : nullptr, mx8 ? row_bytes(scales) : 0};
+    return library.norm(&n, stream_on(x));
+}
+int run_norm_backward(at::Tensor const &grad, at::Tensor const &total, at::Tensor const *weight, at::Tensor const *grad_total, float eps, bool need_weight, at::Tensor &of_x,
+                      at::Tensor &of_weight) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    int64_t const rows = total.size(0), depth = total.size(1);
+    at::Tensor workspace;
+    of_x = fresh({rows, depth}, total.scalar_type(), total);
+    if (need_weight && weight) of_weight = fresh({depth}, weight->scalar_type(), total);
+    nk_amd_rms_norm_backward_t const n = {(nk_size_t)rows, (nk_size_t)depth, eps, dtype_of(&total), total.data_ptr(), row_bytes(total),
+                                          dtype_of(weight), data_of(weight), dtype_of(&grad), grad.data_ptr(), row_bytes(grad), data_of(grad_total),
+                                          stride_of(grad_total), of_x.data_ptr(), row_bytes(of_x), of_weight.defined() ? of_weight.data_ptr() : nullptr};
+    nk_size_t const room = library.norm_backward_room(&n);
+    if (room) workspace = fresh({(int64_t)room}, at::kByte, total);
+    return library.norm_backward(&n, room ? workspace.data_ptr() : nullptr, room, stream_on(total));
+}
+struct NormWithGradient : torch::autograd::Function<NormWithGradient> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, at::Tensor x, Maybe weight, Maybe residual, double eps, at::ScalarType type) {
+        at::Tensor y, scales, total;
+        check(run_norm(x, present(weight), present(residual), (float)eps, type, false, y, scales, total), "rms_norm");
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({residual ? total : x, weight ? *weight : at::Tensor()});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["there"] = int64_t(1 | (weight ? 2 : 0) | (residual ? 4 : 0));
+        return residual ? torch::autograd::variable_list {y, total} : torch::autograd::variable_list {y};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        auto const saved = ctx->get_saved_variables();
+        at::Tensor const &total = saved[0], &weight = saved[1];
+        at::Tensor of_x, of_weight, of_total = grads.size() > 1 && grads[1].defined() ? rows_of(grads[1]) : at::Tensor();
+        if (!grads[0].defined()) { // nothing came back through y
+            of_x = of_total;
+            if (weight.defined() && needs(ctx, 1)) of_weight = at::zeros_like(weight);
+        } else
+            check(run_norm_backward(rows_of(grads[0]), total, present(weight), present(of_total), (float)ctx->saved_data["eps"].toDouble(), needs(ctx, 1), of_x, of_weight),
+                  "rms_norm_backward");
+        return once({needs(ctx, 0) ? of_x : at::Tensor(), of_weight, needs(ctx, 2) ? of_x : at::Tensor(), at::Tensor(), at::Tensor()});
+    }
+};
+
 /** norm(x, weight or None, residual or None, eps, dtype or None, mx8) -> (y, scales or None, total or None) */
 PyObject *norm(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
     HANDLE_TH_ERRORS
@@ -137,20 +223,22 @@ PyObject *norm(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
         Py_RETURN_NONE;
     int64_t const rows = x->size(0), depth = x->size(1);
     if (!is_vector(weight, depth) || !has_shape(residual, rows, depth) || (residual && residual->scalar_type() != x->scalar_type())) Py_RETURN_NONE;
+    float const eps = (float)PyFloat_AS_DOUBLE(arguments[3]);
     at::Tensor y, scales, total;
-    int status;
-    {
+    if (followed(x, weight, residual)) {
+        if (mx8 || !(eps >= 0) || eps > std::numeric_limits<float>::max() || depth > 32768) Py_RETURN_NONE;
         WithoutLock unlocked;
-        at::AutoDispatchBelowADInplaceOrView guard;
-        if (mx8) y = strided(rows, depth, 16, at::kFloat8_e4m3fn, *x), scales = strided(rows, (depth + 31) / 32, 4, at::kByte, *x);
-        else y = fresh({rows, depth}, type, *x);
-        if (residual) total = fresh({rows, depth}, x->scalar_type(), *x);
-        nk_amd_rms_norm_t const n = {(nk_size_t)rows, (nk_size_t)depth, (float)PyFloat_AS_DOUBLE(arguments[3]), dtype_of(x), x->data_ptr(), row_bytes(*x), data_of(residual),
-                                     stride_of(residual), residual ? total.data_ptr() : nullptr, residual ? row_bytes(total) : 0, dtype_of(weight), data_of(weight),
-                                     mx8 ? nk_e4m3_k : code_of(type), y.data_ptr(), row_bytes(y), mx8 ? scales.data_ptr() : nullptr, mx8 ? row_bytes(scales) : 0};
-        status = library.norm(&n, stream_of(home));
+        auto found = NormWithGradient::apply(*x, maybe(weight), maybe(residual), (double)eps, type);
+        y = found[0];
+        if (residual) total = found[1];
+    } else {
+        int status;
+        {
+            WithoutLock unlocked;
+            status = run_norm(*x, weight, residual, eps, type, mx8, y, scales, total);
+        }
+        if (status) Py_RETURN_NONE;
     }
-    if (status) Py_RETURN_NONE;
     return Py_BuildValue("NNN", wrapped(y), wrapped(scales), wrapped(total));
     END_HANDLE_TH_ERRORS
 }
@@ -167,24 +255,89 @@ PyObject *norm_backward(PyObject *, PyObject *const *arguments, Py_ssize_t count
     int64_t const rows = total->size(0), depth = total->size(1);
     if (!has_shape(grad, rows, depth) || !is_vector(weight, depth) || !has_shape(grad_total, rows, depth) || (grad_total && grad_total->scalar_type() != total->scalar_type()))
         Py_RETURN_NONE;
-    at::Tensor of_x, of_weight, workspace;
+    if (followed(grad, total, weight, grad_total)) Py_RETURN_NONE;
+    at::Tensor of_x, of_weight;
     int status;
     {
         WithoutLock unlocked;
-        at::AutoDispatchBelowADInplaceOrView guard;
-        of_x = fresh({rows, depth}, total->scalar_type(), *total);
-        if (need_weight && weight) of_weight = fresh({depth}, weight->scalar_type(), *total);
-        nk_amd_rms_norm_backward_t const n = {(nk_size_t)rows, (nk_size_t)depth, (float)PyFloat_AS_DOUBLE(arguments[4]), dtype_of(total), total->data_ptr(), row_bytes(*total),
-                                              dtype_of(weight), data_of(weight), dtype_of(grad), grad->data_ptr(), row_bytes(*grad), data_of(grad_total),
-                                              stride_of(grad_total), of_x.data_ptr(), row_bytes(of_x), of_weight.defined() ? of_weight.data_ptr() : nullptr};
-        nk_size_t const room = library.norm_backward_room(&n);
-        if (room) workspace = fresh({(int64_t)room}, at::kByte, *total);
-        status = library.norm_backward(&n, room ? workspace.data_ptr() : nullptr, room, stream_of(home));
+        status = run_norm_backward(*grad, *total, weight, grad_total, (float)PyFloat_AS_DOUBLE(arguments[4]), need_weight, of_x, of_weight);
     }
     if (status) Py_RETURN_NONE;
     return Py_BuildValue("NN", wrapped(of_x), wrapped(of_weight));
     END_HANDLE_TH_ERRORS
 }
+
+int run_linear(Matrix const &a, Matrix const &w, Matrix const &up, at::Tensor const *bias, int activation, at::Tensor const *residual, at::ScalarType type, bool sums, at::Tensor &c,
+               at::Tensor &pre, at::Tensor &pre_up) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    int64_t const height = a.t->size(0), depth = a.t->size(1), width = w.t->size(0);
+    bool const gated = up.t;
+    at::Tensor workspace;
+    c = fresh({height, width}, type, *a.t);
+    if (sums) pre = fresh({height, width}, at::kFloat, *a.t);
+    if (sums && gated) pre_up = fresh({height, width}, at::kFloat, *a.t);
+    nk_amd_linear_t const l = {(nk_size_t)height, (nk_size_t)width, (nk_size_t)depth, gated, a.dtype(), a.t->data_ptr(), row_bytes(*a.t), data_of(a.scales), stride_of(a.scales),
+                               w.dtype(), w.t->data_ptr(), row_bytes(*w.t), data_of(w.scales), stride_of(w.scales), data_of(up.t), stride_of(up.t), data_of(up.scales),
+                               stride_of(up.scales), activation, dtype_of(bias), data_of(bias), dtype_of(residual), data_of(residual), stride_of(residual),
+                               code_of(type), c.data_ptr(), row_bytes(c), sums ? (float *)pre.data_ptr() : nullptr, sums && gated ? (float *)pre_up.data_ptr() : nullptr,
+                               sums ? (nk_size_t)width * 4 : 0};
+    nk_size_t const room = library.linear_room(&l);
+    if (room) workspace = fresh({(int64_t)room}, at::kByte, *a.t);
+    return library.linear(&l, room ? workspace.data_ptr() : nullptr, room, stream_on(*a.t));
+}
+/** `up` and the sums: NULL, if there are none; of_bias: of that type, if `biased`. */
+int run_linear_backward(at::Tensor const &grad, at::Tensor const &a, at::Tensor const &w, at::Tensor const *up, at::Tensor const *sums, at::Tensor const *up_sums, int activation, bool need_a,
+                        bool need_w, bool need_up, bool biased, at::ScalarType bias_type, at::Tensor &of_a, at::Tensor &of_w, at::Tensor &of_up, at::Tensor &of_bias) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    int64_t const height = a.size(0), depth = a.size(1), width = w.size(0);
+    at::Tensor workspace;
+    if (need_a) of_a = fresh({height, depth}, a.scalar_type(), a);
+    if (need_w) of_w = fresh({width, depth}, a.scalar_type(), a);
+    if (need_up && up) of_up = fresh({width, depth}, a.scalar_type(), a);
+    if (biased) of_bias = fresh({width}, bias_type, a);
+    auto const data = [](at::Tensor const &t) { return t.defined() ? t.data_ptr() : nullptr; };
+    nk_size_t const row = (nk_size_t)depth * 2;
+    nk_amd_linear_backward_t const l = {(nk_size_t)height, (nk_size_t)width, (nk_size_t)depth, up != nullptr, dtype_of(&a), a.data_ptr(), row_bytes(a), w.data_ptr(), row_bytes(w),
+                                        data_of(up), stride_of(up), activation, (float const *)data_of(sums), (float const *)data_of(up_sums), stride_of(sums),
+                                        dtype_of(&grad), grad.data_ptr(), row_bytes(grad), data(of_a), row, data(of_w), row, data(of_up), row,
+                                        biased ? code_of(bias_type) : nk_dtype_t(0), data(of_bias)};
+    nk_size_t const room = library.linear_backward_room(&l);
+    if (room) workspace = fresh({(int64_t)room}, at::kByte, a);
+    return library.linear_backward(&l, room ? workspace.data_ptr() : nullptr, room, stream_on(a));
+}
+Matrix plain(at::Tensor const *t) {
+    Matrix m;
+    m.t = t;
+    return m;
+}
+/** Both products: a, w, w_up, bias and residual are the inputs; the gradient of the residual alone does without the sums. */
+struct LinearWithGradient : torch::autograd::Function<LinearWithGradient> {
+    static at::Tensor forward(torch::autograd::AutogradContext *ctx, at::Tensor a, at::Tensor w, Maybe up, Maybe bias, Maybe residual, int64_t activation, at::ScalarType type) {
+        bool const keeps = up || (activation && (a.requires_grad() || w.requires_grad() || (bias && bias->requires_grad())));
+        at::Tensor c, pre, pre_up;
+        check(run_linear(plain(&a), plain(&w), plain(present(up)), present(bias), (int)activation, present(residual), type, keeps, c, pre, pre_up), "linear");
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({a, w, up ? *up : at::Tensor(), pre, pre_up});
+        ctx->saved_data["there"] = int64_t(3 | (up ? 4 : 0) | (bias ? 8 : 0) | (residual ? 16 : 0));
+        ctx->saved_data["activation"] = activation;
+        ctx->saved_data["bias"] = bias ? (int64_t)bias->scalar_type() : int64_t(-1);
+        ctx->saved_data["residual"] = residual ? (int64_t)residual->scalar_type() : int64_t(-1);
+        return c;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        torch::autograd::variable_list found(7);
+        if (!grads[0].defined()) return found;
+        auto const saved = ctx->get_saved_variables();
+        bool const need[4] = {needs(ctx, 0), needs(ctx, 1), needs(ctx, 2), needs(ctx, 3)};
+        int64_t const bias = ctx->saved_data["bias"].toInt(), residual = ctx->saved_data["residual"].toInt();
+        if (need[0] || need[1] || need[2] || need[3])
+            check(run_linear_backward(rows_of(grads[0]), saved[0], saved[1], present(saved[2]), present(saved[3]), present(saved[4]), (int)ctx->saved_data["activation"].toInt(), need[0], need[1],
+                                      need[2], bias >= 0 && need[3], bias >= 0 ? (at::ScalarType)bias : at::kFloat, found[0], found[1], found[2], found[3]),
+                  "linear_backward");
+        if (residual >= 0 && needs(ctx, 4)) found[4] = grads[0].to((at::ScalarType)residual);
+        return once(std::move(found));
+    }
+};
 
 /** linear(a, its scales or None, w, its or None, w_up or None, its or None, bias or None, activation, residual or None, dtype or None, sums)
  *  -> (y, sums or None, the other matrix's or None) */
@@ -206,22 +359,16 @@ PyObject *linear(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
     if (w.t->size(1) != depth || (a.scales && !mx8) || (!mx8 && a.t->scalar_type() != w.t->scalar_type()) || (mx8 && type == at::kFloat) ||
         (gated && (up.t->sizes() != w.t->sizes() || up.t->scalar_type() != w.t->scalar_type())) || !is_vector(bias, width) || !has_shape(residual, height, width))
         Py_RETURN_NONE;
-    at::Tensor c, pre, pre_up, workspace;
-    int status;
-    {
+    at::Tensor c, pre, pre_up;
+    int status = 0;
+    if (followed(a.scales ? nullptr : a.t, mx8 ? nullptr : w.t, mx8 ? nullptr : up.t, bias, residual)) {
+        int64_t const most = 1 << 22; // (the backward pass's)
+        if (mx8 || sums || height >= most || width >= most || depth >= most || w.t->scalar_type() == at::kFloat) Py_RETURN_NONE;
         WithoutLock unlocked;
-        at::AutoDispatchBelowADInplaceOrView guard;
-        c = fresh({height, width}, type, *a.t);
-        if (sums) pre = fresh({height, width}, at::kFloat, *a.t);
-        if (sums && gated) pre_up = fresh({height, width}, at::kFloat, *a.t);
-        nk_amd_linear_t const l = {(nk_size_t)height, (nk_size_t)width, (nk_size_t)depth, gated, a.dtype(), a.t->data_ptr(), row_bytes(*a.t), data_of(a.scales), stride_of(a.scales),
-                                   w.dtype(), w.t->data_ptr(), row_bytes(*w.t), data_of(w.scales), stride_of(w.scales), data_of(up.t), stride_of(up.t), data_of(up.scales),
-                                   stride_of(up.scales), (int)activation, dtype_of(bias), data_of(bias), dtype_of(residual), data_of(residual), stride_of(residual),
-                                   code_of(type), c.data_ptr(), row_bytes(c), sums ? (float *)pre.data_ptr() : nullptr, sums && gated ? (float *)pre_up.data_ptr() : nullptr,
-                                   sums ? (nk_size_t)width * 4 : 0};
-        nk_size_t const room = library.linear_room(&l);
-        if (room) workspace = fresh({(int64_t)room}, at::kByte, *a.t);
-        status = library.linear(&l, room ? workspace.data_ptr() : nullptr, room, stream_of(home));
+        c = LinearWithGradient::apply(*a.t, *w.t, maybe(up.t), maybe(bias), maybe(residual), activation, type);
+    } else {
+        WithoutLock unlocked;
+        status = run_linear(a, w, up, bias, (int)activation, residual, type, sums, c, pre, pre_up);
     }
     if (status) Py_RETURN_NONE;
     return Py_BuildValue("NNN", wrapped(c), wrapped(pre), wrapped(pre_up));
@@ -249,24 +396,12 @@ PyObject *linear_backward(PyObject *, PyObject *const *arguments, Py_ssize_t cou
         (sums && sums->scalar_type() != at::kFloat) || (up_sums && (up_sums->scalar_type() != at::kFloat || !sums || row_bytes(*sums) != row_bytes(*up_sums))) ||
         ((gated || activation) && !sums) || (gated && !up_sums))
         Py_RETURN_NONE;
-    at::Tensor of_a, of_w, of_up, of_bias, workspace;
+    if (followed(grad, a, w, up, sums, up_sums)) Py_RETURN_NONE;
+    at::Tensor of_a, of_w, of_up, of_bias;
     int status;
     {
         WithoutLock unlocked;
-        at::AutoDispatchBelowADInplaceOrView guard;
-        if (need_a) of_a = fresh({height, depth}, a->scalar_type(), *a);
-        if (need_w) of_w = fresh({width, depth}, a->scalar_type(), *a);
-        if (need_up && gated) of_up = fresh({width, depth}, a->scalar_type(), *a);
-        if (biased) of_bias = fresh({width}, bias_type, *a);
-        auto const data = [](at::Tensor const &t) { return t.defined() ? t.data_ptr() : nullptr; };
-        nk_size_t const row = (nk_size_t)depth * 2;
-        nk_amd_linear_backward_t const l = {(nk_size_t)height, (nk_size_t)width, (nk_size_t)depth, gated, dtype_of(a), a->data_ptr(), row_bytes(*a), w->data_ptr(), row_bytes(*w),
-                                            data_of(up), stride_of(up), (int)activation, (float const *)data_of(sums), (float const *)data_of(up_sums), stride_of(sums),
-                                            dtype_of(grad), grad->data_ptr(), row_bytes(*grad), data(of_a), row, data(of_w), row, data(of_up), row,
-                                            biased ? code_of(bias_type) : nk_dtype_t(0), data(of_bias)};
-        nk_size_t const room = library.linear_backward_room(&l);
-        if (room) workspace = fresh({(int64_t)room}, at::kByte, *a);
-        status = library.linear_backward(&l, room ? workspace.data_ptr() : nullptr, room, stream_of(home));
+        status = run_linear_backward(*grad, *a, *w, up, sums, up_sums, (int)activation, need_a, need_w, need_up, biased, bias_type, of_a, of_w, of_up, of_bias);
     }
     if (status) Py_RETURN_NONE;
     return Py_BuildValue("NNNN", wrapped(of_a), wrapped(of_w), wrapped(of_up), wrapped(of_bias));

@@ -80,7 +80,7 @@ def _library():
         except ImportError:  # built for another torch, or not at all
             _dense_calls = None
         else:
-            _dense_calls.bind(*(ctypes.cast(getattr(lib, "nk_amd_" + name), _vp).value for name, *_ in functions))
+            _dense_calls.bind(*(ctypes.cast(getattr(lib, name), _vp).value for name in (*("nk_amd_" + name for name, *_ in functions), "nk_hip_last_error")))
         _CALLS = _dense_calls
     return _LIB
 
