@@ -362,7 +362,12 @@ int launch_few_of(FewArgs const &p, bool gated, hipStream_t stream) {
     if (p.m <= 16) return gated ? launch_few<T, 1, 1, true, 4>(p, stream) : launch_few<T, 1, 1, false, 8>(p, stream);
     return gated ? launch_few<T, 2, 1, true, 4>(p, stream) : launch_few<T, 2, 1, false, 8>(p, stream);
 }
-constexpr uint64_t kFewRows = 32; // (48 x 8192 x 8192 bf16 took 76 us in such a kernel; tiles take 64 rows in 28)
+/**
+ *  Which products go there: those of up to 16 rows, and of up to 64 where the matrix is small. Each workgroup reads all of A, and every 32 rows all of its
+ *  columns, so that tiles win with size: 24 x 8192 x 8192 bf16 38.6 us here and 33 in tiles, 24 x 1024 x 8192 12.5 and 14, 64 x 2048 x 2048 10.9 in
+ *  tiles. (Whole passes over three sets of operands.)
+ */
+bool of_few_rows(uint64_t m, uint64_t n, uint64_t k, bool gated) { return m <= 16 || (m <= 64 && (double)m * (double)n * (double)k * (gated ? 2 : 1) <= 0x1p28); }
 
 // ---- tiles ---------------------------------------------------------------------------------------------------------
 
@@ -531,7 +536,7 @@ LinearLayout linear_layout(nk_amd_linear_t const *l) {
     auto const room = [&](uint64_t size) { uint64_t const at = end; return end += up_to(size, 256), at; };
     y.quantises = mx8 && l->a_dtype != nk_e4m3_k && l->depth;
     y.codes_stride = up_to(l->depth, 128), y.moved_stride = up_to(bytes, 128);
-    y.few = l->height <= kFewRows;
+    y.few = of_few_rows(l->height, l->width, l->depth, l->gated);
     if (y.quantises) y.a_at = room(l->height * y.codes_stride);
     if (y.few) {
         y.scales_stride = y.codes_stride / 32;
