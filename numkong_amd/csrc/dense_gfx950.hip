@@ -426,10 +426,8 @@ int launch_tiles(int dtype, TileForm form, TilePlan const &t, TileArgs p, float 
     return e == hipSuccess ? 0 : mx_fail(e, "join_kernel");
 }
 
-/** Can the tiles read these rows in place? `along`: the depth runs along them. */
-bool in_place(void const *values, uint64_t stride, uint64_t bytes, bool along) {
-    return !((uintptr_t)values & 3) && !(stride & 3) && stride <= kTileStride && (!along || bytes % 16 == 0);
-}
+/** Can the tiles read these rows in place? */
+bool in_place(void const *values, uint64_t stride) { return !((uintptr_t)values & 3) && !(stride & 3) && stride <= kTileStride; }
 
 // ---- the gradient of the sums --------------------------------------------------------------------------------------
 
@@ -544,9 +542,11 @@ LinearLayout linear_layout(nk_amd_linear_t const *l) {
         return y.bytes = end, y;
     }
     y.stages = (bytes + 127) / 128;
-    y.moves_a = !y.quantises && bytes && !in_place(l->a, l->a_stride, bytes, true);
-    y.moves_w = bytes && !in_place(l->w, l->w_stride, bytes, true);
-    y.moves_up = l->gated && bytes && !in_place(l->w_up, l->w_up_stride, bytes, true);
+    y.tiles = tile_plan(l->height, l->width, y.stages, l->gated);
+    bool const ends = y.tiles.shape < 2 || bytes % 16 == 0; // (the depth may end where it does)
+    y.moves_a = !y.quantises && bytes && !(ends && in_place(l->a, l->a_stride));
+    y.moves_w = bytes && !(ends && in_place(l->w, l->w_stride));
+    y.moves_up = l->gated && bytes && !(ends && in_place(l->w_up, l->w_up_stride));
     if (y.moves_a) y.a_at = room(l->height * y.moved_stride);
     if (y.moves_w) y.w_at = room(l->width * y.moved_stride);
     if (y.moves_up) y.up_at = room(l->width * y.moved_stride);
@@ -555,7 +555,6 @@ LinearLayout linear_layout(nk_amd_linear_t const *l) {
         y.a_words_at = room(y.stages * y.a_pitch * 4), y.w_words_at = room(y.stages * y.w_pitch * 4);
         if (l->gated) y.up_words_at = room(y.stages * y.w_pitch * 4);
     }
-    y.tiles = tile_plan(l->height, l->width, y.stages, l->gated);
     y.partial_at = room(partial_bytes(y.tiles, l->height, l->width, l->gated));
     return y.bytes = end, y;
 }
@@ -572,16 +571,16 @@ BackwardLayout backward_layout(nk_amd_linear_backward_t const *l) {
     uint64_t end = 0;
     auto const room = [&](uint64_t size) { uint64_t const at = end; return end += up_to(size, 256), at; };
     bool const gated = l->gated, some = l->height && l->width, of_a = l->grad_a && some && l->depth, of_w = (l->grad_w || l->grad_w_up) && some && l->depth;
-    y.writes_d = (of_a || of_w) && (gated || l->activation || l->grad_dtype != l->dtype || !in_place(l->grad, l->grad_stride, l->width * 2, true));
+    y.writes_d = (of_a || of_w) && (gated || l->activation || l->grad_dtype != l->dtype || l->width % 8 || !in_place(l->grad, l->grad_stride));
     y.sums = l->grad_bias != nullptr;
     y.padded = up_to(l->width, 64), y.d_stride = y.padded * 2 * (gated ? 2 : 1);
     y.rows_each = l->height <= 1u << 21 ? 64 : 128, y.partials = (l->height + y.rows_each - 1) / y.rows_each;
     if (y.writes_d) room(l->height * y.d_stride); // (at 0)
     if (y.sums) y.column_sums_at = room(y.partials * l->width * 4);
     y.moved_stride = up_to(l->depth * 2, 128);
-    y.moves_a = of_w && !in_place(l->a, l->a_stride, 0, false);
-    y.moves_w = of_a && !in_place(l->w, l->w_stride, 0, false);
-    y.moves_up = gated && of_a && !in_place(l->w_up, l->w_up_stride, 0, false);
+    y.moves_a = of_w && !in_place(l->a, l->a_stride);
+    y.moves_w = of_a && !in_place(l->w, l->w_stride);
+    y.moves_up = gated && of_a && !in_place(l->w_up, l->w_up_stride);
     if (y.moves_a) y.a_at = room(l->height * y.moved_stride);
     if (y.moves_w) y.w_at = room(l->width * y.moved_stride);
     if (y.moves_up) y.up_at = room(l->width * y.moved_stride);
@@ -646,8 +645,10 @@ int nk_amd_linear_async(nk_amd_linear_t const *l, void *workspace, nk_size_t wor
     }
     TileArgs p = {};
     p.m = (uint32_t)l->height, p.n = (uint32_t)l->width, p.stages = p.first_stages = (uint32_t)y.stages, p.e = e;
-    uint32_t const k = (uint32_t)(up_to(bytes, 16) / (mx8 ? 1 : 2)); // (what is moved or quantised ends with zeros)
-    p.a.extent = p.m, p.b.extent = p.n, p.a.k = p.b.k = k;
+    p.a.extent = p.m, p.b.extent = p.n, p.a.k = p.b.k = (uint32_t)l->depth;
+    uint32_t const whole = (uint32_t)(up_to(bytes, 16) / (mx8 ? 1 : 2)); // (what is moved or quantised ends with zeros)
+    if (y.quantises || y.moves_a) p.a.k = whole;
+    if (y.moves_w && (!gated || y.moves_up)) p.b.k = whole;
     p.a.pitch = (uint32_t)y.a_pitch, p.b.pitch = (uint32_t)y.w_pitch;
     p.a.values[0] = (uint8_t const *)l->a, p.a.stride[0] = l->a_stride;
     p.b.values[0] = (uint8_t const *)l->w, p.b.stride[0] = l->w_stride;

@@ -37,8 +37,7 @@ struct Epilogue {
 };
 
 /**
- *  One operand: `extent` rows (columns) of tiles and a depth of `k`; rows 4-byte aligned and at most 2^24 bytes apart, and where the depth runs along
- *  them it ends at a multiple of 16 bytes. Two addresses: the matrices of a gated product, or (columns) of two depths one behind the other. Scales of mx8: a word, four blocks, for each stage and
+ *  One operand: `extent` rows (columns) of tiles and a depth of `k`; rows 4-byte aligned and at most 2^24 bytes apart. Two addresses: the matrices of a gated product, or (columns) of two depths one behind the other. Scales of mx8: a word, four blocks, for each stage and
  *  row, [stage][pitch rows].
  */
 struct TileSide {
@@ -123,7 +122,7 @@ struct Bringer {
 #pragma unroll
             for (int i = 0; i < (PAIR ? 2 : 1); ++i) {
                 base[i] = its.values[i] + first * its.stride[i];
-                left[i] = (uint64_t)(its.extent - 1 - first) * its.stride[i] + bytes;
+                left[i] = (uint64_t)(its.extent - 1 - first) * its.stride[i] + (bytes + 3) / 4 * 4;
             }
         } else {
             row = wave * kEachLoad + l / kChunks, lane = ((l % kChunks) ^ swizzle(row)) * 16, beyond = 0;
@@ -161,6 +160,23 @@ struct Bringer {
             for (int i = 0; i < kLoads; ++i) {
                 uint32_t const r = row + i * 4 * kEachLoad;
                 fetch_16(from, to + (i * 4 + wave) * 1024, k0 + r >= side.k ? kNowhere : lane + r * (uint32_t)stride, 0);
+            }
+        }
+    }
+    /** Makes zeros, in the last stage of a depth that runs along the rows, of what stands between its end and the next 16 bytes: a thread a row. */
+    __device__ __forceinline__ void clear_tail(uint8_t *at) const {
+        if constexpr (!COLUMNS) {
+            uint32_t const tail = side.k * kValueBytes<T> % 128;
+            if (tail % 16 == 0) return;
+#pragma unroll
+            for (uint32_t r = threadIdx.x; r < WIDTH; r += 256) {
+                uint32_t *const piece = (uint32_t *)(at + r * 128 + ((tail / 16) ^ (r / 2 & 7)) * 16);
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    uint32_t const from = tail % 16;
+                    if (from <= i * 4) piece[i] = 0;
+                    else if (from < i * 4 + 4) piece[i] &= (1u << (from % 4 * 8)) - 1;
+                }
             }
         }
     }
@@ -304,9 +320,10 @@ __device__ __forceinline__ void arrive_and_meet() {
 /**
  *  A tile of 64 WM x 64 WN results (columns of both matrices, where gated). Loop over the stages: fragments of a step are read while the one before is
  *  multiplied; before the last step of a stage, whose fragments are in registers then, the wavefronts meet, the next stage has to be there, and the
- *  one after that is asked for into the array that has become free.
+ *  one after that is asked for into the array that has become free. TAIL: a depth along rows may end at any byte, not only at multiples of 16 (256 x 256
+ *  would spill with it: their operands are moved to where it does).
  */
-template <class T, int WM, int WN, bool A_COLUMNS, bool B_COLUMNS, bool GATED>
+template <class T, int WM, int WN, bool A_COLUMNS, bool B_COLUMNS, bool GATED, bool TAIL>
 __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void tile_kernel(TileArgs p) {
     constexpr int kRows = 64 * WM, kColumns = 64 * WN, kValues = 128 / kValueBytes<T>;
     constexpr bool kScaled = __is_same(T, Mx8);
@@ -348,6 +365,11 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void tile_kernel(TileArgs
         uint32_t const stages = s < end ? p.stages : 0;
         a.bring(to_a, s, stages, p.first_stages, wave);
         b.bring(to_b, s, stages, p.first_stages, wave);
+    };
+    auto const clear = [&](uint8_t *at_a, uint8_t *at_b, uint32_t s) { // stage `s` is there
+        if (!TAIL || s + 1 != p.stages) return;
+        a.clear_tail(at_a), b.clear_tail(at_b);
+        __syncthreads();
     };
     auto const read = [&](int to, uint8_t const *at_a, uint8_t const *at_b, int j) {
 #pragma unroll
@@ -403,6 +425,7 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void tile_kernel(TileArgs
             in_turn(Number<0>());
         }
         arrive_and_meet();
+        clear(next_a, next_b, s + 1);
         read(0, next_a, next_b, 0);
         bring(at_a, at_b, s + 2, slot);
         multiply(Number<1>());
@@ -412,6 +435,7 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void tile_kernel(TileArgs
     if (begin < end) {
         bring(a0, b0, begin, Number<0>());
         arrive_and_meet();
+        clear(a0, b0, begin);
         bring(a1, b1, begin + 1, Number<1>());
         read(0, a0, b0, 0);
         for (uint32_t s = begin; s < end; s += 2) { // (an odd number of stages ends with one of zeros)
@@ -516,20 +540,27 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void tile_kernel(TileArgs
 }
 
 /** Queues the kernel of a form; the grid is a workgroup for each tile and split. */
-template <class T, int WM, int WN, bool A_COLUMNS, bool B_COLUMNS, bool GATED>
+template <class T, int WM, int WN, bool A_COLUMNS, bool B_COLUMNS, bool GATED, bool TAIL>
 int launch_tile(TileArgs const &p, hipStream_t stream) {
-    hipLaunchKernelGGL((tile_kernel<T, WM, WN, A_COLUMNS, B_COLUMNS, GATED>), dim3(p.tiles_m * p.tiles_n * p.splits), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((tile_kernel<T, WM, WN, A_COLUMNS, B_COLUMNS, GATED, TAIL>), dim3(p.tiles_m * p.tiles_n * p.splits), dim3(256), 0, stream, p);
     hipError_t const e = hipGetLastError();
     return e == hipSuccess ? 0 : mx_fail(e, "tile_kernel");
 }
+template <class T, bool A_COLUMNS, bool B_COLUMNS, bool GATED, bool TAIL>
+int launch_shape(int shape, TileArgs const &p, hipStream_t stream) {
+    if (shape == 0) return launch_tile<T, 1, GATED ? 2 : 1, A_COLUMNS, B_COLUMNS, GATED, TAIL>(p, stream);
+    if (shape == 1) return launch_tile<T, 2, 2, A_COLUMNS, B_COLUMNS, GATED, TAIL>(p, stream);
+    if constexpr (TAIL) return mx_fail("tile_kernel: no such form");
+    else return launch_tile<T, 4, 4, A_COLUMNS, B_COLUMNS, GATED, false>(p, stream);
+}
 template <class T>
 int launch_tiles_of(TileForm const &f, TileArgs const &p, hipStream_t stream) {
-    if (f.gated) return f.shape == 0 ? launch_tile<T, 1, 2, false, false, true>(p, stream) : f.shape == 1 ? launch_tile<T, 2, 2, false, false, true>(p, stream) : launch_tile<T, 4, 4, false, false, true>(p, stream);
-    if (!f.b_columns) return f.shape == 0 ? launch_tile<T, 1, 1, false, false, false>(p, stream) : f.shape == 1 ? launch_tile<T, 2, 2, false, false, false>(p, stream) : launch_tile<T, 4, 4, false, false, false>(p, stream);
-    if constexpr (!__is_same(T, Mx8)) {
-        if (!f.a_columns) return f.shape == 0 ? launch_tile<T, 1, 1, false, true, false>(p, stream) : f.shape == 1 ? launch_tile<T, 2, 2, false, true, false>(p, stream) : launch_tile<T, 4, 4, false, true, false>(p, stream);
-        return f.shape == 0 ? launch_tile<T, 1, 1, true, true, false>(p, stream) : f.shape == 1 ? launch_tile<T, 2, 2, true, true, false>(p, stream) : launch_tile<T, 4, 4, true, true, false>(p, stream);
+    if (!f.b_columns) {
+        bool const tail = p.a.k * kValueBytes<T> % 16 || p.b.k * kValueBytes<T> % 16;
+        if (f.gated) return tail ? launch_shape<T, false, false, true, true>(f.shape, p, stream) : launch_shape<T, false, false, true, false>(f.shape, p, stream);
+        return tail ? launch_shape<T, false, false, false, true>(f.shape, p, stream) : launch_shape<T, false, false, false, false>(f.shape, p, stream);
     }
+    if constexpr (!__is_same(T, Mx8)) return f.a_columns ? launch_shape<T, true, true, false, false>(f.shape, p, stream) : launch_shape<T, false, true, false, false>(f.shape, p, stream);
     return mx_fail("tile_kernel: no such form");
 }
 int launch_tiles_bf16(TileForm const &, TileArgs const &, hipStream_t);

@@ -194,8 +194,8 @@ struct Raw {
 
 /**
  *  Threads (x) share a row, rows (y) a workgroup, as forward; a workgroup has every gridDim.x-th of such groups and keeps its part of the weight's
- *  gradient in registers until the last. Rows of at most 8192 values of 16 bits (HALF: all operands) are asked for before the one before is worked on; of others
- *  two do not fit the registers. Memory is what bounds it (8192 x 4096 bf16
+ *  gradient in registers until the last. Rows of at most 8192 values are asked for before the one before is worked on (of longer ones two do
+ *  not fit the registers; HALF: all operands are of 16 bits). Memory is what bounds it (8192 x 4096 bf16
  *  with the total's gradient: 62 us without the weight's, 113 with it, when rows were loaded in turn and 1024 parts added up by 128 workgroups).
  */
 template <class T, int P, bool HALF>
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(NormBackwardArg
     __shared__ float sums[2][16][2];
     extern __shared__ float parts[]; // rows of a workgroup but the first: theirs of the weight's gradient
     float of_weight[P][8] = {};
-    constexpr bool kAhead = HALF && P == 1;
+    constexpr bool kAhead = P == 1;
     Raw<HALF> w, ahead[3];
     auto const load_weight = [&](uint32_t col) { if (p.weight) w.load(p.weight_kind, (uint8_t const *)p.weight, col, p.k); };
     auto const load_row = [&](uint64_t row, uint32_t col, Raw<HALF> (&raw)[3], bool rest) { // total, gradient, the total's gradient
@@ -329,10 +329,10 @@ int with_float(int dtype, Call call) {
     return dtype == nk_f32_k ? call(float()) : dtype == nk_bf16_k ? call(__bf16()) : call(_Float16());
 }
 
-/** Workgroups of a backward pass: what 1024 threads a compute unit are, or groups of rows, if there are fewer. */
+/** Workgroups of a backward pass: as many as run at once, with 1024 threads a compute unit, or groups of rows, if there are fewer. */
 uint32_t norm_backward_workgroups(uint64_t rows, uint64_t k) {
     NormShape const shape = norm_shape(k);
-    uint64_t const groups = (rows + shape.rows - 1) / shape.rows, most = 256 * 1024 / (shape.threads * shape.rows);
+    uint64_t const groups = (rows + shape.rows - 1) / shape.rows, most = 256 * (1024 / (shape.threads * shape.rows));
     return (uint32_t)(groups < most ? groups : most);
 }
 
