@@ -133,7 +133,8 @@ __global__ __launch_bounds__(256) void join_kernel(float const *partial, uint32_
     if (row >= m) return;
     uint32_t const col = (uint32_t)(at - row * each) * 8;
     float v[1][8] = {}, q[1][8] = {};
-    for (uint32_t i = 0; i < splits; ++i) {
+#pragma unroll 4
+    for (uint32_t i = 0; i < splits; ++i) { // (several parts on their way at a time)
         float part[8];
         load_adjacent(partial + i * plane * (GATED ? 2 : 1) + row * n, col, n, part);
 #pragma unroll
@@ -574,7 +575,10 @@ BackwardLayout backward_layout(nk_amd_linear_backward_t const *l) {
     y.writes_d = (of_a || of_w) && (gated || l->activation || l->grad_dtype != l->dtype || l->width % 8 || !in_place(l->grad, l->grad_stride));
     y.sums = l->grad_bias != nullptr;
     y.padded = up_to(l->width, 64), y.d_stride = y.padded * 2 * (gated ? 2 : 1);
-    y.rows_each = l->height <= 1u << 21 ? 64 : 128, y.partials = (l->height + y.rows_each - 1) / y.rows_each;
+    // Rows of a workgroup that makes d: 64 (128, where a grid would be too high), fewer until there are 1024 workgroups (343 x 1150 gated: 51 us with 64).
+    y.rows_each = l->height <= 1u << 21 ? 64 : 128;
+    while (y.rows_each > 4 && (l->height + y.rows_each - 1) / y.rows_each * ((y.padded + 511) / 512) < 1024) y.rows_each /= 2;
+    y.partials = (l->height + y.rows_each - 1) / y.rows_each;
     if (y.writes_d) room(l->height * y.d_stride); // (at 0)
     if (y.sums) y.column_sums_at = room(y.partials * l->width * 4);
     y.moved_stride = up_to(l->depth * 2, 128);

@@ -175,13 +175,14 @@ struct Raw {
             if (size == 4) high = *(v4u_anywhere const *)(at + 16);
             return;
         }
-        low = high = v4u {0, 0, 0, 0};
+        uint32_t words[8] = {};
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i)
             if (col + i < k) {
-                if (size == 4) (i < 4 ? low : high)[i % 4] = ((uint32_t const *)at)[i];
-                else low[i / 2] |= (uint32_t)((uint16_t const *)at)[i] << 16 * (i % 2);
+                if (size == 4) words[i] = ((uint32_t const *)at)[i];
+                else words[i / 2] |= (uint32_t)((uint16_t const *)at)[i] << 16 * (i % 2);
             }
+        low = v4u {words[0], words[1], words[2], words[3]}, high = v4u {words[4], words[5], words[6], words[7]};
     }
     __device__ __forceinline__ void widen_to(uint32_t kind, float (&v)[8]) const {
         if (!HALF && kind == kF32) {
