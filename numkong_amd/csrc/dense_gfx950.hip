@@ -380,9 +380,10 @@ struct TilePlan {
  *  The shape of tiles and the splits of the depth that take the least time by a simple account, in microseconds of a compute unit, from what was
  *  measured with bf16: a stage of a workgroup that is alone (512 x 4096 x 4096 and 64 x 8192 x 8192), one among as many as fit (8192 x 8192 by depths of 64 to
  *  4096), what a tile's beginning and end add, and a launch and the partial sums' way through memory where there are splits. It is within a
- *  sixth of the times of ten products between 64 x 8192 x 8192 and 4096 x 4096 x 1024.
+ *  sixth of the times of ten products between 64 x 8192 x 8192 and 4096 x 4096 x 1024. The transposing reads of depths along columns cost tiles of 128 rows more (the
+ *  gradient of 4096 x 2048 over 16384: 316 us in such tiles).
  */
-TilePlan tile_plan(uint64_t m, uint64_t n, uint64_t stages, bool gated) {
+TilePlan tile_plan(uint64_t m, uint64_t n, uint64_t stages, bool gated, bool b_columns = false) {
     static constexpr double kAlone[3] = {0.45, 0.57, 1.48}, kEach[3] = {0.173, 0.442, 1.48}, kEnds[3] = {0.8, 2.5, 13.5};
     static constexpr uint64_t kResident[3] = {4, 2, 1};
     uint64_t const found = (uint64_t)compute_unit_count(), units = found ? found : 256; // (a size may be asked for where there is no GPU)
@@ -391,7 +392,7 @@ TilePlan tile_plan(uint64_t m, uint64_t n, uint64_t stages, bool gated) {
     for (int shape = 0; shape < 3; ++shape) {
         uint64_t const rows = 64u << shape, columns = gated ? (shape == 2 ? 128 : 64) : rows;
         uint64_t const tiles = ((m + rows - 1) / rows) * ((n + columns - 1) / columns);
-        double const each = gated && shape == 0 ? 0.3 : kEach[shape];
+        double const each = gated && shape == 0 ? 0.3 : b_columns && shape == 1 ? 0.54 : kEach[shape];
         auto const together = [&](uint64_t workgroups) { return workgroups * each > kAlone[shape] ? workgroups * each : workgroups ? kAlone[shape] : 0.0; };
         for (uint64_t splits = 1; splits <= 16; splits *= 2) {
             if (splits > 1 && (stages < splits * 4 || tiles * splits > units * 4)) break;
@@ -589,7 +590,7 @@ BackwardLayout backward_layout(nk_amd_linear_backward_t const *l) {
     if (y.moves_w) y.w_at = room(l->width * y.moved_stride);
     if (y.moves_up) y.up_at = room(l->width * y.moved_stride);
     y.first_stages = y.padded / 64, y.stages = y.first_stages * (gated ? 2 : 1);
-    y.of_a = tile_plan(l->height, l->depth, y.stages, false), y.of_w = tile_plan(l->width, l->depth, (l->height + 63) / 64, false);
+    y.of_a = tile_plan(l->height, l->depth, y.stages, false, true), y.of_w = tile_plan(l->width, l->depth, (l->height + 63) / 64, false, true);
     uint64_t const a_bytes = of_a ? partial_bytes(y.of_a, l->height, l->depth, false) : 0, w_bytes = of_w ? partial_bytes(y.of_w, l->width, l->depth, false) : 0;
     y.partial_at = room(a_bytes > w_bytes ? a_bytes : w_bytes);
     return y.bytes = end, y;
