@@ -721,10 +721,12 @@ int nk_amd_linear_backward_async(nk_amd_linear_backward_t const *l, void *worksp
             uint64_t const rows = i ? l->width : l->height, stride = i == 0 ? l->grad_a_stride : i == 1 ? l->grad_w_stride : l->grad_w_up_stride;
             void *const to = i == 0 ? l->grad_a : i == 1 ? l->grad_w : l->grad_w_up;
             if (!to || !rows || !l->depth) continue;
-            FewArgs p = {}; // (no depth: zeros)
-            p.m = (uint32_t)rows, p.n = (uint32_t)l->depth;
-            p.e.c = (uint8_t *)to, p.e.c_stride = stride, p.e.c_kind = kind;
-            if (int const status = launch_few<__bf16, 2, 1, false, 8>(p, stream)) return status;
+            for (uint64_t first = 0; first < rows; first += 1u << 20) { // (a grid is at most 65535 high)
+                FewArgs p = {};                                          // (no depth: zeros)
+                p.m = (uint32_t)(rows - first < 1u << 20 ? rows - first : 1u << 20), p.n = (uint32_t)l->depth;
+                p.e.c = (uint8_t *)to + first * stride, p.e.c_stride = stride, p.e.c_kind = kind;
+                if (int const status = launch_few<__bf16, 2, 1, false, 8>(p, stream)) return status;
+            }
         }
         return 0;
     }

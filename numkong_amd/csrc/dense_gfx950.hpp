@@ -163,8 +163,7 @@ __device__ __forceinline__ float scale_of(uint32_t byte) {
 
 /**
  *  Activations and their slopes in 32 bits, off by a few units in the last place. The sigmoid is 1 / (1 + e^-x) by the part's own 2^x and reciprocal
- *  (one unit each; the library's forms cost three times the instructions, and tiles would wait for them: f16 8192 x 8191 x 1000 with relu in a
- *  switch for each value and these took 60 us more). The tanh of gelu_tanh is written as 1 - 2 / (1 + e^2z), so that 0.5 x (1 + tanh z) = x / (1 + e^-2z).
+ *  (one unit each; with the library's forms, chosen by a switch for each value, bias and relu of f16 8192 x 8191 x 1000 took 60 us more). The tanh of gelu_tanh is written as 1 - 2 / (1 + e^2z), so that 0.5 x (1 + tanh z) = x / (1 + e^-2z).
  *  Gelu: with h = erfc(|x| / sqrt 2) / 2 it is x - x h, or x h below zero, and h = e^(-x^2/2) t P(t), t = 1 / (1 + 0.35 |x|): P is fitted
  *  to that quotient over all |x| <= 16 by least squares weighted towards the largest relative error (8 degrees, 5 units of 2^-24 with its
  *  evaluation). What is beyond +-16 (+-110 for slopes) is at its limit.

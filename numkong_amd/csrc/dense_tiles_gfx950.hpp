@@ -9,15 +9,18 @@
  *               lanes of a fragment, which read as many rows, meet no bank twice
  *      columns  the depth runs from row to row (the gradients' operands): LDS holds 64 rows of the tile's columns, and the reads that
  *               transpose (ds_read_b64_tr_b16: of 16 lanes, four rows of 16 columns) give each lane its column; position p of row r holds
- *               the 16 bytes p ^ 4 (r % 4)
+ *               the 16 bytes p ^ 4 (r % 4), or, in rows of 64 columns, p ^ 4 (r / 2 % 2)
  *
  *  Which depth is in which place of a fragment is the same for both, 8 adjacent values a lane, so either kind meets either. Of 8-bit values the
  *  instruction takes 64 of the depth, a lane 16 of its first 32 and 16 of its second, and the scale of row or column l % 32 for block l / 32
  *  from lane l: two fragments one behind the other.
  *
  *  The products are made transposed (the matrix instruction's rows are C's columns), so that a lane has four adjacent results of one
- *  row; 32 rows at a time they go through LDS, where eight adjacent ones of a row come together: bias, activation and residual are
+ *  row; 64 rows at a time they go through LDS, where adjacent ones of a row come together: bias, activation and residual are
  *  added there, in 32 bits, and whole lines are written.
+ *
+ *  Measured: 256 x 256 bf16 8192 x 8192 x 4096 416 us (1.32 PFLOP/s), 8192^3 797 us (1.38), gated 8192 x 8192 x 4096 832 us; columns 8192 x 4096 x 4096 206 us (both operands)
+ *  and 216 (one); 8 bits 8192^3 400 us (2.75). Power bounds them: matrix instructions take 65 % of the cycles at 1.6 to 1.9 GHz, waits 10 to 14 %.
  */
 #ifndef NUMKONG_AMD_DENSE_TILES_GFX950_HPP
 #define NUMKONG_AMD_DENSE_TILES_GFX950_HPP

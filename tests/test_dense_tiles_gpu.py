@@ -157,6 +157,13 @@ def test_empty_ones_have_gradients():
         assert of_x.shape == x.shape and (m or not of_scale.any())
 
 
+def test_gradients_of_many_rows_without_width():
+    m = (1 << 21) + 70000  # more rows than one grid of the kernel that writes the zeros is high
+    a, w = torch.ones((m, 24), dtype=torch.float16, device=DEV), torch.empty((0, 24), dtype=torch.float16, device=DEV)
+    of_a, of_w, _ = nk.linear_backward(torch.empty((m, 0), dtype=torch.float16, device=DEV), a, w)
+    assert of_a.shape == a.shape and not of_a.any() and of_w.shape == w.shape
+
+
 def test_gradients_have_none_of_their_own_and_say_so():
     x, w = (normal(20, 64, torch.float16, seed).to(DEV).requires_grad_() for seed in (1, 2))
     for y in (nk.linear(x, w, activation="silu"), nk.gated_linear(x, w, w), nk.rms_norm(x, w[0])):
