@@ -17,8 +17,8 @@
  *  allocates nor synchronises, may be captured into a HIP graph (after one eager call, which loads the kernels), and returns 0
  *  or a status that `nk_hip_last_error()` explains; a refused call has queued nothing. Strides are in bytes; results share memory
  *  neither with one another nor with operands, unless it says so. A workspace is device memory, 256-byte aligned, of the
- *  bytes that the call's `*_workspace_size` says (0: NULL will do), and belongs to the call until the stream has run it. Sums are
- *  held in 32 bits; no result depends on the order in which workgroups run.
+ *  bytes that the call's `*_workspace_size` says of the very same structure (addresses and strides count; 0: NULL will do), and belongs to
+ *  the call until the stream has run it. Sums are held in 32 bits; no result depends on the order in which workgroups run.
  */
 #ifndef NUMKONG_AMD_DENSE_H
 #define NUMKONG_AMD_DENSE_H
