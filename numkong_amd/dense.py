@@ -464,6 +464,34 @@ def _operand(m, codes):
     return codes[m.dtype], m.data_ptr(), _row_bytes(m), None, 0
 
 
+def _rows_in_memory(t):
+    """(address, rows, bytes from one to the next, bytes of one) of a vector or matrix."""
+    rows = t.shape[0] if t.dim() == 2 else 1
+    return t.data_ptr(), rows, _row_bytes(t) if t.dim() == 2 else 0, t.shape[-1] * t.itemsize
+
+
+def _share_memory(x, y) -> bool:
+    """Do two operands have bytes in common? (Rows that lie between one another's, at one distance, have none.)"""
+    if not x.numel() or not y.numel():
+        return False
+    (x0, x_rows, x_step, x_size), (y0, y_rows, y_step, y_size) = _rows_in_memory(x), _rows_in_memory(y)
+    if x0 + (x_rows - 1) * x_step + x_size <= y0 or y0 + (y_rows - 1) * y_step + y_size <= x0:
+        return False
+    if x_step != y_step or x_step < max(x_size, y_size):
+        return True
+    return (y0 - x0) % x_step < x_size or (x0 - y0) % x_step < y_size
+
+
+def _check_out_alone(out, residual, **operands):
+    """A result may be its residual, but no other operand: workgroups read those at any time."""
+    if residual is not None and _share_memory(out, residual) and (out.data_ptr(), out.dtype, _row_bytes(out)) != (residual.data_ptr(), residual.dtype, _row_bytes(residual)):
+        raise ValueError("out shares memory with residual, but is not residual itself")
+    for name, m in operands.items():
+        for t in (m.codes, m.scales) if isinstance(m, Mx8Matrix) else () if m is None else (m,):
+            if _share_memory(out, t):
+                raise ValueError(f"out shares memory with {name}")
+
+
 def _parts(m):
     """An operand and its scales, if it has any."""
     return (m.codes, m.scales) if type(m) is Mx8Matrix else (m, None)
@@ -476,6 +504,8 @@ def _multiply(a, w, w_up, bias, activation, residual, out, out_dtype, sums, wher
     width, device = w.shape[0], a.device
     like = a.codes if isinstance(a, Mx8Matrix) else a
     result = _result(torch, out, (height, width), out_dtype, like)
+    if out is not None:
+        _check_out_alone(result, residual, a=a, w=w, w_up=w_up, bias=bias)
     kept = [mx._new(torch, height, width, torch.float32, device) for _ in range(0 if not sums else 1 if w_up is None else 2)]
     l = _Linear(height, width, depth, w_up is not None, *_operand(a, dtype_codes), *_operand(w, dtype_codes), *_operand(w_up, dtype_codes)[1:], activation,
                 0 if bias is None else dtype_codes[bias.dtype], _address(bias), 0 if residual is None else dtype_codes[residual.dtype],
@@ -498,7 +528,7 @@ def linear(a, w, bias=None, activation=None, residual=None, out=None, out_dtype=
     are bfloat16 or float16 alike, or ``w`` is an ``Mx8Matrix`` and ``a`` is one too, or floats that are quantised on the way exactly as
     ``mx8_quantize`` does. ``activation``: None, "relu", "silu", "gelu" (erf's) or "gelu_tanh"; ``bias`` (width) and ``residual`` (height x
     width) are floats of any type. The result has ``out_dtype`` (or ``out``'s; default: ``a``'s type), 16 bits where ``w`` is 8-bit;
-    ``out`` may be the residual itself.
+    ``out`` may be the residual itself, and shares memory with no other operand.
 
     16-bit products have gradients for ``a``, ``w``, ``bias`` and ``residual``, which autograd follows; 8-bit ones have none and refuse
     operands that require one while autograd records. With ``sums`` the result is ``(y, a @ w.T + bias)``, as ``linear_backward`` takes them."""

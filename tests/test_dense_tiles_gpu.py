@@ -157,6 +157,26 @@ def test_empty_ones_have_gradients():
         assert of_x.shape == x.shape and (m or not of_scale.any())
 
 
+def test_results_over_operands_are_refused():
+    store = torch.zeros((64, 200), dtype=torch.bfloat16, device=DEV)
+    a, w = store[:, :64], torch.ones((64, 64), dtype=torch.bfloat16, device=DEV)
+    for call in (lambda out: nk.linear(a, w, out=out), lambda out: nk.gated_linear(a, w, w, out=out)):
+        for out in (a, store[:, 10:74], store[:, 63:127], w):
+            with pytest.raises(ValueError, match="shares memory"):
+                call(out)
+        call(store[:, 64:128])  # rows between those of A
+        assert not store.any()
+    with pytest.raises(ValueError, match="residual itself"):
+        nk.linear(a, w, residual=store[:, 70:134], out=store[:, 71:135])
+    row = torch.zeros(64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="bias"):
+        nk.linear(a[:1], w, row, out=row[None])
+    m = nk.mx8_quantize(w)
+    over = torch.empty(0, dtype=torch.bfloat16, device=DEV).set_(m.codes.untyped_storage(), 0, (32, 64), (64, 1))  # the codes' memory
+    with pytest.raises(ValueError, match="shares memory with w"):
+        nk.linear(a[:32], m, out=over)
+
+
 def test_gradients_of_many_rows_without_width():
     m = (1 << 21) + 70000  # more rows than one grid of the kernel that writes the zeros is high
     a, w = torch.ones((m, 24), dtype=torch.float16, device=DEV), torch.empty((0, 24), dtype=torch.float16, device=DEV)
