@@ -451,7 +451,8 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void tile_kernel(TileArgs
     // has the same columns in all of them: eight, or four where C is of 32 bits and so written in whole lines (8192 x 8192 x 64 to f32: 82 us, and
     // 93 with eight, two stores with gaps; to bf16 72 and 57; with the sums for the gradients beside bf16 eight again, 8192 x 4096 x 4096 282 and 328).
     // Two or four rows are finished at a time.
-    __syncthreads();
+    // (The arrays are free once every wavefront's loads into them have arrived: those of the stages past the end bring zeros.)
+    arrive_and_meet();
     constexpr int kHigh = WM < 2 ? WM : 2;
     constexpr uint32_t kWidth = WN * 32, kPieces = kWidth / 4, kOut = GATED ? kWidth / 2 : kWidth; // kOut: results of a row
     float *const room = (float *)(wave == 0 ? a0 : wave == 1 ? a1 : wave == 2 ? b0 : b1);
