@@ -372,6 +372,8 @@ bool of_few_rows(uint64_t m, uint64_t n, uint64_t k, bool gated) { return m <= 1
 
 // ---- tiles ---------------------------------------------------------------------------------------------------------
 
+constexpr uint64_t kMostTiles = (1ull << 24) - 1; // of a launch, which has fewer than 2^32 threads
+
 struct TilePlan {
     int shape;
     uint32_t splits, split_stages;
@@ -392,6 +394,7 @@ TilePlan tile_plan(uint64_t m, uint64_t n, uint64_t stages, bool gated, bool b_c
     for (int shape = 0; shape < 3; ++shape) {
         uint64_t const rows = 64u << shape, columns = gated ? (shape == 2 ? 128 : 64) : rows;
         uint64_t const tiles = ((m + rows - 1) / rows) * ((n + columns - 1) / columns);
+        if (tiles > kMostTiles) continue; // (2^30 x 8 in tiles of 64 rows)
         double const each = gated && shape == 0 ? 0.3 : b_columns && shape == 1 ? 0.54 : kEach[shape];
         auto const together = [&](uint64_t workgroups) { return workgroups * each > kAlone[shape] ? workgroups * each : workgroups ? kAlone[shape] : 0.0; };
         for (uint64_t splits = 1; splits <= 16; splits *= 2) {
@@ -405,10 +408,10 @@ TilePlan tile_plan(uint64_t m, uint64_t n, uint64_t stages, bool gated, bool b_c
     }
     return best;
 }
-/** Are there more results than the tiles of one launch make? */
+/** Are there more results than the tiles of one launch make? (Then those of every shape are too many.) */
 bool too_many(TilePlan const &t, uint64_t m, uint64_t n, bool gated) {
     uint64_t const rows = 64u << t.shape, columns = gated ? (t.shape == 2 ? 128 : 64) : rows;
-    return ((m + rows - 1) / rows) * ((n + columns - 1) / columns) * t.splits * 256 >= (1ull << 32);
+    return ((m + rows - 1) / rows) * ((n + columns - 1) / columns) * t.splits > kMostTiles;
 }
 uint64_t partial_bytes(TilePlan const &t, uint64_t m, uint64_t n, bool gated) { return t.splits > 1 ? up_to(t.splits * m * n * (gated ? 8 : 4), 256) : 0; }
 

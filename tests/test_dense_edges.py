@@ -2,8 +2,15 @@
 import os
 import re
 
+import pytest
+import torch
+
+from numkong_amd import api
+from numkong_amd import dense as binding
 from tests import support
 
+BF16, F16, E4M3 = api.NK_BF16, api.NK_F16, api.NK_E4M3
+SOME = 1 << 20  # an address that no refused call reads
 CSRC = os.path.join(support.ROOT, "numkong_amd", "csrc")
 
 
@@ -17,3 +24,25 @@ def test_tiles_wait_for_every_load_into_lds_before_they_put_sums_there():
     behind = kernel[kernel.index("stage(a1, b1, a0, b0, s + 1"):]
     before_sums = re.sub(r"//.*", "", behind[:behind.index("float *const room")])
     assert "arrive_and_meet();" in before_sums and "__syncthreads" not in before_sums and "s_barrier" not in before_sums
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="what is not refused would run, on addresses of nothing")
+@pytest.mark.parametrize("height,width,depth,gated", [(1 << 30, 8, 64, 0), ((1 << 31) - 1, 1, 64, 0), (1 << 30, 64, 128, 1), (17, (1 << 31) - 128, 64, 1), (70, (1 << 31) - 1, 64, 0)])
+def test_many_short_rows_are_not_refused_for_tiles_that_others_hold(height, width, depth, gated):
+    """Tiles of 64 rows would be 2^24 or more, which no launch has; those of 128 or 256 fit. (Without a GPU the launch is what fails.)"""
+    lib = binding._library()[0]
+    l = binding._Linear(height=height, width=width, depth=depth, gated=gated, a_dtype=BF16, a=SOME, a_stride=256, w_dtype=BF16, w=SOME, w_stride=256,
+                        w_up=SOME if gated else None, w_up_stride=256, c_dtype=BF16, c=SOME, c_stride=width * 2)
+    needed = lib.nk_amd_linear_workspace_size(l)
+    assert lib.nk_amd_linear_async(l, SOME, needed, None) != 0
+    message = lib.nk_hip_last_error().decode()
+    assert "more results" not in message and "tile_kernel" in message
+
+
+@pytest.mark.parametrize("height,width", [(17, (1 << 31) - 127), (1 << 30, 1 << 20)])
+def test_results_of_more_tiles_than_a_launch_has_are_refused(height, width):
+    lib = binding._library()[0]
+    l = binding._Linear(height=height, width=width, depth=64, gated=1, a_dtype=BF16, a=SOME, a_stride=128, w_dtype=BF16, w=SOME, w_stride=128, w_up=SOME, w_up_stride=128,
+                        c_dtype=BF16, c=SOME, c_stride=width * 2)
+    assert lib.nk_amd_linear_async(l, SOME, lib.nk_amd_linear_workspace_size(l), None) != 0
+    assert "more results" in lib.nk_hip_last_error().decode()
