@@ -35,12 +35,13 @@ struct Home {
         return t.get_device() == index;
     }
 };
-/** The tensor that an argument is, if it is one on that GPU, of `dims` dimensions, its rows of adjacent values. */
+/** The tensor that an argument is, if it is one on that GPU, of `dims` dimensions, its rows of adjacent values, without a tangent. */
 at::Tensor const *tensor_of(PyObject *argument, int64_t dims, Home &home) {
     if (!THPVariable_CheckExact(argument)) return nullptr;
     at::Tensor const &t = THPVariable_Unpack(argument);
     if (!home.has(t) || t.layout() != at::kStrided || t.dim() != dims) return nullptr;
     if (dims && t.size(dims - 1) > 1 && t.stride(dims - 1) != 1) return nullptr;
+    if (t._fw_grad(0).defined()) return nullptr; // (forward mode: the Python side refuses it)
     return &t;
 }
 nk_dtype_t code_of(at::ScalarType type) {

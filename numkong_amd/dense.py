@@ -7,7 +7,8 @@ row. ``mx8_quantize`` makes one, ``rms_norm_mx8`` gives its result as one, and a
 
 Operands live in GPU memory, and the work is queued on torch's current stream of their device, without waiting for it, as
 torch's own calls are; workspaces come from torch's allocator for that stream. Operands in host memory (numpy arrays, torch
-CPU tensors) are copied to the current GPU, and the result back: those calls return when it is there.
+CPU tensors) are copied to the current GPU, and the result back: those calls return when it is there. There are no forward-mode
+derivatives: operands with a tangent are refused.
 """
 from __future__ import annotations
 

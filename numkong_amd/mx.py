@@ -145,7 +145,9 @@ def _autograd():
 
 
 def _tracked(torch, *operands) -> bool:
-    """Does autograd follow one of the operands?"""
+    """Does autograd follow one of the operands? One that has a tangent is refused (torch.no_grad() does not end forward mode, so it is not asked)."""
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in operands):
+        raise NumKongAmdError("the operators have no forward-mode derivatives: an operand has a tangent, unpack it (torch.autograd.forward_ad.unpack_dual)")
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands)
 
 

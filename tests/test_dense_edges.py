@@ -5,6 +5,7 @@ import re
 import pytest
 import torch
 
+import numkong_amd as nk
 from numkong_amd import api
 from numkong_amd import dense as binding
 from tests import support
@@ -46,3 +47,18 @@ def test_results_of_more_tiles_than_a_launch_has_are_refused(height, width):
                         c_dtype=BF16, c=SOME, c_stride=width * 2)
     assert lib.nk_amd_linear_async(l, SOME, lib.nk_amd_linear_workspace_size(l), None) != 0
     assert "more results" in lib.nk_hip_last_error().decode()
+
+
+def test_operands_with_a_tangent_are_refused():
+    """Forward mode, which torch.no_grad() does not end: the results would carry no tangent on."""
+    forward = torch.autograd.forward_ad
+    x = torch.ones((2, 8), dtype=torch.bfloat16)
+    assert not binding._tracked(torch, x, None) and binding._tracked(torch, x.clone().requires_grad_(), None)
+    with forward.dual_level():
+        dual = forward.make_dual(x, torch.ones_like(x))
+        for operands in ((dual,), (None, x, dual)):
+            with pytest.raises(nk.NumKongAmdError, match="forward-mode"):
+                binding._tracked(torch, *operands)
+            with torch.no_grad(), pytest.raises(nk.NumKongAmdError, match="forward-mode"):
+                binding._tracked(torch, *operands)
+        assert not binding._tracked(torch, x, forward.unpack_dual(dual).primal)

@@ -19,3 +19,34 @@ def test_more_short_rows_than_one_launch_has_tiles_of_64():
     y = nk.linear(a, w, activation="relu")
     some = torch.cat([torch.arange(300, device=DEV), rows - 1 - torch.arange(300, device=DEV), torch.randint(0, rows, (4000,), device=DEV, generator=torch.Generator(DEV).manual_seed(3))])
     ds.Linear(a[some].double().cpu(), w.double().cpu(), activation="relu").check(y[some])
+
+
+def test_operands_with_a_tangent_are_refused():
+    forward = torch.autograd.forward_ad
+    x, w, v = (normal(m, 64, torch.bfloat16, m).to(DEV) for m in (5, 64, 1))
+    v, w8, logits = v[0], nk.mx8_quantize(w), normal(5, 8, torch.float32, 9).to(DEV)
+    packed = nk.mx_pack(nk.mx_quantize(w))
+    stack = nk.mx_pack(w.expand(8, 64, 64).contiguous())
+    weights, chosen = nk.experts_route(logits, 2)
+    plan = nk.experts_plan(chosen, 8)
+    calls = [  # every operand that could have a derivative, in turn
+        (lambda t: nk.rms_norm(t, v, x), x), (lambda t: nk.rms_norm(x, t), v), (lambda t: nk.rms_norm(x, v, t), x), (lambda t: nk.rms_norm_mx8(t, v), x),
+        (lambda t: nk.rms_norm_mx8(x, t), v), (lambda t: nk.linear(t, w), x), (lambda t: nk.linear(x, t, activation="gelu"), w), (lambda t: nk.linear(x, w, t), v),
+        (lambda t: nk.linear(x, w, residual=t), x), (lambda t: nk.linear(t, w8), x), (lambda t: nk.linear(x, w8, t), v), (lambda t: nk.gated_linear(t, w, w), x),
+        (lambda t: nk.gated_linear(x, t, w), w), (lambda t: nk.gated_linear(x, w, t), w), (lambda t: nk.gated_linear(t, w8, w8), x),
+        (lambda t: nk.mx_dots_packed(t, packed), x), (lambda t: nk.experts_route(t, 2), logits), (lambda t: nk.mx_dots_experts(t, stack, plan), x),
+        (lambda t: nk.mx_dots_experts(x, stack, plan, t), weights),
+    ]
+    with forward.dual_level():
+        for call, t in calls:
+            call(t)
+            dual = forward.make_dual(t, torch.ones_like(t))
+            with pytest.raises(nk.NumKongAmdError, match="forward-mode"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(nk.NumKongAmdError, match="forward-mode"):
+                call(dual)
+            with pytest.raises(nk.NumKongAmdError, match="forward-mode"):
+                call(forward.make_dual(t.clone().requires_grad_(), torch.ones_like(t)))
+        same = forward.make_dual(x, torch.ones_like(x))
+        codes = nk.mx8_quantize(same)  # (numbers that no gradient passes)
+        assert torch.equal(codes.codes.view(torch.uint8), nk.mx8_quantize(x).codes.view(torch.uint8))
