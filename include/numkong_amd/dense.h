@@ -118,7 +118,7 @@ typedef struct {
     nk_dtype_t c_dtype;        /* nk_f32_k, nk_bf16_k or nk_f16_k */
     void *c;
     nk_size_t c_stride;
-    float *pre;                /* for the gradients: A * W^T + bias before the activation, height x width, or NULL */
+    float *pre;                /* for the gradients, of 16-bit matrices: A * W^T + bias before the activation, height x width, or NULL */
     float *pre_up;             /* and A * W_up^T, gated only; both or none */
     nk_size_t pre_stride;
 } nk_amd_linear_t;

@@ -501,6 +501,7 @@ int check_linear(nk_amd_linear_t const *l) {
     if (l->activation < nk_amd_no_activation || l->activation > nk_amd_gelu_tanh) return mx_fail("linear: there is no such activation");
     if (l->gated && (l->bias || l->residual)) return mx_fail("linear: a gated product takes no bias and no residual");
     if ((l->bias && !float_bytes(l->bias_dtype)) || (l->residual && !float_bytes(l->residual_dtype))) return mx_fail("linear: bias and residual have to be f32, bf16 or f16");
+    if (mx8 && (l->pre || l->pre_up)) return mx_fail("linear: sums are left by products of 16-bit matrices (those of mx8 have no gradient, and not the bits of f32)");
     if (l->gated ? !l->pre != !l->pre_up : l->pre_up != nullptr) return mx_fail("linear: a gated product leaves both sums or none, another has one");
     return 0;
 }

@@ -444,10 +444,12 @@ def _left(a, w):
     return a
 
 
-def _product_dtype(a, w, out, out_dtype):
+def _product_dtype(a, w, out, out_dtype, sums):
     """The type of a product's results: A's, or bfloat16 where A is 8-bit or 32-bit and W 8-bit."""
     lib, torch, dtype_codes = _library()
     eight = isinstance(w, Mx8Matrix)
+    if eight and sums:
+        raise TypeError("sums are given by products of 16-bit matrices: those of 8-bit ones have no gradient, and not the bits of float32")
     if out_dtype is None and out is None:
         return torch.bfloat16 if isinstance(a, Mx8Matrix) or a.dtype == torch.float32 else a.dtype
     out_dtype = mx._out_dtype(out, out_dtype)
@@ -532,7 +534,7 @@ def linear(a, w, bias=None, activation=None, residual=None, out=None, out_dtype=
     ``out`` may be the residual itself, and shares memory with no other operand.
 
     16-bit products have gradients for ``a``, ``w``, ``bias`` and ``residual``, which autograd follows; 8-bit ones have none and refuse
-    operands that require one while autograd records. With ``sums`` the result is ``(y, a @ w.T + bias)``, as ``linear_backward`` takes them."""
+    operands that require one while autograd records. With ``sums`` (16-bit) the result is ``(y, a @ w.T + bias)``, as ``linear_backward`` takes them."""
     lib, torch, dtype_codes = _LIB or _library()
     if _CALLS is not None and out is None:
         if (made := _CALLS.linear(*_parts(a), *_parts(w), None, None, bias, ACTIVATIONS.get(activation), residual, out_dtype, sums)) is not None:
@@ -545,7 +547,7 @@ def linear(a, w, bias=None, activation=None, residual=None, out=None, out_dtype=
         residual = _floats(residual, "residual")
         if tuple(residual.shape) != (height, width):
             raise ValueError(f"residual must have shape {(height, width)}, got {tuple(residual.shape)}")
-    out_dtype = _product_dtype(t, w, out, out_dtype)
+    out_dtype = _product_dtype(t, w, out, out_dtype, sums)
     index = _home(t, w, bias, residual)
     if index is None:
         _check_host_out(out, (height, width), out_dtype)
@@ -568,7 +570,7 @@ def linear(a, w, bias=None, activation=None, residual=None, out=None, out_dtype=
 
 def gated_linear(a, w_gate, w_up, activation="silu", out=None, out_dtype=None, sums: bool = False):
     """``activation(a @ w_gate.T) * (a @ w_up.T)``, both products in one kernel. Operands, types and gradients as in ``linear``; the two
-    matrices have one type and shape. With ``sums`` the result is ``(y, a @ w_gate.T, a @ w_up.T)``, as ``gated_linear_backward`` takes them."""
+    matrices have one type and shape. With ``sums`` (16-bit) the result is ``(y, a @ w_gate.T, a @ w_up.T)``, as ``gated_linear_backward`` takes them."""
     lib, torch, dtype_codes = _LIB or _library()
     if _CALLS is not None and out is None and w_up is not None:
         if (made := _CALLS.linear(*_parts(a), *_parts(w_gate), *_parts(w_up), None, ACTIVATIONS.get(activation), None, out_dtype, sums)) is not None:
@@ -577,7 +579,7 @@ def gated_linear(a, w_gate, w_up, activation="silu", out=None, out_dtype=None, s
     if gate.shape != up.shape or isinstance(gate, Mx8Matrix) != isinstance(up, Mx8Matrix) or getattr(gate, "dtype", None) != getattr(up, "dtype", None):
         raise ValueError("w_gate and w_up must have the same shape and type")
     t, code = _left(a, gate), _activation(activation)
-    out_dtype = _product_dtype(t, gate, out, out_dtype)
+    out_dtype = _product_dtype(t, gate, out, out_dtype, sums)
     shape = t.shape[0], gate.shape[0]
     index = _home(t, gate, up)
     if index is None:

@@ -62,3 +62,19 @@ def test_operands_with_a_tangent_are_refused():
             with torch.no_grad(), pytest.raises(nk.NumKongAmdError, match="forward-mode"):
                 binding._tracked(torch, *operands)
         assert not binding._tracked(torch, x, forward.unpack_dual(dual).primal)
+
+
+def test_8_bit_products_give_no_sums():
+    """Results of 8-bit products are 16-bit for the bits that the matrix instruction drops: 32-bit sums would show them, and no backward pass takes them."""
+    lib = binding._library()[0]
+    fields = dict(height=100, width=64, depth=96, a_dtype=BF16, a=SOME, a_stride=192, w_dtype=E4M3, w=SOME, w_stride=96, w_scales=SOME, w_scales_stride=4, c_dtype=BF16, c=SOME,
+                  c_stride=128, pre_stride=256)
+    gated = dict(gated=1, w_up=SOME, w_up_stride=96, w_up_scales=SOME, w_up_scales_stride=4)
+    for l in (binding._Linear(**fields, pre=SOME), binding._Linear(**fields, **gated, pre=SOME, pre_up=SOME), binding._Linear(**fields, **gated, pre_up=SOME)):
+        assert lib.nk_amd_linear_async(l, None, 0, None) != 0 and "16-bit matrices" in lib.nk_hip_last_error().decode()
+        assert lib.nk_amd_linear_workspace_size(l) == 0
+    x = torch.zeros((4, 64), dtype=torch.bfloat16)
+    w8 = nk.Mx8Matrix(torch.zeros((8, 64), dtype=torch.uint8), torch.zeros((8, 2), dtype=torch.uint8))
+    for call in (lambda: nk.linear(x, w8, sums=True), lambda: nk.linear(w8, w8, sums=True), lambda: nk.gated_linear(x, w8, w8, sums=True)):
+        with pytest.raises(TypeError, match="16-bit matrices"):
+            call()

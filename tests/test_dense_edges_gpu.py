@@ -50,3 +50,10 @@ def test_operands_with_a_tangent_are_refused():
         same = forward.make_dual(x, torch.ones_like(x))
         codes = nk.mx8_quantize(same)  # (numbers that no gradient passes)
         assert torch.equal(codes.codes.view(torch.uint8), nk.mx8_quantize(x).codes.view(torch.uint8))
+
+
+def test_8_bit_products_give_no_sums():
+    x, w8 = normal(5, 64, torch.bfloat16, 1).to(DEV), nk.mx8_quantize(normal(8, 64, torch.bfloat16, 2).to(DEV))
+    for call in (lambda: nk.linear(x, w8, sums=True), lambda: nk.linear(nk.mx8_quantize(x), w8, sums=True), lambda: nk.gated_linear(x, w8, w8, sums=True)):
+        with pytest.raises(TypeError, match="16-bit matrices"):
+            call()
