@@ -215,6 +215,10 @@ def _result(torch, out, shape, dtype, like):
         raise ValueError("out rows must be contiguous")
     if t.dim() == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1]:
         raise ValueError("out rows share memory")
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise NumKongAmdError("out requires a gradient, which results written into it do not carry: detach it, or call under torch.no_grad()")
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)  # (so that a backward pass that has kept its old values says so)
     return t
 
 

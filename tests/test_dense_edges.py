@@ -78,3 +78,22 @@ def test_8_bit_products_give_no_sums():
     for call in (lambda: nk.linear(x, w8, sums=True), lambda: nk.linear(w8, w8, sums=True), lambda: nk.gated_linear(x, w8, w8, sums=True)):
         with pytest.raises(TypeError, match="16-bit matrices"):
             call()
+
+
+def test_results_in_out_are_seen_by_autograd():
+    """A tensor that a backward pass has kept, and that a call has written over since, has to be noticed; one that requires a gradient is refused."""
+    out = torch.zeros((2, 8))
+    version = out._version
+    assert binding._result(torch, out, (2, 8), torch.float32, out) is out and out._version > version
+    leaf = torch.zeros((2, 8), requires_grad=True)
+    kept = (leaf * leaf.sin())  # (keeps the sine)
+    for t in (leaf, kept):
+        with pytest.raises(nk.NumKongAmdError, match="requires a gradient"):
+            binding._result(torch, t, (2, 8), torch.float32, t)
+    with torch.no_grad():
+        binding._result(torch, leaf, (2, 8), torch.float32, leaf)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.sum().backward()
+    with torch.inference_mode():
+        t = torch.zeros((2, 8))
+        assert binding._result(torch, t, (2, 8), torch.float32, t) is t

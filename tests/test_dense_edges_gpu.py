@@ -57,3 +57,19 @@ def test_8_bit_products_give_no_sums():
     for call in (lambda: nk.linear(x, w8, sums=True), lambda: nk.linear(nk.mx8_quantize(x), w8, sums=True), lambda: nk.gated_linear(x, w8, w8, sums=True)):
         with pytest.raises(TypeError, match="16-bit matrices"):
             call()
+
+
+def test_results_in_out_are_seen_by_autograd():
+    x, w = normal(8, 64, torch.bfloat16, 1).to(DEV), normal(64, 64, torch.bfloat16, 2).to(DEV)
+    leaf, buffer, w8, packed = torch.ones_like(x).requires_grad_(), x.clone(), nk.mx8_quantize(w), nk.mx_pack(w)
+    calls = (lambda out: nk.linear(x, w, out=out), lambda out: nk.linear(x, w, residual=out, out=out), lambda out: nk.linear(x, w8, out=out), lambda out: nk.gated_linear(x, w, w, out=out),
+             lambda out: nk.mx_dots_packed(x, packed, out=out))
+    for call in calls:
+        loss = (leaf * buffer).sum()  # (keeps the buffer)
+        call(buffer)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        with pytest.raises(nk.NumKongAmdError, match="requires? a gradient"):
+            call(leaf)
+    with torch.no_grad():
+        assert torch.equal(nk.linear(x, w, out=leaf), nk.linear(x, w))
