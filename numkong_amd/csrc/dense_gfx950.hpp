@@ -162,11 +162,14 @@ __device__ __forceinline__ float scale_of(uint32_t byte) {
 }
 
 /**
- *  Activations and their slopes in 32 bits, off by a few units in the last place. The sigmoid is 1 / (1 + e^-x) by the part's own 2^x and reciprocal
+ *  Activations and their slopes in 32 bits. An activation is off by at most 16 + 4 z units of 2^-24 of itself, z the magnitude of the exponent (x, for gelu_tanh
+ *  1.6 (x + 0.045 x^3)), a slope by as many of the largest slope, and both by what the limits below leave out. The sigmoid is 1 / (1 + e^-x) by the part's own 2^x and reciprocal
  *  (one unit each; with the library's forms, chosen by a switch for each value, bias and relu of f16 8192 x 8191 x 1000 took 60 us more). The tanh of gelu_tanh is written as 1 - 2 / (1 + e^2z), so that 0.5 x (1 + tanh z) = x / (1 + e^-2z).
  *  Gelu: with h = erfc(|x| / sqrt 2) / 2 it is x - x h, or x h below zero, and h = e^(-x^2/2) t P(t), t = 1 / (1 + 0.35 |x|): P is fitted
  *  to that quotient over all |x| <= 16 by least squares weighted towards the largest relative error (8 degrees, 5 units of 2^-24 with its
- *  evaluation). What is beyond +-16 (+-110 for slopes) is at its limit.
+ *  evaluation).
+ *  Limits: the reciprocal of what is above 2^126 is zero, so that silu ends at -87.3 and gelu_tanh at -10.0 (both were below 1.1e-36 there). Gelu and its slope
+ *  are at their limits beyond +-16, as e^(-x^2/2) is 0 in 32 bits already, silu's slope beyond +-80 (off by 1.5e-33), gelu_tanh's beyond +-9 (2.6e-27).
  */
 __device__ __forceinline__ float power_of_2(float x) {
 #ifdef NK_MX_DEVICE_BUILTINS

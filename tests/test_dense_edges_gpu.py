@@ -73,3 +73,24 @@ def test_results_in_out_are_seen_by_autograd():
             call(leaf)
     with torch.no_grad():
         assert torch.equal(nk.linear(x, w, out=leaf), nk.linear(x, w))
+
+
+@pytest.mark.parametrize("kind", ds.ACTIVATIONS[1:])
+def test_activations_and_slopes_over_their_whole_range(kind):
+    """Every activation and slope of any 32-bit x, through a product of zeros with x as its bias, and through the bias's gradient, both in 32 bits. What may
+    be off: roundings (of the exponent z four: z units each), and below 1.1e-36 (silu's end), of slopes 2.6e-27 (gelu_tanh's)."""
+    ends = torch.tensor([9.0, 10.0, 13.2, 16.0, 80.0, 87.3, 88.0, 89.0, 92.0, 104.0, 128.0, 129.0, 1e4, 3e38, 1e-20, 1e-38, 1e-44, 0.0])
+    x = torch.cat([torch.linspace(-130, 130, 40001), torch.linspace(-12, 12, 20001), ends, -ends, torch.nextafter(ends, ends + 1), -torch.nextafter(ends, ends + 1)])
+    n = len(x)
+    zeros = torch.zeros((n, 1), dtype=torch.bfloat16, device=DEV)
+    got = nk.linear(zeros[:1], zeros, x.to(DEV), kind, out_dtype=torch.float32)[0]
+    p = x.double()
+    near = p.clamp(-128, 128)  # (what is beyond is at its limit, and its exponent with it)
+    z = 1.6 * (near.abs() + 0.045 * near.abs() ** 3) if kind == "gelu_tanh" else near.abs()
+    truth = torch.where(p > 128, p, torch.where(p < -128, 0.0, ds.activate(kind, near)))
+    ds.assert_within(got, truth, (16 + 4 * z.clamp(max=128)) * ds.UNIT * truth.abs() + 1.1e-36, kind)
+    slopes = nk.linear_backward(torch.ones((1, n), device=DEV), zeros[:1], zeros, x.to(DEV)[None], kind, need_a=False, need_w=False, bias_dtype=torch.float32)[2]
+    truth = torch.where(p > 128, 1.0, torch.where(p < -128, 0.0, ds.slope(kind, near)))
+    if kind == "relu":
+        truth = (p > 0).double()  # (0 at 0)
+    ds.assert_within(slopes, truth, (16 + 4 * z.clamp(max=128)) * ds.UNIT * ds.STEEPEST + 2.6e-27, f"slope of {kind}")
