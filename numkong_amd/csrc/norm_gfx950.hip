@@ -195,9 +195,11 @@ struct Raw {
 
 /**
  *  Threads (x) share a row, rows (y) a workgroup, as forward; a workgroup has every gridDim.x-th of such groups and keeps its part of the weight's
- *  gradient in registers until the last. Rows of at most 8192 values are asked for before the one before is worked on (of longer ones two do
- *  not fit the registers; HALF: all operands are of 16 bits). Memory is what bounds it (8192 x 4096 bf16
- *  with the total's gradient: 62 us without the weight's, 113 with it, when rows were loaded in turn and 1024 parts added up by 128 workgroups).
+ *  gradient in registers until the last. Where a thread has eight values of a row (P = 1: rows of at most 512 values, and of 1025 to 8192) a row is asked for before
+ *  the one before is worked on; of others a row is read twice, the second time out of the caches. HALF: all operands are of 16 bits.
+ *  Memory is what bounds it up to there (with the weight's and the total's gradient: 8192 x 4096 bf16 56 to 60 us, 4.5 to 4.8 TB/s, f32 110, 4.9; 8192 x 8192 bf16 104, 5.2;
+ *  16384 x 1024 bf16 37, 3.7). Rows of more than 8192 values do not fit the 128 registers of 1024 threads: with P = 2 some 16 to 19 of f32 or mixed types go to
+ *  scratch memory (4096 x 16384 bf16 147 us, 3.6 TB/s, f32 339, 3.2), with P = 4 109 to 221 of every type (2000 x 32768 bf16 396 us, 1.3 TB/s; f32 694), which bounds these.
  */
 template <class T, int P, bool HALF>
 __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(NormBackwardArgs p) {
@@ -205,7 +207,6 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(NormBackwardArg
     __shared__ float sums[2][16][2];
     extern __shared__ float parts[]; // rows of a workgroup but the first: theirs of the weight's gradient
     float of_weight[P][8] = {};
-    constexpr bool kAhead = P == 1;
     Raw<HALF> w, ahead[3];
     auto const load_weight = [&](uint32_t col) { if (p.weight) w.load(p.weight_kind, (uint8_t const *)p.weight, col, p.k); };
     auto const load_row = [&](uint64_t row, uint32_t col, Raw<HALF> (&raw)[3], bool rest) { // total, gradient, the total's gradient
@@ -216,15 +217,12 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(NormBackwardArg
     if (P == 1) load_weight(threadIdx.x * 8); // (of longer rows it comes out of the caches each time, and so do their values for the second loop)
     uint64_t const step = (uint64_t)gridDim.x * blockDim.y;
     uint64_t row = (uint64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    if (kAhead && row < p.rows) load_row(row, threadIdx.x * 8, ahead, true);
+    if (P == 1 && row < p.rows) load_row(row, threadIdx.x * 8, ahead, true);
     for (uint32_t turn = 0; row < p.rows; row += step, turn ^= 1) { // (two sets of sums: no wavefront writes what another still reads)
         float square = 0, inner = 0;
         Raw<HALF> now[3];
-        if (P == 1) {
-            if (kAhead) now[0] = ahead[0], now[1] = ahead[1], now[2] = ahead[2];
-            else load_row(row, threadIdx.x * 8, now, true);
-        }
-        if (kAhead && row + step < p.rows) load_row(row + step, threadIdx.x * 8, ahead, true);
+        if (P == 1) now[0] = ahead[0], now[1] = ahead[1], now[2] = ahead[2];
+        if (P == 1 && row + step < p.rows) load_row(row + step, threadIdx.x * 8, ahead, true);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             uint32_t const col = (i * blockDim.x + threadIdx.x) * 8;
@@ -305,7 +303,7 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(float const *values, u
     store_1(kind, out, col, sum);
 }
 
-constexpr uint64_t kMaxNormDepth = 32768; // (1024 threads of 32 values; with 64 the kernels spill)
+constexpr uint64_t kMaxNormDepth = 32768; // (1024 threads of 32 values, which the forward kernels hold; those of the backward pass spill)
 
 /** Threads for a row and how many times eight values one has. */
 struct NormShape {
