@@ -94,3 +94,73 @@ def test_activations_and_slopes_over_their_whole_range(kind):
     if kind == "relu":
         truth = (p > 0).double()  # (0 at 0)
     ds.assert_within(slopes, truth, (16 + 4 * z.clamp(max=128)) * ds.UNIT * ds.STEEPEST + 2.6e-27, f"slope of {kind}")
+
+
+SEGMENT = 22 << 20  # (the allocator asks the driver for so much by itself: what is behind it is no tensor's)
+
+
+@pytest.fixture
+def at_end():
+    """Makes copies of matrices and vectors that end with the last byte of an allocation from the driver, their rows `pad` values further apart, NaN before and between."""
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    kept = []
+
+    def place(x, pad=0):
+        room = torch.empty(SEGMENT, dtype=torch.uint8, device=DEV)
+        ends = [s["address"] + s["total_size"] for s in torch.cuda.memory_snapshot()]
+        if room.data_ptr() + SEGMENT not in ends:
+            pytest.skip("the allocator cuts its segments otherwise")
+        values = room.view(x.dtype if x.dtype != torch.float8_e4m3fn else torch.uint8)
+        values.fill_(float("nan") if x.dtype.is_floating_point and x.dtype != torch.float8_e4m3fn else 127)
+        rows, depth = x.shape if x.dim() == 2 else (1, x.shape[0])
+        start = values.numel() - ((rows - 1) * (depth + pad) + depth)
+        view = values.view(x.dtype).as_strided(x.shape, (depth + pad, 1) if x.dim() == 2 else (1,), start)
+        view.copy_(x)
+        kept.append(room)
+        assert view.data_ptr() + (view.shape[0] - 1) * view.stride(0) * view.itemsize + view.shape[-1] * view.itemsize == room.data_ptr() + SEGMENT or x.dim() == 1
+        return view
+
+    yield place
+    torch.cuda.synchronize()
+    kept.clear()
+    torch.cuda.empty_cache()
+
+
+# few rows; tiles of 64, 128 and 256; depths that end within 16 bytes and, of rows apart, are read in place; rows at odd addresses, which are moved
+@pytest.mark.parametrize("m,n,k,pad", [(1, 100, 999, 0), (3, 64, 1000, 3), (16, 33, 130, 0), (17, 512, 130, 0), (65, 257, 72, 4), (100, 130, 66, 2), (129, 255, 8, 0), (200, 96, 6, 2),
+                                       (257, 511, 1001, 0), (300, 520, 1002, 6), (513, 1030, 328, 0)])
+def test_products_of_operands_at_the_last_bytes_of_memory(at_end, m, n, k, pad):
+    a, w, up = (normal(r, k, torch.bfloat16, s) for r, s in ((m, 1), (n, 2), (n, 3)))
+    bias, residual, grad = normal(1, n, torch.float32, 4)[0], normal(m, n, torch.float16, 5), normal(m, n, torch.bfloat16, 6)
+    ga, gw, gu = at_end(a, pad), at_end(w, pad), at_end(up, pad)
+    truth = ds.Linear(a.double(), w.double(), None, bias.double(), "gelu", residual.double())
+    y, sums = nk.linear(ga, gw, at_end(bias), "gelu", at_end(residual, pad), out=at_end(torch.zeros_like(grad), pad), sums=True)
+    truth.check(y)
+    of_a, of_w, of_bias = nk.linear_backward(at_end(grad, pad), ga, gw, at_end(sums, pad), "gelu", bias_dtype=torch.float32)
+    truth.check_gradients(grad, a=of_a, w=of_w, bias=of_bias)
+    gated = ds.Linear(a.double(), w.double(), up.double(), None, "silu")
+    y, gate_sums, up_sums = nk.gated_linear(ga, gw, gu, sums=True)
+    gated.check(y)
+    of_a, of_w, of_up = nk.gated_linear_backward(at_end(grad, pad), ga, gw, gu, at_end(gate_sums, pad), at_end(up_sums, pad))
+    gated.check_gradients(grad, a=of_a, w=of_w, w_up=of_up)
+    a8, w8, up8 = (nk.mx8_quantize(t) for t in (ga, gw, gu))
+    placed = [nk.Mx8Matrix(at_end(t.codes, pad), at_end(t.scales, pad)) for t in (a8, w8, up8)]
+    assert torch.equal(nk.linear(placed[0], placed[1]), nk.linear(a8, w8)) and torch.equal(nk.linear(ga, placed[1]), nk.linear(a8, w8))
+    assert torch.equal(nk.gated_linear(*placed), nk.gated_linear(a8, w8, up8))
+    assert torch.equal(nk.mx8_dequantize(placed[0], torch.bfloat16), nk.mx8_dequantize(a8, torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", ds.FLOATS)
+@pytest.mark.parametrize("rows,depth,pad", [(1, 1, 0), (5, 7, 0), (9, 129, 3), (5, 513, 0), (3, 2049, 1), (3, 8191, 0), (2, 16385, 1), (1, 32767, 0)])
+def test_norms_of_operands_at_the_last_bytes_of_memory(at_end, dtype, rows, depth, pad):
+    x, r, g, w = normal(rows, depth, dtype, 1), normal(rows, depth, dtype, 2), normal(rows, depth, dtype, 3), (1 + 0.3 * normal(1, depth, torch.float32, 4, 0.0)[0]).to(dtype)
+    operands = [t.to(DEV) for t in (x, w, r)]
+    placed = at_end(x, pad), at_end(w), at_end(r, pad)
+    for got, want in zip(nk.rms_norm(*placed), nk.rms_norm(*operands)):
+        assert torch.equal(got, want)
+    (got, total), (want, _) = nk.rms_norm_mx8(*placed), nk.rms_norm_mx8(*operands)
+    assert torch.equal(got.codes.view(torch.uint8), want.codes.view(torch.uint8)) and torch.equal(got.scales, want.scales)
+    of = nk.rms_norm_backward(at_end(g, pad), at_end(total, pad), placed[1], at_end(r, pad))
+    for got, want in zip(of, nk.rms_norm_backward(g.to(DEV), total, operands[1], operands[2])):
+        assert torch.equal(got, want)
