@@ -365,8 +365,8 @@ int launch_few_of(FewArgs const &p, bool gated, hipStream_t stream) {
 }
 /**
  *  Which products go there: those of up to 16 rows, and of up to 64 where the matrix is small. Each workgroup reads all of A, and every 32 rows all of its
- *  columns, so that tiles win with size: 24 x 8192 x 8192 bf16 38.6 us here and 33 in tiles, 24 x 1024 x 8192 12.5 and 14, 64 x 2048 x 2048 10.9 in
- *  tiles. (Whole passes over three sets of operands.)
+ *  columns, so that tiles win with size: 24 x 8192 x 8192 bf16 38.6 us here and 33 in tiles, 24 x 1024 x 8192 12.5 and 14, 64 x 2048 x 2048, the largest that goes here, 6.4 and 10.9.
+ *  (Whole passes over three sets of operands, bf16; 8 bits go by the same limit, with 24 x 8192 x 8192 20 us in tiles.)
  */
 bool of_few_rows(uint64_t m, uint64_t n, uint64_t k, bool gated) { return m <= 16 || (m <= 64 && (double)m * (double)n * (double)k * (gated ? 2 : 1) <= 0x1p28); }
 
@@ -380,10 +380,14 @@ struct TilePlan {
 };
 /**
  *  The shape of tiles and the splits of the depth that take the least time by a simple account, in microseconds of a compute unit, from what was
- *  measured with bf16: a stage of a workgroup that is alone (512 x 4096 x 4096 and 64 x 8192 x 8192), one among as many as fit (8192 x 8192 by depths of 64 to
+ *  measured with bf16: a stage of a workgroup that is alone (512 x 4096 x 4096 and 64 x 8192 x 8192), one among as many as the account takes to fit (8192 x 8192 by depths of 64 to
  *  4096), what a tile's beginning and end add, and a launch and the partial sums' way through memory where there are splits. It is within a
- *  sixth of the times of ten products between 64 x 8192 x 8192 and 4096 x 4096 x 1024. The transposing reads of depths along columns cost tiles of 128 rows more (the
+ *  sixth of the times of ten bf16 products between 64 x 8192 x 8192 and 4096 x 4096 x 1024. The transposing reads of depths along columns cost tiles of 128 rows more (the
  *  gradient of 4096 x 2048 over 16384: 316 us in such tiles).
+ *
+ *  All types and forms go by it, some of them worse. Of gated tiles of 64 rows three fit, where four are counted, and of those in 8 bits with depths that end at any byte two:
+ *  1001 x 2050 x 1000 has 528 tiles for 512 places, so that it takes 19 to 20.5 us and not 9.6. The results' bytes are not counted: f16 8192 x 8191 x 1000 to f32 takes 190 to 222 us and
+ *  not 149 (153 for tiles of 128 rows).
  */
 TilePlan tile_plan(uint64_t m, uint64_t n, uint64_t stages, bool gated, bool b_columns = false) {
     static constexpr double kAlone[3] = {0.45, 0.57, 1.48}, kEach[3] = {0.173, 0.442, 1.48}, kEnds[3] = {0.8, 2.5, 13.5};

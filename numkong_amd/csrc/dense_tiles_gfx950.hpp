@@ -19,7 +19,7 @@
  *  row; 64 rows at a time they go through LDS, where adjacent ones of a row come together: bias, activation and residual are
  *  added there, in 32 bits, and whole lines are written.
  *
- *  Measured: 256 x 256 bf16 8192 x 8192 x 4096 416 us (1.32 PFLOP/s), 8192^3 797 us (1.38), gated 8192 x 8192 x 4096 832 us; columns 8192 x 4096 x 4096 206 us (both operands)
+ *  Measured: 256 x 256 bf16 8192 x 8192 x 4096 416 us (1.32 PFLOP/s), 8192^3 797 us (1.38), gated 8192 x 8192 x 4096 868 to 880 us; columns 8192 x 4096 x 4096 206 us (both operands)
  *  and 216 (one); 8 bits 8192^3 400 us (2.75). Power bounds them: matrix instructions take 65 % of the cycles at 1.6 to 1.9 GHz, waits 10 to 14 %.
  */
 #ifndef NUMKONG_AMD_DENSE_TILES_GFX950_HPP

@@ -379,7 +379,7 @@ def rms_norm_mx8(x, weight=None, residual=None, eps: float = 1e-6):
 def rms_norm_backward(grad, total, weight=None, grad_total=None, eps: float = 1e-6, need_weight: bool = True):
     """The gradients ``(of x, of weight)`` from ``grad``, that of ``y``: ``total`` is what was normed (``x``, or the sum that ``rms_norm``
     returned), ``grad_total`` the gradient that the sum has got from elsewhere. That of the residual is that of ``x``. The second is
-    None without a ``weight``, or where it is not needed."""
+    None without a ``weight``, or where it is not needed. Autograd does not follow this call."""
     lib, torch, dtype_codes = _LIB or _library()
     if _CALLS is not None and (made := _CALLS.norm_backward(grad, total, weight, grad_total, eps, need_weight)) is not None:
         return made
@@ -651,7 +651,8 @@ def _backward(grad, a, w, w_up, sums, activation, need_a, need_w, need_up, bias_
 def linear_backward(grad, a, w, sums=None, activation=None, need_a: bool = True, need_w: bool = True, bias_dtype=None):
     """The gradients ``(of a, of w, of bias)`` of a 16-bit ``linear`` from ``grad``, that of its result; that of the residual is ``grad``
     itself. ``sums`` are those that ``linear`` gave (not looked at without an activation). What is not needed is None; the bias's is given
-    where ``bias_dtype`` says its type."""
+    where ``bias_dtype`` says its type. The gradient of ``a @ w.T`` is rounded to the matrices' type on the way, and has its range: with float16, scale
+    ``grad`` so that it fits. Autograd does not follow this call."""
     if activation is not None and sums is None:
         raise ValueError("an activation's gradient needs the sums that linear(..., sums=True) gives")
     of_a, of_w, _, of_bias = _backward(grad, a, w, None, () if sums is None else (sums,), activation, need_a, need_w, False, bias_dtype, "linear_backward")
@@ -661,7 +662,7 @@ def linear_backward(grad, a, w, sums=None, activation=None, need_a: bool = True,
 def gated_linear_backward(grad, a, w_gate, w_up, gate_sums, up_sums, activation="silu", need_a: bool = True, need_gate: bool = True,
                           need_up: bool = True):
     """The gradients ``(of a, of w_gate, of w_up)`` of a 16-bit ``gated_linear`` from ``grad``, that of its result, and the sums that it
-    gave. What is not needed is None."""
+    gave. What is not needed is None. Those of the two products are rounded as in ``linear_backward``. Autograd does not follow this call."""
     if w_up is None:
         raise TypeError("w_up must be a matrix")
     return _backward(grad, a, w_gate, w_up, (gate_sums, up_sums), activation, need_a, need_gate, need_up, None, "gated_linear_backward")[:3]
