@@ -145,8 +145,11 @@ bool needs(torch::autograd::AutogradContext *ctx, int64_t i) {
     return there >> i & 1 && ctx->needs_input_grad((size_t)__builtin_popcountll((uint64_t)there & ((1ull << i) - 1)));
 }
 void check(int status, char const *where) { TORCH_CHECK(!status, where, ": ", library.last_error()); }
-/** A gradient as the kernels read it: autograd hands on expanded and transposed ones too. */
-at::Tensor rows_of(at::Tensor const &t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
+/** A gradient as the kernels read it: autograd hands on expanded and transposed ones too, and ones with a tangent. */
+at::Tensor rows_of(at::Tensor const &t) {
+    TORCH_CHECK(!t._fw_grad(0).defined(), "the operators have no forward-mode derivatives: a gradient has a tangent");
+    return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous();
+}
 /** Gradients that no gradient passes: asked for one, they say so. */
 torch::autograd::variable_list once(torch::autograd::variable_list found) {
     if (!c10::GradMode::is_enabled()) return found;

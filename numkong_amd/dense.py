@@ -16,7 +16,7 @@ import ctypes
 
 from . import mx
 from .api import NK_BF16, NK_E4M3, NK_F16, NK_F32, NumKongAmdError, _is_numpy
-from .mx import _check, _check_host_out, _floats, _home, _result, _row_bytes, _tensor, _to_host, _tracked
+from .mx import _check, _check_host_out, _floats, _home, _no_tangent, _result, _row_bytes, _tensor, _to_host, _tracked
 
 BLOCK = 32  # values of a row that share a scale
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
@@ -391,6 +391,7 @@ def rms_norm_backward(grad, total, weight=None, grad_total=None, eps: float = 1e
         grad_total = _floats(grad_total, "grad_total")
         if grad_total.shape != t.shape or grad_total.dtype != t.dtype:
             raise ValueError(f"grad_total must be {tuple(t.shape)} of {t.dtype} as total is")
+    _no_tangent(torch, g, t, weight, grad_total)
     index = _home(g, t, weight, grad_total)
     if index is None:
         found = rms_norm_backward(_to_gpu(g), _to_gpu(t), _to_gpu(weight), _to_gpu(grad_total), eps, need_weight)
@@ -624,6 +625,7 @@ def _backward(grad, a, w, w_up, sums, activation, need_a, need_w, need_up, bias_
     sums = [_floats(one, "sums") for one in sums]
     if any(one.dtype != torch.float32 or tuple(one.shape) != (height, width) for one in sums):
         raise ValueError(f"sums must be {(height, width)} of float32, as the product gives them")
+    _no_tangent(torch, g, t, w, w_up, *sums)
     index = _home(g, t, w, w_up, *sums)
     if index is None:
         found = _backward(_to_gpu(g), _to_gpu(t), _to_gpu(w), _to_gpu(w_up), [_to_gpu(one) for one in sums], activation, need_a, need_w, need_up, bias_dtype, where)

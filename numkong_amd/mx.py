@@ -144,10 +144,15 @@ def _autograd():
         _PRODUCT, _ROUTE = Product, Route
 
 
-def _tracked(torch, *operands) -> bool:
-    """Does autograd follow one of the operands? One that has a tangent is refused (torch.no_grad() does not end forward mode, so it is not asked)."""
+def _no_tangent(torch, *operands) -> None:
+    """Refuses operands that have a tangent, which no result would carry on (torch.no_grad() does not end forward mode, so it is not asked)."""
     if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in operands):
         raise NumKongAmdError("the operators have no forward-mode derivatives: an operand has a tangent, unpack it (torch.autograd.forward_ad.unpack_dual)")
+
+
+def _tracked(torch, *operands) -> bool:
+    """Does autograd follow one of the operands? One that has a tangent is refused."""
+    _no_tangent(torch, *operands)
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands)
 
 
@@ -526,6 +531,7 @@ def experts_route_backward(grad_weights, logits, experts, score: str = "softmax"
         raise ValueError(f"grad_weights {tuple(grad_weights.shape)} and experts {tuple(experts.shape)} must be tokens x top_k, tokens {tokens}")
     if grad_weights.dtype != torch.float32 or experts.dtype != torch.int32:
         raise TypeError("grad_weights must be float32 and experts int32")
+    _no_tangent(torch, grad_weights, t)
     index = _home(t, grad_weights, experts)
     if index is None:
         found = experts_route_backward(_to_gpu(grad_weights), _to_gpu(t), _to_gpu(experts), score, renormalize, scale)

@@ -64,6 +64,19 @@ def test_operands_with_a_tangent_are_refused():
         assert not binding._tracked(torch, x, forward.unpack_dual(dual).primal)
 
 
+def test_gradients_with_a_tangent_are_refused():
+    forward = torch.autograd.forward_ad
+    x, w, v = torch.ones((2, 8), dtype=torch.bfloat16), torch.ones((8, 8), dtype=torch.bfloat16), torch.ones(8)
+    weights, chosen = torch.ones((2, 2)), torch.zeros((2, 2), dtype=torch.int32)
+    calls = [(lambda t: nk.rms_norm_backward(t, x, v), x), (lambda t: nk.rms_norm_backward(x, t, v), x), (lambda t: nk.rms_norm_backward(x, x, t), v), (lambda t: nk.rms_norm_backward(x, x, v, t), x),
+             (lambda t: nk.linear_backward(t, x, w), x), (lambda t: nk.linear_backward(x, t, w), x), (lambda t: nk.linear_backward(x, x, t), w), (lambda t: nk.linear_backward(x, x, w, t, "silu"), x.float()),
+             (lambda t: nk.gated_linear_backward(x, x, w, t, x.float(), x.float()), w), (lambda t: nk.experts_route_backward(t, x, chosen), weights), (lambda t: nk.experts_route_backward(weights, t, chosen), x)]
+    with forward.dual_level():
+        for call, t in calls:
+            with pytest.raises(nk.NumKongAmdError, match="forward-mode"):
+                call(forward.make_dual(t, torch.ones_like(t)))
+
+
 def test_8_bit_products_give_no_sums():
     """Results of 8-bit products are 16-bit for the bits that the matrix instruction drops: 32-bit sums would show them, and no backward pass takes them."""
     lib = binding._library()[0]

@@ -52,6 +52,29 @@ def test_operands_with_a_tangent_are_refused():
         assert torch.equal(codes.codes.view(torch.uint8), nk.mx8_quantize(x).codes.view(torch.uint8))
 
 
+def test_gradients_with_a_tangent_are_refused():
+    """Forward mode over a backward pass: the pass's own gradients would carry no tangent on."""
+    forward = torch.autograd.forward_ad
+    x, w, v = (normal(m, 64, torch.bfloat16, m).to(DEV) for m in (5, 64, 1))
+    v, logits = v[0], normal(5, 8, torch.float32, 9).to(DEV)
+    leaf, free = x.clone().requires_grad_(), logits.clone().requires_grad_()
+    found = [(nk.rms_norm(leaf, v), leaf), (nk.rms_norm(leaf, v, x)[0], leaf), (nk.rms_norm(leaf, v, x)[1], leaf), (nk.linear(leaf, w, activation="silu"), leaf), (nk.gated_linear(leaf, w, w), leaf),
+             (nk.experts_route(free, 2)[0], free)]
+    with forward.dual_level():
+        for y, t in found:
+            grad = torch.ones_like(y)
+            plain, = torch.autograd.grad(y, t, grad, retain_graph=True)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, t, forward.make_dual(grad, torch.ones_like(grad)), retain_graph=True)
+            assert torch.equal(torch.autograd.grad(y, t, grad)[0], plain)
+    dual_calls = [(lambda t: nk.rms_norm_backward(t, x, v), x), (lambda t: nk.linear_backward(x, t, w), x), (lambda t: nk.gated_linear_backward(x, x, w, t, x.float(), x.float()), w)]
+    with forward.dual_level():
+        for call, t in dual_calls:
+            call(t)
+            with pytest.raises(nk.NumKongAmdError, match="forward-mode"):
+                call(forward.make_dual(t, torch.ones_like(t)))
+
+
 def test_8_bit_products_give_no_sums():
     x, w8 = normal(5, 64, torch.bfloat16, 1).to(DEV), nk.mx8_quantize(normal(8, 64, torch.bfloat16, 2).to(DEV))
     for call in (lambda: nk.linear(x, w8, sums=True), lambda: nk.linear(nk.mx8_quantize(x), w8, sums=True), lambda: nk.gated_linear(x, w8, w8, sums=True)):
